@@ -1,4 +1,5 @@
-"""ctypes binding of ``libdsr_sampling.so`` (declared in include/dsr_sampling.h).
+"""ctypes binding of ``libdsr_sampling.so`` (declared in include/dsr_sampling.h
+and include/dsr_tree.h).
 
 The library is built in-tree by ``deepseekrpc_amd.build`` and is loaded from
 next to this file.  There is no fallback: if the library is missing, or its
@@ -53,6 +54,22 @@ EXPORTS = (
     "dsr_vocab_head", "dsr_verify_drafts_head", "dsr_prob_stats_rows", "dsr_verify_probs_workspace_bytes",
     "dsr_verify_probs", "dsr_rows_finite", "dsr_count_scan", "dsr_sample_rows_head",
 )
+# include/dsr_tree.h
+TREE_EXPORTS = (
+    "dsr_plan_workspace_bytes", "dsr_tree_attention_workspace_bytes", "dsr_plan_blocks", "dsr_rotary",
+    "dsr_tree_attention", "dsr_commit_tree",
+)
+F16 = 4
+E_LENGTH = 16
+E_BLOCKS = 17
+E_CAPACITY = 18
+E_TREE = 19
+E_BLOCK = 20
+TREE_MAX_NODES = 64
+TREE_MAX_PAGE = 1024
+TREE_MAX_REQUESTS = 16384
+ROTARY_MAX_DIM = 512
+ATTENTION_MAX_DIM = 256
 NOALLOC_SCRATCH_BYTES = 268435456
 HEAD_TILE = 128
 STATS_MAX_ROWS = 16
@@ -120,6 +137,52 @@ class HeadArgs(ctypes.Structure):
     ]
 
 
+class PlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("lengths", _p), ("added", _p), ("parents", _p), ("held_in", _p), ("pool_state_in", _p), ("table", _p),
+        ("pool", _p), ("requests", _i64), ("table_ld", _i64), ("capacity", _i64), ("width", _i32), ("page", _i32),
+        ("pool_size", _i32), ("blocks", _i32), ("held_out", _p), ("pool_state_out", _p), ("offsets", _p),
+        ("kv_lengths", _p), ("status", _p), ("slots", _p), ("positions", _p), ("owners", _p), ("visible", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("q_out", _p), ("k", _p), ("k_out", _p), ("v", _p), ("positions", _p), ("freqs", _p), ("slots", _p),
+        ("k_cache", _p), ("v_cache", _p), ("status", _p), ("dtype", _i32), ("q_heads", _i32), ("kv_heads", _i32),
+        ("head_dim", _i32), ("v_dim", _i32), ("rot_start", _i32), ("rot_dim", _i32), ("interleaved", _i32),
+        ("inverse", _i32), ("page", _i32), ("blocks", _i32), ("reserved", _i32), ("magnitude", _f64),
+        ("tokens", _i64), ("q_token", _i64), ("q_head", _i64), ("qo_token", _i64), ("qo_head", _i64),
+        ("k_token", _i64), ("k_head", _i64), ("ko_token", _i64), ("ko_head", _i64), ("v_token", _i64),
+        ("v_head", _i64), ("kc_block", _i64), ("kc_token", _i64), ("kc_head", _i64), ("vc_block", _i64),
+        ("vc_token", _i64), ("vc_head", _i64),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("k_cache", _p), ("v_cache", _p), ("table", _p), ("offsets", _p), ("kv_lengths", _p),
+        ("visible", _p), ("out", _p), ("lse", _p), ("status", _p), ("dtype", _i32), ("q_heads", _i32),
+        ("kv_heads", _i32), ("head_dim", _i32), ("page", _i32), ("width", _i32), ("blocks", _i32),
+        ("scale", ctypes.c_float), ("requests", _i64), ("tokens", _i64), ("table_ld", _i64), ("q_token", _i64),
+        ("q_head", _i64), ("out_token", _i64), ("out_head", _i64), ("k_block", _i64), ("k_token", _i64),
+        ("k_head", _i64), ("v_block", _i64), ("v_token", _i64), ("v_head", _i64), ("workspace", _p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class CommitArgs(ctypes.Structure):
+    _fields_ = [
+        ("parents", _p), ("tokens_in", _p), ("sampled", _p), ("offsets", _p), ("kv_lengths", _p), ("table", _p),
+        ("output_limit", _p), ("eos_off", _p), ("eos_ids", _p), ("caches", _p), ("path", _p), ("ids", _p),
+        ("accepted", _p), ("count", _p), ("pending", _p), ("stop", _p), ("lengths", _p), ("status", _p),
+        ("requests", _i64), ("tokens", _i64), ("table_ld", _i64), ("width", _i32), ("page", _i32), ("blocks", _i32),
+        ("cache_count", _i32), ("heads", _i32), ("row_bytes", _i32), ("c_block", _i64), ("c_token", _i64),
+        ("c_head", _i64),
+    ]
+
+
 class NativeUnavailable(RuntimeError):
     """The HIP library is missing or incompatible; there is no CPU fallback."""
 
@@ -179,6 +242,14 @@ def load(path: str = LIB_PATH):
     lib.dsr_sample_rows_head.argtypes = [ctypes.POINTER(SampleArgs), _p, _p]
     lib.dsr_count_scan.restype = _i32
     lib.dsr_count_scan.argtypes = [_p, _i32, _i64, _p, _p]
+    lib.dsr_plan_workspace_bytes.restype = ctypes.c_size_t
+    lib.dsr_plan_workspace_bytes.argtypes = [_i64]
+    lib.dsr_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.dsr_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
+    for name, args in (("dsr_plan_blocks", PlanArgs), ("dsr_rotary", RotaryArgs),
+                       ("dsr_tree_attention", TreeAttentionArgs), ("dsr_commit_tree", CommitArgs)):
+        getattr(lib, name).restype = _i32
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), _p]
     _lib = lib
     return lib
 

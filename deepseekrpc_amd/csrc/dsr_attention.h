@@ -1,0 +1,501 @@
+// Attention of a step's new tokens over a paged cache (dsr_tree_attention).
+//
+// For one request and key head the rows are (new token, query head of the
+// group) pairs: rows = new x group.  They share the head's keys and values, so
+// a workgroup takes a tile of rows and a chunk of the request's tokens and
+// reads each key and value of the chunk once.  When the tiles of all requests
+// do not fill the chip, requests are cut into chunks of tokens (attn_unit),
+// whose partial results k_tree_combine joins.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dsr_tree.h"
+
+namespace dsr {
+
+typedef float attn_f32x4 __attribute__((ext_vector_type(4)));
+
+// Rows of bf16 or f16: vector types and matrix products.
+template <class T>
+struct AttnType;
+template <>
+struct AttnType<__bf16> {
+  typedef __bf16 x4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kExponent = 0x7F80u;  // all ones: infinity or NaN
+  static constexpr float kLift = 0.f;
+  static __device__ __forceinline__ attn_f32x4 mfma16(x8 a, x8 b, attn_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct AttnType<_Float16> {
+  typedef _Float16 x4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kExponent = 0x7C00u;
+  // Weights are 2^7 times larger (at most 2^15), so that those of a long
+  // context's many small terms keep their bits: f16 has no normal number
+  // below 2^-14.
+  static constexpr float kLift = 7.f;
+  static __device__ __forceinline__ attn_f32x4 mfma16(x8 a, x8 b, attn_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Transposing LDS read: of the 16 lanes of a group, lane i points at four
+// elements of row i / 4 (columns 4 (i % 4) ...) of a 4 x 16 block and gets the
+// four rows' elements of column i.
+template <class T>
+__device__ __forceinline__ typename AttnType<T>::x4 attn_read_tr(const T* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(typename AttnType<T>::x4,
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnWaves = 4;
+constexpr int kAttnTile = 32;             // tokens a wave takes at a time
+constexpr int kAttnChunk = 128;           // chunks are multiples of this many tokens
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// What the host decides for one call.
+struct AttnPlan {
+  int tile_rows;      // rows of a tile
+  int target;         // units (tile x chunk x head) aimed at
+  int min_chunk;      // tokens, a multiple of kAttnChunk
+  int tiles_bound;    // row tiles of all requests at most
+  int64_t max_parts;  // partial results the workspace holds
+  float* part_o;      // [max_parts, tile_rows, head dim of the kernel]
+  float2* part_ml;    // [max_parts, tile_rows]: base (log2) and sum
+  int32_t* part_bad;  // [max_parts]: a page id outside the cache
+};
+
+struct AttnRequest {
+  int lo, n, kv;  // first new token, new tokens, cached tokens (0: nothing to read)
+  int rows, tiles;
+  bool fine;
+};
+
+__device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_args_t& a, int group, int tile_rows,
+                                                    int r) {
+  AttnRequest q;
+  int lo = a.offsets[r], hi = a.offsets[r + 1];
+  const int N = (int)a.tokens;
+  lo = lo < 0 ? 0 : lo > N ? N : lo;
+  hi = hi < lo ? lo : hi > N ? N : hi;
+  q.lo = lo;
+  q.n = hi - lo;
+  const int kv = a.kv_lengths[r];
+  q.fine = kv >= q.n && kv <= (int64_t)a.width * a.page && !(a.visible && q.n > DSR_TREE_MAX_NODES);
+  q.rows = q.n * group;
+  q.kv = q.fine && q.n > 0 ? kv : 0;
+  q.tiles = q.rows > tile_rows ? (q.rows + tile_rows - 1) / tile_rows : 1;
+  return q;
+}
+
+// One unit of work: rows of a tile against a chunk of a request's tokens.
+struct AttnUnit {
+  int r, head, tile, tiles, chunk, chunks, size;  // size: tokens per chunk
+  int64_t part;                                   // partial result of chunk 0 (chunks > 1), `tiles * heads` apart
+  bool any;
+};
+
+// Unit `u` of the launch, found by every wave for itself from the requests'
+// lengths (64 at a time).  The chunk size makes about `target` units of equal
+// size out of the tokens that the row tiles have to pass over.  `chunked`
+// false: units are tiles alone (k_tree_combine).
+__device__ __forceinline__ AttnUnit attn_unit(const dsr_tree_attention_args_t& a, const AttnPlan& p, int u,
+                                              bool chunked) {
+  const int l = threadIdx.x & 63, R = (int)a.requests, H = a.kv_heads, group = a.q_heads / a.kv_heads;
+  AttnUnit out;
+  out.any = false;
+  out.head = u % H;
+  const int w = u / H;
+  int64_t load = 0;
+  AttnRequest q;
+  for (int r0 = 0; r0 < R; r0 += 64) {
+    const int r = r0 + l < R ? r0 + l : R - 1;
+    q = attn_request(a, group, p.tile_rows, r);
+    if (r0 + l < R) load += (int64_t)q.tiles * q.kv;
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) load += __shfl_xor(load, s);
+  int64_t size = (load * H + p.target - 1) / p.target;
+  size = (size + kAttnChunk - 1) / kAttnChunk * kAttnChunk;
+  if (size < p.min_chunk) size = p.min_chunk;
+  if (size > (1 << 30)) size = 1 << 30;
+  int before = 0;         // units of the requests passed
+  int64_t parts = 0;      // partial results of the requests passed
+  for (int r0 = 0; r0 < R; r0 += 64) {
+    const int r = r0 + l < R ? r0 + l : R - 1;
+    if (R > 64) q = attn_request(a, group, p.tile_rows, r);
+    // Equal chunks: as many as the size asks for, each a multiple of kAttnChunk.
+    const int chunks = q.kv > size ? (int)((q.kv + size - 1) / size) : 1;
+    const int units = r0 + l < R ? (chunked ? q.tiles * chunks : q.tiles) : 0;
+    int sum = units;
+    int64_t psum = r0 + l < R && chunks > 1 ? (int64_t)q.tiles * chunks : 0;
+    const int64_t own = psum;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int x = __shfl_up(sum, s);
+      const int64_t y = __shfl_up(psum, s);
+      if (l >= s) {
+        sum += x;
+        psum += y;
+      }
+    }
+    const uint64_t past = __ballot(before + sum > w);
+    if (past) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      const int rem = w - before - __shfl(sum - units, at);
+      const int tiles = __shfl(q.tiles, at), n_chunks = __shfl(chunks, at);
+      out.part = (parts + __shfl(psum - own, at)) * H;
+      out.r = r0 + at;
+      out.tiles = tiles;
+      out.chunks = n_chunks;
+      out.tile = rem % tiles;
+      out.chunk = chunked ? rem / tiles : 0;
+      const int kv = __shfl(q.kv, at);
+      out.size = n_chunks > 1 ? ((kv + n_chunks - 1) / n_chunks + kAttnTile - 1) / kAttnTile * kAttnTile : kv;
+      out.any = rem >= 0 && out.chunk < n_chunks && (n_chunks == 1 || out.part + (int64_t)tiles * n_chunks * H <= p.max_parts);
+      return out;
+    }
+    before += __shfl(sum, 63);
+    parts += __shfl(psum, 63);
+  }
+  return out;
+}
+
+template <class T>
+__device__ __forceinline__ bool attn_not_finite(typename AttnType<T>::x8 v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  constexpr uint32_t E = AttnType<T>::kExponent;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
+  return bad;
+}
+
+// Few rows (up to 16 NB of a tile): the four waves take the chunk's 32-token
+// tiles in turn, each for itself, and join their results at the end.
+//
+// S^T = K Q^T and O^T = V^T P^T, so that a lane holds one row's scores (row
+// lane % 16) and outputs: statistics and rescaling stay in the lane, and the
+// scores are the second product's operand as they lie, with the k index of
+// both operands permuted alike (lane group g takes tokens 4 g + i and
+// 16 + 4 g + i).  Keys go from memory to the product's registers directly;
+// values pass through the wave's own LDS rows, from which the transposing
+// read hands each lane four tokens of its dimension.  The next tile's keys
+// and values are in flight while a tile is worked on.
+//
+// The running maximum is raised only when a score passes it by 8 (log2): the
+// weights then stay below 2^8, far inside every type's range, and most tiles
+// need no rescaling.
+template <class T, int DP, int NB>
+__global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_tree_attention(
+    dsr_tree_attention_args_t a, AttnPlan p) {
+  typedef typename AttnType<T>::x4 x4;
+  typedef typename AttnType<T>::x8 x8;
+  constexpr int KS = DP / 32;   // k steps of the score product
+  constexpr int DB = DP / 16;   // 16-wide output blocks
+  constexpr int VS = DP + 16;   // LDS row of values: 32 bytes of padding spread the transposing reads over the banks
+  __shared__ T vals[kAttnWaves][kAttnTile][VS];
+  __shared__ float sm[kAttnWaves][16 * NB], sl[kAttnWaves][16 * NB];
+  __shared__ int sbad;
+
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const AttnUnit u = attn_unit(a, p, blockIdx.x, true);
+  if (!u.any) return;  // the same for the whole workgroup
+  if (threadIdx.x == 0) sbad = 0;
+  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
+  const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
+  const int ctx = q.kv - q.n;
+  const int begin = u.chunk * u.size;
+  const int end = min(begin + u.size, q.kv);
+  const int row0 = u.tile * p.tile_rows;
+
+  // This lane's rows: token index, mask, query operand.
+  x8 qv[NB][KS];
+  int tok[NB];
+  uint64_t mask[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int row = row0 + 16 * b + n;
+    const bool in = row < q.rows;
+    const int t = in ? row / group : 0, h = in ? row - t * group : 0;
+    tok[b] = t;
+    mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
+    const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + h) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 32 * s + 8 * g;
+      qv[b][s] = in && d < dim ? *(const x8*)(src + d) : x8{};
+    }
+  }
+
+  attn_f32x4 acc[NB][DB];
+  float m[NB], sum[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b] = -INFINITY;
+    sum[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[b][d] = attn_f32x4{};
+  }
+  const float scale = a.scale * kLog2e;
+  const int32_t* pages = a.table + u.r * a.table_ld;
+  const T* kb = (const T*)a.k_cache + u.head * a.k_head;
+  const T* vb = (const T*)a.v_cache + u.head * a.v_head;
+  const int shift = __ffs(a.page) - 1;
+  bool any_bad = false;
+
+  // Token tiles of this wave: 32 (4 i + w) past the chunk's begin.  Places
+  // past the last token read the last token (their scores are masked).
+  int ids[2];
+  uint32_t bad_next = 0;
+  x8 kr[2][KS], vr[2][KS];
+  auto load_ids = [&](int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) ids[b] = pages[min(p0 + 16 * b + n, end - 1) >> shift];
+  };
+  auto load_rows = [&](int p0) __attribute__((always_inline)) {
+    bad_next = 0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int place = min(p0 + 16 * b + n, end - 1) & (a.page - 1);
+      const bool bad = (unsigned)ids[b] >= (unsigned)a.blocks;
+      bad_next |= (uint32_t)(__ballot(bad) & 0xFFFF) << (16 * b);
+      const int64_t id = bad ? 0 : ids[b];
+      const T* ks = kb + id * a.k_block + place * a.k_token;
+      const T* vs = vb + id * a.v_block + place * a.v_token;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = min(32 * s + 8 * g, dim - 8);  // past the head: any of its values, dropped below
+        kr[b][s] = *(const x8*)(ks + d);
+        vr[b][s] = *(const x8*)(vs + d);
+      }
+    }
+  };
+  const int first = begin + kAttnTile * w, step = kAttnTile * kAttnWaves;
+  if (first < end) {
+    load_ids(first);
+    load_rows(first);
+    if (first + step < end) load_ids(first + step);
+  }
+  __syncthreads();  // sbad
+  for (int p0 = first; p0 < end; p0 += step) {
+    const uint32_t bad = bad_next;
+    const bool masked = p0 + kAttnTile > ctx || bad;  // some row may not see some token
+    any_bad |= bad != 0;
+    bool poison = false;
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) poison |= attn_not_finite<T>(vr[b][s]);
+      poison = __ballot(poison) != 0;
+    }
+    // Scores.
+    attn_f32x4 sc[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sc[b][k] = attn_f32x4{};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const x8 key = 32 * s + 8 * g < dim ? kr[k][s] : x8{};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) sc[b][k] = AttnType<T>::mfma16(key, qv[b][s], sc[b][k]);
+      }
+    // Values to LDS; then the next tile's loads.
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) *(x8*)&vals[w][16 * k + n][32 * s + 8 * g] = vr[k][s];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (p0 + step < end) {
+      load_rows(p0 + step);
+      if (p0 + 2 * step < end) load_ids(p0 + 2 * step);
+    }
+    // Softmax.  A lane's scores: tokens p0 + 16 k + 4 g + e of its row.
+    x8 pv[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = sc[b][k][e] * scale;
+          if (masked) {
+            const int j = p0 + 16 * k + 4 * g + e - ctx;
+            const bool see = j < 0 || (a.visible ? j < 64 && (mask[b] >> (j & 63) & 1) : j <= tok[b]);
+            x = see && j < q.n && p0 + 16 * k + 4 * g + e < end && !(bad >> (16 * k + 4 * g + e) & 1) ? x : -INFINITY;
+          }
+          sc[b][k][e] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__ballot(top - AttnType<T>::kLift > m[b] + 8.f)) {
+        const float next = fmaxf(m[b], top - AttnType<T>::kLift);
+        const float f = m[b] == next ? 1.f : __builtin_amdgcn_exp2f(m[b] - next);
+        m[b] = next;
+        sum[b] *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[b][d] *= f;
+      }
+      const float base = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(sc[b][k][e] - base);
+          sum[b] += x;
+          pv[b][4 * k + e] = (T)x;
+        }
+    }
+    if (!poison) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const T* at = &vals[w][4 * g + (n >> 2)][16 * d + 4 * (n & 3)];
+        const x4 lo = attn_read_tr<T>(at), hi = attn_read_tr<T>(at + 16 * VS);
+        const x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b][d] = AttnType<T>::mfma16(v, pv[b], acc[b][d]);
+      }
+    } else {
+      // An infinity or NaN among values that some row must not see: token by
+      // token, and only where the row sees it (0 x infinity would be NaN).
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            for (int from = 0; from < 4; ++from) {
+              const int t = 16 * k + 4 * from + e;
+              const float x = __shfl((float)pv[b][4 * k + e], n + 16 * from);
+              const float seen = __shfl(sc[b][k][e], n + 16 * from);
+              if (seen == -INFINITY) continue;
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[b][d][i] += x * (float)vals[w][t][16 * d + 4 * g + i];
+            }
+    }
+  }
+
+  // The four waves' results: statistics, then one row block at a time.
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    sum[b] += __shfl_xor(sum[b], 16);
+    sum[b] += __shfl_xor(sum[b], 32);
+    if (g == 0) {
+      sm[w][16 * b + n] = m[b];
+      sl[w][16 * b + n] = sum[b];
+    }
+  }
+  if (any_bad && l == 0) sbad = 1;
+  __syncthreads();
+  const bool split = u.chunks > 1;
+  const int64_t part = u.part + ((int64_t)u.chunk * u.tiles + u.tile) * a.kv_heads + u.head;
+  constexpr int OS = DP + 4;  // LDS row of outputs
+  static_assert(16 * OS * sizeof(float) <= kAttnTile * VS * sizeof(T), "a wave's outputs fit its rows of values");
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float top = fmaxf(fmaxf(sm[0][16 * b + n], sm[1][16 * b + n]), fmaxf(sm[2][16 * b + n], sm[3][16 * b + n]));
+    const float f = m[b] == top ? 1.f : __builtin_amdgcn_exp2f(m[b] - top);  // a wave without tokens: 0
+    float* mine = (float*)&vals[w][0][0];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *(attn_f32x4*)&mine[n * OS + 16 * d + 4 * g] = acc[b][d] * f;
+    __syncthreads();
+    for (int x = threadIdx.x; x < 16 * (DP / 4); x += kAttnThreads) {
+      const int row = x / (DP / 4), d = x % (DP / 4) * 4, rr = 16 * b + row;
+      float M = sm[0][rr];
+#pragma unroll
+      for (int i = 1; i < kAttnWaves; ++i) M = fmaxf(M, sm[i][rr]);
+      float L = 0.f;
+      attn_f32x4 o = {};
+#pragma unroll
+      for (int i = 0; i < kAttnWaves; ++i) {
+        L += sl[i][rr] * (sm[i][rr] == M ? 1.f : __builtin_amdgcn_exp2f(sm[i][rr] - M));
+        o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
+      }
+      if (split) {
+        *(attn_f32x4*)&p.part_o[(part * p.tile_rows + rr) * DP + d] = o;
+        if (d == 0) p.part_ml[part * p.tile_rows + rr] = float2{M, L};
+      } else if (row0 + rr < q.rows && d < dim) {
+        const int t = (row0 + rr) / group, h = row0 + rr - t * group;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+        *(x4*)((T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + h) * a.out_head + d) = y;
+        if (a.lse && d == 0)
+          a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    if (split)
+      p.part_bad[part] = sbad;
+    else if (u.head == 0 && u.tile == 0)
+      a.status[u.r] = !q.fine ? DSR_E_LENGTH : sbad ? DSR_E_BLOCK : DSR_OK;
+  }
+}
+
+// Joins the chunks of a (request, tile, head): out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
+template <class T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void k_tree_combine(dsr_tree_attention_args_t a, AttnPlan p) {
+  typedef typename AttnType<T>::x4 x4;
+  const AttnUnit u = attn_unit(a, p, blockIdx.x, false);
+  if (!u.any || u.chunks == 1) return;
+  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
+  const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
+  const int row0 = u.tile * p.tile_rows;
+  const int rows = min(p.tile_rows, q.rows - row0);
+  const int64_t part = u.part + (int64_t)u.tile * a.kv_heads + u.head, next = (int64_t)u.tiles * a.kv_heads;
+  for (int x = threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
+    const int row = x / (DP / 4), d = x % (DP / 4) * 4;
+    if (d >= dim) continue;
+    float M = -INFINITY, L = 0.f;
+    attn_f32x4 o = {};
+    for (int c = 0; c < u.chunks; ++c) {
+      const int64_t at = (part + c * next) * p.tile_rows + row;
+      const float2 ml = p.part_ml[at];
+      const attn_f32x4 y = *(const attn_f32x4*)&p.part_o[at * DP + d];
+      const float top = fmaxf(M, ml.x);
+      const float f = M == top ? 1.f : __builtin_amdgcn_exp2f(M - top), f2 = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+      M = top;
+      L = L * f + ml.y * f2;
+      o = o * f + y * f2;
+    }
+    const int t = (row0 + row) / group, h = row0 + row - t * group;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+    *(x4*)((T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + h) * a.out_head + d) = y;
+    if (a.lse && d == 0)
+      a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  }
+  if (threadIdx.x == 0 && u.head == 0 && u.tile == 0) a.status[u.r] = DSR_OK;
+  __syncthreads();
+  if (u.head == 0 && u.tile == 0) {
+    // Any chunk of the request with a page id outside the cache (its first tile and head looked at all of them).
+    for (int c = threadIdx.x; c < u.chunks; c += kAttnThreads)
+      if (p.part_bad[part + c * next]) a.status[u.r] = DSR_E_BLOCK;
+  }
+}
+
+}  // namespace dsr

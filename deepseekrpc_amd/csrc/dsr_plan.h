@@ -1,0 +1,300 @@
+// Block tables, slot maps, positions and tree masks of a step's new tokens
+// (dsr_plan_blocks), from request lengths that only the device knows.
+//
+// Two parts.  plan_scan: one workgroup turns lengths and counts into
+// offsets, grants and the pool's ring index of each request's first new page
+// (prefix sums in 64 bits: counts come unchecked from device memory).
+// plan_tokens / plan_trees: every token's slot and position, 64 tokens to a
+// wave, and every new table entry, written by the token that first touches
+// the page (a new page lies wholly past the old tokens, so its first slot is
+// always a new token's).
+//
+// What bounds it is latency: a call reads and writes a few KB to a few MB,
+// and its chain is load -> three scans -> offset search -> table entry ->
+// store.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "dsr_tree.h"
+
+namespace dsr {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+
+// What plan_scan leaves for the second part, per request (a.workspace).
+struct PlanRow {
+  int32_t ring;  // granted: pool index of the first page taken; ended: of the first page given back
+  int32_t old;   // pages held before
+  int32_t mode;  // kPlanRefused / kPlanGranted / kPlanEnded
+};
+constexpr int kPlanRefused = 0, kPlanGranted = 1, kPlanEnded = 2;
+
+__device__ __forceinline__ int64_t plan_wave_scan(int64_t x) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int64_t y = __shfl_up(x, s);
+    if ((int)(threadIdx.x & 63) >= s) x += y;
+  }
+  return x;
+}
+
+// Inclusive sums of x and y over the workgroup's 1,024 threads, and their totals.
+__device__ __forceinline__ void plan_block_scan(int64_t& x, int64_t& y, int64_t* part, int64_t& tx, int64_t& ty) {
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  x = plan_wave_scan(x);
+  y = plan_wave_scan(y);
+  __syncthreads();  // the last call's readers are done
+  if (l == 63) {
+    part[w] = x;
+    part[kPlanWaves + w] = y;
+  }
+  __syncthreads();
+  tx = ty = 0;
+  int64_t bx = 0, by = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanWaves; ++i) {
+    const int64_t px = part[i], py = part[kPlanWaves + i];
+    if (i < w) {
+      bx += px;
+      by += py;
+    }
+    tx += px;
+    ty += py;
+  }
+  x += bx;
+  y += by;
+}
+
+// One workgroup of 1,024 threads.
+__device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
+  __shared__ int64_t part[2 * kPlanWaves];
+  const int R = (int)a.requests;
+  PlanRow* rows = (PlanRow*)a.workspace;
+  int head = a.pool_state_in[0], count = a.pool_state_in[1];
+  if (head < 0 || head >= a.pool_size || count < 0 || count > a.pool_size) head = count = 0;  // not a pool: empty
+  int64_t tokens = 0, pages = 0, back = 0, taken = 0, given = 0;  // sums over the requests before this round's
+  for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
+    const int r = r0 + (int)threadIdx.x;
+    const bool in = r < R;
+    const int64_t L = in ? a.lengths[r] : 0, A = in ? a.added[r] : 0, held = in ? a.held_in[r] : 0;
+    int status = DSR_OK;
+    if (L < 0 || A < -1 || held < 0 || held > a.width || L > held * a.page || L + A > (int64_t)a.width * a.page)
+      status = DSR_E_LENGTH;
+    const bool ended = A == -1;
+    const int64_t take = A > 0 ? A : 0;
+    int64_t ends = take, wants = 0, total, unused;
+    plan_block_scan(ends, wants, part, total, unused);
+    ends += tokens;
+    if (status == DSR_OK && take > 0 && ends > a.capacity) status = DSR_E_CAPACITY;
+    int64_t need = 0, give = 0;
+    if (status == DSR_OK && !ended) need = (L + take + a.page - 1) / a.page - held;
+    if (need < 0) need = 0;
+    if (status == DSR_OK && ended) give = held;
+    int64_t need_to = need, give_to = give, needs, gives;
+    plan_block_scan(need_to, give_to, part, needs, gives);
+    need_to += pages;
+    give_to += back;
+    if (need > 0 && need_to > count) status = DSR_E_BLOCKS;
+    if (give > 0 && give_to > (int64_t)a.pool_size - count) status = DSR_E_BLOCKS;
+    const bool granted = status == DSR_OK && !ended, frees = status == DSR_OK && ended;
+    if (in) {
+      PlanRow p;
+      p.ring = granted ? (int)((head + need_to - need) % a.pool_size)
+                       : frees ? (int)(((int64_t)head + count + give_to - give) % a.pool_size) : 0;
+      p.old = (int)held;
+      p.mode = granted ? kPlanGranted : frees ? kPlanEnded : kPlanRefused;
+      rows[r] = p;
+      a.offsets[r + 1] = (int)(ends < a.capacity ? ends : a.capacity);
+      if (r == 0) a.offsets[0] = 0;
+      a.kv_lengths[r] = granted ? (int)(L + take) : 0;
+      a.held_out[r] = granted ? (int)(held + need) : frees ? 0 : (int)held;
+      a.status[r] = status;
+    }
+    // Pages really taken and given: the sums up to the last request served.
+    int64_t t = granted ? need : 0, g = frees ? give : 0, tt, gg;
+    plan_block_scan(t, g, part, tt, gg);
+    tokens += total;
+    pages += needs;
+    back += gives;
+    taken += tt;
+    given += gg;
+  }
+  if (threadIdx.x == 0) {
+    if (R == 0) a.offsets[0] = 0;
+    a.pool_state_out[0] = (int)((head + taken) % a.pool_size);
+    a.pool_state_out[1] = (int)(count - taken + given);
+  }
+}
+
+// The slot of place `p` of request r, and, if this is the first slot of a
+// new page, the page's table entry.
+__device__ __forceinline__ int plan_slot(const dsr_plan_args_t& a, const PlanRow& row, int64_t r, int p) {
+  const int b = p / a.page, o = p & (a.page - 1);
+  int id;
+  if (b < row.old) {
+    id = a.table[r * a.table_ld + b];
+  } else {
+    id = a.pool[(int)(((int64_t)row.ring + b - row.old) % a.pool_size)];
+    if (o == 0) a.table[r * a.table_ld + b] = id;
+  }
+  if ((unsigned)id >= (unsigned)a.blocks) {
+    a.status[r] = DSR_E_BLOCK;
+    a.kv_lengths[r] = 0;
+    return -1;
+  }
+  return id * a.page + o;
+}
+
+__device__ __forceinline__ void plan_write(const dsr_plan_args_t& a, int64_t i, int slot, int position, int owner,
+                                           uint64_t mask) {
+  a.slots[i] = slot;
+  a.positions[i] = position;
+  if (a.owners) a.owners[i] = owner;
+  if (a.visible) a.visible[i] = mask;
+}
+
+// The number of requests whose tokens end at or before token i (its owner),
+// for a whole wave at once: 64 offsets per round.
+__device__ __forceinline__ int plan_owner(const dsr_plan_args_t& a, int i) {
+  const int l = threadIdx.x & 63;
+  int lo = 0, n = (int)a.requests;
+  while (n > 0) {
+    const int stride = (n + 63) / 64, end = lo + n;
+    const int at = lo + l * stride + stride - 1;
+    const uint64_t le = __ballot(at < end && a.offsets[at < end ? at + 1 : 0] <= i);
+    lo += __popcll(le) * stride;
+    n = end - lo < stride - 1 ? end - lo : stride - 1;
+  }
+  return lo;
+}
+
+// How many of the wave's 64 non-decreasing x are <= i, for each lane's own i.
+__device__ __forceinline__ int plan_count(int x, int i) {
+  int c = 0;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1)
+    if (__shfl(x, c + s - 1) <= i) c += s;
+  return __shfl(x, c) <= i ? c + 1 : c;
+}
+
+// Tokens i0 .. i0 + 63 (one wave).
+__device__ __forceinline__ void plan_tokens(const dsr_plan_args_t& a, int i0) {
+  const int l = threadIdx.x & 63, R = (int)a.requests;
+  const int i = i0 + l;
+  // Each token's owner lies as many requests behind token i0's as end at or
+  // before the token; 64 requests a round (empty ones can make it more).
+  int base = plan_owner(a, i0), r = base, c;
+  do {
+    c = plan_count(base + l < R ? a.offsets[base + l + 1] : INT_MAX, i);
+    r += r == base ? c : 0;
+    base += 64;
+  } while (__ballot(c == 64));
+  if (i >= a.capacity) return;
+  if (r >= R || i >= a.offsets[R]) {
+    plan_write(a, i, -1, 0, -1, 0);
+    return;
+  }
+  const PlanRow row = ((const PlanRow*)a.workspace)[r];
+  if (row.mode != kPlanGranted) {
+    plan_write(a, i, -1, 0, r, 0);
+    return;
+  }
+  const int p = a.lengths[r] + i - a.offsets[r];
+  const int slot = plan_slot(a, row, r, p);
+  plan_write(a, i, slot, slot < 0 ? 0 : p, r, 0);
+}
+
+// Request r's pages back to the pool, if it ended (one wave).
+__device__ __forceinline__ void plan_release(const dsr_plan_args_t& a, int r) {
+  const PlanRow row = ((const PlanRow*)a.workspace)[r];
+  if (row.mode != kPlanEnded) return;
+  for (int b = threadIdx.x & 63; b < row.old; b += 64)
+    a.pool[(int)(((int64_t)row.ring + b) % a.pool_size)] = a.table[r * a.table_ld + b];
+}
+
+// Request r's tree, one node per lane: masks and depths by pointer doubling
+// (after round k a node knows its nearest 2^k ancestors).
+__device__ __forceinline__ void plan_tree(const dsr_plan_args_t& a, int r) {
+  const int l = threadIdx.x & 63;
+  const PlanRow row = ((const PlanRow*)a.workspace)[r];
+  const int lo = a.offsets[r], n = a.offsets[r + 1] - lo;
+  if (row.mode != kPlanGranted) {
+    for (int i = l; i < n; i += 64) plan_write(a, lo + i, -1, 0, r, 0);
+    return;
+  }
+  const int par = l < n ? a.parents[lo + l] : -1;
+  if (__ballot(par >= l || par < -1) || n > DSR_TREE_MAX_NODES) {
+    for (int i = l; i < n; i += 64) {
+      plan_write(a, lo + i, -1, 0, r, 0);
+      // Pages already taken stay with the request, table entries included.
+      const int p = a.lengths[r] + i;
+      if (p / a.page >= row.old && (p & (a.page - 1)) == 0) plan_slot(a, row, r, p);
+    }
+    if (l == 0) {
+      a.status[r] = DSR_E_TREE;
+      a.kv_lengths[r] = 0;
+    }
+    return;
+  }
+  uint64_t mask = 1ull << l;
+  int depth = par >= 0 ? 1 : 0, up = par;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const int at = up < 0 ? l : up;
+    const uint64_t m = __shfl(mask, at);
+    const int d = __shfl(depth, at), u = __shfl(up, at);
+    if (up >= 0) {
+      mask |= m;
+      depth += d;
+      up = u;
+    }
+  }
+  if (l >= n) return;
+  const int p = a.lengths[r] + l;
+  const int slot = plan_slot(a, row, r, p);
+  plan_write(a, lo + l, slot, slot < 0 ? 0 : a.lengths[r] + depth, r, slot < 0 ? 0 : mask);
+}
+
+// Tokens past the last request's (tree plans: the trees write their own).
+__device__ __forceinline__ void plan_padding(const dsr_plan_args_t& a, int i) {
+  if (i < a.capacity && i >= a.offsets[a.requests]) plan_write(a, i, -1, 0, -1, 0);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_plan_scan(dsr_plan_args_t a) { plan_scan(a); }
+
+// 256 threads: workgroups [0, token_groups) take 256 tokens each, the others four requests each.
+__global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_groups) {
+  const int w = threadIdx.x >> 6, b = blockIdx.x;
+  if (b < token_groups) {
+    if (a.parents)
+      plan_padding(a, b * 256 + (int)threadIdx.x);
+    else
+      plan_tokens(a, b * 256 + w * 64);
+    return;
+  }
+  const int r = (b - token_groups) * 4 + w;
+  if (r >= a.requests) return;
+  if (a.parents) plan_tree(a, r);
+  plan_release(a, r);
+}
+
+// The whole plan in one workgroup, for calls that fit it.
+__global__ __launch_bounds__(kPlanThreads) void k_plan_small(dsr_plan_args_t a) {
+  plan_scan(a);
+  __threadfence_block();
+  __syncthreads();
+  const int w = threadIdx.x >> 6;
+  if (a.parents) {
+    for (int i = threadIdx.x; i < a.capacity; i += kPlanThreads) plan_padding(a, i);
+    for (int r = w; r < a.requests; r += kPlanWaves) plan_tree(a, r);
+  } else {
+    for (int i = w * 64; i < a.capacity; i += kPlanThreads) plan_tokens(a, i);
+  }
+  for (int r = w; r < a.requests; r += kPlanWaves) plan_release(a, r);
+}
+
+}  // namespace dsr

@@ -32,6 +32,7 @@
 #include "dsr_split.h"
 #include "dsr_verify.h"
 #include "dsr_wide.h"
+#include "dsr_tree.h"
 #include "dsr_wide_verify.h"
 
 namespace dsr {
@@ -1179,6 +1180,11 @@ const char* dsr_status_message(int32_t code) {
     case DSR_E_HISTORY: return "history needs bounded exact integer token IDs";
     case DSR_E_APPEND: return "a history append holds at most 16384 tokens per row";
     case DSR_E_HINT: return "request contradicts the call's DSR_HINT_VERIFY_FAST promise";
+    case DSR_E_LENGTH: return "a length, page count or offset lies outside its bounds";
+    case DSR_E_BLOCKS: return "the page pool cannot serve the request";
+    case DSR_E_CAPACITY: return "the new tokens do not fit the token arrays";
+    case DSR_E_TREE: return "drafted nodes are not a tree of at most 64 nodes in parent-first order";
+    case DSR_E_BLOCK: return "a page id or slot lies outside the cache";
     default: return "unknown sampling status";
   }
 }

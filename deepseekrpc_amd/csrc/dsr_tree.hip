@@ -1,0 +1,227 @@
+// C ABI of dsr_tree.h: argument checks and launches.
+#include "dsr_tree.h"
+
+#include "dsr_attention.h"
+#include "dsr_commit.h"
+#include "dsr_plan.h"
+#include "dsr_rotary.h"
+
+using namespace dsr;
+
+namespace {
+
+int32_t launched() { return hipGetLastError() == hipSuccess ? 0 : DSR_ERR_LAUNCH; }
+
+bool page_ok(int32_t page, int32_t blocks) {
+  return page >= 1 && page <= DSR_TREE_MAX_PAGE && (page & (page - 1)) == 0 && blocks >= 1 &&
+         (int64_t)blocks * page <= INT_MAX;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Plans of at most this many tokens and requests run in one workgroup.
+constexpr int kPlanSmallTokens = 4096, kPlanSmallRequests = 256;
+
+template <class T>
+int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
+  constexpr int VE = 16 / sizeof(T);
+  const int half = a.rot_dim / 2;
+  auto rows = [&](const void* p, int64_t t, int64_t h) { return !p || (aligned16(p) && t % VE == 0 && h % VE == 0); };
+  const bool wide = a.head_dim % VE == 0 && a.rot_start % VE == 0 &&
+                    (a.interleaved ? a.rot_dim % VE == 0 : half % VE == 0) && (!a.v || a.v_dim % VE == 0) &&
+                    rows(a.q, a.q_token, a.q_head) && rows(a.q_out, a.qo_token, a.qo_head) &&
+                    rows(a.k, a.k_token, a.k_head) && rows(a.k_out, a.ko_token, a.ko_head) &&
+                    rows(a.v, a.v_token, a.v_head) &&
+                    (!a.k_cache || (rows(a.k_cache, a.kc_token, a.kc_head) && a.kc_block % VE == 0)) &&
+                    (!a.v_cache || (rows(a.v_cache, a.vc_token, a.vc_head) && a.vc_block % VE == 0));
+  const int64_t items = (int64_t)(a.q_heads + a.kv_heads) * a.head_dim / (wide ? VE : 1);
+  // Few tokens: a token's rows are shared by several workgroups, so that the chip is filled.
+  int64_t parts = (1024 + a.tokens - 1) / a.tokens, most = (items + kRotaryThreads - 1) / kRotaryThreads;
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  const dim3 grid((unsigned)a.tokens, (unsigned)parts);
+  if (wide)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE>), grid, dim3(kRotaryThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1>), grid, dim3(kRotaryThreads), 0, s, a);
+  return launched();
+}
+
+// Dimensions of the kernel that takes a head dimension.
+int attn_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+
+// Host part of the work split, from sizes alone.
+AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
+  AttnPlan p{};
+  const int64_t group = a.q_heads / a.kv_heads;
+  const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
+  p.tile_rows = rows <= 16 || a.head_dim > 128 ? 16 : 32;
+  p.target = 512;
+  p.min_chunk = 256;
+  p.tiles_bound = (int)(a.tokens * group / p.tile_rows + a.requests);
+  p.max_parts = 2 * (int64_t)p.target + 64;
+  return p;
+}
+
+int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
+
+struct AttnSizes {
+  int64_t o, ml, bad, all;
+};
+AttnSizes attn_sizes(const dsr_tree_attention_args_t& a, const AttnPlan& p) {
+  AttnSizes s;
+  s.o = round256(p.max_parts * p.tile_rows * attn_dim(a.head_dim) * 4);
+  s.ml = round256(p.max_parts * p.tile_rows * 8);
+  s.bad = round256(p.max_parts * 4);
+  s.all = s.o + s.ml + s.bad;
+  return s;
+}
+
+bool attn_shape_ok(const dsr_tree_attention_args_t& a) {
+  return (a.dtype == DSR_BF16 || a.dtype == DSR_F16) && a.q_heads >= 1 && a.kv_heads >= 1 &&
+         a.q_heads % a.kv_heads == 0 && a.head_dim >= 8 && a.head_dim <= DSR_ATTENTION_MAX_DIM &&
+         a.head_dim % 8 == 0 && a.requests >= 0 && a.requests <= DSR_TREE_MAX_REQUESTS && a.tokens >= 0 &&
+         a.tokens * a.q_heads <= INT_MAX / 2;
+}
+
+template <class T, int DP>
+int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
+  const int64_t units = (int64_t)p.target + (int64_t)p.tiles_bound * a.kv_heads;
+  if (units > INT_MAX) return DSR_ERR_ARG;
+  const dim3 grid((unsigned)units), threads(kAttnThreads);
+  if (p.tile_rows == 16) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 1>), grid, threads, 0, s, a, p);
+  } else if constexpr (DP <= 128) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 2>), grid, threads, 0, s, a, p);
+  }
+  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+  if ((int64_t)a.width * a.page > p.min_chunk)  // else no request can have two chunks
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_combine<T, DP>), dim3((unsigned)(p.tiles_bound * a.kv_heads)), threads, 0,
+                       s, a, p);
+  return launched();
+}
+
+template <class T>
+int32_t attn_typed(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
+  switch (attn_dim(a.head_dim)) {
+    case 64: return attn_launch<T, 64>(a, p, s);
+    case 128: return attn_launch<T, 128>(a, p, s);
+    case 192: return attn_launch<T, 192>(a, p, s);
+    default: return attn_launch<T, 256>(a, p, s);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dsr_plan_workspace_bytes(int64_t requests) {
+  return requests > 0 && requests <= DSR_TREE_MAX_REQUESTS ? (size_t)requests * sizeof(PlanRow) : 0;
+}
+
+int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_plan_args_t& a = *args;
+  if (a.requests < 0 || a.requests > DSR_TREE_MAX_REQUESTS || a.capacity < 1 || a.capacity > (1 << 30) ||
+      !page_ok(a.page, a.blocks) || a.width < 1 || (int64_t)a.width * a.page > INT_MAX || a.table_ld < a.width ||
+      a.pool_size < 1)
+    return DSR_ERR_ARG;
+  if (!a.pool_state_in || !a.pool || !a.pool_state_out || !a.offsets || !a.slots || !a.positions ||
+      (a.parents && !a.visible) || (!a.parents && a.visible))
+    return DSR_ERR_ARG;
+  if (a.requests > 0 && (!a.lengths || !a.added || !a.held_in || !a.table || !a.held_out || !a.kv_lengths || !a.status))
+    return DSR_ERR_ARG;
+  if (a.requests > 0 && (!a.workspace || ((uintptr_t)a.workspace & 3u) ||
+                         a.workspace_bytes < dsr_plan_workspace_bytes(a.requests)))
+    return DSR_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  if (a.capacity <= kPlanSmallTokens && a.requests <= kPlanSmallRequests) {
+    hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(kPlanThreads), 0, s, a);
+    return launched();
+  }
+  hipLaunchKernelGGL(k_plan_scan, dim3(1), dim3(kPlanThreads), 0, s, a);
+  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+  const int token_groups = (int)((a.capacity + 255) / 256);
+  hipLaunchKernelGGL(k_plan_fill, dim3((unsigned)(token_groups + (a.requests + 3) / 4)), dim3(256), 0, s, a,
+                     token_groups);
+  return launched();
+}
+
+int32_t dsr_rotary(const dsr_rotary_args_t* args, void* stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_rotary_args_t& a = *args;
+  if ((a.dtype != DSR_BF16 && a.dtype != DSR_F16 && a.dtype != DSR_F32) || a.reserved != 0 || a.tokens < 0 ||
+      a.tokens > (1 << 30) || a.q_heads < 0 || a.kv_heads < 0 || a.q_heads > 65536 || a.kv_heads > 65536 ||
+      a.q_heads + a.kv_heads < 1 || a.head_dim < 2 || a.head_dim > DSR_ROTARY_MAX_DIM || a.rot_dim < 2 ||
+      a.rot_dim % 2 != 0 || a.rot_start < 0 || a.rot_start + a.rot_dim > a.head_dim ||
+      !(a.magnitude > 0.0 && a.magnitude < 1e30))
+    return DSR_ERR_ARG;
+  if (a.tokens == 0) return 0;
+  if (!a.positions || !a.freqs) return DSR_ERR_ARG;
+  if ((a.q_heads > 0) != (a.q != nullptr) || (a.q != nullptr) != (a.q_out != nullptr) ||
+      (a.kv_heads > 0) != (a.k != nullptr) || (a.k != nullptr) != (a.k_out || a.k_cache) ||
+      (a.v != nullptr) != (a.v_cache != nullptr) || (a.v && !a.k) ||
+      (a.v && (a.v_dim < 1 || a.v_dim > DSR_ROTARY_MAX_DIM)))
+    return DSR_ERR_ARG;
+  if ((a.k_cache || a.v_cache) && (!page_ok(a.page, a.blocks) || !a.slots)) return DSR_ERR_ARG;
+  if (!(a.k_cache || a.v_cache) && a.slots) return DSR_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  switch (a.dtype) {
+    case DSR_BF16: return rotary_typed<__bf16>(a, s);
+    case DSR_F16: return rotary_typed<_Float16>(a, s);
+    default: return rotary_typed<float>(a, s);
+  }
+}
+
+size_t dsr_tree_attention_workspace_bytes(const dsr_tree_attention_args_t* args) {
+  if (!args || !attn_shape_ok(*args)) return 0;
+  return (size_t)attn_sizes(*args, attn_plan(*args)).all;
+}
+
+int32_t dsr_tree_attention(const dsr_tree_attention_args_t* args, void* stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_tree_attention_args_t& a = *args;
+  if (!attn_shape_ok(a) || !page_ok(a.page, a.blocks) || a.width < 1 || (int64_t)a.width * a.page > INT_MAX ||
+      a.table_ld < a.width || !(a.scale == a.scale) || a.scale - a.scale != 0.f)
+    return DSR_ERR_ARG;
+  if (a.requests == 0) return a.tokens == 0 ? 0 : DSR_ERR_ARG;
+  if (!a.table || !a.offsets || !a.kv_lengths || !a.status || !a.k_cache || !a.v_cache ||
+      (a.tokens > 0 && (!a.q || !a.out)))
+    return DSR_ERR_ARG;
+  if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return DSR_ERR_ARG;
+  for (int64_t st : {a.q_token, a.q_head, a.out_token, a.out_head, a.k_block, a.k_token, a.k_head, a.v_block,
+                     a.v_token, a.v_head})
+    if (st % 8 != 0) return DSR_ERR_ARG;
+  AttnPlan p = attn_plan(a);
+  const AttnSizes z = attn_sizes(a, p);
+  if (!a.workspace || ((uintptr_t)a.workspace & 255u) || a.workspace_bytes < (size_t)z.all) return DSR_ERR_WORKSPACE;
+  p.part_o = (float*)a.workspace;
+  p.part_ml = (float2*)((char*)a.workspace + z.o);
+  p.part_bad = (int32_t*)((char*)a.workspace + z.o + z.ml);
+  hipStream_t s = (hipStream_t)stream;
+  return a.dtype == DSR_BF16 ? attn_typed<__bf16>(a, p, s) : attn_typed<_Float16>(a, p, s);
+}
+
+int32_t dsr_commit_tree(const dsr_commit_args_t* args, void* stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_commit_args_t& a = *args;
+  if (a.requests < 0 || a.requests > DSR_TREE_MAX_REQUESTS || a.tokens < 0 || a.tokens > INT_MAX ||
+      !page_ok(a.page, a.blocks) || a.width < 1 || (int64_t)a.width * a.page > INT_MAX || a.table_ld < a.width ||
+      a.cache_count < 0 || a.cache_count > 65535)
+    return DSR_ERR_ARG;
+  if (a.cache_count > 0 && (!a.caches || a.heads < 1 || a.heads > 65536 || a.row_bytes < 16 || a.row_bytes > 65536 ||
+                            a.row_bytes % 16 != 0 || a.c_block % 16 != 0 || a.c_token % 16 != 0 || a.c_head % 16 != 0))
+    return DSR_ERR_ARG;
+  if (a.requests == 0) return 0;
+  if (!a.offsets || !a.kv_lengths || !a.table || !a.output_limit || !a.path || !a.ids || !a.accepted || !a.count ||
+      !a.pending || !a.stop || !a.lengths || !a.status || a.lengths == a.kv_lengths ||
+      (a.tokens > 0 && (!a.parents || !a.tokens_in || !a.sampled)) || (a.eos_off && !a.eos_ids))
+    return DSR_ERR_ARG;
+  const int per = commit_caches(a);
+  const int groups = a.cache_count > 0 ? (a.cache_count + per - 1) / per : 1;
+  hipLaunchKernelGGL(k_commit_tree, dim3((unsigned)a.requests, (unsigned)groups), dim3(kCommitThreads), 0,
+                     (hipStream_t)stream, a);
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,153 @@
+"""include/dsr_tree.h against the binding and the library, without a GPU:
+exports, constants, struct layouts, argument errors ahead of any launch."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+
+from deepseekrpc_amd import _native as N
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "dsr_tree.h")
+STRUCTS = {"dsr_plan_args_t": N.PlanArgs, "dsr_rotary_args_t": N.RotaryArgs,
+           "dsr_tree_attention_args_t": N.TreeAttentionArgs, "dsr_commit_args_t": N.CommitArgs}
+
+
+def test_exports_and_constants():
+    text = open(HEADER).read()
+    lib = N.load()
+    names = set(re.findall(r"^\s*(?:int32_t|size_t)\s+(dsr_\w+)\s*\(", text, re.M))
+    assert names == set(N.TREE_EXPORTS)
+    for name in names:
+        assert hasattr(lib, name), name
+    defs = {m.group(1): int(m.group(2)) for m in re.finditer(r"#define (DSR_\w+) \(?(-?\d+)u?\)?", text)}
+    for name in ("F16", "E_LENGTH", "E_BLOCKS", "E_CAPACITY", "E_TREE", "E_BLOCK", "TREE_MAX_NODES", "TREE_MAX_PAGE",
+                 "TREE_MAX_REQUESTS", "ROTARY_MAX_DIM", "ATTENTION_MAX_DIM"):
+        assert getattr(N, name) == defs["DSR_" + name], name
+    for code in range(N.E_LENGTH, N.E_BLOCK + 1):
+        assert "unknown" not in N.status_message(code)
+
+
+def test_struct_layouts(tmp_path):
+    lines = [f'printf("{c} size %zu\\n", sizeof({c}));' for c in STRUCTS]
+    lines += [f'printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for c, s in STRUCTS.items() for f, _ in s._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "dsr_tree.h"\nint main(void) {\n'
+                   + "\n".join(lines) + "\nreturn 0; }\n")
+    subprocess.run(["gcc", "-std=c99", f"-I{os.path.dirname(HEADER)}", str(src), "-o", str(exe)], check=True)
+    got = {}
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        c, f, off = line.split()
+        got[c, f] = int(off)
+    for c, s in STRUCTS.items():
+        assert got[c, "size"] == ctypes.sizeof(s), c
+        for f, _ in s._fields_:
+            assert got[c, f] == getattr(s, f).offset, (c, f)
+
+
+def refused(call, a, bad, rc=-1):
+    """Every (field, value) of ``bad`` alone makes the call return ``rc``."""
+    for field, value in bad:
+        good = getattr(a, field)
+        setattr(a, field, value)
+        assert call(ctypes.byref(a), None) == rc, (field, value)
+        setattr(a, field, good)
+
+
+@pytest.mark.parametrize("name", ["dsr_plan_blocks", "dsr_rotary", "dsr_tree_attention", "dsr_commit_tree"])
+def test_null_arguments(name):
+    lib = N.load()
+    args = dict(dsr_plan_blocks=N.PlanArgs, dsr_rotary=N.RotaryArgs, dsr_tree_attention=N.TreeAttentionArgs,
+                dsr_commit_tree=N.CommitArgs)[name]
+    assert getattr(lib, name)(None, None) == -1
+    assert getattr(lib, name)(ctypes.byref(args()), None) == -1
+
+
+def test_plan_arguments():
+    lib = N.load()
+    a = N.PlanArgs()
+    for f in ("lengths", "added", "held_in", "pool_state_in", "table", "pool", "held_out", "pool_state_out", "offsets",
+              "kv_lengths", "status", "slots", "positions", "workspace"):
+        setattr(a, f, 4096)
+    a.requests, a.table_ld, a.capacity, a.width, a.page, a.pool_size, a.blocks = 4, 8, 16, 8, 16, 9, 9
+    a.workspace_bytes = lib.dsr_plan_workspace_bytes(4)
+    refused(lib.dsr_plan_blocks, a, [("requests", -1), ("requests", N.TREE_MAX_REQUESTS + 1), ("table_ld", 7),
+                                     ("capacity", 0), ("capacity", 2**30 + 1), ("width", 0), ("page", 0), ("page", 24),
+                                     ("page", 2048), ("pool_size", 0), ("blocks", 0), ("blocks", 2**28),
+                                     ("lengths", None), ("added", None), ("held_in", None), ("pool_state_in", None),
+                                     ("table", None), ("pool", None), ("held_out", None), ("pool_state_out", None),
+                                     ("offsets", None), ("kv_lengths", None), ("status", None), ("slots", None),
+                                     ("positions", None), ("parents", 4096), ("visible", 4096)])
+    refused(lib.dsr_plan_blocks, a, [("workspace", None), ("workspace", 4098),
+                                     ("workspace_bytes", a.workspace_bytes - 1)], -3)
+    assert lib.dsr_plan_workspace_bytes(-1) == 0 and lib.dsr_plan_workspace_bytes(N.TREE_MAX_REQUESTS + 1) == 0
+
+
+def test_rotary_arguments():
+    lib = N.load()
+    a = N.RotaryArgs()
+    for f in ("q", "q_out", "k", "v", "positions", "freqs", "slots", "k_cache", "v_cache"):
+        setattr(a, f, 4096)
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim, a.v_dim, a.rot_dim = N.BF16, 2, 1, 64, 64, 64
+    a.page, a.blocks, a.magnitude, a.tokens = 16, 4, 1.0, 3
+    refused(lib.dsr_rotary, a, [("dtype", N.F64), ("dtype", 0), ("tokens", -1), ("q_heads", -1), ("kv_heads", -1),
+                                ("head_dim", 1), ("head_dim", 513), ("rot_dim", 0), ("rot_dim", 63), ("rot_dim", 66),
+                                ("rot_start", -1), ("rot_start", 2), ("reserved", 1), ("magnitude", 0.0),
+                                ("magnitude", float("nan")), ("magnitude", float("inf")), ("positions", None),
+                                ("freqs", None), ("q", None), ("q_out", None), ("k", None), ("v", None),
+                                ("v_cache", None), ("v_dim", 0), ("v_dim", 513), ("slots", None), ("page", 3),
+                                ("blocks", 0)])
+    a.tokens = 0
+    assert lib.dsr_rotary(ctypes.byref(a), None) == 0
+
+
+def test_attention_arguments():
+    lib = N.load()
+    a = N.TreeAttentionArgs()
+    for f in ("q", "k_cache", "v_cache", "table", "offsets", "kv_lengths", "out", "status", "workspace"):
+        setattr(a, f, 4096)
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim, a.page, a.width, a.blocks = N.BF16, 8, 2, 128, 16, 4, 9
+    a.scale, a.requests, a.tokens, a.table_ld = 0.1, 2, 5, 4
+    a.workspace_bytes = lib.dsr_tree_attention_workspace_bytes(ctypes.byref(a))
+    assert a.workspace_bytes > 0
+    refused(lib.dsr_tree_attention, a, [("dtype", N.F32), ("q_heads", 7), ("q_heads", 0), ("kv_heads", 0),
+                                        ("head_dim", 4), ("head_dim", 100), ("head_dim", 264), ("page", 5),
+                                        ("width", 0), ("blocks", 0), ("scale", float("nan")), ("scale", float("inf")),
+                                        ("requests", -1), ("requests", 0), ("requests", N.TREE_MAX_REQUESTS + 1),
+                                        ("tokens", -1), ("tokens", 2**31), ("table_ld", 3), ("q", None), ("out", None),
+                                        ("q", 4104), ("out", 4104), ("k_cache", 4104), ("v_cache", 4104),
+                                        ("table", None), ("offsets", None), ("kv_lengths", None), ("status", None),
+                                        ("q_token", 4), ("q_head", 4), ("out_token", 1), ("out_head", 2),
+                                        ("k_block", 4), ("k_token", 12), ("k_head", 4), ("v_block", 4),
+                                        ("v_token", 4), ("v_head", 4)])
+    refused(lib.dsr_tree_attention, a, [("workspace", None), ("workspace", 4352 - 128),
+                                        ("workspace_bytes", a.workspace_bytes - 1)], -3)
+    a.requests = a.tokens = 0
+    assert lib.dsr_tree_attention(ctypes.byref(a), None) == 0
+    a.head_dim = 100
+    assert lib.dsr_tree_attention_workspace_bytes(ctypes.byref(a)) == 0
+    assert lib.dsr_tree_attention_workspace_bytes(None) == 0
+
+
+def test_commit_arguments():
+    lib = N.load()
+    a = N.CommitArgs()
+    for f in ("parents", "tokens_in", "sampled", "offsets", "kv_lengths", "table", "output_limit", "caches", "path",
+              "ids", "accepted", "count", "pending", "stop", "status"):
+        setattr(a, f, 4096)
+    a.lengths = 8192
+    a.requests, a.tokens, a.table_ld, a.width, a.page, a.blocks = 2, 8, 4, 4, 16, 9
+    a.cache_count, a.heads, a.row_bytes, a.c_block, a.c_token, a.c_head = 3, 2, 256, 8192, 512, 256
+    refused(lib.dsr_commit_tree, a, [("requests", -1), ("requests", N.TREE_MAX_REQUESTS + 1), ("tokens", -1),
+                                     ("table_ld", 3), ("width", 0), ("page", 12), ("blocks", 0), ("cache_count", -1),
+                                     ("cache_count", 65536), ("caches", None), ("heads", 0), ("row_bytes", 0),
+                                     ("row_bytes", 24), ("c_block", 8), ("c_token", 8), ("c_head", 8),
+                                     ("parents", None), ("tokens_in", None), ("sampled", None), ("offsets", None),
+                                     ("kv_lengths", None), ("table", None), ("output_limit", None), ("path", None),
+                                     ("ids", None), ("accepted", None), ("count", None), ("pending", None),
+                                     ("stop", None), ("lengths", None), ("lengths", 4096), ("status", None),
+                                     ("eos_off", 4096)])
+    a.requests = 0
+    assert lib.dsr_commit_tree(ctypes.byref(a), None) == 0
