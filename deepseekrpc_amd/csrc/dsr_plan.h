@@ -3,7 +3,7 @@
 //
 // Two parts.  plan_scan: one workgroup turns lengths and counts into
 // offsets, grants and the pool's ring index of each request's first new page
-// (prefix sums in 64 bits: counts come unchecked from device memory).
+// by prefix sums.
 // plan_tokens / plan_trees: every token's slot and position, 64 tokens to a
 // wave, and every new table entry, written by the token that first touches
 // the page (a new page lies wholly past the old tokens, so its first slot is
@@ -33,112 +33,109 @@ struct PlanRow {
 };
 constexpr int kPlanRefused = 0, kPlanGranted = 1, kPlanEnded = 2;
 
-__device__ __forceinline__ int64_t plan_wave_scan(int64_t x) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t y = __shfl_up(x, s);
-    if ((int)(threadIdx.x & 63) >= s) x += y;
-  }
+// Sums of counts that are at most 2^30 each: they stop at 2^31 - 1, above
+// every bound they are compared with, so that 32 bits are enough for counts
+// that come unchecked from device memory.
+__device__ __forceinline__ int plan_add(int x, int y) { return __builtin_elementwise_add_sat(x, y); }
+
+// Inclusive sums over the lanes of a wave (row shifts, then the rows' last
+// lanes handed on), without LDS.
+__device__ __forceinline__ int plan_wave_scan(int x) {
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // lane - 1 in its row of 16
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // rows 1 and 3 get the row before
+  x = plan_add(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // rows 2 and 3 get lane 31
   return x;
 }
 
-// Inclusive sums of x and y over the workgroup's 1,024 threads, and their totals.
-__device__ __forceinline__ void plan_block_scan(int64_t& x, int64_t& y, int64_t* part, int64_t& tx, int64_t& ty) {
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  x = plan_wave_scan(x);
-  y = plan_wave_scan(y);
-  __syncthreads();  // the last call's readers are done
-  if (l == 63) {
-    part[w] = x;
-    part[kPlanWaves + w] = y;
-  }
-  __syncthreads();
-  tx = ty = 0;
-  int64_t bx = 0, by = 0;
-#pragma unroll
-  for (int i = 0; i < kPlanWaves; ++i) {
-    const int64_t px = part[i], py = part[kPlanWaves + i];
-    if (i < w) {
-      bx += px;
-      by += py;
-    }
-    tx += px;
-    ty += py;
-  }
-  x += bx;
-  y += by;
-}
+constexpr int kPlanSums = 3;  // tokens, pages wanted, pages given back
 
-// One workgroup of 1,024 threads.
+// One workgroup of 1,024 threads, a request per thread and round.
+//
+// One scan of the three counts serves every decision.  A request that does
+// not fit the token arrays, or finds the pool short, still counts in the sums
+// of those behind it: by then no later request with tokens, or without its
+// pages, can be granted either, and the others want none.
 __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
-  __shared__ int64_t part[2 * kPlanWaves];
+  __shared__ int part[kPlanSums][kPlanWaves];
+  __shared__ int done[2];  // pages taken and given back in all
   const int R = (int)a.requests;
+  const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int shift = __ffs(a.page) - 1;
+  const uint32_t most = (uint32_t)a.width << shift;
+  const int capacity = (int)a.capacity, pool_size = a.pool_size;
   PlanRow* rows = (PlanRow*)a.workspace;
   int head = a.pool_state_in[0], count = a.pool_state_in[1];
-  if (head < 0 || head >= a.pool_size || count < 0 || count > a.pool_size) head = count = 0;  // not a pool: empty
-  int64_t tokens = 0, pages = 0, back = 0, taken = 0, given = 0;  // sums over the requests before this round's
+  if (head < 0 || head >= pool_size || count < 0 || count > pool_size) head = count = 0;  // not a pool: empty
+  auto wrap = [&](int x) { return x >= pool_size ? x - pool_size : x; };
+  if (threadIdx.x < 2) done[threadIdx.x] = 0;
+  if (threadIdx.x == 0) a.offsets[0] = 0;
+  int base[kPlanSums] = {0, 0, 0};  // sums over the requests before this round's
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + (int)threadIdx.x;
     const bool in = r < R;
-    const int64_t L = in ? a.lengths[r] : 0, A = in ? a.added[r] : 0, held = in ? a.held_in[r] : 0;
-    int status = DSR_OK;
-    if (L < 0 || A < -1 || held < 0 || held > a.width || L > held * a.page || L + A > (int64_t)a.width * a.page)
-      status = DSR_E_LENGTH;
+    const int L = in ? a.lengths[r] : 0, A = in ? a.added[r] : 0, held = in ? a.held_in[r] : 0;
     const bool ended = A == -1;
-    const int64_t take = A > 0 ? A : 0;
-    int64_t ends = take, wants = 0, total, unused;
-    plan_block_scan(ends, wants, part, total, unused);
-    ends += tokens;
-    if (status == DSR_OK && take > 0 && ends > a.capacity) status = DSR_E_CAPACITY;
-    int64_t need = 0, give = 0;
-    if (status == DSR_OK && !ended) need = (L + take + a.page - 1) / a.page - held;
-    if (need < 0) need = 0;
-    if (status == DSR_OK && ended) give = held;
-    int64_t need_to = need, give_to = give, needs, gives;
-    plan_block_scan(need_to, give_to, part, needs, gives);
-    need_to += pages;
-    give_to += back;
-    if (need > 0 && need_to > count) status = DSR_E_BLOCKS;
-    if (give > 0 && give_to > (int64_t)a.pool_size - count) status = DSR_E_BLOCKS;
+    const int take = A > 0 ? A : 0;
+    int status = DSR_OK;
+    if (L < 0 || A < -1 || (uint32_t)held > (uint32_t)a.width || (uint32_t)L > (uint32_t)held << shift ||
+        (uint32_t)L + (uint32_t)take > most)
+      status = DSR_E_LENGTH;
+    const int wants = (int)(((uint32_t)L + (uint32_t)take + (uint32_t)a.page - 1) >> shift) - held;
+    const int need = status == DSR_OK && !ended && wants > 0 ? wants : 0;
+    const int give = status == DSR_OK && ended ? held : 0;
+    int sum[kPlanSums] = {plan_wave_scan(take <= capacity ? take : capacity + 1), plan_wave_scan(need),
+                          plan_wave_scan(give)};
+    __syncthreads();  // the last round's readers are done
+    if (l == 63)
+#pragma unroll
+      for (int k = 0; k < kPlanSums; ++k) part[k][w] = sum[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPlanSums; ++k) {
+      const int waves_to = plan_wave_scan(l < kPlanWaves ? part[k][l] : 0);  // lane i: waves 0 .. i
+      const int before = w > 0 ? __builtin_amdgcn_readlane(waves_to, w - 1) : 0;
+      sum[k] = plan_add(sum[k], plan_add(base[k], before));
+      base[k] = plan_add(base[k], __builtin_amdgcn_readlane(waves_to, 63));
+    }
+    if (status == DSR_OK && take > 0 && sum[0] > capacity) status = DSR_E_CAPACITY;
+    if (status == DSR_OK && need > 0 && sum[1] > count) status = DSR_E_BLOCKS;
+    if (status == DSR_OK && give > 0 && sum[2] > pool_size - count) status = DSR_E_BLOCKS;
     const bool granted = status == DSR_OK && !ended, frees = status == DSR_OK && ended;
     if (in) {
       PlanRow p;
-      p.ring = granted ? (int)((head + need_to - need) % a.pool_size)
-                       : frees ? (int)(((int64_t)head + count + give_to - give) % a.pool_size) : 0;
-      p.old = (int)held;
+      p.ring = granted && need > 0 ? wrap(head + sum[1] - need)
+                                   : frees && give > 0 ? wrap(wrap(head + count) + sum[2] - give) : 0;
+      p.old = held;
       p.mode = granted ? kPlanGranted : frees ? kPlanEnded : kPlanRefused;
       rows[r] = p;
-      a.offsets[r + 1] = (int)(ends < a.capacity ? ends : a.capacity);
-      if (r == 0) a.offsets[0] = 0;
-      a.kv_lengths[r] = granted ? (int)(L + take) : 0;
-      a.held_out[r] = granted ? (int)(held + need) : frees ? 0 : (int)held;
+      a.offsets[r + 1] = sum[0] < capacity ? sum[0] : capacity;
+      a.kv_lengths[r] = granted ? L + take : 0;
+      a.held_out[r] = granted ? held + need : frees ? 0 : held;
       a.status[r] = status;
     }
-    // Pages really taken and given: the sums up to the last request served.
-    int64_t t = granted ? need : 0, g = frees ? give : 0, tt, gg;
-    plan_block_scan(t, g, part, tt, gg);
-    tokens += total;
-    pages += needs;
-    back += gives;
-    taken += tt;
-    given += gg;
+    if (granted && need > 0) atomicMax(&done[0], sum[1]);
+    if (frees && give > 0) atomicMax(&done[1], sum[2]);
   }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    if (R == 0) a.offsets[0] = 0;
-    a.pool_state_out[0] = (int)((head + taken) % a.pool_size);
-    a.pool_state_out[1] = (int)(count - taken + given);
+    a.pool_state_out[0] = wrap(head + done[0]);
+    a.pool_state_out[1] = count - done[0] + done[1];
   }
 }
 
 // The slot of place `p` of request r, and, if this is the first slot of a
 // new page, the page's table entry.
 __device__ __forceinline__ int plan_slot(const dsr_plan_args_t& a, const PlanRow& row, int64_t r, int p) {
-  const int b = p / a.page, o = p & (a.page - 1);
+  const int shift = __ffs(a.page) - 1, b = p >> shift, o = p & (a.page - 1);
   int id;
   if (b < row.old) {
     id = a.table[r * a.table_ld + b];
   } else {
-    id = a.pool[(int)(((int64_t)row.ring + b - row.old) % a.pool_size)];
+    const int at = row.ring + b - row.old;
+    id = a.pool[at >= a.pool_size ? at - a.pool_size : at];
     if (o == 0) a.table[r * a.table_ld + b] = id;
   }
   if ((unsigned)id >= (unsigned)a.blocks) {
@@ -146,7 +143,7 @@ __device__ __forceinline__ int plan_slot(const dsr_plan_args_t& a, const PlanRow
     a.kv_lengths[r] = 0;
     return -1;
   }
-  return id * a.page + o;
+  return (id << shift) + o;
 }
 
 __device__ __forceinline__ void plan_write(const dsr_plan_args_t& a, int64_t i, int slot, int position, int owner,
@@ -212,8 +209,10 @@ __device__ __forceinline__ void plan_tokens(const dsr_plan_args_t& a, int i0) {
 __device__ __forceinline__ void plan_release(const dsr_plan_args_t& a, int r) {
   const PlanRow row = ((const PlanRow*)a.workspace)[r];
   if (row.mode != kPlanEnded) return;
-  for (int b = threadIdx.x & 63; b < row.old; b += 64)
-    a.pool[(int)(((int64_t)row.ring + b) % a.pool_size)] = a.table[r * a.table_ld + b];
+  for (int b = threadIdx.x & 63; b < row.old; b += 64) {
+    const int at = row.ring + b;
+    a.pool[at >= a.pool_size ? at - a.pool_size : at] = a.table[r * a.table_ld + b];
+  }
 }
 
 // Request r's tree, one node per lane: masks and depths by pointer doubling
@@ -232,7 +231,7 @@ __device__ __forceinline__ void plan_tree(const dsr_plan_args_t& a, int r) {
       plan_write(a, lo + i, -1, 0, r, 0);
       // Pages already taken stay with the request, table entries included.
       const int p = a.lengths[r] + i;
-      if (p / a.page >= row.old && (p & (a.page - 1)) == 0) plan_slot(a, row, r, p);
+      if (p >= row.old * a.page && (p & (a.page - 1)) == 0) plan_slot(a, row, r, p);
     }
     if (l == 0) {
       a.status[r] = DSR_E_TREE;

@@ -40,10 +40,15 @@ int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
   if (parts > most) parts = most;
   if (parts < 1) parts = 1;
   const dim3 grid((unsigned)a.tokens, (unsigned)parts);
-  if (wide)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE>), grid, dim3(kRotaryThreads), 0, s, a);
+  const dim3 threads(kRotaryThreads);
+  if (wide && a.interleaved)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE, true>), grid, threads, 0, s, a);
+  else if (wide)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE, false>), grid, threads, 0, s, a);
+  else if (a.interleaved)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1, true>), grid, threads, 0, s, a);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1>), grid, dim3(kRotaryThreads), 0, s, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1, false>), grid, threads, 0, s, a);
   return launched();
 }
 
@@ -124,7 +129,7 @@ int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
   const dsr_plan_args_t& a = *args;
   if (a.requests < 0 || a.requests > DSR_TREE_MAX_REQUESTS || a.capacity < 1 || a.capacity > (1 << 30) ||
       !page_ok(a.page, a.blocks) || a.width < 1 || (int64_t)a.width * a.page > INT_MAX || a.table_ld < a.width ||
-      a.pool_size < 1)
+      a.pool_size < 1 || a.pool_size > (1 << 30))
     return DSR_ERR_ARG;
   if (!a.pool_state_in || !a.pool || !a.pool_state_out || !a.offsets || !a.slots || !a.positions ||
       (a.parents && !a.visible) || (!a.parents && a.visible))

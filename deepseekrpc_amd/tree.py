@@ -162,8 +162,8 @@ class PreparedPlan(_Prepared):
         a.held_in = _array(held, "held", torch.int32, dev, R)
         a.pool = _array(pool, "pool", torch.int32, dev)
         a.pool_state_in = _array(state, "state", torch.int32, dev, 2)
-        if pool.numel() < 1:
-            raise ValueError("pool must have an entry")
+        if not 1 <= pool.numel() <= 1 << 30:
+            raise ValueError("pool must have 1 to 2^30 entries")
         a.table, a.table_ld, a.width = _table(table, R, dev)
         if a.width * page > 2**31 - 1:
             raise ValueError("a table row must span less than 2^31 tokens")

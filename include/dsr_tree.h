@@ -83,7 +83,7 @@ typedef struct dsr_plan_args {
   int64_t capacity;            /* tokens in the per-token arrays, 1 .. 2^30 */
   int32_t width;               /* pages per table row, >= 1; width * page < 2^31 */
   int32_t page;
-  int32_t pool_size;           /* >= 1 */
+  int32_t pool_size;           /* 1 .. 2^30 */
   int32_t blocks;              /* pages of the cache; blocks * page < 2^31 */
   int32_t* held_out;           /* [requests] */
   int32_t* pool_state_out;     /* [2] */
