@@ -25,7 +25,8 @@ SOURCES = {
     "dsr_sampling.hip": ["dsr_common.h", "dsr_wave.h", "dsr_general.h", "dsr_fast.h", "dsr_topk.h", "dsr_full.h",
                          "dsr_verify.h", "dsr_history.h", "dsr_split.h", "dsr_numpy.h", "dsr_head.h", "dsr_f32.h",
                          "dsr_wide.h", "dsr_wide_verify.h"],
-    "dsr_tree.hip": ["dsr_plan.h", "dsr_rotary.h", "dsr_attention.h", "dsr_commit.h"],
+    "dsr_tree.hip": ["dsr_plan.h", "dsr_rotary.h", "dsr_attention.h", "dsr_attention_wide.h",
+                     "dsr_commit.h"],
 }
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -169,15 +169,88 @@ __device__ __forceinline__ AttnUnit attn_unit(const dsr_tree_attention_args_t& a
   return out;
 }
 
+// v with 0 in the place of infinities and NaN; whether there were any.
 template <class T>
-__device__ __forceinline__ bool attn_not_finite(typename AttnType<T>::x8 v) {
+__device__ __forceinline__ bool attn_make_finite(typename AttnType<T>::x8& v) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  u32x4 w = __builtin_bit_cast(u32x4, v);
   constexpr uint32_t E = AttnType<T>::kExponent;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (w[i] & E) == E, hi = ((w[i] >> 16) & E) == E;
+    bad |= lo || hi;
+    w[i] = w[i] & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
+  }
+  v = __builtin_bit_cast(typename AttnType<T>::x8, w);
   return bad;
+}
+
+// Infinities and NaN among values that some row must not see were taken out
+// of the products (0 x infinity would be NaN).  Here, after the workgroup's
+// results are written, the rows that do see such a value get weight x value
+// added in memory: what they hold becomes infinite or NaN as the sum would
+// have.  Adding a term that was in the product already changes nothing, so the
+// tokens from `from` on are all looked at.  A thread takes a row; `base` is
+// its scores' base.  Nothing of this runs for ordinary values.
+template <class T, int DP>
+__device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, const AttnPlan& p, const AttnUnit& u,
+                                            const AttnRequest& q, int from, int end, const float* base, int64_t part) {
+  typedef typename AttnType<T>::x8 x8;
+  const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = a.q_heads / a.kv_heads, ctx = q.kv - q.n;
+  if (r >= p.tile_rows || row >= q.rows) return;
+  const int t = row / group, h = u.head * group + row - t * group;
+  const T* query = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)h * a.q_head;
+  T* out = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)h * a.out_head;
+  float* o = &p.part_o[(part * p.tile_rows + r) * DP];
+#pragma unroll 1
+  for (int at = from; at < end; ++at) {
+    const int id = a.table[u.r * a.table_ld + at / a.page], place = at & (a.page - 1);
+    if ((unsigned)id >= (unsigned)a.blocks) continue;
+    const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
+    const T* k = (const T*)a.k_cache + id * a.k_block + place * a.k_token + u.head * a.k_head;
+    const int j = at - ctx;
+    if (j >= 0 && !(a.visible ? a.visible[q.lo + t] >> j & 1 : j <= t)) continue;
+    float weight = -1.f;
+#pragma unroll 1
+    for (int d = 0; d < a.head_dim; d += 8) {
+      x8 x = *(const x8*)(v + d);
+      const x8 whole = x;
+      if (!attn_make_finite<T>(x)) continue;
+      if (weight < 0.f) {  // this row's weight of the token, once
+        float dot = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < a.head_dim; ++i) dot += (float)query[i] * (float)k[i];
+        weight = __builtin_amdgcn_exp2f(dot * a.scale * kLog2e - base[r]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if ((float)x[i] == (float)whole[i]) continue;
+        if (u.chunks > 1)
+          o[d + i] += weight * (float)whole[i];
+        else
+          out[d + i] = (T)((float)out[d + i] + weight * (float)whole[i]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t attn_low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
+// Which of the 32 tokens from place p0 on a row sees, a bit each: the
+// context, of the new tokens those of `mask` (or, without masks, those up to
+// the row's own token `tok`), none at or past `end`, none of `bad`.
+__device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok, int p0, int ctx, int end,
+                                              uint32_t bad) {
+  const int s = p0 - ctx;  // the first token's index among the new ones
+  uint32_t see;
+  if (masks)
+    see = attn_low_bits(-s) | (uint32_t)(s >= 64 || s <= -32 ? 0ull : s >= 0 ? mask >> s : mask << -s);
+  else
+    see = attn_low_bits(tok + 1 - s);
+  return see & attn_low_bits(end - p0) & ~bad;
 }
 
 // Few rows (up to 16 NB of a tile): the four waves take the chunk's 32-token
@@ -205,12 +278,13 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   constexpr int VS = DP + 16;   // LDS row of values: 32 bytes of padding spread the transposing reads over the banks
   __shared__ T vals[kAttnWaves][kAttnTile][VS];
   __shared__ float sm[kAttnWaves][16 * NB], sl[kAttnWaves][16 * NB];
-  __shared__ int sbad;
+  __shared__ float sbase[16 * NB];
+  __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
-  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const AttnUnit u = attn_unit(a, p, blockIdx.x, true);
   if (!u.any) return;  // the same for the whole workgroup
-  if (threadIdx.x == 0) sbad = 0;
+  if (threadIdx.x == 0) sbad = spoison = 0;
   const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
   const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
   const int ctx = q.kv - q.n;
@@ -218,7 +292,10 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   const int end = min(begin + u.size, q.kv);
   const int row0 = u.tile * p.tile_rows;
 
-  // This lane's rows: token index, mask, query operand.
+  // This lane's rows: token index, mask, query operand.  A negative scale
+  // changes the queries' sign, so that scores only grow with their products;
+  // scale 0 is queries of 0.
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   x8 qv[NB][KS];
   int tok[NB];
   uint64_t mask[NB];
@@ -233,7 +310,8 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = 32 * s + 8 * g;
-      qv[b][s] = in && d < dim ? *(const x8*)(src + d) : x8{};
+      const x8 v = in && d < dim && a.scale != 0.f ? *(const x8*)(src + d) : x8{};
+      qv[b][s] = a.scale < 0.f ? -v : v;
     }
   }
 
@@ -246,7 +324,6 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = attn_f32x4{};
   }
-  const float scale = a.scale * kLog2e;
   const int32_t* pages = a.table + u.r * a.table_ld;
   const T* kb = (const T*)a.k_cache + u.head * a.k_head;
   const T* vb = (const T*)a.v_cache + u.head * a.v_head;
@@ -286,18 +363,18 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
     load_rows(first);
     if (first + step < end) load_ids(first + step);
   }
-  __syncthreads();  // sbad
+  __syncthreads();  // the flags
   for (int p0 = first; p0 < end; p0 += step) {
     const uint32_t bad = bad_next;
     const bool masked = p0 + kAttnTile > ctx || bad;  // some row may not see some token
     any_bad |= bad != 0;
-    bool poison = false;
     if (masked) {
+      bool poison = false;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) poison |= attn_not_finite<T>(vr[b][s]);
-      poison = __ballot(poison) != 0;
+        for (int s = 0; s < KS; ++s) poison |= attn_make_finite<T>(vr[b][s]);
+      if (poison) spoison = 1;
     }
     // Scores.
     attn_f32x4 sc[NB][2];
@@ -330,67 +407,44 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float top = -INFINITY;
+      if (masked) {
+        const uint32_t see = attn_sees(a.visible, mask[b], tok[b], p0, ctx, end, bad) >> (4 * g);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[b][k][e] = see >> (16 * k + e) & 1 ? sc[b][k][e] : -INFINITY;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = sc[b][k][e] * scale;
-          if (masked) {
-            const int j = p0 + 16 * k + 4 * g + e - ctx;
-            const bool see = j < 0 || (a.visible ? j < 64 && (mask[b] >> (j & 63) & 1) : j <= tok[b]);
-            x = see && j < q.n && p0 + 16 * k + 4 * g + e < end && !(bad >> (16 * k + 4 * g + e) & 1) ? x : -INFINITY;
-          }
-          sc[b][k][e] = x;
-          top = fmaxf(top, x);
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[b][k][e]);
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (__ballot(top - AttnType<T>::kLift > m[b] + 8.f)) {
-        const float next = fmaxf(m[b], top - AttnType<T>::kLift);
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale - AttnType<T>::kLift;
+      if (__ballot(top > m[b] + 8.f)) {
+        const float next = fmaxf(m[b], top);
         const float f = m[b] == next ? 1.f : __builtin_amdgcn_exp2f(m[b] - next);
         m[b] = next;
         sum[b] *= f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[b][d] *= f;
       }
-      const float base = m[b] == -INFINITY ? 0.f : m[b];
+      const float base = m[b] == -INFINITY ? 0.f : -m[b];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(sc[b][k][e] - base);
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][k][e], scale, base));
           sum[b] += x;
           pv[b][4 * k + e] = (T)x;
         }
     }
-    if (!poison) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const T* at = &vals[w][4 * g + (n >> 2)][16 * d + 4 * (n & 3)];
-        const x4 lo = attn_read_tr<T>(at), hi = attn_read_tr<T>(at + 16 * VS);
-        const x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int d = 0; d < DB; ++d) {
+      const T* at = &vals[w][4 * g + (n >> 2)][16 * d + 4 * (n & 3)];
+      const x4 lo = attn_read_tr<T>(at), hi = attn_read_tr<T>(at + 16 * VS);
+      const x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b][d] = AttnType<T>::mfma16(v, pv[b], acc[b][d]);
-      }
-    } else {
-      // An infinity or NaN among values that some row must not see: token by
-      // token, and only where the row sees it (0 x infinity would be NaN).
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            for (int from = 0; from < 4; ++from) {
-              const int t = 16 * k + 4 * from + e;
-              const float x = __shfl((float)pv[b][4 * k + e], n + 16 * from);
-              const float seen = __shfl(sc[b][k][e], n + 16 * from);
-              if (seen == -INFINITY) continue;
-#pragma unroll
-              for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][d][i] += x * (float)vals[w][t][16 * d + 4 * g + i];
-            }
+      for (int b = 0; b < NB; ++b) acc[b][d] = AttnType<T>::mfma16(v, pv[b], acc[b][d]);
     }
   }
 
@@ -430,6 +484,7 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
         L += sl[i][rr] * (sm[i][rr] == M ? 1.f : __builtin_amdgcn_exp2f(sm[i][rr] - M));
         o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
       }
+      if (d == 0) sbase[rr] = M;
       if (split) {
         *(attn_f32x4*)&p.part_o[(part * p.tile_rows + rr) * DP + d] = o;
         if (d == 0) p.part_ml[part * p.tile_rows + rr] = float2{M, L};
@@ -444,8 +499,11 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
           a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
       }
     }
+    __threadfence_block();
     __syncthreads();
   }
+  if (spoison)
+    attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), end, sbase, part);
   if (threadIdx.x == 0) {
     if (split)
       p.part_bad[part] = sbad;
@@ -453,6 +511,8 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
       a.status[u.r] = !q.fine ? DSR_E_LENGTH : sbad ? DSR_E_BLOCK : DSR_OK;
   }
 }
+
+constexpr int kCombineRows = 16;  // rows of a tile per workgroup (blockIdx.y)
 
 // Joins the chunks of a (request, tile, head): out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
 template <class T, int DP>
@@ -463,9 +523,9 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_combine(dsr_tree_attentio
   const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
   const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
   const int row0 = u.tile * p.tile_rows;
-  const int rows = min(p.tile_rows, q.rows - row0);
+  const int rows = min((int)blockIdx.y * kCombineRows + kCombineRows, min(p.tile_rows, q.rows - row0));
   const int64_t part = u.part + (int64_t)u.tile * a.kv_heads + u.head, next = (int64_t)u.tiles * a.kv_heads;
-  for (int x = threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
+  for (int x = blockIdx.y * kCombineRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
     const int row = x / (DP / 4), d = x % (DP / 4) * 4;
     if (d >= dim) continue;
     float M = -INFINITY, L = 0.f;
@@ -489,9 +549,9 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_combine(dsr_tree_attentio
     if (a.lse && d == 0)
       a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   }
-  if (threadIdx.x == 0 && u.head == 0 && u.tile == 0) a.status[u.r] = DSR_OK;
-  __syncthreads();
-  if (u.head == 0 && u.tile == 0) {
+  if (u.head == 0 && u.tile == 0 && blockIdx.y == 0) {
+    if (threadIdx.x == 0) a.status[u.r] = DSR_OK;
+    __syncthreads();
     // Any chunk of the request with a page id outside the cache (its first tile and head looked at all of them).
     for (int c = threadIdx.x; c < u.chunks; c += kAttnThreads)
       if (p.part_bad[part + c * next]) a.status[u.r] = DSR_E_BLOCK;

@@ -2,6 +2,7 @@
 #include "dsr_tree.h"
 
 #include "dsr_attention.h"
+#include "dsr_attention_wide.h"
 #include "dsr_commit.h"
 #include "dsr_plan.h"
 #include "dsr_rotary.h"
@@ -60,8 +61,9 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   AttnPlan p{};
   const int64_t group = a.q_heads / a.kv_heads;
   const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
-  p.tile_rows = rows <= 16 || a.head_dim > 128 ? 16 : 32;
-  p.target = 512;
+  const bool big = a.head_dim > 128;
+  p.tile_rows = rows <= 16 || (big && rows <= 32) ? 16 : rows <= 32 ? 32 : rows <= 64 && !big ? 64 : rows <= 128 || big ? 128 : 256;
+  p.target = p.tile_rows <= 16 ? 1024 : p.tile_rows <= 128 && !big ? 512 : 256;
   p.min_chunk = 256;
   p.tiles_bound = (int)(a.tokens * group / p.tile_rows + a.requests);
   p.max_parts = 2 * (int64_t)p.target + 64;
@@ -94,15 +96,23 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
   const int64_t units = (int64_t)p.target + (int64_t)p.tiles_bound * a.kv_heads;
   if (units > INT_MAX) return DSR_ERR_ARG;
   const dim3 grid((unsigned)units), threads(kAttnThreads);
-  if (p.tile_rows == 16) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 1>), grid, threads, 0, s, a, p);
-  } else if constexpr (DP <= 128) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 2>), grid, threads, 0, s, a, p);
+  switch (p.tile_rows) {
+    case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 1>), grid, threads, 0, s, a, p); break;
+    case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, a, p); break;
+    default:
+      if constexpr (DP <= 128) {
+        if (p.tile_rows == 32)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 1>), grid, threads, 0, s, a, p);
+        else if (p.tile_rows == 64)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 2>), grid, threads, 0, s, a, p);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 2, 4>), grid, threads, 0, s, a, p);
+      }
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   if ((int64_t)a.width * a.page > p.min_chunk)  // else no request can have two chunks
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_combine<T, DP>), dim3((unsigned)(p.tiles_bound * a.kv_heads)), threads, 0,
-                       s, a, p);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_combine<T, DP>), dim3((unsigned)(p.tiles_bound * a.kv_heads), (unsigned)(p.tile_rows / kCombineRows)),
+                       threads, 0, s, a, p);
   return launched();
 }
 
