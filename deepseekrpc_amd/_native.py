@@ -56,8 +56,7 @@ EXPORTS = (
 )
 # include/dsr_tree.h
 TREE_EXPORTS = (
-    "dsr_plan_workspace_bytes", "dsr_tree_attention_workspace_bytes", "dsr_plan_blocks", "dsr_rotary",
-    "dsr_tree_attention", "dsr_commit_tree",
+    "dsr_plan_workspace_bytes", "dsr_tree_attention_workspace_bytes", "dsr_plan_blocks", "dsr_rotary", "dsr_tree_attention", "dsr_commit_tree",
 )
 F16 = 4
 E_LENGTH = 16

@@ -2,10 +2,8 @@
 //
 // For one request and key head the rows are (new token, query head of the
 // group) pairs: rows = new x group.  They share the head's keys and values, so
-// a workgroup takes a tile of rows and a chunk of the request's tokens and
-// reads each key and value of the chunk once.  When the tiles of all requests
-// do not fill the chip, requests are cut into chunks of tokens (attn_unit),
-// whose partial results k_tree_combine joins.
+// a workgroup takes a tile of rows and reads each key and value once for all
+// of them.  How tiles and tokens are dealt out is at AttnWork.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -57,20 +55,19 @@ __device__ __forceinline__ typename AttnType<T>::x4 attn_read_tr(const T* p) {
 constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = 4;
 constexpr int kAttnTile = 32;             // tokens a wave takes at a time
-constexpr int kAttnChunk = 128;           // chunks are multiples of this many tokens
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // What the host decides for one call.
 struct AttnPlan {
   int tile_rows;      // rows of a tile
-  int target;         // units (tile x chunk x head) aimed at
-  int min_chunk;      // tokens, a multiple of kAttnChunk
-  int tiles_bound;    // row tiles of all requests at most
-  int64_t max_parts;  // partial results the workspace holds
-  float* part_o;      // [max_parts, tile_rows, head dim of the kernel]
-  float2* part_ml;    // [max_parts, tile_rows]: base (log2) and sum
-  int32_t* part_bad;  // [max_parts]: a page id outside the cache
+  int groups;         // workgroups, a multiple of 8
+  int tokens;         // of a step of the work split: a multiple of the kernel's own
+  int min_steps;      // fewest steps worth a workgroup
+  bool cut;           // some tile may be cut into parts
+  float* part_o;      // [2 groups, tile_rows, head dim of the kernel]
+  float2* part_ml;    // [2 groups, tile_rows]: base (log2) and sum
+  int32_t* part_bad;  // [2 groups]: a page id outside the cache
 };
 
 struct AttnRequest {
@@ -96,77 +93,150 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   return q;
 }
 
-// One unit of work: rows of a tile against a chunk of a request's tokens.
-struct AttnUnit {
-  int r, head, tile, tiles, chunk, chunks, size;  // size: tokens per chunk
-  int64_t part;                                   // partial result of chunk 0 (chunks > 1), `tiles * heads` apart
-  bool any;
+// A value that all lanes share, in scalar registers.
+__device__ __forceinline__ int attn_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t attn_uniform(int64_t x) {
+  const uint32_t lo = (uint32_t)attn_uniform((int)(uint32_t)x), hi = (uint32_t)attn_uniform((int)(x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ int64_t attn_div(int64_t x, int64_t d) {  // both >= 0, d > 0
+  return (uint64_t)x >> 32 || (uint64_t)d >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+}
+
+// One segment of a workgroup's work: the rows of a tile against tokens begin .. end - 1.
+struct AttnSegment {
+  int r, head, tile, begin, end;
+  bool whole;         // all of the tile's tokens
+  int64_t part;       // else: where its result goes
+  int64_t from, to;   // the tile's place in the order of all steps
 };
 
-// Unit `u` of the launch, found by every wave for itself from the requests'
-// lengths (64 at a time).  The chunk size makes about `target` units of equal
-// size out of the tokens that the row tiles have to pass over.  `chunked`
-// false: units are tiles alone (k_tree_combine).
-__device__ __forceinline__ AttnUnit attn_unit(const dsr_tree_attention_args_t& a, const AttnPlan& p, int u,
-                                              bool chunked) {
-  const int l = threadIdx.x & 63, R = (int)a.requests, H = a.kv_heads, group = a.q_heads / a.kv_heads;
-  AttnUnit out;
-  out.any = false;
-  out.head = u % H;
-  const int w = u / H;
-  int64_t load = 0;
-  AttnRequest q;
-  for (int r0 = 0; r0 < R; r0 += 64) {
-    const int r = r0 + l < R ? r0 + l : R - 1;
-    q = attn_request(a, group, p.tile_rows, r);
-    if (r0 + l < R) load += (int64_t)q.tiles * q.kv;
+// A workgroup's share of the work.
+//
+// All work is put in one order of steps (`tokens` tokens of a tile): request
+// by request, head by head, tile by tile, token by token.  Each workgroup
+// takes an equal, contiguous part of it, so that requests of any lengths
+// load the chip evenly; a tile that crosses a border is written in parts,
+// which k_tree_join joins.  (Joining in this launch, by the workgroup that
+// finishes a tile last, needs the parts made visible across the XCDs' caches:
+// with the fences for that, 32 requests of 8,064 tokens and 128 rows took
+// 447 us instead of 274.)  Every wave finds the place for itself from the
+// requests' lengths, 64 at a time.  Neighbouring shares, which often have
+// keys and values in common, go to one XCD.
+struct AttnWork {
+  int64_t at, stop, quota;  // steps
+  int64_t base;             // steps of the requests before r
+  int r, me;
+
+  static __device__ __forceinline__ int steps_of(const AttnRequest& q, int tokens) {
+    return q.rows == 0 ? 0 : q.kv > tokens ? (q.kv + tokens - 1) / tokens : 1;
   }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) load += __shfl_xor(load, s);
-  int64_t size = (load * H + p.target - 1) / p.target;
-  size = (size + kAttnChunk - 1) / kAttnChunk * kAttnChunk;
-  if (size < p.min_chunk) size = p.min_chunk;
-  if (size > (1 << 30)) size = 1 << 30;
-  int before = 0;         // units of the requests passed
-  int64_t parts = 0;      // partial results of the requests passed
-  for (int r0 = 0; r0 < R; r0 += 64) {
-    const int r = r0 + l < R ? r0 + l : R - 1;
-    if (R > 64) q = attn_request(a, group, p.tile_rows, r);
-    // Equal chunks: as many as the size asks for, each a multiple of kAttnChunk.
-    const int chunks = q.kv > size ? (int)((q.kv + size - 1) / size) : 1;
-    const int units = r0 + l < R ? (chunked ? q.tiles * chunks : q.tiles) : 0;
-    int sum = units;
-    int64_t psum = r0 + l < R && chunks > 1 ? (int64_t)q.tiles * chunks : 0;
-    const int64_t own = psum;
+
+  // `border` 0: this workgroup's share.  Else the work from where share `border` begins.
+  __device__ __forceinline__ AttnWork(const dsr_tree_attention_args_t& a, const AttnPlan& p, int border) {
+    const int tokens = p.tokens;
+    const int l = threadIdx.x & 63, R = (int)a.requests, group = a.q_heads / a.kv_heads;
+    AttnRequest q;
+    int64_t sum = 0, mine = 0;
+    for (int r0 = 0; r0 < R; r0 += 64) {
+      q = attn_request(a, group, p.tile_rows, r0 + l < R ? r0 + l : R - 1);
+      mine = r0 + l < R ? (int64_t)q.tiles * steps_of(q, tokens) * a.kv_heads : 0;
+      sum += mine;
+    }
+    int64_t upto = sum;  // inclusive sums over the lanes
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-      const int x = __shfl_up(sum, s);
-      const int64_t y = __shfl_up(psum, s);
-      if (l >= s) {
-        sum += x;
-        psum += y;
+      const int64_t x = __shfl_up(upto, s);
+      if (l >= s) upto += x;
+    }
+    const int64_t total = attn_uniform(__shfl(upto, 63));
+    quota = attn_div(total + p.groups - 1, p.groups);
+    if (quota < p.min_steps) quota = p.min_steps;
+    const int each = (int)attn_div(total + 8 * quota - 1, 8 * quota);  // workgroups with work, per XCD
+    const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
+    me = x * each + y;
+    at = y < each ? me * quota : total;
+    if (border) {
+      me = border;
+      at = border < 8 * each ? border * quota : total;
+    }
+    stop = at + quota < total ? at + quota : total;
+    r = 0;
+    base = 0;
+    if (at >= stop) return;
+    for (int r0 = 0; r0 < R; r0 += 64) {
+      if (R > 64) {
+        q = attn_request(a, group, p.tile_rows, r0 + l < R ? r0 + l : R - 1);
+        mine = r0 + l < R ? (int64_t)q.tiles * steps_of(q, tokens) * a.kv_heads : 0;
+        upto = mine;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+          const int64_t z = __shfl_up(upto, s);
+          if (l >= s) upto += z;
+        }
       }
+      const uint64_t past = __ballot(base + upto > at);
+      if (past) {
+        const int hit = __ffsll((unsigned long long)past) - 1;
+        base += attn_uniform(__shfl(upto - mine, hit));
+        r = r0 + hit;
+        break;
+      }
+      base += attn_uniform(__shfl(upto, 63));
     }
-    const uint64_t past = __ballot(before + sum > w);
-    if (past) {
-      const int at = __ffsll((unsigned long long)past) - 1;
-      const int rem = w - before - __shfl(sum - units, at);
-      const int tiles = __shfl(q.tiles, at), n_chunks = __shfl(chunks, at);
-      out.part = (parts + __shfl(psum - own, at)) * H;
-      out.r = r0 + at;
-      out.tiles = tiles;
-      out.chunks = n_chunks;
-      out.tile = rem % tiles;
-      out.chunk = chunked ? rem / tiles : 0;
-      const int kv = __shfl(q.kv, at);
-      out.size = n_chunks > 1 ? ((kv + n_chunks - 1) / n_chunks + kAttnTile - 1) / kAttnTile * kAttnTile : kv;
-      out.any = rem >= 0 && out.chunk < n_chunks && (n_chunks == 1 || out.part + (int64_t)tiles * n_chunks * H <= p.max_parts);
-      return out;
-    }
-    before += __shfl(sum, 63);
-    parts += __shfl(psum, 63);
   }
-  return out;
+
+  // The next segment and its request; false at the end.
+  __device__ __forceinline__ bool next(const dsr_tree_attention_args_t& a, const AttnPlan& p, AttnSegment& s,
+                                       AttnRequest& q) {
+    if (at >= stop) return false;
+    const int tokens = p.tokens;
+    const int group = a.q_heads / a.kv_heads;
+    int steps;
+    int64_t length;
+    for (;;) {  // past requests that end here or have no rows; one with steps left exists, as at < stop
+      if (r >= a.requests) return false;
+      q = attn_request(a, group, p.tile_rows, r);
+      q.lo = attn_uniform(q.lo);
+      q.n = attn_uniform(q.n);
+      q.kv = attn_uniform(q.kv);
+      q.rows = attn_uniform(q.rows);
+      q.tiles = attn_uniform(q.tiles);
+      steps = steps_of(q, tokens);
+      length = (int64_t)q.tiles * steps * a.kv_heads;
+      if (at < base + length) break;
+      base += length;
+      ++r;
+    }
+    const int64_t unit = attn_div(at - base, steps);
+    const int s0 = (int)(at - base - unit * steps);
+    const int s1 = stop - at < steps - s0 ? s0 + (int)(stop - at) : steps;
+    s.r = r;
+    s.head = (int)attn_div(unit, q.tiles);
+    s.tile = (int)(unit - (int64_t)s.head * q.tiles);
+    s.begin = s0 * tokens;
+    s.end = s1 == steps ? q.kv : s1 * tokens;
+    if (!a.visible && q.kv > 0) {  // causal rows: nothing past the tile's last one
+      const int64_t last = ((int64_t)(s.tile + 1) * p.tile_rows - 1) / group;
+      if (s.end > q.kv - q.n + last + 1) s.end = (int)(q.kv - q.n + last + 1);
+    }
+    s.whole = s0 == 0 && s1 == steps;
+    s.part = 2 * (int64_t)me + (s0 > 0 ? 0 : 1);  // a tile begun elsewhere can only be a workgroup's first
+    s.from = base + unit * steps;
+    s.to = s.from + steps;
+    at += s1 - s0;
+    return true;
+  }
+};
+
+// Requests without rows have no work: their status, by the launch's first workgroup.
+__device__ __forceinline__ void attn_idle(const dsr_tree_attention_args_t& a, const AttnPlan& p) {
+  if (blockIdx.x != 0) return;
+  for (int r = threadIdx.x; r < a.requests; r += kAttnThreads) {
+    const AttnRequest q = attn_request(a, a.q_heads / a.kv_heads, p.tile_rows, r);
+    if (q.rows == 0) a.status[r] = q.fine ? DSR_OK : DSR_E_LENGTH;
+  }
 }
 
 // v with 0 in the place of infinities and NaN; whether there were any.
@@ -194,17 +264,17 @@ __device__ __forceinline__ bool attn_make_finite(typename AttnType<T>::x8& v) {
 // tokens from `from` on are all looked at.  A thread takes a row; `base` is
 // its scores' base.  Nothing of this runs for ordinary values.
 template <class T, int DP>
-__device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, const AttnPlan& p, const AttnUnit& u,
-                                            const AttnRequest& q, int from, int end, const float* base, int64_t part) {
+__device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, const AttnPlan& p, const AttnSegment& u,
+                                            const AttnRequest& q, int from, const float* base) {
   typedef typename AttnType<T>::x8 x8;
   const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = a.q_heads / a.kv_heads, ctx = q.kv - q.n;
   if (r >= p.tile_rows || row >= q.rows) return;
   const int t = row / group, h = u.head * group + row - t * group;
   const T* query = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)h * a.q_head;
   T* out = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)h * a.out_head;
-  float* o = &p.part_o[(part * p.tile_rows + r) * DP];
+  float* o = &p.part_o[(u.part * p.tile_rows + r) * DP];
 #pragma unroll 1
-  for (int at = from; at < end; ++at) {
+  for (int at = from; at < u.end; ++at) {
     const int id = a.table[u.r * a.table_ld + at / a.page], place = at & (a.page - 1);
     if ((unsigned)id >= (unsigned)a.blocks) continue;
     const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
@@ -226,13 +296,24 @@ __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if ((float)x[i] == (float)whole[i]) continue;
-        if (u.chunks > 1)
+        if (!u.whole)
           o[d + i] += weight * (float)whole[i];
         else
           out[d + i] = (T)((float)out[d + i] + weight * (float)whole[i]);
       }
     }
   }
+}
+
+// What a segment says of its page ids: the request's status, or its part's
+// (its first tile and head speak for all: every tile sees the same pages).
+__device__ __forceinline__ void attn_report(const dsr_tree_attention_args_t& a, const AttnPlan& p,
+                                            const AttnSegment& u, const AttnRequest& q, int bad) {
+  if (threadIdx.x != 0) return;
+  if (!u.whole)
+    p.part_bad[u.part] = bad;
+  else if (u.head == 0 && u.tile == 0)
+    a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
 }
 
 __device__ __forceinline__ uint32_t attn_low_bits(int n) {
@@ -282,14 +363,15 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  const AttnUnit u = attn_unit(a, p, blockIdx.x, true);
-  if (!u.any) return;  // the same for the whole workgroup
-  if (threadIdx.x == 0) sbad = spoison = 0;
   const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
-  const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
-  const int ctx = q.kv - q.n;
-  const int begin = u.chunk * u.size;
-  const int end = min(begin + u.size, q.kv);
+  attn_idle(a, p);
+  AttnWork work(a, p, 0);
+  AttnSegment u;
+  AttnRequest q;
+  while (work.next(a, p, u, q)) {  // the same for the whole workgroup
+  __syncthreads();  // the last segment's LDS is read
+  if (threadIdx.x == 0) sbad = spoison = 0;
+  const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
   const int row0 = u.tile * p.tile_rows;
 
   // This lane's rows: token index, mask, query operand.  A negative scale
@@ -460,8 +542,8 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   }
   if (any_bad && l == 0) sbad = 1;
   __syncthreads();
-  const bool split = u.chunks > 1;
-  const int64_t part = u.part + ((int64_t)u.chunk * u.tiles + u.tile) * a.kv_heads + u.head;
+  const bool split = !u.whole;
+  const int64_t part = u.part;
   constexpr int OS = DP + 4;  // LDS row of outputs
   static_assert(16 * OS * sizeof(float) <= kAttnTile * VS * sizeof(T), "a wave's outputs fit its rows of values");
 #pragma unroll
@@ -502,44 +584,46 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
     __threadfence_block();
     __syncthreads();
   }
-  if (spoison)
-    attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), end, sbase, part);
-  if (threadIdx.x == 0) {
-    if (split)
-      p.part_bad[part] = sbad;
-    else if (u.head == 0 && u.tile == 0)
-      a.status[u.r] = !q.fine ? DSR_E_LENGTH : sbad ? DSR_E_BLOCK : DSR_OK;
+  if (spoison) attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
+  attn_report(a, p, u, q, sbad);
   }
 }
 
-constexpr int kCombineRows = 16;  // rows of a tile per workgroup (blockIdx.y)
+constexpr int kJoinRows = 16;  // rows of a tile per workgroup (blockIdx.y)
 
-// Joins the chunks of a (request, tile, head): out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
+// Joins the parts of the tiles that borders between shares cut, in the order
+// of the tokens: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
+// Workgroup x takes the tile whose first border is the one before share x + 1.
 template <class T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void k_tree_combine(dsr_tree_attention_args_t a, AttnPlan p) {
+__global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_args_t a, AttnPlan p) {
   typedef typename AttnType<T>::x4 x4;
-  const AttnUnit u = attn_unit(a, p, blockIdx.x, false);
-  if (!u.any || u.chunks == 1) return;
-  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
-  const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
-  const int row0 = u.tile * p.tile_rows;
-  const int rows = min((int)blockIdx.y * kCombineRows + kCombineRows, min(p.tile_rows, q.rows - row0));
-  const int64_t part = u.part + (int64_t)u.tile * a.kv_heads + u.head, next = (int64_t)u.tiles * a.kv_heads;
-  for (int x = blockIdx.y * kCombineRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
+  const int border = blockIdx.x + 1;
+  AttnWork work(a, p, border);
+  AttnSegment u;
+  AttnRequest q;
+  const int64_t at = work.at;
+  if (!work.next(a, p, u, q) || u.from == at) return;  // no work there; a tile begins there
+  const int64_t first = attn_div(u.from, work.quota), last = attn_div(u.to - 1, work.quota);
+  if (first != border - 1) return;
+  const int group = a.q_heads / a.kv_heads, row0 = u.tile * p.tile_rows;
+  const int rows = min((int)blockIdx.y * kJoinRows + kJoinRows, min(p.tile_rows, q.rows - row0));
+  // The first part is its workgroup's last (an odd place), the others their workgroups' first.
+  for (int x = blockIdx.y * kJoinRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
     const int row = x / (DP / 4), d = x % (DP / 4) * 4;
-    if (d >= dim) continue;
     float M = -INFINITY, L = 0.f;
     attn_f32x4 o = {};
-    for (int c = 0; c < u.chunks; ++c) {
-      const int64_t at = (part + c * next) * p.tile_rows + row;
-      const float2 ml = p.part_ml[at];
-      const attn_f32x4 y = *(const attn_f32x4*)&p.part_o[at * DP + d];
+    for (int64_t c = first; c <= last; ++c) {
+      const int64_t part = (2 * c + (c == first)) * p.tile_rows + row;
+      const float2 ml = p.part_ml[part];
+      const attn_f32x4 y = *(const attn_f32x4*)&p.part_o[part * DP + d];
       const float top = fmaxf(M, ml.x);
-      const float f = M == top ? 1.f : __builtin_amdgcn_exp2f(M - top), f2 = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+      const float f = M == top ? 1.f : __builtin_amdgcn_exp2f(M - top);
+      const float f2 = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
       M = top;
       L = L * f + ml.y * f2;
       o = o * f + y * f2;
     }
+    if (d >= a.head_dim) continue;
     const int t = (row0 + row) / group, h = row0 + row - t * group;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     x4 y;
@@ -549,12 +633,10 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_combine(dsr_tree_attentio
     if (a.lse && d == 0)
       a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   }
-  if (u.head == 0 && u.tile == 0 && blockIdx.y == 0) {
-    if (threadIdx.x == 0) a.status[u.r] = DSR_OK;
-    __syncthreads();
-    // Any chunk of the request with a page id outside the cache (its first tile and head looked at all of them).
-    for (int c = threadIdx.x; c < u.chunks; c += kAttnThreads)
-      if (p.part_bad[part + c * next]) a.status[u.r] = DSR_E_BLOCK;
+  if (u.head == 0 && u.tile == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    int bad = 0;
+    for (int64_t c = first; c <= last; ++c) bad |= p.part_bad[2 * c + (c == first)];
+    a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
   }
 }
 

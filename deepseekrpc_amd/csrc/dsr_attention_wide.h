@@ -65,15 +65,16 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  const AttnUnit u = attn_unit(a, p, blockIdx.x, true);
-  if (!u.any) return;  // the same for the whole workgroup
+  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
+  attn_idle(a, p);
+  AttnWork work(a, p, 0);
+  AttnSegment u;
+  AttnRequest q;
+  while (work.next(a, p, u, q)) {  // the same for the whole workgroup
+  __syncthreads();  // the last segment's LDS is read
   if (threadIdx.x < 4 * WK) sbits[threadIdx.x / WK][threadIdx.x % WK] = 0;
   if (threadIdx.x == 0) sbad = spoison = 0;
-  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
-  const AttnRequest q = attn_request(a, group, p.tile_rows, u.r);
-  const int ctx = q.kv - q.n;
-  const int begin = u.chunk * u.size;
-  const int end = min(begin + u.size, q.kv);
+  const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
   const int clear = min(ctx, end);  // every row sees the tokens before
   const int steps = end > begin ? (end - begin + NT - 1) / NT : 0;
   const int row0 = u.tile * p.tile_rows + 32 * RB * wr;
@@ -365,8 +366,8 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       }
     }
   }
-  const bool split = u.chunks > 1;
-  const int64_t part = u.part + ((int64_t)u.chunk * u.tiles + u.tile) * a.kv_heads + u.head;
+  const bool split = !u.whole;
+  const int64_t part = u.part;
   if (wk == 0) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -404,13 +405,8 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   }
   __threadfence_block();
   __syncthreads();
-  if (spoison)
-    attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, clear - NT), end, sbase, part);
-  if (threadIdx.x == 0) {
-    if (split)
-      p.part_bad[part] = sbad;
-    else if (u.head == 0 && u.tile == 0)
-      a.status[u.r] = !q.fine ? DSR_E_LENGTH : sbad ? DSR_E_BLOCK : DSR_OK;
+  if (spoison) attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, clear - NT), sbase);
+  attn_report(a, p, u, q, sbad);
   }
 }
 

@@ -56,6 +56,8 @@ int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
 // Dimensions of the kernel that takes a head dimension.
 int attn_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
+constexpr int kAttnShort = 1024;  // tokens, a multiple of every kernel's step
+
 // Host part of the work split, from sizes alone.
 AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   AttnPlan p{};
@@ -63,24 +65,30 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
   const bool big = a.head_dim > 128;
   p.tile_rows = rows <= 16 || (big && rows <= 32) ? 16 : rows <= 32 ? 32 : rows <= 64 && !big ? 64 : rows <= 128 || big ? 128 : 256;
-  p.target = p.tile_rows <= 16 ? 1024 : p.tile_rows <= 128 && !big ? 512 : 256;
-  p.min_chunk = 256;
-  p.tiles_bound = (int)(a.tokens * group / p.tile_rows + a.requests);
-  p.max_parts = 2 * (int64_t)p.target + 64;
+  // As many workgroups as the chip holds at once (256 CUs, one or two each).
+  p.groups = p.tile_rows == 256 || p.tile_rows == 32 || big ? 256 : 512;
+  // Causal tiles have unlike lengths: several workgroups for each place even them out.
+  if (!a.visible && a.tokens > 64 * a.requests) p.groups *= 4;
+  p.min_steps = p.tile_rows == 16 ? 2 : 8;
+  p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
+  // Where a whole table row is a short way for one workgroup, a tile is one
+  // step: nothing is cut, and no joining launch follows.
+  p.cut = (int64_t)a.width * a.page > kAttnShort;
+  if (!p.cut) p.tokens = kAttnShort, p.min_steps = 1;
   return p;
 }
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 struct AttnSizes {
-  int64_t o, ml, bad, all;
+  int64_t o, ml, all;
 };
 AttnSizes attn_sizes(const dsr_tree_attention_args_t& a, const AttnPlan& p) {
   AttnSizes s;
-  s.o = round256(p.max_parts * p.tile_rows * attn_dim(a.head_dim) * 4);
-  s.ml = round256(p.max_parts * p.tile_rows * 8);
-  s.bad = round256(p.max_parts * 4);
-  s.all = s.o + s.ml + s.bad;
+  const int64_t parts = 2 * (int64_t)p.groups;
+  s.o = round256(parts * p.tile_rows * attn_dim(a.head_dim) * 4);
+  s.ml = round256(parts * p.tile_rows * 8);
+  s.all = s.o + s.ml + round256(parts * 4);
   return s;
 }
 
@@ -93,9 +101,7 @@ bool attn_shape_ok(const dsr_tree_attention_args_t& a) {
 
 template <class T, int DP>
 int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
-  const int64_t units = (int64_t)p.target + (int64_t)p.tiles_bound * a.kv_heads;
-  if (units > INT_MAX) return DSR_ERR_ARG;
-  const dim3 grid((unsigned)units), threads(kAttnThreads);
+  const dim3 grid((unsigned)p.groups), threads(kAttnThreads);
   switch (p.tile_rows) {
     case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 1>), grid, threads, 0, s, a, p); break;
     case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, a, p); break;
@@ -110,8 +116,8 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
       }
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
-  if ((int64_t)a.width * a.page > p.min_chunk)  // else no request can have two chunks
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_combine<T, DP>), dim3((unsigned)(p.tiles_bound * a.kv_heads), (unsigned)(p.tile_rows / kCombineRows)),
+  if (p.cut)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP>), dim3((unsigned)p.groups - 1, (unsigned)(p.tile_rows / kJoinRows)),
                        threads, 0, s, a, p);
   return launched();
 }

@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as N
-from .batch import Workspace, _stream_handle
+from .batch import _stream_handle
 
 MAX_NODES = N.TREE_MAX_NODES
 _ROTARY_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16, torch.float32: N.F32}
@@ -90,14 +90,17 @@ class _Prepared:
         self._keep, self._name = keep, name
         self._call = getattr(N.load(), name)
         self._ref = ctypes.byref(args)
-        self._scratch, self._workspace = scratch, Workspace()
+        self._scratch, self._buffers = scratch, {}
         self._home = self._bound = _stream_handle(device)
         if scratch:
             self._bind(self._home)
 
     def _bind(self, handle):
         if self._scratch:
-            ws = self._workspace.get(self._scratch, self.device, handle=handle)
+            # One buffer per stream, made while the stream is current.
+            ws = self._buffers.get(handle)
+            if ws is None:
+                ws = self._buffers[handle] = torch.empty(self._scratch, dtype=torch.uint8, device=self.device)
             self.args.workspace, self.args.workspace_bytes = ws.data_ptr(), ws.numel()
         if handle != self._home:
             # Memory of the stream it was made on: not reused before this stream is done with it.
