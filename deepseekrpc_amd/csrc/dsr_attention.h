@@ -93,28 +93,29 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   return q;
 }
 
-// A value that all lanes share, in scalar registers.
-__device__ __forceinline__ int attn_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t attn_uniform(int64_t x) {
-  const uint32_t lo = (uint32_t)attn_uniform((int)(uint32_t)x), hi = (uint32_t)attn_uniform((int)(x >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-__device__ __forceinline__ int64_t attn_div(int64_t x, int64_t d) {  // both >= 0, d > 0
-  return (uint64_t)x >> 32 || (uint64_t)d >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+// Inclusive sums over the lanes of a wave, without LDS (row shifts, then the
+// rows' last lanes handed on).  Sums stop at 2^31 - 1.
+__device__ __forceinline__ int attn_wave_scan(int x) {
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = __builtin_elementwise_add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return x;
 }
 
 // One segment of a workgroup's work: the rows of a tile against tokens begin .. end - 1.
 struct AttnSegment {
   int r, head, tile, begin, end;
   bool whole;         // all of the tile's tokens
-  int64_t part;       // else: where its result goes
-  int64_t from, to;   // the tile's place in the order of all steps
+  int part;           // else: where its result goes
+  uint32_t from, to;  // the tile's place in the order of all steps
 };
 
 // A workgroup's share of the work.
 //
-// All work is put in one order of steps (`tokens` tokens of a tile): request
+// All work is put in one order of steps (p.tokens tokens of a tile): request
 // by request, head by head, tile by tile, token by token.  Each workgroup
 // takes an equal, contiguous part of it, so that requests of any lengths
 // load the chip evenly; a tile that crosses a border is written in parts,
@@ -124,66 +125,66 @@ struct AttnSegment {
 // 447 us instead of 274.)  Every wave finds the place for itself from the
 // requests' lengths, 64 at a time.  Neighbouring shares, which often have
 // keys and values in common, go to one XCD.
+// The host chooses p.tokens so that the steps of a call number less than 2^31.
+// HOLD: each lane keeps its request of the 64 looked at last (for kernels with
+// registers to spare), else a segment's request is read again.
+template <bool HOLD>
 struct AttnWork {
-  int64_t at, stop, quota;  // steps
-  int64_t base;             // steps of the requests before r
+  uint32_t at, stop, quota;  // steps
+  uint32_t base;             // steps of the requests before r
   int r, me;
+  int r0;                    // lane l holds request r0 + l:
+  AttnRequest mine;
 
-  static __device__ __forceinline__ int steps_of(const AttnRequest& q, int tokens) {
-    return q.rows == 0 ? 0 : q.kv > tokens ? (q.kv + tokens - 1) / tokens : 1;
+  __device__ __forceinline__ int steps_of(const AttnPlan& p, const AttnRequest& q) {
+    return q.rows == 0 ? 0 : q.kv > p.tokens ? (q.kv + p.tokens - 1) / p.tokens : 1;
+  }
+
+  // Steps of the lane's request of the 64 from `first` on.
+  __device__ __forceinline__ int hold(const dsr_tree_attention_args_t& a, const AttnPlan& p, int first) {
+    const int l = threadIdx.x & 63, R = (int)a.requests;
+    r0 = first;
+    mine = attn_request(a, a.q_heads / a.kv_heads, p.tile_rows, first + l < R ? first + l : R - 1);
+    return first + l < R ? mine.tiles * steps_of(p, mine) * a.kv_heads : 0;
   }
 
   // `border` 0: this workgroup's share.  Else the work from where share `border` begins.
   __device__ __forceinline__ AttnWork(const dsr_tree_attention_args_t& a, const AttnPlan& p, int border) {
-    const int tokens = p.tokens;
-    const int l = threadIdx.x & 63, R = (int)a.requests, group = a.q_heads / a.kv_heads;
-    AttnRequest q;
-    int64_t sum = 0, mine = 0;
-    for (int r0 = 0; r0 < R; r0 += 64) {
-      q = attn_request(a, group, p.tile_rows, r0 + l < R ? r0 + l : R - 1);
-      mine = r0 + l < R ? (int64_t)q.tiles * steps_of(q, tokens) * a.kv_heads : 0;
-      sum += mine;
+    const int R = (int)a.requests;
+    int upto = 0, steps = 0;
+    uint32_t total = 0;
+    for (int first = 0; first < R; first += 64) {
+      steps = hold(a, p, first);
+      upto = attn_wave_scan(steps);
+      total += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
     }
-    int64_t upto = sum;  // inclusive sums over the lanes
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int64_t x = __shfl_up(upto, s);
-      if (l >= s) upto += x;
-    }
-    const int64_t total = attn_uniform(__shfl(upto, 63));
-    quota = attn_div(total + p.groups - 1, p.groups);
-    if (quota < p.min_steps) quota = p.min_steps;
-    const int each = (int)attn_div(total + 8 * quota - 1, 8 * quota);  // workgroups with work, per XCD
-    const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
-    me = x * each + y;
-    at = y < each ? me * quota : total;
-    if (border) {
+    quota = (total + p.groups - 1) / (uint32_t)p.groups;
+    if (quota < (uint32_t)p.min_steps) quota = p.min_steps;
+    const uint32_t each = (total + 8 * quota - 1) / (8 * quota);  // workgroups with work, per XCD
+    if (border == 0) {
+      me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+      at = (blockIdx.x >> 3) < each ? me * quota : total;
+    } else {
       me = border;
-      at = border < 8 * each ? border * quota : total;
+      at = (uint32_t)border < 8 * each ? border * quota : total;
     }
     stop = at + quota < total ? at + quota : total;
-    r = 0;
+    r = R;
     base = 0;
     if (at >= stop) return;
-    for (int r0 = 0; r0 < R; r0 += 64) {
+    for (int first = 0; first < R; first += 64) {
       if (R > 64) {
-        q = attn_request(a, group, p.tile_rows, r0 + l < R ? r0 + l : R - 1);
-        mine = r0 + l < R ? (int64_t)q.tiles * steps_of(q, tokens) * a.kv_heads : 0;
-        upto = mine;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-          const int64_t z = __shfl_up(upto, s);
-          if (l >= s) upto += z;
-        }
+        steps = hold(a, p, first);
+        upto = attn_wave_scan(steps);
       }
-      const uint64_t past = __ballot(base + upto > at);
+      const uint64_t past = __ballot(base + (uint32_t)upto > at);
       if (past) {
         const int hit = __ffsll((unsigned long long)past) - 1;
-        base += attn_uniform(__shfl(upto - mine, hit));
-        r = r0 + hit;
-        break;
+        base += (uint32_t)__builtin_amdgcn_readlane(upto - steps, hit);
+        r = first + hit;
+        return;
       }
-      base += attn_uniform(__shfl(upto, 63));
+      base += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
     }
   }
 
@@ -191,38 +192,40 @@ struct AttnWork {
   __device__ __forceinline__ bool next(const dsr_tree_attention_args_t& a, const AttnPlan& p, AttnSegment& s,
                                        AttnRequest& q) {
     if (at >= stop) return false;
-    const int tokens = p.tokens;
     const int group = a.q_heads / a.kv_heads;
-    int steps;
-    int64_t length;
-    for (;;) {  // past requests that end here or have no rows; one with steps left exists, as at < stop
+    uint32_t steps, length;
+    for (;;) {  // past requests that end here or have no rows
       if (r >= a.requests) return false;
-      q = attn_request(a, group, p.tile_rows, r);
-      q.lo = attn_uniform(q.lo);
-      q.n = attn_uniform(q.n);
-      q.kv = attn_uniform(q.kv);
-      q.rows = attn_uniform(q.rows);
-      q.tiles = attn_uniform(q.tiles);
-      steps = steps_of(q, tokens);
-      length = (int64_t)q.tiles * steps * a.kv_heads;
-      if (at < base + length) break;
+      if (!HOLD || r - r0 >= 64) {
+        r0 = r;
+        mine = attn_request(a, group, p.tile_rows, HOLD && r + (int)(threadIdx.x & 63) < a.requests ? r + (threadIdx.x & 63) : r);
+      }
+      const int l = r - r0;
+      q.lo = __builtin_amdgcn_readlane(mine.lo, l);
+      q.n = __builtin_amdgcn_readlane(mine.n, l);
+      q.kv = __builtin_amdgcn_readlane(mine.kv, l);
+      q.rows = __builtin_amdgcn_readlane(mine.rows, l);
+      q.tiles = __builtin_amdgcn_readlane(mine.tiles, l);
+      q.fine = __builtin_amdgcn_readlane((int)mine.fine, l);
+      steps = steps_of(p, q);
+      length = q.tiles * steps * a.kv_heads;
+      if (at - base < length) break;
       base += length;
       ++r;
     }
-    const int64_t unit = attn_div(at - base, steps);
-    const int s0 = (int)(at - base - unit * steps);
-    const int s1 = stop - at < steps - s0 ? s0 + (int)(stop - at) : steps;
+    const uint32_t unit = (at - base) / steps, s0 = at - base - unit * steps;
+    const uint32_t s1 = stop - at < steps - s0 ? s0 + stop - at : steps;
     s.r = r;
-    s.head = (int)attn_div(unit, q.tiles);
-    s.tile = (int)(unit - (int64_t)s.head * q.tiles);
-    s.begin = s0 * tokens;
-    s.end = s1 == steps ? q.kv : s1 * tokens;
+    s.head = unit / (uint32_t)q.tiles;
+    s.tile = unit - (uint32_t)s.head * q.tiles;
+    s.begin = s0 * p.tokens;
+    s.end = s1 == steps ? q.kv : s1 * p.tokens;
     if (!a.visible && q.kv > 0) {  // causal rows: nothing past the tile's last one
-      const int64_t last = ((int64_t)(s.tile + 1) * p.tile_rows - 1) / group;
-      if (s.end > q.kv - q.n + last + 1) s.end = (int)(q.kv - q.n + last + 1);
+      const int last = (int)(((uint32_t)(s.tile + 1) * p.tile_rows - 1) / group);
+      if (s.end - (q.kv - q.n) > last + 1) s.end = q.kv - q.n + last + 1;
     }
     s.whole = s0 == 0 && s1 == steps;
-    s.part = 2 * (int64_t)me + (s0 > 0 ? 0 : 1);  // a tile begun elsewhere can only be a workgroup's first
+    s.part = 2 * me + (s0 > 0 ? 0 : 1);  // a tile begun elsewhere can only be a workgroup's first
     s.from = base + unit * steps;
     s.to = s.from + steps;
     at += s1 - s0;
@@ -231,9 +234,9 @@ struct AttnWork {
 };
 
 // Requests without rows have no work: their status, by the launch's first workgroup.
-__device__ __forceinline__ void attn_idle(const dsr_tree_attention_args_t& a, const AttnPlan& p) {
+__device__ __forceinline__ void attn_idle(const dsr_tree_attention_args_t& a, const AttnPlan& p, int threads) {
   if (blockIdx.x != 0) return;
-  for (int r = threadIdx.x; r < a.requests; r += kAttnThreads) {
+  for (int r = threadIdx.x; r < a.requests; r += threads) {
     const AttnRequest q = attn_request(a, a.q_heads / a.kv_heads, p.tile_rows, r);
     if (q.rows == 0) a.status[r] = q.fine ? DSR_OK : DSR_E_LENGTH;
   }
@@ -272,7 +275,7 @@ __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, 
   const int t = row / group, h = u.head * group + row - t * group;
   const T* query = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)h * a.q_head;
   T* out = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)h * a.out_head;
-  float* o = &p.part_o[(u.part * p.tile_rows + r) * DP];
+  float* o = &p.part_o[((int64_t)u.part * p.tile_rows + r) * DP];
 #pragma unroll 1
   for (int at = from; at < u.end; ++at) {
     const int id = a.table[u.r * a.table_ld + at / a.page], place = at & (a.page - 1);
@@ -334,38 +337,45 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
   return see & attn_low_bits(end - p0) & ~bad;
 }
 
-// Few rows (up to 16 NB of a tile): the four waves take the chunk's 32-token
-// tiles in turn, each for itself, and join their results at the end.
+// Few rows (16 of a tile): the waves take the segment's 32-token tiles in
+// turn, each for itself, and join their results at the end.
 //
 // S^T = K Q^T and O^T = V^T P^T, so that a lane holds one row's scores (row
 // lane % 16) and outputs: statistics and rescaling stay in the lane, and the
 // scores are the second product's operand as they lie, with the k index of
 // both operands permuted alike (lane group g takes tokens 4 g + i and
-// 16 + 4 g + i).  Keys go from memory to the product's registers directly;
-// values pass through the wave's own LDS rows, from which the transposing
-// read hands each lane four tokens of its dimension.  The next tile's keys
-// and values are in flight while a tile is worked on.
+// 16 + 4 g + i).  Keys and values pass through the wave's own LDS rows, from
+// which the transposing read hands each lane four tokens of a value's
+// dimension.  The next tile's keys and values are in flight while a tile is
+// worked on, and no wave waits for another.
 //
 // The running maximum is raised only when a score passes it by 8 (log2): the
 // weights then stay below 2^8, far inside every type's range, and most tiles
 // need no rescaling.
-template <class T, int DP, int NB>
-__global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_tree_attention(
+//
+// WAVES: four, two workgroups a CU, for long contexts; eight where one
+// workgroup takes a whole short context and its latency counts (32 query
+// heads over 1,001 tokens: ? us with eight, ? with four).
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
     dsr_tree_attention_args_t a, AttnPlan p) {
+  constexpr int NB = 1;         // 16-row blocks of a tile
+  constexpr int kThreads = 64 * WAVES;
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
   constexpr int KS = DP / 32;   // k steps of the score product
   constexpr int DB = DP / 16;   // 16-wide output blocks
   constexpr int VS = DP + 16;   // LDS row of values: 32 bytes of padding spread the transposing reads over the banks
-  __shared__ T vals[kAttnWaves][kAttnTile][VS];
-  __shared__ float sm[kAttnWaves][16 * NB], sl[kAttnWaves][16 * NB];
+  __shared__ __align__(16) T keys[WAVES][kAttnTile][DP + 8];  // 16 bytes of padding for the 16-byte reads of 16 keys
+  __shared__ __align__(16) T vals[WAVES][kAttnTile][VS];
+  __shared__ float sm[WAVES][16 * NB], sl[WAVES][16 * NB];
   __shared__ float sbase[16 * NB];
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
-  attn_idle(a, p);
-  AttnWork work(a, p, 0);
+  attn_idle(a, p, kThreads);
+  AttnWork<DP <= 128> work(a, p, 0);
   AttnSegment u;
   AttnRequest q;
   while (work.next(a, p, u, q)) {  // the same for the whole workgroup
@@ -412,38 +422,53 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   const int shift = __ffs(a.page) - 1;
   bool any_bad = false;
 
-  // Token tiles of this wave: 32 (4 i + w) past the chunk's begin.  Places
-  // past the last token read the last token (their scores are masked).
-  int ids[2];
+  // Tiles of this wave: 32 tokens from begin + 32 (WAVES i + w) on.  LPR lanes
+  // read a token's row, 16 bytes each side by side (lanes next to each other
+  // on different rows, as the product wants them, would take a cache access
+  // each: 16 bytes a cycle and CU in place of 64), and each of them NI tokens
+  // in a row, which share a page unless it is smaller.  Places past the last
+  // token read the last token (their scores are masked).
+  constexpr int LPR = DP / 8 <= 8 ? 8 : DP / 8 <= 16 ? 16 : 32;
+  constexpr int NI = kAttnTile / (64 / LPR);
+  const int sub = l / LPR * NI, chunk = 8 * (l & (LPR - 1)), d0 = min(chunk, dim - 8);
+  const bool stores = chunk < DP;  // 192 dimensions: 24 of 32 lanes
+  const bool tiny = a.page < NI;   // several pages: their ids are read with the rows
+  int id_next = 0;
   uint32_t bad_next = 0;
-  x8 kr[2][KS], vr[2][KS];
-  auto load_ids = [&](int p0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) ids[b] = pages[min(p0 + 16 * b + n, end - 1) >> shift];
-  };
+  x8 kr[NI], vr[NI];
+  auto load_id = [&](int p0) __attribute__((always_inline)) { id_next = pages[min(p0 + sub, end - 1) >> shift]; };
   auto load_rows = [&](int p0) __attribute__((always_inline)) {
     bad_next = 0;
+    auto load = [&](int i, int id, int place) __attribute__((always_inline)) {
+      const int64_t at = (unsigned)id < (unsigned)a.blocks ? id : 0;
+      place &= a.page - 1;
+      kr[i] = *(const x8*)(kb + at * a.k_block + place * a.k_token + d0);
+      vr[i] = *(const x8*)(vb + at * a.v_block + place * a.v_token + d0);
+    };
+    if (!tiny) {
+      const uint64_t bad = __ballot((unsigned)id_next >= (unsigned)a.blocks);
+      if (bad)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int place = min(p0 + 16 * b + n, end - 1) & (a.page - 1);
-      const bool bad = (unsigned)ids[b] >= (unsigned)a.blocks;
-      bad_next |= (uint32_t)(__ballot(bad) & 0xFFFF) << (16 * b);
-      const int64_t id = bad ? 0 : ids[b];
-      const T* ks = kb + id * a.k_block + place * a.k_token;
-      const T* vs = vb + id * a.v_block + place * a.v_token;
+        for (int j = 0; j < 64 / LPR; ++j)
+          if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = min(32 * s + 8 * g, dim - 8);  // past the head: any of its values, dropped below
-        kr[b][s] = *(const x8*)(ks + d);
-        vr[b][s] = *(const x8*)(vs + d);
+      for (int i = 0; i < NI; ++i) load(i, id_next, min(p0 + sub + i, end - 1));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int place = min(p0 + sub + i, end - 1), id = pages[place >> shift];
+        const uint64_t bad = __ballot((unsigned)id >= (unsigned)a.blocks);
+#pragma unroll
+        for (int j = 0; j < 64 / LPR; ++j) bad_next |= (uint32_t)(bad >> (j * LPR) & 1) << (NI * j + i);
+        load(i, id, place);
       }
     }
   };
-  const int first = begin + kAttnTile * w, step = kAttnTile * kAttnWaves;
+  const int first = begin + kAttnTile * w, step = kAttnTile * WAVES;
   if (first < end) {
-    load_ids(first);
+    load_id(first);
     load_rows(first);
-    if (first + step < end) load_ids(first + step);
+    load_id(first + step);
   }
   __syncthreads();  // the flags
   for (int p0 = first; p0 < end; p0 += step) {
@@ -453,10 +478,26 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
     if (masked) {
       bool poison = false;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int s = 0; s < KS; ++s) poison |= attn_make_finite<T>(vr[b][s]);
+      for (int i = 0; i < NI; ++i) poison |= attn_make_finite<T>(vr[i]);
       if (poison) spoison = 1;
+    }
+    // Keys and values to the wave's LDS rows; then the next tile's loads.
+    __builtin_amdgcn_wave_barrier();
+    if (DP == 8 * LPR || stores) {
+      if (chunk >= dim)  // dimensions past the head's
+#pragma unroll
+        for (int i = 0; i < NI; ++i) kr[i] = x8{};
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        *(x8*)&keys[w][sub + i][chunk] = kr[i];
+        *(x8*)&vals[w][sub + i][chunk] = vr[i];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (p0 + step < end) {
+      load_rows(p0 + step);
+      load_id(p0 + 2 * step);
     }
     // Scores.
     attn_f32x4 sc[NB][2];
@@ -465,25 +506,13 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
       for (int k = 0; k < 2; ++k) sc[b][k] = attn_f32x4{};
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const x8 key = 32 * s + 8 * g < dim ? kr[k][s] : x8{};
+      for (int k = 0; k < 2; ++k) {
+        const x8 key = *(const x8*)&keys[w][16 * k + n][32 * s + 8 * g];
 #pragma unroll
         for (int b = 0; b < NB; ++b) sc[b][k] = AttnType<T>::mfma16(key, qv[b][s], sc[b][k]);
       }
-    // Values to LDS; then the next tile's loads.
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) *(x8*)&vals[w][16 * k + n][32 * s + 8 * g] = vr[k][s];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (p0 + step < end) {
-      load_rows(p0 + step);
-      if (p0 + 2 * step < end) load_ids(p0 + 2 * step);
-    }
     // Softmax.  A lane's scores: tokens p0 + 16 k + 4 g + e of its row.
     x8 pv[NB];
 #pragma unroll
@@ -530,7 +559,7 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
     }
   }
 
-  // The four waves' results: statistics, then one row block at a time.
+  // The waves' results: statistics, then one row block at a time.
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     sum[b] += __shfl_xor(sum[b], 16);
@@ -548,21 +577,23 @@ __global__ __launch_bounds__(kAttnThreads, NB == 1 && DP <= 128 ? 2 : 1) void k_
   static_assert(16 * OS * sizeof(float) <= kAttnTile * VS * sizeof(T), "a wave's outputs fit its rows of values");
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const float top = fmaxf(fmaxf(sm[0][16 * b + n], sm[1][16 * b + n]), fmaxf(sm[2][16 * b + n], sm[3][16 * b + n]));
+    float top = sm[0][16 * b + n];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) top = fmaxf(top, sm[i][16 * b + n]);
     const float f = m[b] == top ? 1.f : __builtin_amdgcn_exp2f(m[b] - top);  // a wave without tokens: 0
     float* mine = (float*)&vals[w][0][0];
 #pragma unroll
     for (int d = 0; d < DB; ++d) *(attn_f32x4*)&mine[n * OS + 16 * d + 4 * g] = acc[b][d] * f;
     __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (DP / 4); x += kAttnThreads) {
+    for (int x = threadIdx.x; x < 16 * (DP / 4); x += kThreads) {
       const int row = x / (DP / 4), d = x % (DP / 4) * 4, rr = 16 * b + row;
       float M = sm[0][rr];
 #pragma unroll
-      for (int i = 1; i < kAttnWaves; ++i) M = fmaxf(M, sm[i][rr]);
+      for (int i = 1; i < WAVES; ++i) M = fmaxf(M, sm[i][rr]);
       float L = 0.f;
       attn_f32x4 o = {};
 #pragma unroll
-      for (int i = 0; i < kAttnWaves; ++i) {
+      for (int i = 0; i < WAVES; ++i) {
         L += sl[i][rr] * (sm[i][rr] == M ? 1.f : __builtin_amdgcn_exp2f(sm[i][rr] - M));
         o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
       }
@@ -598,30 +629,30 @@ template <class T, int DP>
 __global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_args_t a, AttnPlan p) {
   typedef typename AttnType<T>::x4 x4;
   const int border = blockIdx.x + 1;
-  AttnWork work(a, p, border);
+  AttnWork<false> work(a, p, border);
   AttnSegment u;
   AttnRequest q;
-  const int64_t at = work.at;
+  const uint32_t at = work.at;
   if (!work.next(a, p, u, q) || u.from == at) return;  // no work there; a tile begins there
-  const int64_t first = attn_div(u.from, work.quota), last = attn_div(u.to - 1, work.quota);
+  const int first = u.from / work.quota, last = (u.to - 1) / work.quota;
   if (first != border - 1) return;
   const int group = a.q_heads / a.kv_heads, row0 = u.tile * p.tile_rows;
   const int rows = min((int)blockIdx.y * kJoinRows + kJoinRows, min(p.tile_rows, q.rows - row0));
   // The first part is its workgroup's last (an odd place), the others their workgroups' first.
   for (int x = blockIdx.y * kJoinRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
     const int row = x / (DP / 4), d = x % (DP / 4) * 4;
+    // The maximum first, so that the parts' loads do not wait for each other.
+    auto part = [&](int c) { return (int64_t)(2 * c + (c == first)) * p.tile_rows + row; };
     float M = -INFINITY, L = 0.f;
     attn_f32x4 o = {};
-    for (int64_t c = first; c <= last; ++c) {
-      const int64_t part = (2 * c + (c == first)) * p.tile_rows + row;
-      const float2 ml = p.part_ml[part];
-      const attn_f32x4 y = *(const attn_f32x4*)&p.part_o[part * DP + d];
-      const float top = fmaxf(M, ml.x);
-      const float f = M == top ? 1.f : __builtin_amdgcn_exp2f(M - top);
-      const float f2 = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-      M = top;
-      L = L * f + ml.y * f2;
-      o = o * f + y * f2;
+#pragma unroll 4
+    for (int c = first; c <= last; ++c) M = fmaxf(M, p.part_ml[part(c)].x);
+#pragma unroll 4
+    for (int c = first; c <= last; ++c) {
+      const float2 ml = p.part_ml[part(c)];
+      const float f = ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+      L += ml.y * f;
+      o += *(const attn_f32x4*)&p.part_o[part(c) * DP + d] * f;
     }
     if (d >= a.head_dim) continue;
     const int t = (row0 + row) / group, h = row0 + row - t * group;
@@ -635,7 +666,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_a
   }
   if (u.head == 0 && u.tile == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     int bad = 0;
-    for (int64_t c = first; c <= last; ++c) bad |= p.part_bad[2 * c + (c == first)];
+    for (int c = first; c <= last; ++c) bad |= p.part_bad[2 * c + (c == first)];
     a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
   }
 }

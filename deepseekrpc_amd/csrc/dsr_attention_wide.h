@@ -66,8 +66,8 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
   const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
-  attn_idle(a, p);
-  AttnWork work(a, p, 0);
+  attn_idle(a, p, kAttnThreads);
+  AttnWork<false> work(a, p, 0);
   AttnSegment u;
   AttnRequest q;
   while (work.next(a, p, u, q)) {  // the same for the whole workgroup

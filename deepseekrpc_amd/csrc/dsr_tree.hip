@@ -75,6 +75,9 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   // step: nothing is cut, and no joining launch follows.
   p.cut = (int64_t)a.width * a.page > kAttnShort;
   if (!p.cut) p.tokens = kAttnShort, p.min_steps = 1;
+  const int64_t tiles = (a.tokens * group / p.tile_rows + a.requests) * a.kv_heads;
+  while (((int64_t)a.width * a.page / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
+  if (!p.cut && tiles < p.groups) p.groups = (int)((tiles + 7) / 8 * 8);
   return p;
 }
 
@@ -103,7 +106,14 @@ template <class T, int DP>
 int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.groups), threads(kAttnThreads);
   switch (p.tile_rows) {
-    case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 1>), grid, threads, 0, s, a, p); break;
+    case 16:
+      if constexpr (DP <= 128)
+        if (!p.cut) {
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 8>), grid, dim3(512), 0, s, a, p);
+          break;
+        }
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4>), grid, threads, 0, s, a, p);
+      break;
     case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, a, p); break;
     default:
       if constexpr (DP <= 128) {
