@@ -60,9 +60,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // What the host decides for one call.
 struct AttnPlan {
-  int tile_rows;      // rows of a tile
+  int tile_rows;      // rows of a tile, a power of two
+  int tile_shift, token_shift, page_shift, group_shift;  // their logarithms; -1: not a power of two
+  int group;          // query heads per key head
   int groups;         // workgroups, a multiple of 8
-  int tokens;         // of a step of the work split: a multiple of the kernel's own
+  int tokens;         // of a step of the work split: a power of two times the kernel's own
   int min_steps;      // fewest steps worth a workgroup
   bool cut;           // some tile may be cut into parts
   float* part_o;      // [2 groups, tile_rows, head dim of the kernel]
@@ -76,8 +78,12 @@ struct AttnRequest {
   bool fine;
 };
 
-__device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_args_t& a, int group, int tile_rows,
-                                                    int r) {
+// A row's token among the request's new ones.
+__device__ __forceinline__ int attn_token(const AttnPlan& p, int row) {
+  return p.group_shift >= 0 ? row >> p.group_shift : row / p.group;
+}
+
+__device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_args_t& a, const AttnPlan& p, int r) {
   AttnRequest q;
   int lo = a.offsets[r], hi = a.offsets[r + 1];
   const int N = (int)a.tokens;
@@ -87,9 +93,9 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   q.n = hi - lo;
   const int kv = a.kv_lengths[r];
   q.fine = kv >= q.n && kv <= (int64_t)a.width * a.page && !(a.visible && q.n > DSR_TREE_MAX_NODES);
-  q.rows = q.n * group;
+  q.rows = q.n * p.group;
   q.kv = q.fine && q.n > 0 ? kv : 0;
-  q.tiles = q.rows > tile_rows ? (q.rows + tile_rows - 1) / tile_rows : 1;
+  q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
   return q;
 }
 
@@ -137,14 +143,14 @@ struct AttnWork {
   AttnRequest mine;
 
   __device__ __forceinline__ int steps_of(const AttnPlan& p, const AttnRequest& q) {
-    return q.rows == 0 ? 0 : q.kv > p.tokens ? (q.kv + p.tokens - 1) / p.tokens : 1;
+    return q.rows == 0 ? 0 : q.kv > p.tokens ? (q.kv + p.tokens - 1) >> p.token_shift : 1;
   }
 
   // Steps of the lane's request of the 64 from `first` on.
   __device__ __forceinline__ int hold(const dsr_tree_attention_args_t& a, const AttnPlan& p, int first) {
     const int l = threadIdx.x & 63, R = (int)a.requests;
     r0 = first;
-    mine = attn_request(a, a.q_heads / a.kv_heads, p.tile_rows, first + l < R ? first + l : R - 1);
+    mine = attn_request(a, p, first + l < R ? first + l : R - 1);
     return first + l < R ? mine.tiles * steps_of(p, mine) * a.kv_heads : 0;
   }
 
@@ -192,13 +198,12 @@ struct AttnWork {
   __device__ __forceinline__ bool next(const dsr_tree_attention_args_t& a, const AttnPlan& p, AttnSegment& s,
                                        AttnRequest& q) {
     if (at >= stop) return false;
-    const int group = a.q_heads / a.kv_heads;
     uint32_t steps, length;
     for (;;) {  // past requests that end here or have no rows
       if (r >= a.requests) return false;
       if (!HOLD || r - r0 >= 64) {
         r0 = r;
-        mine = attn_request(a, group, p.tile_rows, HOLD && r + (int)(threadIdx.x & 63) < a.requests ? r + (threadIdx.x & 63) : r);
+        mine = attn_request(a, p, HOLD && r + (int)(threadIdx.x & 63) < a.requests ? r + (threadIdx.x & 63) : r);
       }
       const int l = r - r0;
       q.lo = __builtin_amdgcn_readlane(mine.lo, l);
@@ -221,7 +226,7 @@ struct AttnWork {
     s.begin = s0 * p.tokens;
     s.end = s1 == steps ? q.kv : s1 * p.tokens;
     if (!a.visible && q.kv > 0) {  // causal rows: nothing past the tile's last one
-      const int last = (int)(((uint32_t)(s.tile + 1) * p.tile_rows - 1) / group);
+      const int last = attn_token(p, (s.tile + 1) * p.tile_rows - 1);
       if (s.end - (q.kv - q.n) > last + 1) s.end = q.kv - q.n + last + 1;
     }
     s.whole = s0 == 0 && s1 == steps;
@@ -237,7 +242,7 @@ struct AttnWork {
 __device__ __forceinline__ void attn_idle(const dsr_tree_attention_args_t& a, const AttnPlan& p, int threads) {
   if (blockIdx.x != 0) return;
   for (int r = threadIdx.x; r < a.requests; r += threads) {
-    const AttnRequest q = attn_request(a, a.q_heads / a.kv_heads, p.tile_rows, r);
+    const AttnRequest q = attn_request(a, p, r);
     if (q.rows == 0) a.status[r] = q.fine ? DSR_OK : DSR_E_LENGTH;
   }
 }
@@ -270,15 +275,15 @@ template <class T, int DP>
 __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, const AttnPlan& p, const AttnSegment& u,
                                             const AttnRequest& q, int from, const float* base) {
   typedef typename AttnType<T>::x8 x8;
-  const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = a.q_heads / a.kv_heads, ctx = q.kv - q.n;
+  const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = p.group, ctx = q.kv - q.n;
   if (r >= p.tile_rows || row >= q.rows) return;
-  const int t = row / group, h = u.head * group + row - t * group;
+  const int t = attn_token(p, row), h = u.head * group + row - t * group;
   const T* query = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)h * a.q_head;
   T* out = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)h * a.out_head;
   float* o = &p.part_o[((int64_t)u.part * p.tile_rows + r) * DP];
 #pragma unroll 1
   for (int at = from; at < u.end; ++at) {
-    const int id = a.table[u.r * a.table_ld + at / a.page], place = at & (a.page - 1);
+    const int id = a.table[u.r * a.table_ld + (at >> p.page_shift)], place = at & (a.page - 1);
     if ((unsigned)id >= (unsigned)a.blocks) continue;
     const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
     const T* k = (const T*)a.k_cache + id * a.k_block + place * a.k_token + u.head * a.k_head;
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
+  const int group = p.group, dim = a.head_dim;
   attn_idle(a, p, kThreads);
   AttnWork<DP <= 128> work(a, p, 0);
   AttnSegment u;
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   for (int b = 0; b < NB; ++b) {
     const int row = row0 + 16 * b + n;
     const bool in = row < q.rows;
-    const int t = in ? row / group : 0, h = in ? row - t * group : 0;
+    const int t = in ? attn_token(p, row) : 0, h = in ? row - t * group : 0;
     tok[b] = t;
     mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
     const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + h) * a.q_head;
@@ -419,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   const int32_t* pages = a.table + u.r * a.table_ld;
   const T* kb = (const T*)a.k_cache + u.head * a.k_head;
   const T* vb = (const T*)a.v_cache + u.head * a.v_head;
-  const int shift = __ffs(a.page) - 1;
+  const int shift = p.page_shift;
   bool any_bad = false;
 
   // Tiles of this wave: 32 tokens from begin + 32 (WAVES i + w) on.  LPR lanes
@@ -446,13 +451,27 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
       vr[i] = *(const x8*)(vb + at * a.v_block + place * a.v_token + d0);
     };
     if (!tiny) {
-      const uint64_t bad = __ballot((unsigned)id_next >= (unsigned)a.blocks);
+      const bool outside = (unsigned)id_next >= (unsigned)a.blocks;
+      const uint64_t bad = __ballot(outside);
       if (bad)
 #pragma unroll
         for (int j = 0; j < 64 / LPR; ++j)
           if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
+      if (p0 + kAttnTile <= end) {
+        const int64_t at = outside ? 0 : id_next, place = (p0 + sub) & (a.page - 1);
+        const T* k = kb + (at * a.k_block + place * a.k_token + d0);
+        const T* v = vb + (at * a.v_block + place * a.v_token + d0);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) load(i, id_next, min(p0 + sub + i, end - 1));
+        for (int i = 0; i < NI; ++i) {
+          kr[i] = *(const x8*)k;
+          vr[i] = *(const x8*)v;
+          k += a.k_token;
+          v += a.v_token;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) load(i, id_next, min(p0 + sub + i, end - 1));
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -602,7 +621,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
         *(attn_f32x4*)&p.part_o[(part * p.tile_rows + rr) * DP + d] = o;
         if (d == 0) p.part_ml[part * p.tile_rows + rr] = float2{M, L};
       } else if (row0 + rr < q.rows && d < dim) {
-        const int t = (row0 + rr) / group, h = row0 + rr - t * group;
+        const int t = attn_token(p, row0 + rr), h = row0 + rr - t * group;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         x4 y;
 #pragma unroll
@@ -636,7 +655,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_a
   if (!work.next(a, p, u, q) || u.from == at) return;  // no work there; a tile begins there
   const int first = u.from / work.quota, last = (u.to - 1) / work.quota;
   if (first != border - 1) return;
-  const int group = a.q_heads / a.kv_heads, row0 = u.tile * p.tile_rows;
+  const int group = p.group, row0 = u.tile * p.tile_rows;
   const int rows = min((int)blockIdx.y * kJoinRows + kJoinRows, min(p.tile_rows, q.rows - row0));
   // The first part is its workgroup's last (an odd place), the others their workgroups' first.
   for (int x = blockIdx.y * kJoinRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
@@ -655,7 +674,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_a
       o += *(const attn_f32x4*)&p.part_o[part(c) * DP + d] * f;
     }
     if (d >= a.head_dim) continue;
-    const int t = (row0 + row) / group, h = row0 + row - t * group;
+    const int t = attn_token(p, row0 + row), h = row0 + row - t * group;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     x4 y;
 #pragma unroll

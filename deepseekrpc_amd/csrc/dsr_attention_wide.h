@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  const int group = a.q_heads / a.kv_heads, dim = a.head_dim;
+  const int group = p.group, dim = a.head_dim;
   attn_idle(a, p, kAttnThreads);
   AttnWork<false> work(a, p, 0);
   AttnSegment u;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   for (int b = 0; b < RB; ++b) {
     const int row = row0 + 32 * b + n;
     const bool in = row < q.rows;
-    const int t = in ? row / group : 0, hh = in ? row - t * group : 0;
+    const int t = in ? attn_token(p, row) : 0, hh = in ? row - t * group : 0;
     tok[b] = t;
     mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
     const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + hh) * a.q_head;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   const int32_t* pages = a.table + u.r * a.table_ld;
   const T* kb = (const T*)a.k_cache + u.head * a.k_head;
   const T* vb = (const T*)a.v_cache + u.head * a.v_head;
-  const int shift = __ffs(a.page) - 1;
+  const int shift = p.page_shift;
   bool any_bad = false;
 
   // Staging: chunk c of token t of a step's NT; the step's places past the
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
                 attn_f32x4{acc[b][d][4 * e], acc[b][d][4 * e + 1], acc[b][d][4 * e + 2], acc[b][d][4 * e + 3]};
         if (h == 0) p.part_ml[part * p.tile_rows + in_tile] = float2{m[b], sum[b]};
       } else {
-        const int t = row / group, hh = row - t * group;
+        const int t = attn_token(p, row), hh = row - t * group;
         const float inv = sum[b] == 0.f ? 0.f : 1.f / sum[b];
         T* o = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + hh) * a.out_head;
 #pragma unroll

@@ -77,6 +77,10 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   if (!p.cut) p.tokens = kAttnShort, p.min_steps = 1;
   const int64_t tiles = (a.tokens * group / p.tile_rows + a.requests) * a.kv_heads;
   while (((int64_t)a.width * a.page / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
+  auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
+  p.group = (int)group;
+  p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
+  p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
   if (!p.cut && tiles < p.groups) p.groups = (int)((tiles + 7) / 8 * 8);
   return p;
 }

@@ -26,11 +26,16 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as N
-from .batch import _stream_handle
+from . import batch
 
 MAX_NODES = N.TREE_MAX_NODES
 _ROTARY_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16, torch.float32: N.F32}
 _ATTENTION_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16}
+
+
+# torch's raw accessors, as batch uses them: the public ones cost microseconds a launch.
+_raw_stream = batch._raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = batch._current_device or torch.cuda.current_device
 
 
 def _device_of(t, name):
@@ -91,7 +96,8 @@ class _Prepared:
         self._call = getattr(N.load(), name)
         self._ref = ctypes.byref(args)
         self._scratch, self._buffers = scratch, {}
-        self._home = self._bound = _stream_handle(device)
+        self._index = device.index
+        self._home = self._bound = _raw_stream(self._index)
         if scratch:
             self._bind(self._home)
 
@@ -110,10 +116,10 @@ class _Prepared:
         self._bound = handle
 
     def launch(self):
-        handle = _stream_handle(self.device)
+        handle = _raw_stream(self._index)
         if handle != self._bound:
             self._bind(handle)
-        if torch.cuda.current_device() == self.device.index:
+        if _current_device() == self._index:
             rc = self._call(self._ref, handle)
         else:
             with torch.cuda.device(self.device):
