@@ -72,6 +72,20 @@ struct AttnPlan {
   int32_t* part_bad;  // [2 groups]: a page id outside the cache
 };
 
+// The kernels' argument, read anew where a part of it begins: kept in
+// scalar registers from its start to its end they would not fit, and a third
+// of the few-row kernel's instructions were moves of spilled ones.
+struct AttnCall {
+  dsr_tree_attention_args_t a;
+  AttnPlan p;
+};
+__device__ __forceinline__ const AttnCall& attn_call() {
+  typedef const AttnCall __attribute__((address_space(4))) * Args;
+  Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  return *(const AttnCall*)args;
+}
+
 struct AttnRequest {
   int lo, n, kv;  // first new token, new tokens, cached tokens (0: nothing to read)
   int rows, tiles;
@@ -363,7 +377,7 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
 // heads over 1,001 tokens: ? us with eight, ? with four).
 template <class T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
-    dsr_tree_attention_args_t a, AttnPlan p) {
+    AttnCall) {
   constexpr int NB = 1;         // 16-row blocks of a tile
   constexpr int kThreads = 64 * WAVES;
   typedef typename AttnType<T>::x4 x4;
@@ -378,16 +392,18 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  const int group = p.group, dim = a.head_dim;
-  attn_idle(a, p, kThreads);
-  AttnWork<DP <= 128> work(a, p, 0);
+  attn_idle(attn_call().a, attn_call().p, kThreads);
+  AttnWork<DP <= 128> work(attn_call().a, attn_call().p, 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(a, p, u, q)) {  // the same for the whole workgroup
+  while (work.next(attn_call().a, attn_call().p, u, q)) {  // the same for the whole workgroup
+  const dsr_tree_attention_args_t& a = attn_call().a;
+  const AttnPlan& p = attn_call().p;
+  const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
   __syncthreads();  // the last segment's LDS is read
   if (threadIdx.x == 0) sbad = spoison = 0;
   const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
-  const int row0 = u.tile * p.tile_rows;
+  const int row0 = u.tile << row_shift;
 
   // This lane's rows: token index, mask, query operand.  A negative scale
   // changes the queries' sign, so that scores only grow with their products;
@@ -421,10 +437,14 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = attn_f32x4{};
   }
-  const int32_t* pages = a.table + u.r * a.table_ld;
-  const T* kb = (const T*)a.k_cache + u.head * a.k_head;
-  const T* vb = (const T*)a.v_cache + u.head * a.v_head;
-  const int shift = p.page_shift;
+  const dsr_tree_attention_args_t& c = attn_call().a;
+  const int32_t* pages = c.table + u.r * c.table_ld;
+  const T* kb = (const T*)c.k_cache + u.head * c.k_head;
+  const T* vb = (const T*)c.v_cache + u.head * c.v_head;
+  const int shift = attn_call().p.page_shift, page = c.page;
+  const unsigned blocks = c.blocks;
+  const int64_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
+  const bool masks = c.visible != nullptr;
   bool any_bad = false;
 
   // Tiles of this wave: 32 tokens from begin + 32 (WAVES i + w) on.  LPR lanes
@@ -437,7 +457,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   constexpr int NI = kAttnTile / (64 / LPR);
   const int sub = l / LPR * NI, chunk = 8 * (l & (LPR - 1)), d0 = min(chunk, dim - 8);
   const bool stores = chunk < DP;  // 192 dimensions: 24 of 32 lanes
-  const bool tiny = a.page < NI;   // several pages: their ids are read with the rows
+  const bool tiny = page < NI;   // several pages: their ids are read with the rows
   int id_next = 0;
   uint32_t bad_next = 0;
   x8 kr[NI], vr[NI];
@@ -445,28 +465,28 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   auto load_rows = [&](int p0) __attribute__((always_inline)) {
     bad_next = 0;
     auto load = [&](int i, int id, int place) __attribute__((always_inline)) {
-      const int64_t at = (unsigned)id < (unsigned)a.blocks ? id : 0;
-      place &= a.page - 1;
-      kr[i] = *(const x8*)(kb + at * a.k_block + place * a.k_token + d0);
-      vr[i] = *(const x8*)(vb + at * a.v_block + place * a.v_token + d0);
+      const int64_t at = (unsigned)id < blocks ? id : 0;
+      place &= page - 1;
+      kr[i] = *(const x8*)(kb + at * k_block + place * k_token + d0);
+      vr[i] = *(const x8*)(vb + at * v_block + place * v_token + d0);
     };
     if (!tiny) {
-      const bool outside = (unsigned)id_next >= (unsigned)a.blocks;
+      const bool outside = (unsigned)id_next >= blocks;
       const uint64_t bad = __ballot(outside);
       if (bad)
 #pragma unroll
         for (int j = 0; j < 64 / LPR; ++j)
           if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
       if (p0 + kAttnTile <= end) {
-        const int64_t at = outside ? 0 : id_next, place = (p0 + sub) & (a.page - 1);
-        const T* k = kb + (at * a.k_block + place * a.k_token + d0);
-        const T* v = vb + (at * a.v_block + place * a.v_token + d0);
+        const int64_t at = outside ? 0 : id_next, place = (p0 + sub) & (page - 1);
+        const T* k = kb + (at * k_block + place * k_token + d0);
+        const T* v = vb + (at * v_block + place * v_token + d0);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
           kr[i] = *(const x8*)k;
           vr[i] = *(const x8*)v;
-          k += a.k_token;
-          v += a.v_token;
+          k += k_token;
+          v += v_token;
         }
       } else {
 #pragma unroll
@@ -476,7 +496,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int place = min(p0 + sub + i, end - 1), id = pages[place >> shift];
-        const uint64_t bad = __ballot((unsigned)id >= (unsigned)a.blocks);
+        const uint64_t bad = __ballot((unsigned)id >= blocks);
 #pragma unroll
         for (int j = 0; j < 64 / LPR; ++j) bad_next |= (uint32_t)(bad >> (j * LPR) & 1) << (NI * j + i);
         load(i, id, place);
@@ -538,7 +558,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     for (int b = 0; b < NB; ++b) {
       float top = -INFINITY;
       if (masked) {
-        const uint32_t see = attn_sees(a.visible, mask[b], tok[b], p0, ctx, end, bad) >> (4 * g);
+        const uint32_t see = attn_sees(masks, mask[b], tok[b], p0, ctx, end, bad) >> (4 * g);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -590,6 +610,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   }
   if (any_bad && l == 0) sbad = 1;
   __syncthreads();
+  const AttnCall& e = attn_call();
   const bool split = !u.whole;
   const int64_t part = u.part;
   constexpr int OS = DP + 4;  // LDS row of outputs
@@ -618,24 +639,24 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
       }
       if (d == 0) sbase[rr] = M;
       if (split) {
-        *(attn_f32x4*)&p.part_o[(part * p.tile_rows + rr) * DP + d] = o;
-        if (d == 0) p.part_ml[part * p.tile_rows + rr] = float2{M, L};
+        *(attn_f32x4*)&e.p.part_o[(((int64_t)part << row_shift) + rr) * DP + d] = o;
+        if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + rr] = float2{M, L};
       } else if (row0 + rr < q.rows && d < dim) {
-        const int t = attn_token(p, row0 + rr), h = row0 + rr - t * group;
+        const int t = attn_token(e.p, row0 + rr), h = row0 + rr - t * group;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         x4 y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
-        *(x4*)((T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + h) * a.out_head + d) = y;
-        if (a.lse && d == 0)
-          a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        *(x4*)((T*)e.a.out + (int64_t)(q.lo + t) * e.a.out_token + (int64_t)(u.head * group + h) * e.a.out_head + d) = y;
+        if (e.a.lse && d == 0)
+          e.a.lse[(int64_t)(q.lo + t) * e.a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
       }
     }
     __threadfence_block();
     __syncthreads();
   }
-  if (spoison) attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
-  attn_report(a, p, u, q, sbad);
+  if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
+  attn_report(e.a, e.p, u, q, sbad);
   }
 }
 
@@ -645,16 +666,18 @@ constexpr int kJoinRows = 16;  // rows of a tile per workgroup (blockIdx.y)
 // of the tokens: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
 // Workgroup x takes the tile whose first border is the one before share x + 1.
 template <class T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void k_tree_join(dsr_tree_attention_args_t a, AttnPlan p) {
+__global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   typedef typename AttnType<T>::x4 x4;
   const int border = blockIdx.x + 1;
-  AttnWork<false> work(a, p, border);
+  AttnWork<false> work(attn_call().a, attn_call().p, border);
   AttnSegment u;
   AttnRequest q;
   const uint32_t at = work.at;
-  if (!work.next(a, p, u, q) || u.from == at) return;  // no work there; a tile begins there
+  if (!work.next(attn_call().a, attn_call().p, u, q) || u.from == at) return;  // no work there; a tile begins there
   const int first = u.from / work.quota, last = (u.to - 1) / work.quota;
   if (first != border - 1) return;
+  const dsr_tree_attention_args_t& a = attn_call().a;
+  const AttnPlan& p = attn_call().p;
   const int group = p.group, row0 = u.tile * p.tile_rows;
   const int rows = min((int)blockIdx.y * kJoinRows + kJoinRows, min(p.tile_rows, q.rows - row0));
   // The first part is its workgroup's last (an odd place), the others their workgroups' first.

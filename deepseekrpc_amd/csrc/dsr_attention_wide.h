@@ -43,7 +43,7 @@ struct AttnWideShared {
 // values pass from memory through registers (two steps in flight) into LDS.
 template <class T, int DP, int RB, int WR>
 __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_tree_attention_wide(
-    dsr_tree_attention_args_t a, AttnPlan p) {
+    AttnCall) {
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
   typedef AttnWideShared<DP, WR> Sh;
@@ -65,19 +65,21 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  const int group = p.group, dim = a.head_dim;
-  attn_idle(a, p, kAttnThreads);
-  AttnWork<false> work(a, p, 0);
+  attn_idle(attn_call().a, attn_call().p, kAttnThreads);
+  AttnWork<false> work(attn_call().a, attn_call().p, 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(a, p, u, q)) {  // the same for the whole workgroup
+  while (work.next(attn_call().a, attn_call().p, u, q)) {  // the same for the whole workgroup
+  const dsr_tree_attention_args_t& a = attn_call().a;
+  const AttnPlan& p = attn_call().p;
+  const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
   __syncthreads();  // the last segment's LDS is read
   if (threadIdx.x < 4 * WK) sbits[threadIdx.x / WK][threadIdx.x % WK] = 0;
   if (threadIdx.x == 0) sbad = spoison = 0;
   const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
   const int clear = min(ctx, end);  // every row sees the tokens before
   const int steps = end > begin ? (end - begin + NT - 1) / NT : 0;
-  const int row0 = u.tile * p.tile_rows + 32 * RB * wr;
+  const int row0 = (u.tile << row_shift) + 32 * RB * wr;
 
   // A negative scale changes the queries' sign, so that scores only grow
   // with their products; scale 0 is queries of 0.
@@ -110,10 +112,14 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = attn_f32x16{};
   }
-  const int32_t* pages = a.table + u.r * a.table_ld;
-  const T* kb = (const T*)a.k_cache + u.head * a.k_head;
-  const T* vb = (const T*)a.v_cache + u.head * a.v_head;
-  const int shift = p.page_shift;
+  const dsr_tree_attention_args_t& c = attn_call().a;
+  const int32_t* pages = c.table + u.r * c.table_ld;
+  const T* kb = (const T*)c.k_cache + u.head * c.k_head;
+  const T* vb = (const T*)c.v_cache + u.head * c.v_head;
+  const int shift = attn_call().p.page_shift, page = c.page;
+  const unsigned blocks = c.blocks;
+  const int64_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
+  const bool masks = c.visible != nullptr;
   bool any_bad = false;
 
   // Staging: chunk c of token t of a step's NT; the step's places past the
@@ -134,8 +140,8 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = (int)(threadIdx.x + kAttnThreads * i) % CH;
-      const int64_t b = (unsigned)id[i] < (unsigned)a.blocks ? id[i] : 0;
-      r[i] = *(const x8*)(base + b * block + (place_of(step, i) & (a.page - 1)) * token + min(8 * c, dim - 8));
+      const int64_t b = (unsigned)id[i] < blocks ? id[i] : 0;
+      r[i] = *(const x8*)(base + b * block + (place_of(step, i) & (page - 1)) * token + min(8 * c, dim - 8));
     }
   };
   auto store_keys = [&](int buf, const x8* r, const int* id, int step) __attribute__((always_inline)) {
@@ -144,7 +150,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
     for (int i = 0; i < NL; ++i) {
       const int x = (int)threadIdx.x + kAttnThreads * i, c = x % CH;
       *(x8*)&keys[(buf * NT + x / CH) * KS + 8 * c] = 8 * c < dim ? r[i] : x8{};
-      if ((unsigned)id[i] >= (unsigned)a.blocks) {
+      if ((unsigned)id[i] >= blocks) {
         bad = true;
         atomicOr(&sbits[step & 3][x / CH / 32], 1u << (x / CH % 32));
       }
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   auto store_vals = [&](int buf, x8* r, const int* id, int step) __attribute__((always_inline)) {
     bool bad = begin + (step + 1) * NT > clear;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) bad |= (unsigned)id[i] >= (unsigned)a.blocks;
+    for (int i = 0; i < NL; ++i) bad |= (unsigned)id[i] >= blocks;
     if (__ballot(bad)) {
       bool poison = false;
 #pragma unroll
@@ -187,7 +193,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
     if (p0 + kAttnTile > clear || bad) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const uint32_t see = attn_sees(a.visible, mask[b], tok[b], p0, ctx, end, bad) >> (4 * h);
+        const uint32_t see = attn_sees(masks, mask[b], tok[b], p0, ctx, end, bad) >> (4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[b][e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? s[b][e] : -INFINITY;
       }
@@ -253,14 +259,14 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
     const int last = steps - 1;
     auto keys_of = [&](auto S, int step) __attribute__((always_inline)) {  // registers of keys `step`, ids ahead
       constexpr int c = decltype(S)::value % SETS;
-      load(kr[c], kid[c], min(step, last), kb, a.k_block, a.k_token);
+      load(kr[c], kid[c], min(step, last), kb, k_block, k_token);
       load_ids(nid[c], min(step + SETS, last));
     };
     auto vals_of = [&](auto S, int step) __attribute__((always_inline)) {  // values: on the pages of those keys
       constexpr int c = decltype(S)::value % SETS;
 #pragma unroll
       for (int i = 0; i < NL; ++i) vid[c][i] = kid[c][i];
-      load(vr[c], vid[c], min(step, last), vb, a.v_block, a.v_token);
+      load(vr[c], vid[c], min(step, last), vb, v_block, v_token);
     };
     auto next_ids = [&](auto S) __attribute__((always_inline)) {
       constexpr int c = decltype(S)::value % SETS;
@@ -366,6 +372,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       }
     }
   }
+  const AttnCall& e = attn_call();
   const bool split = !u.whole;
   const int64_t part = u.part;
   if (wk == 0) {
@@ -375,18 +382,18 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       if (row >= q.rows) continue;
       if (h == 0) sbase[in_tile] = m[b];
       if (split) {
-        float* o = &p.part_o[(part * p.tile_rows + in_tile) * DP];
+        float* o = &e.p.part_o[(((int64_t)part << row_shift) + in_tile) * DP];
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             *(attn_f32x4*)&o[32 * d + 8 * e + 4 * h] =
                 attn_f32x4{acc[b][d][4 * e], acc[b][d][4 * e + 1], acc[b][d][4 * e + 2], acc[b][d][4 * e + 3]};
-        if (h == 0) p.part_ml[part * p.tile_rows + in_tile] = float2{m[b], sum[b]};
+        if (h == 0) e.p.part_ml[((int64_t)part << row_shift) + in_tile] = float2{m[b], sum[b]};
       } else {
-        const int t = attn_token(p, row), hh = row - t * group;
+        const int t = attn_token(e.p, row), hh = row - t * group;
         const float inv = sum[b] == 0.f ? 0.f : 1.f / sum[b];
-        T* o = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + hh) * a.out_head;
+        T* o = (T*)e.a.out + (int64_t)(q.lo + t) * e.a.out_token + (int64_t)(u.head * group + hh) * e.a.out_head;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -397,16 +404,16 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
             for (int i = 0; i < 4; ++i) y[i] = (T)(acc[b][d][4 * e + i] * inv);
             if (at < dim) *(x4*)(o + at) = y;
           }
-        if (a.lse && h == 0)
-          a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + hh] =
+        if (e.a.lse && h == 0)
+          e.a.lse[(int64_t)(q.lo + t) * e.a.q_heads + u.head * group + hh] =
               sum[b] == 0.f ? -INFINITY : (m[b] + log2f(sum[b])) * kLn2;
       }
     }
   }
   __threadfence_block();
   __syncthreads();
-  if (spoison) attn_poison<T, DP>(a, p, u, q, sbad ? begin : max(begin, clear - NT), sbase);
-  attn_report(a, p, u, q, sbad);
+  if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, clear - NT), sbase);
+  attn_report(e.a, e.p, u, q, sbad);
   }
 }
 

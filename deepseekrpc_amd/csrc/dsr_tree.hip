@@ -109,30 +109,31 @@ bool attn_shape_ok(const dsr_tree_attention_args_t& a) {
 template <class T, int DP>
 int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.groups), threads(kAttnThreads);
+  const AttnCall call{a, p};
   switch (p.tile_rows) {
     case 16:
       if constexpr (DP <= 128)
         if (!p.cut) {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 8>), grid, dim3(512), 0, s, a, p);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 8>), grid, dim3(512), 0, s, call);
           break;
         }
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4>), grid, threads, 0, s, a, p);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4>), grid, threads, 0, s, call);
       break;
-    case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, a, p); break;
+    case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, call); break;
     default:
       if constexpr (DP <= 128) {
         if (p.tile_rows == 32)
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 1>), grid, threads, 0, s, a, p);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 1>), grid, threads, 0, s, call);
         else if (p.tile_rows == 64)
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 2>), grid, threads, 0, s, a, p);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 2>), grid, threads, 0, s, call);
         else
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 2, 4>), grid, threads, 0, s, a, p);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 2, 4>), grid, threads, 0, s, call);
       }
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   if (p.cut)
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP>), dim3((unsigned)p.groups - 1, (unsigned)(p.tile_rows / kJoinRows)),
-                       threads, 0, s, a, p);
+                       threads, 0, s, call);
   return launched();
 }
 
