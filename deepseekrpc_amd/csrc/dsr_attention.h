@@ -443,7 +443,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   const T* vb = (const T*)c.v_cache + u.head * c.v_head;
   const int shift = attn_call().p.page_shift, page = c.page;
   const unsigned blocks = c.blocks;
-  const int64_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
+  const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
   const bool masks = c.visible != nullptr;
   bool any_bad = false;
 
@@ -465,10 +465,9 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   auto load_rows = [&](int p0) __attribute__((always_inline)) {
     bad_next = 0;
     auto load = [&](int i, int id, int place) __attribute__((always_inline)) {
-      const int64_t at = (unsigned)id < blocks ? id : 0;
-      place &= page - 1;
-      kr[i] = *(const x8*)(kb + at * k_block + place * k_token + d0);
-      vr[i] = *(const x8*)(vb + at * v_block + place * v_token + d0);
+      const uint32_t at = (unsigned)id < blocks ? id : 0, in = place & (page - 1);
+      kr[i] = *(const x8*)(kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token));
+      vr[i] = *(const x8*)(vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token));
     };
     if (!tiny) {
       const bool outside = (unsigned)id_next >= blocks;
@@ -478,9 +477,9 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
         for (int j = 0; j < 64 / LPR; ++j)
           if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
       if (p0 + kAttnTile <= end) {
-        const int64_t at = outside ? 0 : id_next, place = (p0 + sub) & (page - 1);
-        const T* k = kb + (at * k_block + place * k_token + d0);
-        const T* v = vb + (at * v_block + place * v_token + d0);
+        const uint32_t at = outside ? 0 : id_next, in = (p0 + sub) & (page - 1);
+        const T* k = kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token);
+        const T* v = vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
           kr[i] = *(const x8*)k;

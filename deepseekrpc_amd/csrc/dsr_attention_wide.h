@@ -118,7 +118,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   const T* vb = (const T*)c.v_cache + u.head * c.v_head;
   const int shift = attn_call().p.page_shift, page = c.page;
   const unsigned blocks = c.blocks;
-  const int64_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
+  const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
   const bool masks = c.visible != nullptr;
   bool any_bad = false;
 
@@ -135,45 +135,45 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
     for (int i = 0; i < NL; ++i) id[i] = pages[place_of(step, i) >> shift];
   };
-  auto load = [&](x8* r, const int* id, int step, const T* base, int64_t block, int64_t token)
+  auto load = [&](x8* r, const int* id, int step, const T* base, uint32_t block, uint32_t token)
                   __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = (int)(threadIdx.x + kAttnThreads * i) % CH;
-      const int64_t b = (unsigned)id[i] < blocks ? id[i] : 0;
-      r[i] = *(const x8*)(base + b * block + (place_of(step, i) & (page - 1)) * token + min(8 * c, dim - 8));
+      const uint32_t b = (unsigned)id[i] < blocks ? id[i] : 0, place = place_of(step, i) & (page - 1);
+      r[i] = *(const x8*)(base + min(8 * c, dim - 8) + ((uint64_t)b * block + (uint64_t)place * token));
     }
   };
-  auto store_keys = [&](int buf, const x8* r, const int* id, int step) __attribute__((always_inline)) {
-    bool bad = false;
+  auto store = [&](T* rows, int stride, int buf, const x8* r, bool pad) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int x = (int)threadIdx.x + kAttnThreads * i, c = x % CH;
-      *(x8*)&keys[(buf * NT + x / CH) * KS + 8 * c] = 8 * c < dim ? r[i] : x8{};
-      if ((unsigned)id[i] >= blocks) {
-        bad = true;
-        atomicOr(&sbits[step & 3][x / CH / 32], 1u << (x / CH % 32));
-      }
+      *(x8*)&rows[(buf * NT + x / CH) * stride + 8 * c] = !pad || 8 * c < dim ? r[i] : x8{};
     }
-    any_bad |= bad;
+  };
+  auto outside = [&](const int* id) __attribute__((always_inline)) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) bad |= (unsigned)id[i] >= blocks;
+    return bad;
+  };
+  // Keys on pages outside the cache are noted, a bit each (rare).
+  auto check_keys = [&](const int* id, int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if ((unsigned)id[i] >= blocks) {
+        const int x = ((int)threadIdx.x + kAttnThreads * i) / CH;
+        atomicOr(&sbits[step & 3][x / 32], 1u << (x % 32));
+        any_bad = true;
+      }
   };
   // Values that some row may not see have to be finite to be multiplied by
   // 0: where they are not, 0 takes their place (attn_poison adds them in the end).
-  auto store_vals = [&](int buf, x8* r, const int* id, int step) __attribute__((always_inline)) {
-    bool bad = begin + (step + 1) * NT > clear;
+  auto check_vals = [&](x8* r) __attribute__((always_inline)) {
+    bool poison = false;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) bad |= (unsigned)id[i] >= blocks;
-    if (__ballot(bad)) {
-      bool poison = false;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) poison |= attn_make_finite<T>(r[i]);
-      if (poison) spoison = 1;
-    }
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int x = (int)threadIdx.x + kAttnThreads * i, c = x % CH;
-      *(x8*)&vals[(buf * NT + x / CH) * VS + 8 * c] = r[i];
-    }
+    for (int i = 0; i < NL; ++i) poison |= attn_make_finite<T>(r[i]);
+    if (poison) spoison = 1;
   };
   // Scores of a step's keys.
   auto scores = [&](attn_f32x16* s, int buf) __attribute__((always_inline)) {
@@ -186,10 +186,21 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       for (int b = 0; b < RB; ++b) s[b] = attn_mfma32(key, qv[b][k], s[b]);
     }
   };
-  // What rows may not see becomes -inf; then the running maximum.
-  auto settle = [&](attn_f32x16* s, int step) __attribute__((always_inline)) {
+  // The largest of a lane's row among a step's scores.
+  auto largest = [&](attn_f32x16* s, float* top) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float x = s[b][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) x = fmaxf(x, s[b][e]);
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      const u32x2 y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      top[b] = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    }
+  };
+  // What rows may not see becomes -inf (rare); then the running maximum.
+  auto settle = [&](attn_f32x16* s, float* top, int step, uint32_t bad) __attribute__((always_inline)) {
     const int p0 = begin + step * NT + 32 * wk;
-    const uint32_t bad = sbits[step & 3][wk];
     if (p0 + kAttnTile > clear || bad) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
@@ -197,23 +208,19 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[b][e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? s[b][e] : -INFINITY;
       }
+      largest(s, top);
     }
     bool raise = false;
-    float next[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      float top = s[b][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[b][e]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * scale - AttnType<T>::kLift;
-      raise |= top > m[b] + 8.f;
-      next[b] = fmaxf(m[b], top);
+      top[b] = __builtin_fmaf(top[b], scale, -AttnType<T>::kLift);
+      raise |= top[b] > m[b] + 8.f;
     }
     if (__ballot(raise)) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const float f = m[b] == next[b] ? 1.f : __builtin_amdgcn_exp2f(m[b] - next[b]);
-        m[b] = next[b];
+        const float next = fmaxf(m[b], top[b]), f = m[b] == next ? 1.f : __builtin_amdgcn_exp2f(m[b] - next);
+        m[b] = next;
         sum[b] *= f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[b][d] *= f;
@@ -284,41 +291,57 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       vals_of(odd, 1);
     }
     __syncthreads();  // the flags
-    store_keys(0, kr[0], kid[0], 0);
-    store_vals(0, vr[0], vid[0], 0);
+    if (__ballot(outside(kid[0]))) check_keys(kid[0], 0);
+    if (begin + NT > clear || __ballot(outside(vid[0]))) check_vals(vr[0]);
+    store(keys, KS, 0, kr[0], true);
+    store(vals, VS, 0, vr[0], false);
     next_ids(even);
     if constexpr (SETS == 2) {
       keys_of(even, 2);
       vals_of(even, 2);
-      store_keys(1, kr[1], kid[1], 1);
+      if (__ballot(outside(kid[1]))) check_keys(kid[1], 1);
+      store(keys, KS, 1, kr[1], true);
       next_ids(odd);
       keys_of(odd, 3);
     } else {
       keys_of(even, 1);
       vals_of(even, 1);
-      store_keys(1, kr[0], kid[0], 1);
+      if (__ballot(outside(kid[0]))) check_keys(kid[0], 1);
+      store(keys, KS, 1, kr[0], true);
       next_ids(even);
       keys_of(even, 2);
     }
     __syncthreads();
+    float top[RB];
     scores(sc[0], 0);
-    settle(sc[0], 0);
+    largest(sc[0], top);
+    settle(sc[0], top, 0, sbits[0][wk]);
     __syncthreads();  // keys 0 are read
     auto step = [&](auto S, int t) __attribute__((always_inline)) {
       constexpr int c = decltype(S)::value;  // t % 2
       constexpr std::integral_constant<int, c> now{};
       constexpr std::integral_constant<int, c ^ 1> next{};
-      if (threadIdx.x < WK) sbits[(t + 3) & 3][threadIdx.x] = 0;  // last read two steps ago
-      store_keys(c, kr[c % SETS], kid[c % SETS], t + 2);
-      store_vals(c ^ 1, vr[(c ^ 1) % SETS], vid[(c ^ 1) % SETS], t + 1);
+      constexpr int kc = c % SETS, vc = (c ^ 1) % SETS;
+      const bool odd = outside(kid[kc]) || outside(vid[vc]);
+      if (begin + (t + 2) * NT > clear || __ballot(odd)) {
+        check_keys(kid[kc], t + 2);
+        check_vals(vr[vc]);
+      }
+      // From here on no branch: the compiler places the products among the
+      // vector instructions that do not wait for them.
+      sbits[(t + 3) & 3][threadIdx.x & (WK - 1)] = 0;  // last read two steps ago
+      store(keys, KS, c, kr[kc], true);
+      store(vals, VS, c ^ 1, vr[vc], false);
       vals_of(next, t + 1 + SETS);
       next_ids(now);
       keys_of(now, t + 2 + SETS);
+      const uint32_t bad = sbits[(t + 1) & 3][wk];
       x8 pv[RB][2];
-      weigh(sc[c], pv);
       scores(sc[c ^ 1], c ^ 1);
+      weigh(sc[c], pv);
       weighted(pv, c);
-      settle(sc[c ^ 1], t + 1);
+      largest(sc[c ^ 1], top);
+      settle(sc[c ^ 1], top, t + 1, bad);
       __syncthreads();
     };
     // An odd count's last step lies past the end, where no row sees anything.

@@ -227,7 +227,9 @@ int32_t dsr_tree_attention(const dsr_tree_attention_args_t* args, void* stream) 
   if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return DSR_ERR_ARG;
   for (int64_t st : {a.q_token, a.q_head, a.out_token, a.out_head, a.k_block, a.k_token, a.k_head, a.v_block,
                      a.v_token, a.v_head})
-    if (st % 8 != 0) return DSR_ERR_ARG;
+    if (st % 8 != 0 || st < 0) return DSR_ERR_ARG;
+  for (int64_t st : {a.k_block, a.k_token, a.v_block, a.v_token})
+    if (st > INT_MAX) return DSR_ERR_ARG;  // multiplied in 32 x 32 bits
   AttnPlan p = attn_plan(a);
   const AttnSizes z = attn_sizes(a, p);
   if (!a.workspace || ((uintptr_t)a.workspace & 255u) || a.workspace_bytes < (size_t)z.all) return DSR_ERR_WORKSPACE;

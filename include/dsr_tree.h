@@ -172,9 +172,9 @@ typedef struct dsr_tree_attention_args {
   int64_t requests;            /* 0 .. DSR_TREE_MAX_REQUESTS */
   int64_t tokens;              /* rows of q and out */
   int64_t table_ld;
-  int64_t q_token, q_head;     /* strides: multiples of 8; rows 16-byte aligned */
+  int64_t q_token, q_head;     /* strides: >= 0, multiples of 8; rows 16-byte aligned */
   int64_t out_token, out_head;
-  int64_t k_block, k_token, k_head;
+  int64_t k_block, k_token, k_head;  /* of pages and tokens less than 2^31 */
   int64_t v_block, v_token, v_head;
   void* workspace;             /* >= dsr_tree_attention_workspace_bytes(args), 256-byte aligned */
   size_t workspace_bytes;
