@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
   constexpr int CH = DP / 8;                          // 16-byte chunks of a row
   constexpr int NL = NT * CH / kAttnThreads;          // chunks a thread stages per step, of keys and of values
   static_assert(NT * CH % kAttnThreads == 0, "every thread stages as much");
-  constexpr int SETS = NL <= 2 ? 2 : 1;               // steps in flight in registers: 16 KB or more per workgroup
+  constexpr int SETS = NL <= 2 && RB == 1 ? 2 : 1;               // steps in flight in registers: 16 KB or more per workgroup
   __shared__ __align__(16) char attn_lds[(Sh::kKeys + Sh::kVals) * sizeof(T)];
   T* keys = (T*)attn_lds;             // [2][NT][KS]
   T* vals = keys + Sh::kKeys;         // [2][NT][VS]
