@@ -177,10 +177,15 @@ struct AttnWork {
       steps = hold(a, p, first);
       upto = attn_wave_scan(steps);
       total += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+      // Requests without rows have no work: the first workgroup tells their status.
+      const int l = threadIdx.x & 63;
+      if (blockIdx.x == 0 && border == 0 && threadIdx.x < 64 && first + l < R && mine.rows == 0)
+        a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
     }
-    quota = (total + p.groups - 1) / (uint32_t)p.groups;
+    // Most calls of one step per tile have a workgroup for each: no division then.
+    quota = total <= (uint32_t)p.groups ? 1 : (total + p.groups - 1) / (uint32_t)p.groups;
     if (quota < (uint32_t)p.min_steps) quota = p.min_steps;
-    const uint32_t each = (total + 8 * quota - 1) / (8 * quota);  // workgroups with work, per XCD
+    const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
       me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
       at = (blockIdx.x >> 3) < each ? me * quota : total;
@@ -232,10 +237,10 @@ struct AttnWork {
       base += length;
       ++r;
     }
-    const uint32_t unit = (at - base) / steps, s0 = at - base - unit * steps;
+    const uint32_t unit = steps == 1 ? at - base : (at - base) / steps, s0 = at - base - unit * steps;
     const uint32_t s1 = stop - at < steps - s0 ? s0 + stop - at : steps;
     s.r = r;
-    s.head = unit / (uint32_t)q.tiles;
+    s.head = q.tiles == 1 ? unit : unit / (uint32_t)q.tiles;
     s.tile = unit - (uint32_t)s.head * q.tiles;
     s.begin = s0 * p.tokens;
     s.end = s1 == steps ? q.kv : s1 * p.tokens;
@@ -251,15 +256,6 @@ struct AttnWork {
     return true;
   }
 };
-
-// Requests without rows have no work: their status, by the launch's first workgroup.
-__device__ __forceinline__ void attn_idle(const dsr_tree_attention_args_t& a, const AttnPlan& p, int threads) {
-  if (blockIdx.x != 0) return;
-  for (int r = threadIdx.x; r < a.requests; r += threads) {
-    const AttnRequest q = attn_request(a, p, r);
-    if (q.rows == 0) a.status[r] = q.fine ? DSR_OK : DSR_E_LENGTH;
-  }
-}
 
 // v with 0 in the place of infinities and NaN; whether there were any.
 template <class T>
@@ -392,7 +388,6 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  attn_idle(attn_call().a, attn_call().p, kThreads);
   AttnWork<DP <= 128> work(attn_call().a, attn_call().p, 0);
   AttnSegment u;
   AttnRequest q;
@@ -404,29 +399,6 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   if (threadIdx.x == 0) sbad = spoison = 0;
   const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
   const int row0 = u.tile << row_shift;
-
-  // This lane's rows: token index, mask, query operand.  A negative scale
-  // changes the queries' sign, so that scores only grow with their products;
-  // scale 0 is queries of 0.
-  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-  x8 qv[NB][KS];
-  int tok[NB];
-  uint64_t mask[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int row = row0 + 16 * b + n;
-    const bool in = row < q.rows;
-    const int t = in ? attn_token(p, row) : 0, h = in ? row - t * group : 0;
-    tok[b] = t;
-    mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
-    const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + h) * a.q_head;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = 32 * s + 8 * g;
-      const x8 v = in && d < dim && a.scale != 0.f ? *(const x8*)(src + d) : x8{};
-      qv[b][s] = a.scale < 0.f ? -v : v;
-    }
-  }
 
   attn_f32x4 acc[NB][DB];
   float m[NB], sum[NB];
@@ -507,6 +479,28 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     load_id(first);
     load_rows(first);
     load_id(first + step);
+  }
+  // This lane's rows: token index, mask, query operand.  A negative scale
+  // changes the queries' sign, so that scores only grow with their products;
+  // scale 0 is queries of 0.
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+  x8 qv[NB][KS];
+  int tok[NB];
+  uint64_t mask[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int row = row0 + 16 * b + n;
+    const bool in = row < q.rows;
+    const int t = in ? attn_token(p, row) : 0, h = in ? row - t * group : 0;
+    tok[b] = t;
+    mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
+    const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + h) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 32 * s + 8 * g;
+      const x8 v = in && d < dim && a.scale != 0.f ? *(const x8*)(src + d) : x8{};
+      qv[b][s] = a.scale < 0.f ? -v : v;
+    }
   }
   __syncthreads();  // the flags
   for (int p0 = first; p0 < end; p0 += step) {
@@ -602,10 +596,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   for (int b = 0; b < NB; ++b) {
     sum[b] += __shfl_xor(sum[b], 16);
     sum[b] += __shfl_xor(sum[b], 32);
-    if (g == 0) {
-      sm[w][16 * b + n] = m[b];
-      sl[w][16 * b + n] = sum[b];
-    }
+    if (g == 0) sm[w][16 * b + n] = m[b];
   }
   if (any_bad && l == 0) sbad = 1;
   __syncthreads();
@@ -620,23 +611,22 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) top = fmaxf(top, sm[i][16 * b + n]);
     const float f = m[b] == top ? 1.f : __builtin_amdgcn_exp2f(m[b] - top);  // a wave without tokens: 0
+    if (g == 0) sl[w][16 * b + n] = sum[b] * f;
+    if (w == 0 && g == 0) sbase[16 * b + n] = top;
     float* mine = (float*)&vals[w][0][0];
 #pragma unroll
     for (int d = 0; d < DB; ++d) *(attn_f32x4*)&mine[n * OS + 16 * d + 4 * g] = acc[b][d] * f;
     __syncthreads();
     for (int x = threadIdx.x; x < 16 * (DP / 4); x += kThreads) {
       const int row = x / (DP / 4), d = x % (DP / 4) * 4, rr = 16 * b + row;
-      float M = sm[0][rr];
-#pragma unroll
-      for (int i = 1; i < WAVES; ++i) M = fmaxf(M, sm[i][rr]);
+      const float M = sbase[rr];
       float L = 0.f;
       attn_f32x4 o = {};
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) {
-        L += sl[i][rr] * (sm[i][rr] == M ? 1.f : __builtin_amdgcn_exp2f(sm[i][rr] - M));
+        L += sl[i][rr];
         o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
       }
-      if (d == 0) sbase[rr] = M;
       if (split) {
         *(attn_f32x4*)&e.p.part_o[(((int64_t)part << row_shift) + rr) * DP + d] = o;
         if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + rr] = float2{M, L};

@@ -65,7 +65,6 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  attn_idle(attn_call().a, attn_call().p, kAttnThreads);
   AttnWork<false> work(attn_call().a, attn_call().p, 0);
   AttnSegment u;
   AttnRequest q;
