@@ -56,7 +56,7 @@ int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
 // Dimensions of the kernel that takes a head dimension.
 int attn_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
-constexpr int kAttnShort = 1024;  // tokens, a multiple of every kernel's step
+constexpr int kAttnShort = 256, kAttnMany = 1024;  // tokens, powers of two from every kernel's step on
 
 // Host part of the work split, from sizes alone.
 AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
@@ -69,19 +69,23 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   p.groups = p.tile_rows == 256 || p.tile_rows == 32 || big ? 256 : 512;
   // Causal tiles have unlike lengths: several workgroups for each place even them out.
   if (!a.visible && a.tokens > 64 * a.requests) p.groups *= 4;
-  p.min_steps = p.tile_rows == 16 ? 2 : 8;
   p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
-  // Where a whole table row is a short way for one workgroup, a tile is one
-  // step: nothing is cut, and no joining launch follows.
-  p.cut = (int64_t)a.width * a.page > kAttnShort;
-  if (!p.cut) p.tokens = kAttnShort, p.min_steps = 1;
+  p.min_steps = 128 / p.tokens;
+  // Where a whole table row is a short way for one workgroup, or a longer
+  // one and there is a tile for every CU, a tile is one step: nothing is
+  // cut, and no joining launch follows.
   const int64_t tiles = (a.tokens * group / p.tile_rows + a.requests) * a.kv_heads;
+  const int64_t span = (int64_t)a.width * a.page;
+  p.cut = span > (tiles >= 256 ? kAttnMany : kAttnShort);
+  if (!p.cut) p.tokens = kAttnMany, p.min_steps = 1;
   while (((int64_t)a.width * a.page / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
   auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
   p.group = (int)group;
   p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
   p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
-  if (!p.cut && tiles < p.groups) p.groups = (int)((tiles + 7) / 8 * 8);
+  // No more workgroups than shares of the fewest steps.
+  const int64_t shares = tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;
+  if (shares < p.groups) p.groups = (int)((shares + 7) / 8 * 8);
   return p;
 }
 
