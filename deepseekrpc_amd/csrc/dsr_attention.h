@@ -649,14 +649,18 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   }
 }
 
-constexpr int kJoinRows = 16;  // rows of a tile per workgroup (blockIdx.y)
-
-// Joins the parts of the tiles that borders between shares cut, in the order
-// of the tokens: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
-// Workgroup x takes the tile whose first border is the one before share x + 1.
-template <class T, int DP>
+// Joins the parts of the tiles that borders between shares cut:
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  Workgroup (x, y) takes
+// rows JR y .. of the tile whose first border is the one before share x + 1.
+// Few rows leave threads over: these take every SLOTS-th part each (a single
+// long request has a part for each of 64 shares), summed in a fixed order.
+template <class T, int DP, int JR>
 __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   typedef typename AttnType<T>::x4 x4;
+  constexpr int E = JR * DP / 4;  // four dimensions of a row each
+  constexpr int SLOTS = E < kAttnThreads ? kAttnThreads / E : 1;
+  __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
+  __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const int border = blockIdx.x + 1;
   AttnWork<false> work(attn_call().a, attn_call().p, border);
   AttnSegment u;
@@ -667,33 +671,52 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   if (first != border - 1) return;
   const dsr_tree_attention_args_t& a = attn_call().a;
   const AttnPlan& p = attn_call().p;
-  const int group = p.group, row0 = u.tile * p.tile_rows;
-  const int rows = min((int)blockIdx.y * kJoinRows + kJoinRows, min(p.tile_rows, q.rows - row0));
-  // The first part is its workgroup's last (an odd place), the others their workgroups' first.
-  for (int x = blockIdx.y * kJoinRows * (DP / 4) + threadIdx.x; x < rows * (DP / 4); x += kAttnThreads) {
-    const int row = x / (DP / 4), d = x % (DP / 4) * 4;
-    // The maximum first, so that the parts' loads do not wait for each other.
-    auto part = [&](int c) { return (int64_t)(2 * c + (c == first)) * p.tile_rows + row; };
+  const int row0 = u.tile << p.tile_shift, slot = SLOTS > 1 ? threadIdx.x / E : 0;
+  const bool spare = slot >= SLOTS;  // 192 dimensions: 64 threads
+  const int rows = min(p.tile_rows, q.rows - row0);
+  if ((int)blockIdx.y * JR >= rows) return;
+  for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
+    const int in = x / (DP / 4), row = blockIdx.y * JR + in, d = x % (DP / 4) * 4;
+    // The first part is its workgroup's last (an odd place), the others their workgroups' first.
+    auto part = [&](int c) { return ((int64_t)(2 * c + (c == first)) << p.tile_shift) + row; };
+    // The base first, so that the parts' loads do not wait for each other.
     float M = -INFINITY, L = 0.f;
     attn_f32x4 o = {};
 #pragma unroll 4
-    for (int c = first; c <= last; ++c) M = fmaxf(M, p.part_ml[part(c)].x);
+    for (int c = spare ? last + 1 : first + slot; c <= last; c += SLOTS) M = fmaxf(M, p.part_ml[part(c)].x);
+    if constexpr (SLOTS > 1) {
+      if (d == 0 && !spare) sm[slot][in] = M;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) M = fmaxf(M, sm[i][in]);
+    }
 #pragma unroll 4
-    for (int c = first; c <= last; ++c) {
+    for (int c = spare ? last + 1 : first + slot; c <= last; c += SLOTS) {
       const float2 ml = p.part_ml[part(c)];
       const float f = ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
       L += ml.y * f;
       o += *(const attn_f32x4*)&p.part_o[part(c) * DP + d] * f;
     }
-    if (d >= a.head_dim) continue;
-    const int t = attn_token(p, row0 + row), h = row0 + row - t * group;
+    if constexpr (SLOTS > 1) {
+      if (!spare) so[slot][x] = o;
+      if (d == 0 && !spare) sl[slot][in] = L;
+      __syncthreads();
+      if (slot > 0) break;
+#pragma unroll
+      for (int i = 1; i < SLOTS; ++i) o += so[i][x];
+      L = 0.f;
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) L += sl[i][in];
+    }
+    if (row >= rows || d >= a.head_dim) continue;
+    const int t = attn_token(p, row0 + row), h = row0 + row - t * p.group;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     x4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
-    *(x4*)((T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * group + h) * a.out_head + d) = y;
+    *(x4*)((T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)(u.head * p.group + h) * a.out_head + d) = y;
     if (a.lse && d == 0)
-      a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+      a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * p.group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   }
   if (u.head == 0 && u.tile == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     int bad = 0;

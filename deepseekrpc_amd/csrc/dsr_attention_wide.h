@@ -102,7 +102,8 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
     }
   }
 
-  attn_f32x16 acc[RB][DB], sc[2][RB];
+  constexpr int SB = RB == 1 ? 2 : 1;  // scores of two steps, or of one where registers are short
+  attn_f32x16 acc[RB][DB], sc[SB][RB];
   float m[RB], sum[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -336,11 +337,12 @@ __global__ __launch_bounds__(kAttnThreads, RB == 1 && DP <= 128 ? 2 : 1) void k_
       keys_of(now, t + 2 + SETS);
       const uint32_t bad = sbits[(t + 1) & 3][wk];
       x8 pv[RB][2];
-      scores(sc[c ^ 1], c ^ 1);
-      weigh(sc[c], pv);
+      constexpr int s0 = c % SB, s1 = (c ^ 1) % SB;
+      weigh(sc[s0], pv);
+      scores(sc[s1], c ^ 1);
       weighted(pv, c);
-      largest(sc[c ^ 1], top);
-      settle(sc[c ^ 1], top, t + 1, bad);
+      largest(sc[s1], top);
+      settle(sc[s1], top, t + 1, bad);
       __syncthreads();
     };
     // An odd count's last step lies past the end, where no row sees anything.

@@ -135,9 +135,14 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
       }
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
-  if (p.cut)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP>), dim3((unsigned)p.groups - 1, (unsigned)(p.tile_rows / kJoinRows)),
-                       threads, 0, s, call);
+  if (p.cut && p.groups > 1) {
+    const unsigned borders = (unsigned)p.groups - 1;
+    if (p.tile_rows == 16)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 2>), dim3(borders, 8), threads, 0, s, call);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 16>), dim3(borders, (unsigned)(p.tile_rows / 16)), threads, 0,
+                         s, call);
+  }
   return launched();
 }
 

@@ -53,13 +53,20 @@ def test_matches_float64(new, ctx, heads, kv, dim, page, dtype, trees, by_head):
     assert not res.status.any()
 
 
-@pytest.mark.parametrize("heads,kv,dim,n", [(8, 1, 128, 1), (16, 4, 64, 4), (8, 1, 128, 40), (4, 2, 256, 9)])
+@pytest.mark.parametrize("heads,kv,dim,n", [(8, 1, 128, 1), (16, 4, 64, 4), (8, 1, 128, 40), (4, 2, 256, 9),
+                                             (4, 2, 192, 3), (6, 2, 96, 2), (4, 1, 192, 30)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_long_contexts_are_split_and_joined(heads, kv, dim, n, dtype):
     """Contexts that many workgroups share, next to ones that one takes alone."""
     rng = np.random.default_rng([heads, dim, n])
     ctx = [9000, 3, 2500, 0]
     check(Step(rng, [n, n, 1, n], ctx, heads, kv, dim, 16, dtype, trees=True), dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+def test_one_long_request_has_many_parts(dim):
+    rng = np.random.default_rng(dim)
+    check(Step(rng, [1], [20_011], 4, 2, dim, 16, "bf16"), "bf16")
 
 
 def test_many_requests():
