@@ -64,9 +64,9 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   const int64_t group = a.q_heads / a.kv_heads;
   const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
   const bool big = a.head_dim > 128;
-  p.tile_rows = rows <= 16 || (big && rows <= 32) ? 16 : rows <= 32 ? 32 : rows <= 64 && !big ? 64 : rows <= 128 || big ? 128 : 256;
+  p.tile_rows = rows <= 16 || (big && rows <= 32) ? 16 : rows <= 32 ? 32 : rows <= 64 && !big ? 64 : 128;
   // As many workgroups as the chip holds at once (256 CUs, one or two each).
-  p.groups = p.tile_rows == 256 || p.tile_rows == 32 || big ? 256 : 512;
+  p.groups = p.tile_rows == 32 || big ? 256 : 512;
   // Causal tiles have unlike lengths: several workgroups for each place even them out.
   if (!a.visible && a.tokens > 64 * a.requests) p.groups *= 4;
   p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
@@ -110,6 +110,18 @@ bool attn_shape_ok(const dsr_tree_attention_args_t& a) {
          a.tokens * a.q_heads <= INT_MAX / 2;
 }
 
+template <class T, int DP, int WR>
+void attn_wide(dim3 grid, hipStream_t s, const AttnCall& call) {
+  const dsr_tree_attention_args_t& a = call.a;
+  // A round's tokens on one page, and their offsets in 32 bits.
+  constexpr bool whole = kAttnThreads % (DP / 8) == 0;
+  const bool flat = whole && a.page >= attn_round(DP) && a.k_token <= 1 << 24 && a.v_token <= 1 << 24;
+  if (flat)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, WR, whole>), grid, dim3(kAttnThreads), 0, s, call);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, WR, false>), grid, dim3(kAttnThreads), 0, s, call);
+}
+
 template <class T, int DP>
 int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.groups), threads(kAttnThreads);
@@ -123,16 +135,9 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
         }
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4>), grid, threads, 0, s, call);
       break;
-    case 128: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 4>), grid, threads, 0, s, call); break;
-    default:
-      if constexpr (DP <= 128) {
-        if (p.tile_rows == 32)
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 1>), grid, threads, 0, s, call);
-        else if (p.tile_rows == 64)
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 1, 2>), grid, threads, 0, s, call);
-        else
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, 2, 4>), grid, threads, 0, s, call);
-      }
+    case 128: attn_wide<T, DP, 4>(grid, s, call); break;
+    case 64: if constexpr (DP <= 128) attn_wide<T, DP, 2>(grid, s, call); break;
+    default: if constexpr (DP <= 128) attn_wide<T, DP, 1>(grid, s, call);
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   if (p.cut && p.groups > 1) {
