@@ -32,13 +32,14 @@ constexpr int attn_round(int DP) { return kAttnThreads / (DP / 8); }
 // One step of the loop multiplies tile t + 1's keys and tile t's values: the
 // products of the one do not wait for the exponentials of the other, and a
 // wave's vector instructions go on while the matrix cores work.  Keys and
-// values pass from memory through registers (SETS steps in flight) into LDS.
+// values pass from memory through registers into LDS.
 //
 // What bounds a step: the instructions a SIMD has to issue for its two waves
 // (a 32 x 32 x 16 product takes 16 of the issue cycles and 32 of the matrix
 // core's, an exponential 13, others 4), not the products themselves.  64 rows
 // a wave, with half the LDS reads a row, came out no faster (8 trees of 64
-// nodes over 32,065 tokens: 710 us against 706) and wasted more on ragged rows.
+// nodes over 32,065 tokens: 710 us against 706 then) and wasted more on ragged
+// rows.
 //
 // FLAT: a page holds every token of a round of loads, so that a round's page
 // id and address are the same for the workgroup and a lane adds one offset.
@@ -55,7 +56,6 @@ __global__ __launch_bounds__(kAttnThreads, DP <= 128 ? 2 : 1) void k_tree_attent
   constexpr int DB = DP / 32;                         // 32-wide output blocks
   constexpr int CH = DP / 8;                          // 16-byte chunks of a row
   constexpr int NL = NT * CH / kAttnThreads;          // chunks a thread stages per step, of keys and of values
-  constexpr int SETS = NL <= 2 ? 2 : 1;               // steps in flight in registers: 16 KB or more per workgroup
   static_assert(NT * CH % kAttnThreads == 0, "every thread stages as much");
   static_assert(!FLAT || kAttnThreads % CH == 0, "a round is a whole number of tokens");
   constexpr int kKeys = 2 * NT * KS, kVals = 2 * NT * VS;  // elements, double-buffered
@@ -120,8 +120,8 @@ __global__ __launch_bounds__(kAttnThreads, DP <= 128 ? 2 : 1) void k_tree_attent
     // of a step's NT.  Steps past the last read the last one again and are
     // never used.  Places past the last token read that token, or, FLAT, what
     // lies behind it in the page: their scores are masked either way.
-    x8 kr[SETS][NL], vr[SETS][NL];
-    int kid[SETS][NL], vid[SETS][NL], nid[SETS][NL];  // page ids: of the keys and values in registers, of the next keys
+    x8 kr[NL], vr[NL];
+    int kid[NL], vid[NL], nid[NL];  // page ids: of the keys and values in registers, of the next keys
     const uint32_t my_token = threadIdx.x / CH, my_dim = min(8 * (int)(threadIdx.x % CH), dim - 8);
     const uint32_t k_lane = (my_token * k_token + my_dim) * sizeof(T), v_lane = (my_token * v_token + my_dim) * sizeof(T);
     auto place_of = [&](int step, int i) __attribute__((always_inline)) {
@@ -242,82 +242,54 @@ __global__ __launch_bounds__(kAttnThreads, DP <= 128 ? 2 : 1) void k_tree_attent
     };
 
     if (steps > 0) {
-      // Step t finds keys t + 1 and values t in LDS and keys t + 2 .. t + 1 +
-      // SETS and values t + 1 .. t + SETS on their way to registers.  Page
-      // ids are read a step ahead of their rows, and before that step's rows:
-      // waiting for them then leaves the rows in flight.
+      // Step t finds keys t + 1 and values t in LDS and keys t + 2 and values
+      // t + 1 on their way to registers.  Page ids are read a step ahead of
+      // their rows, and before that step's rows: waiting for them then leaves
+      // the rows in flight.
       const int last = steps - 1;
-      auto keys_of = [&](auto S, int step) __attribute__((always_inline)) {  // registers of keys `step`, ids ahead
-        constexpr int c = decltype(S)::value % SETS;
-        load_ids(nid[c], min(step + SETS, last));
-        load(kr[c], kid[c], min(step, last), kb, k_block, k_token, k_lane);
+      auto keys_of = [&](int step) __attribute__((always_inline)) {  // keys, and the ids of the next
+        load_ids(nid, min(step + 1, last));
+        load(kr, kid, min(step, last), kb, k_block, k_token, k_lane);
       };
-      auto vals_of = [&](auto S, int step) __attribute__((always_inline)) {  // values: on the pages of those keys
-        constexpr int c = decltype(S)::value % SETS;
+      auto vals_of = [&](int step) __attribute__((always_inline)) {  // values: on the pages of those keys
 #pragma unroll
-        for (int i = 0; i < NL; ++i) vid[c][i] = kid[c][i];
-        load(vr[c], vid[c], min(step, last), vb, v_block, v_token, v_lane);
+        for (int i = 0; i < NL; ++i) vid[i] = kid[i];
+        load(vr, vid, min(step, last), vb, v_block, v_token, v_lane);
       };
-      auto next_ids = [&](auto S) __attribute__((always_inline)) {
-        constexpr int c = decltype(S)::value % SETS;
+      auto next_ids = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) kid[c][i] = FLAT ? __builtin_amdgcn_readfirstlane(nid[c][i]) : nid[c][i];
+        for (int i = 0; i < NL; ++i) kid[i] = FLAT ? __builtin_amdgcn_readfirstlane(nid[i]) : nid[i];
       };
-      constexpr std::integral_constant<int, 0> even{};
-      constexpr std::integral_constant<int, 1> odd{};
-      load_ids(nid[0], 0);
-      if constexpr (SETS == 2) load_ids(nid[1], min(1, last));
-      next_ids(even);
-      keys_of(even, 0);
-      vals_of(even, 0);
-      if constexpr (SETS == 2) {
-        next_ids(odd);
-        keys_of(odd, 1);
-        vals_of(odd, 1);
-      }
+      load_ids(nid, 0);
+      next_ids();
+      keys_of(0);
+      vals_of(0);
       __syncthreads();  // the flags
-      if (outside(kid[0])) check_keys(kid[0], 0);
-      if (begin + NT > clear || outside(vid[0])) check_vals(vr[0], 0);
-      store(keys, KS, 0, kr[0], true);
-      store(vals, VS, 0, vr[0], false);
-      next_ids(even);
-      if constexpr (SETS == 2) {
-        keys_of(even, 2);
-        vals_of(even, 2);
-        if (outside(kid[1])) check_keys(kid[1], 1);
-        store(keys, KS, 1, kr[1], true);
-        next_ids(odd);
-        keys_of(odd, 3);
-      } else {
-        keys_of(even, 1);
-        vals_of(even, 1);
-        if (outside(kid[0])) check_keys(kid[0], 1);
-        store(keys, KS, 1, kr[0], true);
-        next_ids(even);
-        keys_of(even, 2);
-      }
+      if (outside(kid)) check_keys(kid, 0);
+      if (begin + NT > clear || outside(vid)) check_vals(vr, 0);
+      store(keys, KS, 0, kr, true);
+      store(vals, VS, 0, vr, false);
+      next_ids();
+      keys_of(1);
+      vals_of(1);
+      if (outside(kid)) check_keys(kid, 1);
+      store(keys, KS, 1, kr, true);
+      next_ids();
+      keys_of(2);
       __syncthreads();
       scores(sc[0], 0);
       largest(sc[0]);
       settle(sc[0], 0, sbits[0][wk]);
       __syncthreads();  // keys 0 are read
-      auto step = [&](auto S, int t) __attribute__((always_inline)) {
-        constexpr int c = decltype(S)::value;  // t % 2
-        constexpr std::integral_constant<int, c> now{};
-        constexpr std::integral_constant<int, c ^ 1> next{};
-        constexpr int kc = c % SETS, vc = (c ^ 1) % SETS;
-        if (begin + (t + 2) * NT > clear || outside(kid[kc]) || outside(vid[vc])) {
-          check_keys(kid[kc], t + 2);
-          check_vals(vr[vc], t + 1);
+      auto step = [&](auto C, int t) __attribute__((always_inline)) {
+        constexpr int c = decltype(C)::value;  // t % 2
+        if (begin + (t + 2) * NT > clear || outside(kid) || outside(vid)) {
+          check_keys(kid, t + 2);
+          check_vals(vr, t + 1);
         }
         // From here on no branch: the compiler places the products among the
         // vector instructions that do not wait for them.
         sbits[(t + 3) & 3][threadIdx.x & (WK - 1)] = 0;  // last read two steps ago
-        store(keys, KS, c, kr[kc], true);
-        store(vals, VS, c ^ 1, vr[vc], false);
-        vals_of(next, t + 1 + SETS);
-        next_ids(now);
-        keys_of(now, t + 2 + SETS);
         const uint32_t bad = sbits[(t + 1) & 3][wk];
         x8 pv[2];
         weigh(sc[c], pv);
@@ -325,8 +297,18 @@ __global__ __launch_bounds__(kAttnThreads, DP <= 128 ? 2 : 1) void k_tree_attent
         weighted(pv, c);
         largest(sc[c ^ 1]);
         settle(sc[c ^ 1], t + 1, bad);
+        // The rows in flight are waited for only now, behind the products.
+        // (Stored before the products, with two steps of them in registers:
+        // 706 us on 8 trees of 64 nodes over 32,065 tokens, so 682.)
+        store(keys, KS, c, kr, true);
+        store(vals, VS, c ^ 1, vr, false);
+        vals_of(t + 2);
+        next_ids();
+        keys_of(t + 3);
         __syncthreads();
       };
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
       // An odd count's last step lies past the end, where no row sees anything.
       for (int t = 0; t < steps; t += 2) {
         step(even, t);
