@@ -324,13 +324,14 @@ __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, 
 }
 
 // What a segment says of its page ids: the request's status, or its part's
-// (its first tile and head speak for all: every tile sees the same pages).
+// (its last tile of its first head speaks for all: causal tiles see all of the
+// pages that the ones before them see).
 __device__ __forceinline__ void attn_report(const dsr_tree_attention_args_t& a, const AttnPlan& p,
                                             const AttnSegment& u, const AttnRequest& q, int bad) {
   if (threadIdx.x != 0) return;
   if (!u.whole)
     p.part_bad[u.part] = bad;
-  else if (u.head == 0 && u.tile == 0)
+  else if (u.head == 0 && u.tile == q.tiles - 1)
     a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
 }
 
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
     if (a.lse && d == 0)
       a.lse[(int64_t)(q.lo + t) * a.q_heads + u.head * p.group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   }
-  if (u.head == 0 && u.tile == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+  if (u.head == 0 && u.tile == q.tiles - 1 && blockIdx.y == 0 && threadIdx.x == 0) {
     int bad = 0;
     for (int c = first; c <= last; ++c) bad |= p.part_bad[2 * c + (c == first)];
     a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;

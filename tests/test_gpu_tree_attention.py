@@ -202,6 +202,16 @@ def test_bad_lengths_and_pages():
     assert res.status.tolist() == [O.E_LENGTH] and not res.out.any()
 
 
+@pytest.mark.parametrize("new,ctx", [(150, 0), (200, 1500)])
+def test_bad_page_that_only_a_chunks_last_rows_see(new, ctx):
+    """Causal rows are tiled, and the first tiles end before the last page."""
+    step = Step(np.random.default_rng(new), [new, 7], [ctx, 90], 8, 2, 64, 16, "bf16")
+    step.table[0, (ctx + new - 1) // 16] = step.k.shape[0]
+    args, vis = step.args()
+    res = tree.tree_attention(*args, visible=vis, scale=0.125)
+    assert res.status.tolist() == [O.E_BLOCK, 0]
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^31 elements whose used pages lie at its end."""
     rng = np.random.default_rng(31)
