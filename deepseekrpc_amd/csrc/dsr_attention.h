@@ -242,6 +242,7 @@ struct AttnWork {
     s.r = r;
     s.head = q.tiles == 1 ? unit : unit / (uint32_t)q.tiles;
     s.tile = unit - (uint32_t)s.head * q.tiles;
+    if (!p.cut && !a.visible) s.tile = q.tiles - 1 - s.tile;  // a chunk's longest tiles first
     s.begin = s0 * p.tokens;
     s.end = s1 == steps ? q.kv : s1 * p.tokens;
     if (!a.visible && q.kv > 0) {  // causal rows: nothing past the tile's last one

@@ -1,5 +1,6 @@
-// Attention of many rows over a paged cache: tiles of 32, 64 or 128 rows
-// (dsr_attention.h has the work split and the kernel for few rows).
+// Attention of many rows over a paged cache: tiles of 32 rows (up to 128
+// dimensions), 64 (more dimensions) or 128 (dsr_attention.h has the work split
+// and the kernel for few rows).
 #pragma once
 
 #include <type_traits>
@@ -44,7 +45,7 @@ constexpr int attn_round(int DP) { return kAttnThreads / (DP / 8); }
 // FLAT: a page holds every token of a round of loads, so that a round's page
 // id and address are the same for the workgroup and a lane adds one offset.
 template <class T, int DP, int WR, bool FLAT>
-__global__ __launch_bounds__(kAttnThreads, DP <= 128 ? 2 : 1) void k_tree_attention_wide(AttnCall) {
+__global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_tree_attention_wide(AttnCall) {
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
   typedef float f32x8 __attribute__((ext_vector_type(8)));

@@ -20,8 +20,11 @@ bool page_ok(int32_t page, int32_t blocks) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-// Plans of at most this many tokens and requests run in one workgroup.
-constexpr int kPlanSmallTokens = 4096, kPlanSmallRequests = 256;
+// Plans of at most this many tokens and requests (trees) run in one workgroup
+// and launch.  Us a call in one launch against two: 64 requests of 1 token 5.7
+// and 7.6, of 16 7.3 and 8.2, of 32 8.7 and 8.3; 128 of 8 7.0 and 7.4, 256 of
+// 2 7.6 and 7.0; 16 trees of 8 nodes 5.5 and 6.4, 32 7.5 and 6.9.
+constexpr int kPlanSmallTokens = 1024, kPlanSmallRequests = 128, kPlanSmallTrees = 16;
 
 template <class T>
 int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
@@ -56,28 +59,45 @@ int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
 // Dimensions of the kernel that takes a head dimension.
 int attn_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
-constexpr int kAttnShort = 256, kAttnMany = 1024;  // tokens, powers of two from every kernel's step on
-
-// Host part of the work split, from sizes alone.
+// Host part of the work split, from sizes alone.  The figures are us a call in
+// bf16 with 8 key heads of 128, contexts about as long as the table's rows.
 AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   AttnPlan p{};
   const int64_t group = a.q_heads / a.kv_heads;
   const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
   const bool big = a.head_dim > 128;
-  p.tile_rows = rows <= 16 || (big && rows <= 32) ? 16 : rows <= 32 ? 32 : rows <= 64 && !big ? 64 : 128;
-  // As many workgroups as the chip holds at once (256 CUs, one or two each).
-  p.groups = p.tile_rows == 32 || big ? 256 : 512;
-  // Causal tiles have unlike lengths: several workgroups for each place even them out.
-  if (!a.visible && a.tokens > 64 * a.requests) p.groups *= 4;
+  // A tile for the rows of a usual request, so that its keys and values are
+  // read once.  32 requests over 8,064 tokens: 16 rows 200 in tiles of 16, 210
+  // of 32; 32 rows 228 of 16, 209 of 32, 229 of 64.  64 rows: 237 of 64 and 236
+  // of 128, and 199 and 177 on 100 ragged requests, so that 128 take them.  With
+  // 256 dimensions 32 rows 724 in tiles of 16, 384 of 64, 504 of 128.
+  p.tile_rows = rows <= 16 ? 16 : !big && rows <= 32 ? 32 : big && rows <= 64 ? 64 : 128;
   p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
   p.min_steps = 128 / p.tokens;
-  // Where a whole table row is a short way for one workgroup, or a longer
-  // one and there is a tile for every CU, a tile is one step: nothing is
-  // cut, and no joining launch follows.
   const int64_t tiles = (a.tokens * group / p.tile_rows + a.requests) * a.kv_heads;
   const int64_t span = (int64_t)a.width * a.page;
-  p.cut = span > (tiles >= 256 ? kAttnMany : kAttnShort);
-  if (!p.cut) p.tokens = kAttnMany, p.min_steps = 1;
+  // Where a whole table row is a short way for one workgroup, a longer one if
+  // there are tiles for more of the chip, a tile is one step: nothing is cut,
+  // no parts are written and no joining launch follows.  Uncut against cut, a
+  // token a request: 1 request over 500 tokens 11.9 and 14.2, over 1,000 15.8 and
+  // 15.4; 16 over 1,000 19.9 and 27.8; 32 over 2,000 55 and 65.
+  p.cut = span > (tiles < 64 ? 512 : tiles > 256 ? 2048 : 8 * tiles);
+  // Chunks of prompts have many tiles, and causal ones of unlike lengths.  They
+  // go uncut, the longest first, if no tile can be longer than half as much
+  // again as a workgroup's share of the chunks alone: 16 chunks of 512 tokens 210
+  // and 262, 2 of 512 39 and 116, one of 2,048 130 and 258.
+  if (!a.visible && a.tokens > 64 * a.requests && span * a.requests * 2048 <= 3 * tiles * a.tokens) p.cut = false;
+  if (!p.cut) {
+    while (p.tokens < span) p.tokens *= 2;
+    p.min_steps = 1;
+    p.groups = 1 << 14;
+  } else {
+    // Workgroups that the chip holds at once: 256 CUs, one or two each.  One
+    // where a CU has room for one or waits for memory anyway (a token for each
+    // of 64 requests over 8,192: 370 with 256, 391 with 512), two where a CU's
+    // matrix cores have more to do (8 trees of 64 nodes over 32,000: 822 and 693).
+    p.groups = p.tile_rows < 128 || big ? 256 : 512;
+  }
   while (((int64_t)a.width * a.page / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
   auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
   p.group = (int)group;
@@ -96,7 +116,7 @@ struct AttnSizes {
 };
 AttnSizes attn_sizes(const dsr_tree_attention_args_t& a, const AttnPlan& p) {
   AttnSizes s;
-  const int64_t parts = 2 * (int64_t)p.groups;
+  const int64_t parts = p.cut ? 2 * (int64_t)p.groups : 1;
   s.o = round256(parts * p.tile_rows * attn_dim(a.head_dim) * 4);
   s.ml = round256(parts * p.tile_rows * 8);
   s.all = s.o + s.ml + round256(parts * 4);
@@ -129,14 +149,14 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
   switch (p.tile_rows) {
     case 16:
       if constexpr (DP <= 128)
-        if (!p.cut) {
+        if (!p.cut && p.groups < 128) {
           hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 8>), grid, dim3(512), 0, s, call);
           break;
         }
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4>), grid, threads, 0, s, call);
       break;
     case 128: attn_wide<T, DP, 4>(grid, s, call); break;
-    case 64: if constexpr (DP <= 128) attn_wide<T, DP, 2>(grid, s, call); break;
+    case 64: if constexpr (DP > 128) attn_wide<T, DP, 2>(grid, s, call); break;
     default: if constexpr (DP <= 128) attn_wide<T, DP, 1>(grid, s, call);
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
@@ -185,7 +205,7 @@ int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
                          a.workspace_bytes < dsr_plan_workspace_bytes(a.requests)))
     return DSR_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  if (a.capacity <= kPlanSmallTokens && a.requests <= kPlanSmallRequests) {
+  if (a.capacity <= kPlanSmallTokens && a.requests <= (a.parents ? kPlanSmallTrees : kPlanSmallRequests)) {
     hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(kPlanThreads), 0, s, a);
     return launched();
   }

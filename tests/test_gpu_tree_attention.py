@@ -63,6 +63,28 @@ def test_long_contexts_are_split_and_joined(heads, kv, dim, n, dtype):
     check(Step(rng, [n, n, 1, n], ctx, heads, kv, dim, 16, dtype, trees=True), dtype)
 
 
+@pytest.mark.parametrize("new,ctx", [([20, 18], [3000, 40]), ([31, 2, 25], [7, 0, 300])])
+@pytest.mark.parametrize("dim,dtype", [(256, "bf16"), (248, "f16"), (192, "f16"), (136, "bf16")])
+def test_wide_heads_of_some_rows(new, ctx, dim, dtype):
+    """Between the smallest and the largest tiles, in parts and whole."""
+    rng = np.random.default_rng([dim, ctx[0]])
+    check(Step(rng, new, ctx, 4, 2, dim, 16, dtype, trees=True), dtype)
+    check(Step(rng, new, ctx, 4, 2, dim, 1, dtype, by_head=True), dtype)
+
+
+@pytest.mark.parametrize("new,ctx,heads,kv,dim,page", [
+    ([300], [5000], 4, 1, 64, 16),             # a chunk behind a long context: in parts
+    ([513, 0, 66], [0, 40, 0], 16, 2, 128, 32),  # whole tiles, the longest first
+    ([700, 1], [0, 2000], 8, 1, 96, 1),
+    ([130, 200], [100, 3], 3, 3, 256, 64),
+])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_chunks_whole_and_in_parts(new, ctx, heads, kv, dim, page, dtype):
+    rng = np.random.default_rng([sum(new), dim])
+    res = check(Step(rng, new, ctx, heads, kv, dim, page, dtype), dtype)
+    assert not res.status.any()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 192, 256])
 def test_one_long_request_has_many_parts(dim):
     rng = np.random.default_rng(dim)
