@@ -370,9 +370,13 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
 // weights then stay below 2^8, far inside every type's range, and most tiles
 // need no rescaling.
 //
-// WAVES: four, two workgroups a CU, for long contexts; eight where one
-// workgroup takes a whole short context and its latency counts (32 query
-// heads over 1,001 tokens: ? us with eight, ? with four).
+// WAVES: eight where fewer than 128 workgroups take whole short contexts and
+// their latency counts (a request of 64 query heads over 500 tokens: 11.9 us
+// with eight, 12.8 with four), else four (from 16 requests on the same to
+// 0.2 us).
+//
+// What bounds it: the cache's read.  64 requests of one token over 8,192
+// tokens, 8 heads of 128: 370 us, 5.8 TB/s.
 template <class T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
     AttnCall) {
@@ -656,6 +660,10 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
 // rows JR y .. of the tile whose first border is the one before share x + 1.
 // Few rows leave threads over: these take every SLOTS-th part each (a single
 // long request has a part for each of 64 shares), summed in a fixed order.
+// One pass with a running maximum: a part's outputs are not waited for behind
+// all parts' maxima (a single request over 1,001 tokens 14.4 us a call, so 13.8).
+// What bounds it: the call's second launch, and the parts' way through the
+// caches (5 us of that call's 14; 67 MB in 22 us for 512 shares of 128 rows).
 template <class T, int DP, int JR>
 __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   typedef typename AttnType<T>::x4 x4;
@@ -664,7 +672,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const int border = blockIdx.x + 1;
-  AttnWork<false> work(attn_call().a, attn_call().p, border);
+  AttnWork<true> work(attn_call().a, attn_call().p, border);
   AttnSegment u;
   AttnRequest q;
   const uint32_t at = work.at;
@@ -677,38 +685,35 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   const bool spare = slot >= SLOTS;  // 192 dimensions: 64 threads
   const int rows = min(p.tile_rows, q.rows - row0);
   if ((int)blockIdx.y * JR >= rows) return;
+#pragma unroll
   for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
     const int in = x / (DP / 4), row = blockIdx.y * JR + in, d = x % (DP / 4) * 4;
     // The first part is its workgroup's last (an odd place), the others their workgroups' first.
     auto part = [&](int c) { return ((int64_t)(2 * c + (c == first)) << p.tile_shift) + row; };
-    // The base first, so that the parts' loads do not wait for each other.
     float M = -INFINITY, L = 0.f;
     attn_f32x4 o = {};
-#pragma unroll 4
-    for (int c = spare ? last + 1 : first + slot; c <= last; c += SLOTS) M = fmaxf(M, p.part_ml[part(c)].x);
-    if constexpr (SLOTS > 1) {
-      if (d == 0 && !spare) sm[slot][in] = M;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i) M = fmaxf(M, sm[i][in]);
-    }
+    auto add = [&](float m, float l, attn_f32x4 x) {
+      const float both = fmaxf(M, m), f = M == both ? 1.f : __builtin_amdgcn_exp2f(M - both);
+      const float g = m == both ? 1.f : __builtin_amdgcn_exp2f(m - both);
+      M = both;
+      L = L * f + l * g;
+      o = o * f + x * g;
+    };
 #pragma unroll 4
     for (int c = spare ? last + 1 : first + slot; c <= last; c += SLOTS) {
       const float2 ml = p.part_ml[part(c)];
-      const float f = ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-      L += ml.y * f;
-      o += *(const attn_f32x4*)&p.part_o[part(c) * DP + d] * f;
+      add(ml.x, ml.y, *(const attn_f32x4*)&p.part_o[part(c) * DP + d]);
     }
     if constexpr (SLOTS > 1) {
       if (!spare) so[slot][x] = o;
-      if (d == 0 && !spare) sl[slot][in] = L;
+      if (d == 0 && !spare) {
+        sm[slot][in] = M;
+        sl[slot][in] = L;
+      }
       __syncthreads();
       if (slot > 0) break;
 #pragma unroll
-      for (int i = 1; i < SLOTS; ++i) o += so[i][x];
-      L = 0.f;
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i) L += sl[i][in];
+      for (int i = 1; i < SLOTS; ++i) add(sm[i][in], sl[i][in], so[i][x]);
     }
     if (row >= rows || d >= a.head_dim) continue;
     const int t = attn_token(p, row0 + row), h = row0 + row - t * p.group;
