@@ -378,9 +378,7 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
 // What bounds it: the cache's read.  64 requests of one token over 8,192
 // tokens, 8 heads of 128: 370 us, 5.8 TB/s.
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
-    AttnCall) {
-  constexpr int NB = 1;         // 16-row blocks of a tile
+__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(AttnCall) {
   constexpr int kThreads = 64 * WAVES;
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
@@ -389,8 +387,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   constexpr int VS = DP + 16;   // LDS row of values: 32 bytes of padding spread the transposing reads over the banks
   __shared__ __align__(16) T keys[WAVES][kAttnTile][DP + 8];  // 16 bytes of padding for the 16-byte reads of 16 keys
   __shared__ __align__(16) T vals[WAVES][kAttnTile][VS];
-  __shared__ float sm[WAVES][16 * NB], sl[WAVES][16 * NB];
-  __shared__ float sbase[16 * NB];
+  __shared__ float sm[WAVES][16], sl[WAVES][16];
+  __shared__ float sbase[16];
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
@@ -398,260 +396,235 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   AttnSegment u;
   AttnRequest q;
   while (work.next(attn_call().a, attn_call().p, u, q)) {  // the same for the whole workgroup
-  const dsr_tree_attention_args_t& a = attn_call().a;
-  const AttnPlan& p = attn_call().p;
-  const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
-  __syncthreads();  // the last segment's LDS is read
-  if (threadIdx.x == 0) sbad = spoison = 0;
-  const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
-  const int row0 = u.tile << row_shift;
+    const dsr_tree_attention_args_t& a = attn_call().a;
+    const AttnPlan& p = attn_call().p;
+    const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
+    __syncthreads();  // the last segment's LDS is read
+    if (threadIdx.x == 0) sbad = spoison = 0;
+    const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
+    const int row0 = u.tile << row_shift;
 
-  attn_f32x4 acc[NB][DB];
-  float m[NB], sum[NB];
+    attn_f32x4 acc[DB];
+    float m = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    m[b] = -INFINITY;
-    sum[b] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[b][d] = attn_f32x4{};
-  }
-  const dsr_tree_attention_args_t& c = attn_call().a;
-  const int32_t* pages = c.table + u.r * c.table_ld;
-  const T* kb = (const T*)c.k_cache + u.head * c.k_head;
-  const T* vb = (const T*)c.v_cache + u.head * c.v_head;
-  const int shift = attn_call().p.page_shift, page = c.page;
-  const unsigned blocks = c.blocks;
-  const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
-  const bool masks = c.visible != nullptr;
-  bool any_bad = false;
+    for (int d = 0; d < DB; ++d) acc[d] = attn_f32x4{};
+    const dsr_tree_attention_args_t& c = attn_call().a;
+    const int32_t* pages = c.table + u.r * c.table_ld;
+    const T* kb = (const T*)c.k_cache + u.head * c.k_head;
+    const T* vb = (const T*)c.v_cache + u.head * c.v_head;
+    const int shift = attn_call().p.page_shift, page = c.page;
+    const unsigned blocks = c.blocks;
+    const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
+    const bool masks = c.visible != nullptr;
+    bool any_bad = false;
 
-  // Tiles of this wave: 32 tokens from begin + 32 (WAVES i + w) on.  LPR lanes
-  // read a token's row, 16 bytes each side by side (lanes next to each other
-  // on different rows, as the product wants them, would take a cache access
-  // each: 16 bytes a cycle and CU in place of 64), and each of them NI tokens
-  // in a row, which share a page unless it is smaller.  Places past the last
-  // token read the last token (their scores are masked).
-  constexpr int LPR = DP / 8 <= 8 ? 8 : DP / 8 <= 16 ? 16 : 32;
-  constexpr int NI = kAttnTile / (64 / LPR);
-  const int sub = l / LPR * NI, chunk = 8 * (l & (LPR - 1)), d0 = min(chunk, dim - 8);
-  const bool stores = chunk < DP;  // 192 dimensions: 24 of 32 lanes
-  const bool tiny = page < NI;   // several pages: their ids are read with the rows
-  int id_next = 0;
-  uint32_t bad_next = 0;
-  x8 kr[NI], vr[NI];
-  auto load_id = [&](int p0) __attribute__((always_inline)) { id_next = pages[min(p0 + sub, end - 1) >> shift]; };
-  auto load_rows = [&](int p0) __attribute__((always_inline)) {
-    bad_next = 0;
-    auto load = [&](int i, int id, int place) __attribute__((always_inline)) {
-      const uint32_t at = (unsigned)id < blocks ? id : 0, in = place & (page - 1);
-      kr[i] = *(const x8*)(kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token));
-      vr[i] = *(const x8*)(vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token));
-    };
-    if (!tiny) {
-      const bool outside = (unsigned)id_next >= blocks;
-      const uint64_t bad = __ballot(outside);
-      if (bad)
+    // Tiles of this wave: 32 tokens from begin + 32 (WAVES i + w) on.  LPR lanes
+    // read a token's row, 16 bytes each side by side (lanes next to each other
+    // on different rows, as the product wants them, would take a cache access
+    // each: 16 bytes a cycle and CU in place of 64), and each of them NI tokens
+    // in a row, which share a page unless it is smaller.  Places past the last
+    // token read the last token (their scores are masked).
+    constexpr int LPR = DP / 8 <= 8 ? 8 : DP / 8 <= 16 ? 16 : 32;
+    constexpr int NI = kAttnTile / (64 / LPR);
+    const int sub = l / LPR * NI, chunk = 8 * (l & (LPR - 1)), d0 = min(chunk, dim - 8);
+    const bool stores = chunk < DP;  // 192 dimensions: 24 of 32 lanes
+    const bool tiny = page < NI;   // several pages: their ids are read with the rows
+    int id_next = 0;
+    uint32_t bad_next = 0;
+    x8 kr[NI], vr[NI];
+    auto load_id = [&](int p0) __attribute__((always_inline)) { id_next = pages[min(p0 + sub, end - 1) >> shift]; };
+    auto load_rows = [&](int p0) __attribute__((always_inline)) {
+      bad_next = 0;
+      auto load = [&](int i, int id, int place) __attribute__((always_inline)) {
+        const uint32_t at = (unsigned)id < blocks ? id : 0, in = place & (page - 1);
+        kr[i] = *(const x8*)(kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token));
+        vr[i] = *(const x8*)(vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token));
+      };
+      if (!tiny) {
+        const bool outside = (unsigned)id_next >= blocks;
+        const uint64_t bad = __ballot(outside);
+        if (bad)
 #pragma unroll
-        for (int j = 0; j < 64 / LPR; ++j)
-          if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
-      if (p0 + kAttnTile <= end) {
-        const uint32_t at = outside ? 0 : id_next, in = (p0 + sub) & (page - 1);
-        const T* k = kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token);
-        const T* v = vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token);
+          for (int j = 0; j < 64 / LPR; ++j)
+            if (bad >> (j * LPR) & 1) bad_next |= ((1u << NI) - 1u) << (NI * j);
+        if (p0 + kAttnTile <= end) {
+          const uint32_t at = outside ? 0 : id_next, in = (p0 + sub) & (page - 1);
+          const T* k = kb + d0 + ((uint64_t)at * k_block + (uint64_t)in * k_token);
+          const T* v = vb + d0 + ((uint64_t)at * v_block + (uint64_t)in * v_token);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          kr[i] = *(const x8*)k;
-          vr[i] = *(const x8*)v;
-          k += k_token;
-          v += v_token;
+          for (int i = 0; i < NI; ++i) {
+            kr[i] = *(const x8*)k;
+            vr[i] = *(const x8*)v;
+            k += k_token;
+            v += v_token;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NI; ++i) load(i, id_next, min(p0 + sub + i, end - 1));
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) load(i, id_next, min(p0 + sub + i, end - 1));
-      }
-    } else {
+        for (int i = 0; i < NI; ++i) {
+          const int place = min(p0 + sub + i, end - 1), id = pages[place >> shift];
+          const uint64_t bad = __ballot((unsigned)id >= blocks);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int place = min(p0 + sub + i, end - 1), id = pages[place >> shift];
-        const uint64_t bad = __ballot((unsigned)id >= blocks);
-#pragma unroll
-        for (int j = 0; j < 64 / LPR; ++j) bad_next |= (uint32_t)(bad >> (j * LPR) & 1) << (NI * j + i);
-        load(i, id, place);
+          for (int j = 0; j < 64 / LPR; ++j) bad_next |= (uint32_t)(bad >> (j * LPR) & 1) << (NI * j + i);
+          load(i, id, place);
+        }
       }
+    };
+    const int first = begin + kAttnTile * w, step = kAttnTile * WAVES;
+    if (first < end) {
+      load_id(first);
+      load_rows(first);
+      load_id(first + step);
     }
-  };
-  const int first = begin + kAttnTile * w, step = kAttnTile * WAVES;
-  if (first < end) {
-    load_id(first);
-    load_rows(first);
-    load_id(first + step);
-  }
-  // This lane's rows: token index, mask, query operand.  A negative scale
-  // changes the queries' sign, so that scores only grow with their products;
-  // scale 0 is queries of 0.
-  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-  x8 qv[NB][KS];
-  int tok[NB];
-  uint64_t mask[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int row = row0 + 16 * b + n;
-    const bool in = row < q.rows;
-    const int t = in ? attn_token(p, row) : 0, h = in ? row - t * group : 0;
-    tok[b] = t;
-    mask[b] = in && a.visible ? a.visible[q.lo + t] : 0;
-    const T* src = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)(u.head * group + h) * a.q_head;
+    // This lane's rows: token index, mask, query operand.  A negative scale
+    // changes the queries' sign, so that scores only grow with their products;
+    // scale 0 is queries of 0.
+    const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+    x8 qv[KS];
+    const bool in = row0 + n < q.rows;
+    const int tok = in ? attn_token(p, row0 + n) : 0, head = in ? row0 + n - tok * group : 0;
+    const uint64_t mask = in && a.visible ? a.visible[q.lo + tok] : 0;
+    const T* src = (const T*)a.q + (int64_t)(q.lo + tok) * a.q_token + (int64_t)(u.head * group + head) * a.q_head;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = 32 * s + 8 * g;
       const x8 v = in && d < dim && a.scale != 0.f ? *(const x8*)(src + d) : x8{};
-      qv[b][s] = a.scale < 0.f ? -v : v;
+      qv[s] = a.scale < 0.f ? -v : v;
     }
-  }
-  __syncthreads();  // the flags
-  for (int p0 = first; p0 < end; p0 += step) {
-    const uint32_t bad = bad_next;
-    const bool masked = p0 + kAttnTile > ctx || bad;  // some row may not see some token
-    any_bad |= bad != 0;
-    if (masked) {
-      bool poison = false;
+    __syncthreads();  // the flags
+    for (int p0 = first; p0 < end; p0 += step) {
+      const uint32_t bad = bad_next;
+      const bool masked = p0 + kAttnTile > ctx || bad;  // some row may not see some token
+      any_bad |= bad != 0;
+      if (masked) {
+        bool poison = false;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) poison |= attn_make_finite<T>(vr[i]);
-      if (poison) spoison = 1;
-    }
-    // Keys and values to the wave's LDS rows; then the next tile's loads.
-    __builtin_amdgcn_wave_barrier();
-    if (DP == 8 * LPR || stores) {
-      if (chunk >= dim)  // dimensions past the head's
-#pragma unroll
-        for (int i = 0; i < NI; ++i) kr[i] = x8{};
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        *(x8*)&keys[w][sub + i][chunk] = kr[i];
-        *(x8*)&vals[w][sub + i][chunk] = vr[i];
+        for (int i = 0; i < NI; ++i) poison |= attn_make_finite<T>(vr[i]);
+        if (poison) spoison = 1;
       }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (p0 + step < end) {
-      load_rows(p0 + step);
-      load_id(p0 + 2 * step);
-    }
-    // Scores.
-    attn_f32x4 sc[NB][2];
+      // Keys and values to the wave's LDS rows; then the next tile's loads.
+      __builtin_amdgcn_wave_barrier();
+      if (DP == 8 * LPR || stores) {
+        if (chunk >= dim)  // dimensions past the head's
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+          for (int i = 0; i < NI; ++i) kr[i] = x8{};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) sc[b][k] = attn_f32x4{};
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const x8 key = *(const x8*)&keys[w][16 * k + n][32 * s + 8 * g];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) sc[b][k] = AttnType<T>::mfma16(key, qv[b][s], sc[b][k]);
+        for (int i = 0; i < NI; ++i) {
+          *(x8*)&keys[w][sub + i][chunk] = kr[i];
+          *(x8*)&vals[w][sub + i][chunk] = vr[i];
+        }
       }
-    // Softmax.  A lane's scores: tokens p0 + 16 k + 4 g + e of its row.
-    x8 pv[NB];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (p0 + step < end) {
+        load_rows(p0 + step);
+        load_id(p0 + 2 * step);
+      }
+      // Scores.
+      attn_f32x4 sc[2];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
+      for (int k = 0; k < 2; ++k) sc[k] = attn_f32x4{};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const x8 key = *(const x8*)&keys[w][16 * k + n][32 * s + 8 * g];
+          sc[k] = AttnType<T>::mfma16(key, qv[s], sc[k]);
+        }
+      // Softmax.  A lane's scores: tokens p0 + 16 k + 4 g + e of its row.
+      x8 pv;
       float top = -INFINITY;
       if (masked) {
-        const uint32_t see = attn_sees(masks, mask[b], tok[b], p0, ctx, end, bad) >> (4 * g);
+        const uint32_t see = attn_sees(masks, mask, tok, p0, ctx, end, bad) >> (4 * g);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[b][k][e] = see >> (16 * k + e) & 1 ? sc[b][k][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) sc[k][e] = see >> (16 * k + e) & 1 ? sc[k][e] : -INFINITY;
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[b][k][e]);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[k][e]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32)) * scale - AttnType<T>::kLift;
-      if (__ballot(top > m[b] + 8.f)) {
-        const float next = fmaxf(m[b], top);
-        const float f = m[b] == next ? 1.f : __builtin_amdgcn_exp2f(m[b] - next);
-        m[b] = next;
-        sum[b] *= f;
+      if (__ballot(top > m + 8.f)) {
+        const float next = fmaxf(m, top);
+        const float f = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        sum *= f;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc[b][d] *= f;
+        for (int d = 0; d < DB; ++d) acc[d] *= f;
       }
-      const float base = m[b] == -INFINITY ? 0.f : -m[b];
+      const float base = m == -INFINITY ? 0.f : -m;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][k][e], scale, base));
-          sum[b] += x;
-          pv[b][4 * k + e] = (T)x;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][e], scale, base));
+          sum += x;
+          pv[4 * k + e] = (T)x;
         }
-    }
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      const T* at = &vals[w][4 * g + (n >> 2)][16 * d + 4 * (n & 3)];
-      const x4 lo = attn_read_tr<T>(at), hi = attn_read_tr<T>(at + 16 * VS);
-      const x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b][d] = AttnType<T>::mfma16(v, pv[b], acc[b][d]);
+      for (int d = 0; d < DB; ++d) {
+        const T* at = &vals[w][4 * g + (n >> 2)][16 * d + 4 * (n & 3)];
+        const x4 lo = attn_read_tr<T>(at), hi = attn_read_tr<T>(at + 16 * VS);
+        const x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[d] = AttnType<T>::mfma16(v, pv, acc[d]);
+      }
     }
-  }
 
-  // The waves' results: statistics, then one row block at a time.
+    // The waves' results: statistics, then the rows.
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (g == 0) sm[w][n] = m;
+    if (any_bad && l == 0) sbad = 1;
+    __syncthreads();
+    const AttnCall& e = attn_call();
+    const bool split = !u.whole;
+    const int64_t part = u.part;
+    constexpr int OS = DP + 4;  // LDS row of outputs
+    static_assert(16 * OS * sizeof(float) <= kAttnTile * VS * sizeof(T), "a wave's outputs fit its rows of values");
+    float top = sm[0][n];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    sum[b] += __shfl_xor(sum[b], 16);
-    sum[b] += __shfl_xor(sum[b], 32);
-    if (g == 0) sm[w][16 * b + n] = m[b];
-  }
-  if (any_bad && l == 0) sbad = 1;
-  __syncthreads();
-  const AttnCall& e = attn_call();
-  const bool split = !u.whole;
-  const int64_t part = u.part;
-  constexpr int OS = DP + 4;  // LDS row of outputs
-  static_assert(16 * OS * sizeof(float) <= kAttnTile * VS * sizeof(T), "a wave's outputs fit its rows of values");
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    float top = sm[0][16 * b + n];
-#pragma unroll
-    for (int i = 1; i < WAVES; ++i) top = fmaxf(top, sm[i][16 * b + n]);
-    const float f = m[b] == top ? 1.f : __builtin_amdgcn_exp2f(m[b] - top);  // a wave without tokens: 0
-    if (g == 0) sl[w][16 * b + n] = sum[b] * f;
-    if (w == 0 && g == 0) sbase[16 * b + n] = top;
+    for (int i = 1; i < WAVES; ++i) top = fmaxf(top, sm[i][n]);
+    const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);  // a wave without tokens: 0
+    if (g == 0) sl[w][n] = sum * f;
+    if (w == 0 && g == 0) sbase[n] = top;
     float* mine = (float*)&vals[w][0][0];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *(attn_f32x4*)&mine[n * OS + 16 * d + 4 * g] = acc[b][d] * f;
+    for (int d = 0; d < DB; ++d) *(attn_f32x4*)&mine[n * OS + 16 * d + 4 * g] = acc[d] * f;
     __syncthreads();
     for (int x = threadIdx.x; x < 16 * (DP / 4); x += kThreads) {
-      const int row = x / (DP / 4), d = x % (DP / 4) * 4, rr = 16 * b + row;
-      const float M = sbase[rr];
+      const int row = x / (DP / 4), d = x % (DP / 4) * 4;
+      const float M = sbase[row];
       float L = 0.f;
       attn_f32x4 o = {};
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) {
-        L += sl[i][rr];
+        L += sl[i][row];
         o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
       }
       if (split) {
-        *(attn_f32x4*)&e.p.part_o[(((int64_t)part << row_shift) + rr) * DP + d] = o;
-        if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + rr] = float2{M, L};
-      } else if (row0 + rr < q.rows && d < dim) {
-        const int t = attn_token(e.p, row0 + rr), h = row0 + rr - t * group;
+        *(attn_f32x4*)&e.p.part_o[(((int64_t)part << row_shift) + row) * DP + d] = o;
+        if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + row] = float2{M, L};
+      } else if (row0 + row < q.rows && d < dim) {
+        const int t = attn_token(e.p, row0 + row), head = u.head * group + row0 + row - t * group;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         x4 y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
-        *(x4*)((T*)e.a.out + (int64_t)(q.lo + t) * e.a.out_token + (int64_t)(u.head * group + h) * e.a.out_head + d) = y;
+        *(x4*)((T*)e.a.out + (int64_t)(q.lo + t) * e.a.out_token + (int64_t)head * e.a.out_head + d) = y;
         if (e.a.lse && d == 0)
-          e.a.lse[(int64_t)(q.lo + t) * e.a.q_heads + u.head * group + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+          e.a.lse[(int64_t)(q.lo + t) * e.a.q_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
       }
     }
     __threadfence_block();
     __syncthreads();
-  }
-  if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
-  attn_report(e.a, e.p, u, q, sbad);
+    if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
+    attn_report(e.a, e.p, u, q, sbad);
   }
 }
 
