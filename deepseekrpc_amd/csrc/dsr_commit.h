@@ -13,7 +13,8 @@
 // byte's moves run in path order, or a batch of reads before its writes.  A
 // thread owns a 16-byte column of the rows and does just that.
 // What bounds it: a chain of a few dependent reads (tree, page ids, rows),
-// then 2 x row bytes per move and cache.
+// then 2 x row bytes per move and cache.  64 trees, 48 layers of keys and
+// values, about 35 MB moved: 9.6 us, 3.7 TB/s; 8 trees 3.6 to 4.0.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -24,12 +25,13 @@
 namespace dsr {
 
 constexpr int kCommitThreads = 256;
-constexpr int kCommitBatch = 4;  // rows in flight per thread
+constexpr int kCommitBatch = 4;  // rows in flight per thread (64 trees: 10.1 us with two, 9.6 with four, 9.7 with eight)
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 // Caches per workgroup: as many as its threads cover with one 16-byte column
-// each, at most 8 (the launch then has enough workgroups to fill the chip).
+// each, at most 8 (64 trees: 11.9 us with one, 9.6 with two to sixteen; the
+// fewer, the more often a request's tree is walked).
 __host__ __device__ inline int commit_caches(const dsr_commit_args_t& a) {
   const int columns = a.heads * (a.row_bytes / 16);
   const int c = columns > 0 ? kCommitThreads / columns : 1;

@@ -380,9 +380,9 @@ class PreparedTreeAttention(_Prepared):
             raise ValueError("query heads must be a multiple of key heads")
         if not 8 <= dim <= N.ATTENTION_MAX_DIM or dim % 8:
             raise ValueError(f"the head dimension must be a multiple of 8 up to {N.ATTENTION_MAX_DIM}")
-        if blocks < 1 or blocks * page > 2**31 - 1 or n * heads > 2**30:
-            raise ValueError("the cache must hold 1 to 2^31 - 1 tokens and q at most 2^30 rows")
         R = _requests(kv_lengths.numel())
+        if blocks < 1 or blocks * page > 2**31 - 1 or (n + R) * heads >= 2**29:
+            raise ValueError("the cache must hold 1 to 2^31 - 1 tokens, and (tokens + requests) x heads be below 2^29")
         a = N.TreeAttentionArgs()
         shape = (blocks, page, kv_heads, dim)
         a.q, a.q_token, a.q_head = _rows(q, "q", q.dtype, dev, q.shape)

@@ -170,7 +170,7 @@ typedef struct dsr_tree_attention_args {
   int32_t page, width, blocks;
   float scale;
   int64_t requests;            /* 0 .. DSR_TREE_MAX_REQUESTS */
-  int64_t tokens;              /* rows of q and out */
+  int64_t tokens;              /* rows of q and out; (tokens + requests) * q_heads < 2^29 */
   int64_t table_ld;
   int64_t q_token, q_head;     /* strides: >= 0, multiples of 8; rows 16-byte aligned */
   int64_t out_token, out_head;

@@ -121,11 +121,28 @@ def test_attention_arguments():
                                         ("table", None), ("offsets", None), ("kv_lengths", None), ("status", None),
                                         ("q_token", 4), ("q_head", 4), ("out_token", 1), ("out_head", 2),
                                         ("k_block", 4), ("k_token", 12), ("k_head", 4), ("v_block", 4),
-                                        ("v_token", 4), ("v_head", 4)])
+                                        ("v_token", 4), ("v_head", 4), ("k_block", 2**31), ("k_token", 2**31),
+                                        ("v_block", 2**31), ("v_token", 2**31), ("k_head", -8), ("q_token", -8)])
     refused(lib.dsr_tree_attention, a, [("workspace", None), ("workspace", 4352 - 128),
                                         ("workspace_bytes", a.workspace_bytes - 1)], -3)
     a.requests = a.tokens = 0
     assert lib.dsr_tree_attention(ctypes.byref(a), None) == 0
+    # Sizes whose tiles or steps would not fit 32 bits are refused, and the largest ones are planned.
+    for sizes in (dict(requests=N.TREE_MAX_REQUESTS, tokens=1, q_heads=2**20, kv_heads=2**20, width=2**20, page=1024),
+                  dict(requests=1, tokens=2**30, q_heads=1, kv_heads=1, width=2**20, page=1024),
+                  dict(requests=1, tokens=1, q_heads=2, kv_heads=2, width=2**31 - 1, page=1024),
+                  dict(requests=1, tokens=1, q_heads=2, kv_heads=2, width=0, page=16)):
+        b = N.TreeAttentionArgs.from_buffer_copy(a)
+        for f, v in sizes.items():
+            setattr(b, f, v)
+        assert lib.dsr_tree_attention_workspace_bytes(ctypes.byref(b)) == 0, sizes
+        assert lib.dsr_tree_attention(ctypes.byref(b), None) == -1, sizes
+    for sizes in (dict(requests=N.TREE_MAX_REQUESTS, tokens=2**13, q_heads=2**14, kv_heads=2**14, width=2**20,
+                       page=1024), dict(requests=1, tokens=2**28, q_heads=1, kv_heads=1, width=2**20, page=1024)):
+        b = N.TreeAttentionArgs.from_buffer_copy(a)
+        for f, v in sizes.items():
+            setattr(b, f, v)
+        assert lib.dsr_tree_attention_workspace_bytes(ctypes.byref(b)) > 0, sizes
     a.head_dim = 100
     assert lib.dsr_tree_attention_workspace_bytes(ctypes.byref(a)) == 0
     assert lib.dsr_tree_attention_workspace_bytes(None) == 0
