@@ -388,6 +388,8 @@ class PreparedTreeAttention(_Prepared):
         a.q, a.q_token, a.q_head = _rows(q, "q", q.dtype, dev, q.shape)
         a.k_cache, a.k_block, a.k_token, a.k_head = _rows(k_cache, "k_cache", q.dtype, dev, shape)
         a.v_cache, a.v_block, a.v_token, a.v_head = _rows(v_cache, "v_cache", q.dtype, dev, shape)
+        if max(a.k_block, a.k_token, a.v_block, a.v_token) > 2**31 - 1:
+            raise ValueError("strides of the caches' pages and tokens must be below 2^31")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=dev)
         a.out, a.out_token, a.out_head = _rows(out, "out", q.dtype, dev, q.shape)
