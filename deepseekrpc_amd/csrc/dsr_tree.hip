@@ -68,22 +68,42 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   const int64_t group = a.q_heads / a.kv_heads;
   const int64_t rows = a.requests > 0 ? (a.tokens * group + a.requests - 1) / a.requests : 0;  // of a usual request
   const bool big = a.head_dim > 128;
-  // A tile for the rows of a usual request, so that its keys and values are
-  // read once.  32 requests over 8,064 tokens: 16 rows 200 in tiles of 16, 210
-  // of 32; 32 rows 228 of 16, 209 of 32, 229 of 64.  64 rows: 237 of 64 and 236
-  // of 128, and 199 and 177 on 100 ragged requests, so that 128 take them.  With
-  // 256 dimensions 32 rows 724 in tiles of 16, 384 of 64, 504 of 128.
-  p.tile_rows = rows <= 16 ? 16 : !big && rows <= 32 ? 32 : big && rows <= 64 ? 64 : 128;
-  p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
-  p.min_steps = 128 / p.tokens;
-  const int64_t tiles = (a.tokens * group / p.tile_rows + a.requests) * a.kv_heads;
   const int64_t span = (int64_t)a.width * a.page;
+  auto tiles_of = [&](int r) { return (a.tokens * group / r + a.requests) * a.kv_heads; };
   // Where a whole table row is a short way for one workgroup, a longer one if
   // there are tiles for more of the chip, a tile is one step: nothing is cut,
   // no parts are written and no joining launch follows.  Uncut against cut, a
   // token a request: 1 request over 500 tokens 11.9 and 14.2, over 1,000 15.8 and
   // 15.4; 16 over 1,000 19.9 and 27.8; 32 over 2,000 55 and 65.
-  p.cut = span > (tiles < 64 ? 512 : tiles > 256 ? 2048 : 8 * tiles);
+  auto is_short = [&](int64_t tiles) { return span <= (tiles < 64 ? 512 : tiles > 256 ? 2048 : 8 * tiles); };
+  // A tile for the rows of a usual request, so that its keys and values are
+  // read once.  32 requests over 8,064 tokens: 16 rows 200 in tiles of 16, 210
+  // of 32; 32 rows 228 of 16, 209 of 32, 229 of 64.  64 rows: 237 of 64 and 236
+  // of 128, and 199 and 177 on 100 ragged requests, so that 128 take them.  With
+  // 256 dimensions 32 rows 724 in tiles of 16, 384 of 64, 504 of 128.  Whole
+  // tiles of 32 have a CU each, of 128 two share one: 200 requests of 24 rows over
+  // 480 tokens 111 and 66.
+  //
+  // The kernel for 16 rows has the shortest way from start to end (9 us; 20 in
+  // tiles of 32, 10 of 128; 14 with 256 dimensions, 26 of 64), and takes calls of
+  // any rows whose tiles the chip holds about at once, as long as reading keys
+  // and values again for each costs less.  16 against the other: 4 requests of 64
+  // rows over 2,200 tokens 27 and 36, over 6,000 50 and 42; 16 of 24 over 6,000 96
+  // and 107; 40 of 24 over 30 tokens 11 and 21 (10 of 128), of 64 17 and 10; 256
+  // dimensions, 2 key heads: 16 of 64 over 3,000 50 and 80, 32 of 48 over 8,064 291
+  // and 165.
+  const int64_t again = big ? 3 << 19 : rows <= 32 ? 1 << 21 : 5 << 17;
+  const bool few = tiles_of(16) <= (big ? 384 : 512) && tiles_of(16) * span <= again;
+  if (rows <= 16 || few)
+    p.tile_rows = 16;
+  else if (big)
+    p.tile_rows = rows <= 64 ? 64 : 128;
+  else
+    p.tile_rows = rows <= 32 && !is_short(tiles_of(32)) ? 32 : 128;
+  p.tokens = p.tile_rows == 16 || p.tile_rows == 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
+  p.min_steps = 128 / p.tokens;
+  const int64_t tiles = tiles_of(p.tile_rows);
+  p.cut = !is_short(tiles);
   // Chunks of prompts have many tiles, and causal ones of unlike lengths.  They
   // go uncut, the longest first, if no tile can be longer than half as much
   // again as a workgroup's share of the chunks alone: 16 chunks of 512 tokens 210
@@ -107,6 +127,10 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   p.group = (int)group;
   p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
   p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
+  // Two rows a joining workgroup leave threads over for long rows of parts: one
+  // request of 32 rows over 6,700 tokens 28 in all, 37 with sixteen; tiles of 128
+  // rows cut less often 40 with sixteen, 79 with two.
+  p.few_join = p.tile_rows == 16 || (p.tile_rows == 32 && p.groups > 4 * tiles);
   // No more workgroups than shares of the fewest steps.
   const int64_t shares = tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;
   if (shares < p.groups) p.groups = (int)((shares + 7) / 8 * 8);
@@ -169,8 +193,9 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   if (p.cut && p.groups > 1) {
     const unsigned borders = (unsigned)p.groups - 1;
-    if (p.tile_rows == 16)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 2>), dim3(borders, 8), threads, 0, s, call);
+    if (p.few_join)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 2>), dim3(borders, (unsigned)(p.tile_rows / 2)), threads, 0, s,
+                         call);
     else
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 16>), dim3(borders, (unsigned)(p.tile_rows / 16)), threads, 0,
                          s, call);

@@ -321,3 +321,51 @@ def test_no_tokens_and_refused_arguments():
     odd = torch.empty(2 * 4 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(2, 4, 64)
     with pytest.raises(ValueError):
         tree.tree_attention(odd, k, v, table, off, kv)
+
+
+# The calls above are small, and few-row tiles take them.  Many tiles, or table
+# rows with room for long contexts, bring the kernels with larger tiles.
+
+
+@pytest.mark.parametrize("dim,heads,kv,most", [(128, 64, 8, 5), (72, 64, 8, 5), (64, 32, 8, 20), (128, 32, 8, 20),
+                                               (96, 24, 8, 20), (192, 64, 8, 5), (256, 32, 8, 9), (136, 16, 8, 9),
+                                               (256, 64, 8, 20)])
+@pytest.mark.parametrize("longest,page,trees,by_head", [(100, 32, True, False), (2100, 16, False, True),
+                                                        (2300, 1, True, False)])
+def test_many_tiles(dim, heads, kv, most, longest, page, trees, by_head):
+    """Whole (short table rows) and in parts, each with one long request among short ones."""
+    rng = np.random.default_rng([dim, heads, most, longest])
+    R = 72
+    new, ctx = rng.integers(1, most + 1, R).tolist(), rng.integers(0, 40, R).tolist()
+    ctx[11], new[30] = longest, 0
+    check(Step(rng, new, ctx, heads, kv, dim, page, "f16" if dim in (72, 192) else "bf16", trees, by_head),
+          "f16" if dim in (72, 192) else "bf16")
+
+
+def roomy(step):
+    """The step's arguments with table rows of about four million tokens."""
+    args, vis = Step.plain_args(step)
+    columns = (1 << 22) // step.page - args[3].shape[1]
+    table = torch.nn.functional.pad(args[3], (0, columns), value=-1)
+    return (*args[:3], table, *args[4:]), vis
+
+
+AGAIN = ([(test_matches_float64, (*shape, dtype, *how)) for shape in SHAPES for dtype in ("bf16", "f16")
+          for how in ((False, False), (True, True))]
+         + [(test_long_contexts_are_split_and_joined, (h, k, d, n, "bf16"))
+            for h, k, d, n in ((8, 1, 128, 3), (8, 1, 128, 40), (8, 1, 64, 4), (4, 1, 192, 9), (4, 2, 256, 30))]
+         + [(test_sharp_and_flat_rows, (dtype,)) for dtype in ("bf16", "f16")]
+         + [(test_growing_maximum, ()), (test_bad_lengths_and_pages, ()), (test_long_chunks_of_a_prompt, ())]
+         + [(test_masks_that_leave_rows_empty, (n,)) for n in (20, 64)]
+         + [(test_what_masked_places_hold_never_reaches_a_row, (what, dtype, new))
+            for what in (float("inf"), float("nan")) for dtype in ("bf16", "f16") for new in ([12], [40])]
+         + [(test_wide_heads_of_some_rows, ([20, 18], [300, 40], dim, "f16")) for dim in (192, 256)]
+         + [(test_bad_page_that_only_a_chunks_last_rows_see, (150, 0))])
+
+
+@pytest.mark.parametrize("case", range(len(AGAIN)))
+def test_again_with_larger_tiles(case, monkeypatch):
+    test, args = AGAIN[case]
+    monkeypatch.setattr(Step, "plain_args", Step.args, raising=False)
+    monkeypatch.setattr(Step, "args", roomy)
+    test(*args)
