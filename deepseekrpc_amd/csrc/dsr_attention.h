@@ -67,7 +67,6 @@ struct AttnPlan {
   int tokens;         // of a step of the work split: a power of two times the kernel's own
   int min_steps;      // fewest steps worth a workgroup
   bool cut;           // some tile may be cut into parts
-  bool few_join;      // two rows of a tile per joining workgroup (else sixteen)
   float* part_o;      // [2 groups, tile_rows, head dim of the kernel]
   float2* part_ml;    // [2 groups, tile_rows]: base (log2) and sum
   int32_t* part_bad;  // [2 groups]: a page id outside the cache

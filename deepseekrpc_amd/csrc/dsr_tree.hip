@@ -91,8 +91,8 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   // rows over 2,200 tokens 27 and 36, over 6,000 50 and 42; 16 of 24 over 6,000 96
   // and 107; 40 of 24 over 30 tokens 11 and 21 (10 of 128), of 64 17 and 10; 256
   // dimensions, 2 key heads: 16 of 64 over 3,000 50 and 80, 32 of 48 over 8,064 291
-  // and 165.
-  const int64_t again = big ? 3 << 19 : rows <= 32 ? 1 << 21 : 5 << 17;
+  // and 165; 192 dimensions, one key head: 3 of 200 over up to 19,500 94 and 74.
+  const int64_t again = big && rows <= 64 ? 3 << 19 : rows <= 32 ? 1 << 21 : 5 << 17;
   const bool few = tiles_of(16) <= (big ? 384 : 512) && tiles_of(16) * span <= again;
   if (rows <= 16 || few)
     p.tile_rows = 16;
@@ -127,10 +127,6 @@ AttnPlan attn_plan(const dsr_tree_attention_args_t& a) {
   p.group = (int)group;
   p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
   p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
-  // Two rows a joining workgroup leave threads over for long rows of parts: one
-  // request of 32 rows over 6,700 tokens 28 in all, 37 with sixteen; tiles of 128
-  // rows cut less often 40 with sixteen, 79 with two.
-  p.few_join = p.tile_rows == 16 || (p.tile_rows == 32 && p.groups > 4 * tiles);
   // No more workgroups than shares of the fewest steps.
   const int64_t shares = tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;
   if (shares < p.groups) p.groups = (int)((shares + 7) / 8 * 8);
@@ -193,7 +189,11 @@ int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipSt
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   if (p.cut && p.groups > 1) {
     const unsigned borders = (unsigned)p.groups - 1;
-    if (p.few_join)
+    // Two rows a joining workgroup leave threads over for long rows of parts (256
+    // dimensions, one request over 10,000 tokens: 34 us a call, 52 with sixteen;
+    // one row each: 64 requests of a token 373, 370 with two); tiles of 128 rows
+    // would be too many workgroups (4 requests: 53 with sixteen, 89 with two).
+    if (p.tile_rows == 16)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_join<T, DP, 2>), dim3(borders, (unsigned)(p.tile_rows / 2)), threads, 0, s,
                          call);
     else
