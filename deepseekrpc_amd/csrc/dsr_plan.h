@@ -74,7 +74,7 @@ __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
   auto wrap = [&](int x) { return x >= pool_size ? x - pool_size : x; };
   if (threadIdx.x < 2) done[threadIdx.x] = 0;
   if (threadIdx.x == 0) a.offsets[0] = 0;
-  int base[kPlanSums] = {0, 0, 0};  // sums over the requests before this round's
+  int base[kPlanSums] = {0, 0, 0};  // sums over the requests before these 1,024
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + (int)threadIdx.x;
     const bool in = r < R;
