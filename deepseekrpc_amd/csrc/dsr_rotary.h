@@ -37,7 +37,9 @@ struct RotaryVec<T, 1> {
 };
 
 // VE elements per access: 16 bytes' worth when every row and part allows it,
-// else one (8,192 tokens of 80 rows of 128 in bf16: 64 us and 125).
+// else 8 bytes' worth, else one (8,192 tokens of 80 rows of 128 in bf16: 64 us,
+// one by one 125; with the first 24 dimensions turned by halves 85 in 8 bytes,
+// 182 one by one).
 template <class T, int VE, bool PAIRS>
 __global__ __launch_bounds__(kRotaryThreads) void k_rotary(dsr_rotary_args_t a) {
   typedef RotaryVec<T, VE> V;

@@ -26,19 +26,23 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // 2 7.6 and 7.0; 16 trees of 8 nodes 5.5 and 6.4, 32 7.5 and 6.9.
 constexpr int kPlanSmallTokens = 1024, kPlanSmallRequests = 128, kPlanSmallTrees = 16;
 
+// Whether every row, part and pair of a rotary call can be taken VE elements at a time.
 template <class T>
-int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
-  constexpr int VE = 16 / sizeof(T);
-  const int half = a.rot_dim / 2;
-  auto rows = [&](const void* p, int64_t t, int64_t h) { return !p || (aligned16(p) && t % VE == 0 && h % VE == 0); };
-  const bool wide = a.head_dim % VE == 0 && a.rot_start % VE == 0 &&
-                    (a.interleaved ? a.rot_dim % VE == 0 : half % VE == 0) && (!a.v || a.v_dim % VE == 0) &&
-                    rows(a.q, a.q_token, a.q_head) && rows(a.q_out, a.qo_token, a.qo_head) &&
-                    rows(a.k, a.k_token, a.k_head) && rows(a.k_out, a.ko_token, a.ko_head) &&
-                    rows(a.v, a.v_token, a.v_head) &&
-                    (!a.k_cache || (rows(a.k_cache, a.kc_token, a.kc_head) && a.kc_block % VE == 0)) &&
-                    (!a.v_cache || (rows(a.v_cache, a.vc_token, a.vc_head) && a.vc_block % VE == 0));
-  const int64_t items = (int64_t)(a.q_heads + a.kv_heads) * a.head_dim / (wide ? VE : 1);
+bool rotary_fits(const dsr_rotary_args_t& a, int VE) {
+  auto rows = [&](const void* p, int64_t t, int64_t h) {
+    return !p || ((uintptr_t)p % (VE * sizeof(T)) == 0 && t % VE == 0 && h % VE == 0);
+  };
+  return a.head_dim % VE == 0 && a.rot_start % VE == 0 &&
+         (a.interleaved ? a.rot_dim % VE == 0 : a.rot_dim / 2 % VE == 0) && (!a.v || a.v_dim % VE == 0) &&
+         rows(a.q, a.q_token, a.q_head) && rows(a.q_out, a.qo_token, a.qo_head) && rows(a.k, a.k_token, a.k_head) &&
+         rows(a.k_out, a.ko_token, a.ko_head) && rows(a.v, a.v_token, a.v_head) &&
+         (!a.k_cache || (rows(a.k_cache, a.kc_token, a.kc_head) && a.kc_block % VE == 0)) &&
+         (!a.v_cache || (rows(a.v_cache, a.vc_token, a.vc_head) && a.vc_block % VE == 0));
+}
+
+template <class T, int VE>
+void rotary_launch(const dsr_rotary_args_t& a, hipStream_t s) {
+  const int64_t items = (int64_t)(a.q_heads + a.kv_heads) * a.head_dim / VE;
   // Few tokens: a token's rows are shared by several workgroups, so that the
   // chip is filled (256 tokens of 80 rows of 128: 5.3 us with one each, 4.8 so;
   // 64 tokens 4.9 and 4.5; from 1,024 on the same).
@@ -47,14 +51,21 @@ int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
   if (parts < 1) parts = 1;
   const dim3 grid((unsigned)a.tokens, (unsigned)parts);
   const dim3 threads(kRotaryThreads);
-  if (wide && a.interleaved)
+  if (a.interleaved)
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE, true>), grid, threads, 0, s, a);
-  else if (wide)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE, false>), grid, threads, 0, s, a);
-  else if (a.interleaved)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1, true>), grid, threads, 0, s, a);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, 1, false>), grid, threads, 0, s, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_rotary<T, VE, false>), grid, threads, 0, s, a);
+}
+
+template <class T>
+int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
+  constexpr int VE = 16 / sizeof(T);
+  if (rotary_fits<T>(a, VE))
+    rotary_launch<T, VE>(a, s);
+  else if (rotary_fits<T>(a, 4))  // halves of 12 or 20, say (float32 rows have come here as 16 bytes already)
+    rotary_launch<T, 4>(a, s);
+  else
+    rotary_launch<T, 1>(a, s);
   return launched();
 }
 

@@ -169,3 +169,16 @@ def test_refused_arguments():
             tree.rotary(*a, **kw)
     empty = tree.rotary(q[:0], k[:0], pos[:0], freqs)
     assert empty.q.shape == (0, 4, 16)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,start", [(11, 4, 2, 64, 24, 0), (1100, 3, 3, 20, 8, 4),
+                                                           (5, 2, 1, 128, 40, 84)])
+def test_rows_that_only_8_byte_accesses_fit(dtype, interleaved, tokens, heads, kv, dim, rot, start):
+    test_forward_and_inverse(dtype, interleaved, tokens, heads, kv, dim, rot, start)
+
+
+@pytest.mark.parametrize("dtype,by_head,page,v_dim", [("bf16", False, 16, 20), ("f16", True, 1, 12)])
+def test_cache_writes_of_8_byte_rows(dtype, by_head, page, v_dim):
+    test_cache_writes(dtype, by_head, page, v_dim)
