@@ -47,6 +47,9 @@ __global__ __launch_bounds__(kCommitThreads) void k_commit_tree(dsr_commit_args_
     lo = lo < 0 ? 0 : lo > a.tokens ? (int)a.tokens : lo;
     hi = hi < lo ? lo : hi > a.tokens ? (int)a.tokens : hi;
     const int n = hi - lo, kv = a.kv_lengths[r], limit = a.output_limit[r];
+    const bool before = a.lengths_in != nullptr;
+    const int old = before ? a.lengths_in[r] : 0, waiting = before ? a.pending_in[r] : -1;
+    const int planned = before ? a.plan_status[r] : DSR_OK;
     int par = -1, token = -1, target = -1;
     if (l < n) {
       par = a.parents[lo + l];
@@ -56,8 +59,9 @@ __global__ __launch_bounds__(kCommitThreads) void k_commit_tree(dsr_commit_args_
     const int64_t eos_lo = a.eos_off ? a.eos_off[r] : 0, eos_hi = a.eos_off ? a.eos_off[r + 1] : 0;
     int status = DSR_OK;
     if (n > DSR_TREE_MAX_NODES || __ballot(l < n && (par >= l || par < -1))) status = DSR_E_TREE;
-    if (kv < n || kv > (int64_t)a.width * a.page || limit < 1) status = DSR_E_LENGTH;
-    int kept = 0, said = 0, pending = -1, stop = DSR_STOP_NONE;
+    if (kv < n || kv > (int64_t)a.width * a.page || (limit < 1 && !(before && n == 0))) status = DSR_E_LENGTH;
+    if (planned != DSR_OK) status = planned;
+    int kept = 0, said = 0, pending = waiting, stop = DSR_STOP_NONE;
     int mine_path = -1, mine_id = -1;
     if (status == DSR_OK && n > 0) {
       int cur = 0;
@@ -103,7 +107,8 @@ __global__ __launch_bounds__(kCommitThreads) void k_commit_tree(dsr_commit_args_
     if (status == DSR_OK && __ballot(bad)) status = DSR_E_BLOCK;
     if (status != DSR_OK) {
       kept = said = 0;
-      pending = mine_path = mine_id = -1;
+      mine_path = mine_id = -1;
+      pending = waiting;
       stop = DSR_STOP_NONE;
     }
     if (blockIdx.y == 0) {
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(kCommitThreads) void k_commit_tree(dsr_commit_args_
         a.count[r] = said;
         a.pending[r] = pending;
         a.stop[r] = stop;
-        a.lengths[r] = status == DSR_E_LENGTH ? 0 : ctx + kept;
+        a.lengths[r] = before && status != DSR_OK ? old : status == DSR_E_LENGTH ? 0 : ctx + kept;
         a.status[r] = status;
       }
     }

@@ -331,6 +331,11 @@ int32_t dsr_commit_tree(const dsr_commit_args_t* args, void* stream) {
       !a.pending || !a.stop || !a.lengths || !a.status || a.lengths == a.kv_lengths ||
       (a.tokens > 0 && (!a.parents || !a.tokens_in || !a.sampled)) || (a.eos_off && !a.eos_ids))
     return DSR_ERR_ARG;
+  // What was so before the step is read by every workgroup of a request, and one of them writes what is so after it.
+  if (!a.lengths_in != !a.pending_in || !a.lengths_in != !a.plan_status)
+    return DSR_ERR_ARG;
+  if (a.lengths_in && (a.lengths == a.lengths_in || a.pending == a.pending_in || a.status == a.plan_status))
+    return DSR_ERR_ARG;
   const int per = commit_caches(a);
   const int groups = a.cache_count > 0 ? (a.cache_count + per - 1) / per : 1;
   hipLaunchKernelGGL(k_commit_tree, dim3((unsigned)a.requests, (unsigned)groups), dim3(kCommitThreads), 0,

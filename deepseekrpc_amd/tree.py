@@ -29,6 +29,8 @@ from . import _native as N
 from . import batch
 
 MAX_NODES = N.TREE_MAX_NODES
+# Statuses of requests and tokens.
+E_LENGTH, E_BLOCKS, E_CAPACITY, E_TREE, E_BLOCK = N.E_LENGTH, N.E_BLOCKS, N.E_CAPACITY, N.E_TREE, N.E_BLOCK
 _ROTARY_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16, torch.float32: N.F32}
 _ATTENTION_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16}
 
@@ -443,7 +445,7 @@ class CommitResult:
     ids: torch.Tensor       # int32 [requests, 64] output ids, -1 padded
     accepted: torch.Tensor  # int32 [requests] kept nodes (the root among them)
     count: torch.Tensor     # int32 [requests] output ids
-    pending: torch.Tensor   # int32 [requests] the next step's root token, -1: none
+    pending: torch.Tensor   # int32 [requests] the next step's root token, -1: none (kept where nothing is accepted)
     stop: torch.Tensor      # int32 [requests] STOP_NONE / STOP_EOS / STOP_LENGTH
     lengths: torch.Tensor   # int32 [requests] cached tokens afterwards
     status: torch.Tensor    # int32 [requests]
@@ -453,7 +455,8 @@ class PreparedCommit(_Prepared):
     """See ``commit_tree``."""
 
     def __init__(self, parents, tokens, sampled, offsets, kv_lengths, table, caches, *, output_limit,
-                 eos_offsets=None, eos_ids=None, page: int | None = None, blocks: int | None = None):
+                 eos_offsets=None, eos_ids=None, page: int | None = None, blocks: int | None = None, lengths=None,
+                 pending=None, plan_status=None):
         dev = _device_of(kv_lengths, "kv_lengths")
         R = _requests(kv_lengths.numel())
         n = parents.numel()
@@ -470,6 +473,13 @@ class PreparedCommit(_Prepared):
         if eos_ids is not None and eos_ids.numel() > 0:
             a.eos_off = _array(eos_offsets, "eos_offsets", torch.int64, dev, R + 1)
             a.eos_ids = _array(eos_ids, "eos_ids", torch.int32, dev)
+        before = (lengths, pending, plan_status)
+        if any(t is None for t in before) != all(t is None for t in before):
+            raise ValueError("lengths, pending and plan_status come together")
+        if lengths is not None:
+            a.lengths_in = _array(lengths, "lengths", torch.int32, dev, R)
+            a.pending_in = _array(pending, "pending", torch.int32, dev, R)
+            a.plan_status = _array(plan_status, "plan_status", torch.int32, dev, R)
         caches = list(caches)
         pointers = None
         if caches:
@@ -501,11 +511,12 @@ class PreparedCommit(_Prepared):
         a.requests, a.tokens = R, n
         self._setup("dsr_commit_tree", a, dev, res,
                     (parents, tokens, sampled, offsets, kv_lengths, table, output_limit, eos_offsets, eos_ids,
-                     pointers, *caches, *vars(res).values()))
+                     pointers, *before, *caches, *vars(res).values()))
 
 
 def commit_tree(parents, tokens, sampled, offsets, kv_lengths, table, caches, *, output_limit, eos_offsets=None,
-                eos_ids=None, page: int | None = None, blocks: int | None = None) -> CommitResult:
+                eos_ids=None, page: int | None = None, blocks: int | None = None, lengths=None, pending=None,
+                plan_status=None) -> CommitResult:
     """The accepted path of each request's drafted tree, and its cache rows
     moved together in every one of ``caches``.
 
@@ -514,6 +525,15 @@ def commit_tree(parents, tokens, sampled, offsets, kv_lengths, table, caches, *,
     the path then has exactly the target's distribution).  From node 0, the
     first child whose token was drawn is accepted, and so on; ids, stops and
     pending token follow ``verify_drafts``.  ``lengths`` of the result are the
-    next step's ``lengths``."""
+    next step's ``lengths``.
+
+    ``lengths`` (those given to ``plan_blocks``), ``pending`` (the pending
+    tokens before the step) and ``plan_status`` (``plan_blocks``'s status), all
+    int32 ``[requests]``, come together.  With them a request that the plan
+    refused, or that has a status here, keeps its length and pending token for
+    a later step, and one without new tokens its pending token.  Without them
+    it gets length 0, or none pending: a loop whose pool can run short needs
+    them."""
     return PreparedCommit(parents, tokens, sampled, offsets, kv_lengths, table, caches, output_limit=output_limit,
-                          eos_offsets=eos_offsets, eos_ids=eos_ids, page=page, blocks=blocks).launch()
+                          eos_offsets=eos_offsets, eos_ids=eos_ids, page=page, blocks=blocks, lengths=lengths,
+                          pending=pending, plan_status=plan_status).launch()

@@ -9,7 +9,8 @@ at each of them, and keeps the accepted path:
   -> vocab_head -> sample_rows -> commit_tree
 
 Lengths, block tables, page pool and pending tokens stay on the device.  Greedy
-output is that of decoding one token at a time (``drafts=False``).
+output is that of decoding one token at a time (``drafts=False``).  Requests that
+find the pool short wait for pages that others give back at their end.
 
     python examples/tree_decode.py
 """
@@ -79,16 +80,19 @@ class Model:
 class Output:
     ids: list = field(default_factory=list)
     steps: int = 0
+    waits: int = 0  # steps without pages for it
     free_pages: int = 0
 
 
-def generate(model, prompts, new_tokens, *, drafts=True, page=16, policy=None, uniforms=None):
+def generate(model, prompts, new_tokens, *, drafts=True, page=16, policy=None, uniforms=None, missing=0):
     """``new_tokens`` ids for each prompt (lists of token ids).  ``policy`` and
-    ``uniforms(step, rows)`` make it sample; without them it is greedy."""
+    ``uniforms(step, rows)`` make it sample; without them it is greedy.  The pool
+    is ``missing`` pages short of what all requests could hold together: fewer
+    than there are requests, so that some request always finds its pages."""
     dev, R = model.device, len(prompts)
     longest = max(map(len, prompts)) + new_tokens + len(PARENTS)
     width = -(-longest // page)
-    blocks = R * width
+    blocks = sum(-(-(len(p) + new_tokens + len(PARENTS)) // page) for p in prompts) - missing
     shape = (blocks, page, model.kv, model.head)
     k_caches = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(model.layers)]
     v_caches = [torch.zeros_like(t) for t in k_caches]
@@ -114,6 +118,7 @@ def generate(model, prompts, new_tokens, *, drafts=True, page=16, policy=None, u
     plan = tree.plan_blocks(lengths, i32([len(p) for p in prompts]), table, held, pool, state, blocks=blocks,
                             page=page, capacity=flat.numel())
     hidden = model.forward(flat, plan, k_caches, v_caches)
+    assert not bool(plan.status.any())  # the pool holds all prompts
     pending = draw(model.logits(hidden[plan.offsets[1:].long() - 1]), 0)
     lengths = plan.kv_lengths
     left = torch.full((R,), new_tokens - 1, dtype=torch.int32, device=dev)
@@ -125,8 +130,10 @@ def generate(model, prompts, new_tokens, *, drafts=True, page=16, policy=None, u
     while int(left.max()) > 0:
         step += 1
         busy = left > 0
-        plan = tree.plan_blocks(lengths, torch.where(busy, nodes, 0).to(torch.int32), table, held, pool, state,
-                                blocks=blocks, page=page, capacity=R * nodes, parents=parents)
+        # Requests that are done end, and give their pages back.
+        added = torch.where(busy, nodes, torch.where(held > 0, -1, 0)).to(torch.int32)
+        plan = tree.plan_blocks(lengths, added, table, held, pool, state, blocks=blocks, page=page,
+                                capacity=R * nodes, parents=parents)
         trees = [pending.clamp(min=0)]
         for node in range(1, nodes):  # children of one node take its successors in order
             of = PARENTS[node]
@@ -136,13 +143,16 @@ def generate(model, prompts, new_tokens, *, drafts=True, page=16, policy=None, u
         tokens = torch.stack(trees, 1)[owner, local.clamp(0, nodes - 1)]
         logits = model.logits(model.forward(tokens, plan, k_caches, v_caches))
         done = tree.commit_tree(parents, tokens, draw(logits, step), plan.offsets, plan.kv_lengths, table,
-                                k_caches + v_caches, output_limit=left.clamp(min=1))
-        assert not bool(plan.status.any()) and not bool(done.status.any())
+                                k_caches + v_caches, output_limit=left, lengths=lengths, pending=pending,
+                                plan_status=plan.status)
+        # A request that lacks pages is served when there are some.
+        assert bool(((done.status == 0) | (done.status == tree.E_BLOCKS)).all())
         lengths, pending, left = done.lengths, done.pending, left - done.count
-        for r, (n, row) in enumerate(zip(done.count.tolist(), done.ids.tolist())):
+        for r, (n, row, status) in enumerate(zip(done.count.tolist(), done.ids.tolist(), done.status.tolist())):
             result[r].ids += row[:n]
             result[r].steps += n > 0
-    # Requests end: their pages go back.
+            result[r].waits += status == tree.E_BLOCKS
+    # The others end.
     tree.plan_blocks(lengths, i32([-1] * R), table, held, pool, state, blocks=blocks, page=page, capacity=1)
     for o in result:
         o.free_pages = int(state[1])

@@ -194,7 +194,16 @@ typedef struct dsr_tree_attention_args {
  * DSR_E_TOKEN (a negative sampled token on the path), DSR_E_BLOCK (a page id
  * outside the cache): nothing is accepted or moved then and the length is
  * that before the new tokens (0 with DSR_E_LENGTH).
- * A request without new tokens gives an empty path and no pending token. */
+ * A request without new tokens gives an empty path and no pending token.
+ *
+ * Given what was so before the step (lengths_in and plan_status: the plan's
+ * input and result; pending_in: the pending tokens; all three or none), a
+ * request that the plan refused, or that commit gives a status, keeps its
+ * length and pending token, so that a later step can serve it; the status is
+ * the plan's if it has one.  One without new tokens keeps its pending token,
+ * whatever its output_limit, and has the length kv_lengths (0 if the plan
+ * ended it).  Without the three a refused request's context is lost: the plan
+ * gives kv_lengths 0 for it. */
 typedef struct dsr_commit_args {
   const int32_t* parents;      /* [tokens] as dsr_plan_args_t */
   const int32_t* tokens_in;    /* [tokens] drafted token of each node */
@@ -222,6 +231,9 @@ typedef struct dsr_commit_args {
   int32_t heads;               /* rows per token */
   int32_t row_bytes;           /* bytes of one row, a multiple of 16 */
   int64_t c_block, c_token, c_head; /* strides in bytes, multiples of 16 */
+  const int32_t* lengths_in;   /* [requests] as dsr_plan_args_t.lengths, or NULL; none of these is an output */
+  const int32_t* pending_in;   /* [requests] */
+  const int32_t* plan_status;  /* [requests] as dsr_plan_args_t.status */
 } dsr_commit_args_t;
 
 size_t dsr_plan_workspace_bytes(int64_t requests);

@@ -147,15 +147,16 @@ def attention(q, k_cache, v_cache, table, offsets, kv_lengths, visible, scale):
     return out, lse, size
 
 
-def commit(parents, tokens, sampled, offsets, kv_lengths, limit, eos, width, page):
+def commit(parents, tokens, sampled, offsets, kv_lengths, limit, eos, width, page, before=None):
     """dsr_commit_tree's decisions: a list of dicts, one per request
-    (``eos``: a set of ids per request)."""
+    (``eos``: a set of ids per request; ``before``: lengths, pending tokens and
+    the plan's statuses)."""
     out = []
     for r, kv in enumerate(kv_lengths):
         lo, hi = int(offsets[r]), int(offsets[r + 1])
         par, n, kv = [int(p) for p in parents[lo:hi]], hi - lo, int(kv)
         d = dict(path=[], ids=[], pending=-1, stop=0, status=OK)
-        if kv < n or kv > width * page or limit[r] < 1:
+        if kv < n or kv > width * page or (limit[r] < 1 and (n > 0 or before is None)):
             d["status"] = E_LENGTH
         elif not is_tree(par):
             d["status"] = E_TREE
@@ -177,5 +178,11 @@ def commit(parents, tokens, sampled, offsets, kv_lengths, limit, eos, width, pag
                     d["stop"] = reason
                     break
         d["length"] = 0 if d["status"] == E_LENGTH else kv - n + len(d["path"])
+        if before is not None:
+            length, pending, planned = (int(x[r]) for x in before)
+            if planned != OK or d["status"] != OK:
+                d = dict(path=[], ids=[], pending=pending, stop=0, length=length, status=planned or d["status"])
+            elif n == 0:
+                d["pending"] = pending
         out.append(d)
     return out
