@@ -72,6 +72,7 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
+  if ((int)blockIdx.x >= attn_call().p.groups) return attn_clear<T>(attn_call().p.groups, kAttnThreads);
   AttnWork<false> work(attn_call().a, attn_call().p, 0);
   AttnSegment u;
   AttnRequest q;

@@ -182,7 +182,9 @@ void attn_wide(dim3 grid, hipStream_t s, const AttnCall& call) {
 
 template <class T, int DP>
 int32_t attn_launch(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.groups), threads(kAttnThreads);
+  // Workgroups for rows of no request: one for each 256 KB that all rows have, so that a long padding is spread too.
+  const int64_t clear = (a.tokens * a.q_heads * a.head_dim * 2 + (1 << 18) - 1) >> 18;
+  const dim3 grid((unsigned)p.groups + (unsigned)(clear > 256 ? 256 : clear < 8 ? 8 : clear)), threads(kAttnThreads);
   const AttnCall call{a, p};
   switch (p.tile_rows) {
     case 16:

@@ -431,7 +431,8 @@ def tree_attention(q, k_cache, v_cache, table, offsets, kv_lengths, **kw) -> Att
     ``[tokens]``, as ``plan_blocks`` makes it: at most 64 new tokens a request)
     or, without it, those up to itself.  ``scale`` defaults to ``dim ** -0.5``;
     ``lse`` also returns the logarithm of each row's sum.  Rows that see nothing
-    give 0 and -inf.  ``out`` supplies the output tensor."""
+    give 0 and -inf, and so do those past the last request's tokens.  ``out``
+    supplies the output tensor."""
     return PreparedTreeAttention(q, k_cache, v_cache, table, offsets, kv_lengths, **kw).launch()
 
 

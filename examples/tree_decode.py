@@ -63,9 +63,8 @@ class Model:
             q, k, v = (t.view(n, -1, self.head) for t in (q, k, v))
             q = tree.rotary(q, k, plan.positions, self.freqs, v=v, magnitude=self.magnitude, slots=plan.slots,
                             k_cache=k_caches[i], v_cache=v_caches[i]).q
-            out = torch.zeros(n, self.heads, self.head, dtype=torch.bfloat16, device=self.device)
-            tree.tree_attention(q, k_caches[i], v_caches[i], plan.table, plan.offsets, plan.kv_lengths,
-                                visible=plan.visible, out=out)
+            out = tree.tree_attention(q, k_caches[i], v_caches[i], plan.table, plan.offsets, plan.kv_lengths,
+                                      visible=plan.visible).out
             x = x + out.view(n, -1) @ self.out[i].t()
             a, b = (self.norm(x) @ self.up[i].t()).chunk(2, -1)
             x = x + (torch.nn.functional.silu(a) * b) @ self.down[i].t()

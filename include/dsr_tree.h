@@ -144,8 +144,9 @@ typedef struct dsr_rotary_args {
  * and of its own new tokens (the last ones in the cache) those whose bit is
  * set in visible[t], or without `visible` those up to t itself.  Query head h
  * reads key head h / (q_heads / kv_heads).  A row with no visible token gives
- * out 0 and lse -inf.  Values of tokens that a row does not see never reach
- * it, whatever they hold.
+ * out 0 and lse -inf, and so do the rows of no request: those before
+ * offsets[0] and from offsets[requests] on.  Values of tokens that a row does
+ * not see never reach it, whatever they hold.
  * bf16 or f16 rows; products on the matrix cores, scores, softmax statistics
  * and sums in float32; the weights are rounded to the rows' type before
  * they multiply the values.
