@@ -178,7 +178,7 @@ class CommitArgs(ctypes.Structure):
         ("accepted", _p), ("count", _p), ("pending", _p), ("stop", _p), ("lengths", _p), ("status", _p),
         ("requests", _i64), ("tokens", _i64), ("table_ld", _i64), ("width", _i32), ("page", _i32), ("blocks", _i32),
         ("cache_count", _i32), ("heads", _i32), ("row_bytes", _i32), ("c_block", _i64), ("c_token", _i64),
-        ("c_head", _i64), ("lengths_in", _p), ("pending_in", _p), ("plan_status", _p),
+        ("c_head", _i64), ("lengths_in", _p), ("pending_in", _p), ("plan_status", _p), ("host_caches", _p),
     ]
 
 

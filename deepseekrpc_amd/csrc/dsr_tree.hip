@@ -325,7 +325,7 @@ int32_t dsr_commit_tree(const dsr_commit_args_t* args, void* stream) {
       !page_ok(a.page, a.blocks) || a.width < 1 || (int64_t)a.width * a.page > INT_MAX || a.table_ld < a.width ||
       a.cache_count < 0 || a.cache_count > 65535)
     return DSR_ERR_ARG;
-  if (a.cache_count > 0 && (!a.caches || a.heads < 1 || a.heads > 65536 || a.row_bytes < 16 || a.row_bytes > 65536 ||
+  if (a.cache_count > 0 && (!a.caches == !a.host_caches || a.heads < 1 || a.heads > 65536 || a.row_bytes < 16 || a.row_bytes > 65536 ||
                             a.row_bytes % 16 != 0 || a.c_block % 16 != 0 || a.c_token % 16 != 0 || a.c_head % 16 != 0))
     return DSR_ERR_ARG;
   if (a.requests == 0) return 0;
@@ -339,10 +339,24 @@ int32_t dsr_commit_tree(const dsr_commit_args_t* args, void* stream) {
   if (a.lengths_in && (a.lengths == a.lengths_in || a.pending == a.pending_in || a.status == a.plan_status))
     return DSR_ERR_ARG;
   const int per = commit_caches(a);
-  const int groups = a.cache_count > 0 ? (a.cache_count + per - 1) / per : 1;
-  hipLaunchKernelGGL(k_commit_tree, dim3((unsigned)a.requests, (unsigned)groups), dim3(kCommitThreads), 0,
-                     (hipStream_t)stream, a);
-  return launched();
+  auto grid = [&](int count) { return dim3((unsigned)a.requests, count > 0 ? (unsigned)((count + per - 1) / per) : 1u); };
+  hipStream_t s = (hipStream_t)stream;
+  if (!a.host_caches || a.cache_count == 0) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_commit_tree<0>), grid(a.cache_count), dim3(kCommitThreads), 0, s, a,
+                       CommitCaches<0>{});
+    return launched();
+  }
+  // Each launch decides anew: its inputs are no launch's outputs.
+  for (int first = 0; first < a.cache_count; first += kCommitInline) {
+    dsr_commit_args_t part = a;
+    CommitCaches<kCommitInline> caches;
+    part.cache_count = a.cache_count - first < kCommitInline ? a.cache_count - first : kCommitInline;
+    for (int c = 0; c < kCommitInline; ++c) caches.at[c] = c < part.cache_count ? a.host_caches[first + c] : nullptr;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_commit_tree<kCommitInline>), grid(part.cache_count), dim3(kCommitThreads), 0, s,
+                       part, caches);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+  }
+  return 0;
 }
 
 }  // extern "C"

@@ -215,7 +215,7 @@ typedef struct dsr_commit_args {
   const int32_t* output_limit; /* [requests], >= 1 */
   const int64_t* eos_off;      /* [requests + 1] CSR of EOS ids, or NULL */
   const int32_t* eos_ids;
-  void* const* caches;         /* device array of cache_count device pointers */
+  void* const* caches;         /* device array of cache_count device pointers, or NULL with host_caches */
   int32_t* path;               /* [requests, 64] kept nodes, -1 padded */
   int32_t* ids;                /* [requests, 64] output ids, -1 padded */
   int32_t* accepted;           /* [requests] kept nodes, the root among them */
@@ -235,6 +235,7 @@ typedef struct dsr_commit_args {
   const int32_t* lengths_in;   /* [requests] as dsr_plan_args_t.lengths, or NULL; none of these is an output */
   const int32_t* pending_in;   /* [requests] */
   const int32_t* plan_status;  /* [requests] as dsr_plan_args_t.status */
+  void* const* host_caches;    /* the pointers in host memory instead: read during the call, passed with the launch */
 } dsr_commit_args_t;
 
 size_t dsr_plan_workspace_bytes(int64_t requests);
