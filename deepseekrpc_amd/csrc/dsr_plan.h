@@ -4,7 +4,7 @@
 // Two parts.  plan_scan: one workgroup turns lengths and counts into
 // offsets, grants and the pool's ring index of each request's first new page
 // by prefix sums.
-// plan_tokens / plan_trees: every token's slot and position, 64 tokens to a
+// plan_token / plan_tree: every token's slot and position, 64 tokens to a
 // wave, and every new table entry, written by the token that first touches
 // the page (a new page lies wholly past the old tokens, so its first slot is
 // always a new token's).
@@ -27,7 +27,8 @@ namespace dsr {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 
-// What plan_scan leaves for the second part, per request (a.workspace).
+// What plan_scan leaves for the second part, per request (a.workspace; the
+// checkers' flags, kPlanCheckers, lie behind).
 struct PlanRow {
   int32_t ring;  // granted: pool index of the first page taken; ended: of the first page given back
   int32_t old;   // pages held before
@@ -128,6 +129,43 @@ __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
   }
 }
 
+// A request that touches a page outside the cache gets no slot at all, but its
+// tokens are spread over waves that know nothing of each other.  So workgroups
+// beside the scan's look through all pages that the step may touch; only if
+// they find one do the waves look through their requests' pages.
+constexpr int kPlanCheckers = 64;  // workgroups; a flag for each lane of a wave
+
+__device__ __forceinline__ int32_t* plan_flags(const dsr_plan_args_t& a) {
+  return (int32_t*)((PlanRow*)a.workspace + a.requests);
+}
+
+__device__ __forceinline__ void plan_check(const dsr_plan_args_t& a, int checker) {
+  __shared__ int found;
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  const int R = (int)a.requests, shift = __ffs(a.page) - 1, l = threadIdx.x & 63;
+  const unsigned blocks = a.blocks;
+  bool bad = false;
+  // The pages held already, a request a wave.
+  for (int r = checker * kPlanWaves + (int)(threadIdx.x >> 6); r < R; r += kPlanCheckers * kPlanWaves) {
+    const int L = a.lengths[r], A = a.added[r], held = a.held_in[r];
+    if (L < 0 || A <= 0 || (uint32_t)held > (uint32_t)a.width) continue;
+    const uint32_t end = ((uint32_t)L + (uint32_t)A + (uint32_t)a.page - 1) >> shift;
+    for (uint32_t b = ((uint32_t)L >> shift) + l; b < end && b < (uint32_t)held; b += 64)
+      bad |= (unsigned)a.table[r * a.table_ld + b] >= blocks;
+  }
+  // The pool's first pages: a granted request takes at most one more than its tokens fill.
+  const int head = a.pool_state_in[0], count = a.pool_state_in[1], size = a.pool_size;
+  if (head >= 0 && head < size && count <= size) {
+    const int most = (int)(a.capacity >> shift) + R;
+    for (int i = checker * kPlanThreads + (int)threadIdx.x; i < count && i < most; i += kPlanCheckers * kPlanThreads)
+      bad |= (unsigned)a.pool[head + i >= size ? head + i - size : head + i] >= blocks;
+  }
+  if (bad) found = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) plan_flags(a)[checker] = found;
+}
+
 // The slot of place `p` of request r, and, if this is the first slot of a
 // new page, the page's table entry.
 __device__ __forceinline__ int plan_slot(const dsr_plan_args_t& a, const PlanRow& row, int64_t r, int p) {
@@ -180,8 +218,27 @@ __device__ __forceinline__ int plan_count(int x, int i) {
   return __shfl(x, c) <= i ? c + 1 : c;
 }
 
-// Tokens i0 .. i0 + 63 (one wave).
-__device__ __forceinline__ void plan_tokens(const dsr_plan_args_t& a, int i0) {
+// Whether request r's new tokens touch a page outside the cache (one wave).
+__device__ __forceinline__ bool plan_outside(const dsr_plan_args_t& a, int r) {
+  const int shift = __ffs(a.page) - 1, n = a.offsets[r + 1] - a.offsets[r];
+  const PlanRow row = ((const PlanRow*)a.workspace)[r];
+  const int begin = a.lengths[r] >> shift, end = n > 0 ? ((a.lengths[r] + n - 1) >> shift) + 1 : begin;
+  for (int b0 = begin; b0 < end; b0 += 64) {
+    const int b = b0 + (int)(threadIdx.x & 63), at = row.ring + b - row.old;
+    int id = 0;
+    if (b < end) id = b < row.old ? a.table[r * a.table_ld + b] : a.pool[at >= a.pool_size ? at - a.pool_size : at];
+    if (__ballot((unsigned)id >= (unsigned)a.blocks)) return true;
+  }
+  return false;
+}
+
+struct PlanToken {
+  int owner, slot, position;
+  bool granted;  // its request is served
+};
+
+// Token i0 + lane (one wave).
+__device__ __forceinline__ PlanToken plan_token(const dsr_plan_args_t& a, int i0) {
   const int l = threadIdx.x & 63, R = (int)a.requests;
   const int i = i0 + l;
   // Each token's owner lies as many requests behind token i0's as end at or
@@ -192,19 +249,30 @@ __device__ __forceinline__ void plan_tokens(const dsr_plan_args_t& a, int i0) {
     r += r == base ? c : 0;
     base += 64;
   } while (__ballot(c == 64));
-  if (i >= a.capacity) return;
-  if (r >= R || i >= a.offsets[R]) {
-    plan_write(a, i, -1, 0, -1, 0);
-    return;
-  }
+  PlanToken t{-1, -1, 0, false};
+  if (i >= a.capacity || r >= R || i >= a.offsets[R]) return t;
+  t.owner = r;
   const PlanRow row = ((const PlanRow*)a.workspace)[r];
-  if (row.mode != kPlanGranted) {
-    plan_write(a, i, -1, 0, r, 0);
-    return;
+  if (row.mode != kPlanGranted) return t;
+  t.granted = true;
+  t.position = a.lengths[r] + i - a.offsets[r];
+  t.slot = plan_slot(a, row, r, t.position);
+  return t;
+}
+
+// ... and its results.  `doubt`: some request may touch a page outside the cache.
+__device__ __forceinline__ void plan_store(const dsr_plan_args_t& a, int i0, PlanToken t, bool doubt) {
+  const int i = i0 + (int)(threadIdx.x & 63);
+  if (doubt) {
+    uint64_t left = __ballot(t.granted);
+    while (left) {
+      const int r = __shfl(t.owner, __ffsll((unsigned long long)left) - 1);
+      const bool mine = t.granted && t.owner == r;
+      left &= ~__ballot(mine);
+      if (plan_outside(a, r) && mine) t.slot = -1;
+    }
   }
-  const int p = a.lengths[r] + i - a.offsets[r];
-  const int slot = plan_slot(a, row, r, p);
-  plan_write(a, i, slot, slot < 0 ? 0 : p, r, 0);
+  if (i < a.capacity) plan_write(a, i, t.slot, t.slot < 0 ? 0 : t.position, t.owner, 0);
 }
 
 // Request r's pages back to the pool, if it ended (one wave).
@@ -254,10 +322,9 @@ __device__ __forceinline__ void plan_tree(const dsr_plan_args_t& a, int r) {
       up = u;
     }
   }
-  if (l >= n) return;
-  const int p = a.lengths[r] + l;
-  const int slot = plan_slot(a, row, r, p);
-  plan_write(a, lo + l, slot, slot < 0 ? 0 : a.lengths[r] + depth, r, slot < 0 ? 0 : mask);
+  const int slot = l < n ? plan_slot(a, row, r, a.lengths[r] + l) : 0;
+  const bool outside = __ballot(slot < 0) != 0;  // then no node has a slot
+  if (l < n) plan_write(a, lo + l, outside ? -1 : slot, outside ? 0 : a.lengths[r] + depth, r, outside ? 0 : mask);
 }
 
 // Tokens past the last request's (tree plans: the trees write their own).
@@ -265,16 +332,24 @@ __device__ __forceinline__ void plan_padding(const dsr_plan_args_t& a, int i) {
   if (i < a.capacity && i >= a.offsets[a.requests]) plan_write(a, i, -1, 0, -1, 0);
 }
 
-__global__ __launch_bounds__(kPlanThreads) void k_plan_scan(dsr_plan_args_t a) { plan_scan(a); }
+// The first workgroup scans, the others (for tokens without trees) check.
+__global__ __launch_bounds__(kPlanThreads) void k_plan_scan(dsr_plan_args_t a) {
+  if (blockIdx.x > 0)
+    plan_check(a, blockIdx.x - 1);
+  else
+    plan_scan(a);
+}
 
 // 256 threads: workgroups [0, token_groups) take 256 tokens each, the others four requests each.
 __global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_groups) {
   const int w = threadIdx.x >> 6, b = blockIdx.x;
   if (b < token_groups) {
-    if (a.parents)
+    if (a.parents) {
       plan_padding(a, b * 256 + (int)threadIdx.x);
-    else
-      plan_tokens(a, b * 256 + w * 64);
+    } else {
+      const bool doubt = __ballot(a.requests > 0 && plan_flags(a)[threadIdx.x & (kPlanCheckers - 1)] != 0) != 0;
+      plan_store(a, b * 256 + w * 64, plan_token(a, b * 256 + w * 64), doubt);
+    }
     return;
   }
   const int r = (b - token_groups) * 4 + w;
@@ -285,6 +360,8 @@ __global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_
 
 // The whole plan in one workgroup, for calls that fit it.
 __global__ __launch_bounds__(kPlanThreads) void k_plan_small(dsr_plan_args_t a) {
+  __shared__ int doubt;
+  if (threadIdx.x == 0) doubt = 0;
   plan_scan(a);
   __threadfence_block();
   __syncthreads();
@@ -293,7 +370,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_small(dsr_plan_args_t a) 
     for (int i = threadIdx.x; i < a.capacity; i += kPlanThreads) plan_padding(a, i);
     for (int r = w; r < a.requests; r += kPlanWaves) plan_tree(a, r);
   } else {
-    for (int i = w * 64; i < a.capacity; i += kPlanThreads) plan_tokens(a, i);
+    const PlanToken t = plan_token(a, w * 64);  // a token a thread
+    if (t.granted && t.slot < 0) doubt = 1;
+    __syncthreads();
+    plan_store(a, w * 64, t, doubt != 0);
   }
   for (int r = w; r < a.requests; r += kPlanWaves) plan_release(a, r);
 }

@@ -25,6 +25,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // and 7.6, of 16 7.3 and 8.2, of 32 8.7 and 8.3; 128 of 8 7.0 and 7.4, 256 of
 // 2 7.6 and 7.0; 16 trees of 8 nodes 5.5 and 6.4, 32 7.5 and 6.9.
 constexpr int kPlanSmallTokens = 1024, kPlanSmallRequests = 128, kPlanSmallTrees = 16;
+static_assert(kPlanSmallTokens <= kPlanThreads, "a token a thread");
 
 // Whether every row, part and pair of a rotary call can be taken VE elements at a time.
 template <class T>
@@ -231,7 +232,9 @@ int32_t attn_typed(const dsr_tree_attention_args_t& a, const AttnPlan& p, hipStr
 extern "C" {
 
 size_t dsr_plan_workspace_bytes(int64_t requests) {
-  return requests > 0 && requests <= DSR_TREE_MAX_REQUESTS ? (size_t)requests * sizeof(PlanRow) : 0;
+  return requests > 0 && requests <= DSR_TREE_MAX_REQUESTS
+             ? (size_t)requests * sizeof(PlanRow) + kPlanCheckers * sizeof(int32_t)
+             : 0;
 }
 
 int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
@@ -254,7 +257,8 @@ int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
     hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(kPlanThreads), 0, s, a);
     return launched();
   }
-  hipLaunchKernelGGL(k_plan_scan, dim3(1), dim3(kPlanThreads), 0, s, a);
+  const unsigned checkers = a.parents || a.requests == 0 ? 0 : kPlanCheckers;
+  hipLaunchKernelGGL(k_plan_scan, dim3(1 + checkers), dim3(kPlanThreads), 0, s, a);
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   const int token_groups = (int)((a.capacity + 255) / 256);
   hipLaunchKernelGGL(k_plan_fill, dim3((unsigned)(token_groups + (a.requests + 3) / 4)), dim3(256), 0, s, a,

@@ -59,6 +59,8 @@ extern "C" {
  * call.  A request that lacks pages when the pages wanted up to and
  * including it exceed the free ones is refused (DSR_E_BLOCKS), and so is
  * every later request that lacks pages.
+ * A request whose new tokens touch a page id outside the cache is refused
+ * (DSR_E_BLOCK), and keeps the pages that it took.
  *
  * Per token: its slot, its position (lengths[r] + its index, or + its depth
  * in the tree), its request.  With `parents` (per token: the index of its

@@ -87,8 +87,10 @@ def plan(lengths, added, table, held, pool, state, blocks, page, capacity, paren
             positions[i] = L + len(path) - 1
             if tree is not None:
                 visible[i] = sum(1 << p for p in path)
-        if bad_page:
+        if bad_page:  # a refused request's tokens have no slot, on whatever page they would lie
             st, serves = E_BLOCK, False
+            for i in range(lo, hi):
+                slots[i], positions[i], visible[i] = -1, 0, 0
         kv.append(L + A if serves else 0)
         held_out.append(new_held)
         status.append(st)
