@@ -46,6 +46,12 @@ def _device_of(t, name):
     return t.device
 
 
+def _unrecorded(name, *tensors):
+    """A gradient that would be dropped without a word is an error."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} is not recorded for gradients: call it under torch.no_grad() or on detached tensors")
+
+
 def _array(t, name, dtype, dev, numel=None):
     """A contiguous device array; its pointer."""
     if _device_of(t, name) != dev:
@@ -275,6 +281,7 @@ class PreparedRotary(_Prepared):
                  k_out=None):
         one = q if q is not None else k
         dev = _device_of(one, "q" if q is not None else "k")
+        _unrecorded("rotary", q, k, v, k_cache, v_cache, q_out, k_out)
         if one.dim() != 3 or one.dtype not in _ROTARY_TYPES:
             raise ValueError("q and k must be bf16/f16/f32 of shape [tokens, heads, dim]")
         n, dim, dtype = one.shape[0], one.shape[2], one.dtype
@@ -351,7 +358,11 @@ def rotary(q, k, positions, freqs, **kw) -> RotaryResult:
     With ``slots`` (int32 ``[tokens]``; -1: none) the rotated keys go to
     ``k_cache`` and ``v`` to ``v_cache`` there.  Results go to ``q_out`` and
     ``k_out`` (new tensors by default, ``k_out`` only without a key cache;
-    ``q`` and ``k`` themselves are allowed)."""
+    ``q`` and ``k`` themselves are allowed).
+
+    The call is not recorded for gradients, and refuses tensors that require
+    one unless recording is off.  In a ``torch.autograd.Function`` of a training
+    program the backward pass is ``rotary(grad, ..., inverse=True)``."""
     return PreparedRotary(q, k, positions, freqs, **kw).launch()
 
 
@@ -372,6 +383,7 @@ class PreparedTreeAttention(_Prepared):
     def __init__(self, q, k_cache, v_cache, table, offsets, kv_lengths, *, visible=None, scale: float | None = None,
                  lse: bool = False, out=None):
         dev = _device_of(q, "q")
+        _unrecorded("tree_attention", q, k_cache, v_cache, out)
         if q.dim() != 3 or q.dtype not in _ATTENTION_TYPES:
             raise ValueError("q must be bf16/f16 of shape [tokens, heads, dim]")
         n, heads, dim = q.shape
@@ -432,7 +444,8 @@ def tree_attention(q, k_cache, v_cache, table, offsets, kv_lengths, **kw) -> Att
     or, without it, those up to itself.  ``scale`` defaults to ``dim ** -0.5``;
     ``lse`` also returns the logarithm of each row's sum.  Rows that see nothing
     give 0 and -inf, and so do those past the last request's tokens.  ``out``
-    supplies the output tensor."""
+    supplies the output tensor.  There is no backward pass: tensors that require
+    a gradient are refused unless recording is off."""
     return PreparedTreeAttention(q, k_cache, v_cache, table, offsets, kv_lengths, **kw).launch()
 
 
