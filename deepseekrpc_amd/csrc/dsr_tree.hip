@@ -41,6 +41,9 @@ bool rotary_fits(const dsr_rotary_args_t& a, int VE) {
          (!a.v_cache || (rows(a.v_cache, a.vc_token, a.vc_head) && a.vc_block % VE == 0));
 }
 
+// Tokens of one launch: a workgroup each, and a launch has less than 2^32 threads.
+constexpr int64_t kRotaryTokens = 1 << 23;
+
 template <class T, int VE>
 void rotary_launch(const dsr_rotary_args_t& a, hipStream_t s) {
   const int64_t items = (int64_t)(a.q_heads + a.kv_heads) * a.head_dim / VE;
@@ -61,13 +64,27 @@ void rotary_launch(const dsr_rotary_args_t& a, hipStream_t s) {
 template <class T>
 int32_t rotary_typed(const dsr_rotary_args_t& a, hipStream_t s) {
   constexpr int VE = 16 / sizeof(T);
-  if (rotary_fits<T>(a, VE))
-    rotary_launch<T, VE>(a, s);
-  else if (rotary_fits<T>(a, 4))  // halves of 12 or 20, say (float32 rows have come here as 16 bytes already)
-    rotary_launch<T, 4>(a, s);
-  else
-    rotary_launch<T, 1>(a, s);
-  return launched();
+  const bool wide = rotary_fits<T>(a, VE);
+  const bool half = rotary_fits<T>(a, 4);  // halves of 12 or 20, say (float32 rows are wide then)
+  for (int64_t first = 0; first < a.tokens; first += kRotaryTokens) {
+    dsr_rotary_args_t part = a;
+    part.tokens = a.tokens - first < kRotaryTokens ? a.tokens - first : kRotaryTokens;
+    part.positions += first;
+    if (a.slots) part.slots += first;
+    if (a.status) part.status += first;
+    if (a.q) part.q = (const T*)a.q + first * a.q_token, part.q_out = (T*)a.q_out + first * a.qo_token;
+    if (a.k) part.k = (const T*)a.k + first * a.k_token;
+    if (a.k_out) part.k_out = (T*)a.k_out + first * a.ko_token;
+    if (a.v) part.v = (const T*)a.v + first * a.v_token;
+    if (wide)
+      rotary_launch<T, VE>(part, s);
+    else if (half)
+      rotary_launch<T, 4>(part, s);
+    else
+      rotary_launch<T, 1>(part, s);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+  }
+  return 0;
 }
 
 // Dimensions of the kernel that takes a head dimension (the rest are zeros in LDS).
