@@ -27,14 +27,23 @@ namespace dsr {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 
-// What plan_scan leaves for the second part, per request (a.workspace; the
-// checkers' flags, kPlanCheckers, lie behind).
+// What plan_scan leaves for the second part, per request (a.workspace; a
+// PlanTail lies behind).
 struct PlanRow {
   int32_t ring;  // granted: pool index of the first page taken; ended: of the first page given back
   int32_t old;   // pages held before
+  int32_t held;  // and after
   int32_t mode;  // kPlanRefused / kPlanGranted / kPlanEnded
 };
 constexpr int kPlanRefused = 0, kPlanGranted = 1, kPlanEnded = 2;
+constexpr int kPlanCheckers = 64;  // workgroups; a flag for each lane of a wave
+struct PlanTail {
+  int32_t flags[kPlanCheckers];  // a page outside the cache (plan_check)
+  int32_t state[2];              // the pool's afterwards
+};
+__device__ __forceinline__ PlanTail* plan_tail(const dsr_plan_args_t& a) {
+  return (PlanTail*)((PlanRow*)a.workspace + a.requests);
+}
 
 // Sums of counts that are at most 2^30 each: they stop at 2^31 - 1, above
 // every bound they are compared with, so that 32 bits are enough for counts
@@ -55,13 +64,15 @@ __device__ __forceinline__ int plan_wave_scan(int x) {
 
 constexpr int kPlanSums = 3;  // tokens, pages wanted, pages given back
 
-// One workgroup of 1,024 threads, a request per thread and round.
+// One workgroup of 1,024 threads, a request per thread and round.  `checked`:
+// other workgroups are reading pages held and pool state, whose new values,
+// which may replace them, wait in the workspace for the second part.
 //
 // One scan of the three counts serves every decision.  A request that does
 // not fit the token arrays, or finds the pool short, still counts in the sums
 // of those behind it: by then no later request with tokens, or without its
 // pages, can be granted either, and the others want none.
-__device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
+__device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a, bool checked) {
   __shared__ int part[kPlanSums][kPlanWaves];
   __shared__ int done[2];  // pages taken and given back in all
   const int R = (int)a.requests;
@@ -112,11 +123,12 @@ __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
       p.ring = granted && need > 0 ? wrap(head + sum[1] - need)
                                    : frees && give > 0 ? wrap(wrap(head + count) + sum[2] - give) : 0;
       p.old = held;
+      p.held = granted ? held + need : frees ? 0 : held;
       p.mode = granted ? kPlanGranted : frees ? kPlanEnded : kPlanRefused;
       rows[r] = p;
       a.offsets[r + 1] = sum[0] < capacity ? sum[0] : capacity;
       a.kv_lengths[r] = granted ? L + take : 0;
-      a.held_out[r] = granted ? held + need : frees ? 0 : held;
+      if (!checked) a.held_out[r] = p.held;
       a.status[r] = status;
     }
     if (granted && need > 0) atomicMax(&done[0], sum[1]);
@@ -124,8 +136,9 @@ __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    a.pool_state_out[0] = wrap(head + done[0]);
-    a.pool_state_out[1] = count - done[0] + done[1];
+    int32_t* state = checked ? plan_tail(a)->state : a.pool_state_out;
+    state[0] = wrap(head + done[0]);
+    state[1] = count - done[0] + done[1];
   }
 }
 
@@ -133,12 +146,6 @@ __device__ __forceinline__ void plan_scan(const dsr_plan_args_t& a) {
 // tokens are spread over waves that know nothing of each other.  So workgroups
 // beside the scan's look through all pages that the step may touch; only if
 // they find one do the waves look through their requests' pages.
-constexpr int kPlanCheckers = 64;  // workgroups; a flag for each lane of a wave
-
-__device__ __forceinline__ int32_t* plan_flags(const dsr_plan_args_t& a) {
-  return (int32_t*)((PlanRow*)a.workspace + a.requests);
-}
-
 __device__ __forceinline__ void plan_check(const dsr_plan_args_t& a, int checker) {
   __shared__ int found;
   if (threadIdx.x == 0) found = 0;
@@ -163,7 +170,7 @@ __device__ __forceinline__ void plan_check(const dsr_plan_args_t& a, int checker
   }
   if (bad) found = 1;
   __syncthreads();
-  if (threadIdx.x == 0) plan_flags(a)[checker] = found;
+  if (threadIdx.x == 0) plan_tail(a)->flags[checker] = found;
 }
 
 // The slot of place `p` of request r, and, if this is the first slot of a
@@ -337,23 +344,27 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_scan(dsr_plan_args_t a) {
   if (blockIdx.x > 0)
     plan_check(a, blockIdx.x - 1);
   else
-    plan_scan(a);
+    plan_scan(a, gridDim.x > 1);
 }
 
 // 256 threads: workgroups [0, token_groups) take 256 tokens each, the others four requests each.
-__global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_groups) {
+__global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_groups, bool checked) {
   const int w = threadIdx.x >> 6, b = blockIdx.x;
   if (b < token_groups) {
     if (a.parents) {
       plan_padding(a, b * 256 + (int)threadIdx.x);
     } else {
-      const bool doubt = __ballot(a.requests > 0 && plan_flags(a)[threadIdx.x & (kPlanCheckers - 1)] != 0) != 0;
+      const bool doubt = checked && __ballot(plan_tail(a)->flags[threadIdx.x & (kPlanCheckers - 1)] != 0) != 0;
       plan_store(a, b * 256 + w * 64, plan_token(a, b * 256 + w * 64), doubt);
     }
     return;
   }
   const int r = (b - token_groups) * 4 + w;
   if (r >= a.requests) return;
+  if (checked) {  // new values that waited
+    if ((threadIdx.x & 63) == 0) a.held_out[r] = ((const PlanRow*)a.workspace)[r].held;
+    if (r == 0 && threadIdx.x < 2) a.pool_state_out[threadIdx.x] = plan_tail(a)->state[threadIdx.x];
+  }
   if (a.parents) plan_tree(a, r);
   plan_release(a, r);
 }
@@ -362,7 +373,7 @@ __global__ __launch_bounds__(256) void k_plan_fill(dsr_plan_args_t a, int token_
 __global__ __launch_bounds__(kPlanThreads) void k_plan_small(dsr_plan_args_t a) {
   __shared__ int doubt;
   if (threadIdx.x == 0) doubt = 0;
-  plan_scan(a);
+  plan_scan(a, false);
   __threadfence_block();
   __syncthreads();
   const int w = threadIdx.x >> 6;

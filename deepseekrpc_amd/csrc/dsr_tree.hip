@@ -250,7 +250,7 @@ extern "C" {
 
 size_t dsr_plan_workspace_bytes(int64_t requests) {
   return requests > 0 && requests <= DSR_TREE_MAX_REQUESTS
-             ? (size_t)requests * sizeof(PlanRow) + kPlanCheckers * sizeof(int32_t)
+             ? (size_t)requests * sizeof(PlanRow) + sizeof(PlanTail)
              : 0;
 }
 
@@ -279,7 +279,7 @@ int32_t dsr_plan_blocks(const dsr_plan_args_t* args, void* stream) {
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   const int token_groups = (int)((a.capacity + 255) / 256);
   hipLaunchKernelGGL(k_plan_fill, dim3((unsigned)(token_groups + (a.requests + 3) / 4)), dim3(256), 0, s, a,
-                     token_groups);
+                     token_groups, checkers > 0);
   return launched();
 }
 

@@ -60,3 +60,17 @@ def test_bad_pages_that_the_step_does_not_touch():
     c["pool"][(c["state"][0] + np.arange(used, c["state"][1])) % len(c["pool"])] = -3  # not taken this time
     want = check(c)
     assert not want["status"].any()
+
+
+@pytest.mark.parametrize("R,new_hi", [(16384, 1), (9000, 9), (2000, 70)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_pages_held_and_pool_replaced_in_place(R, new_hi, in_place):
+    """The pages are looked through while the scan settles what is held and
+    free: in many requests and in place, bad pages are found all the same."""
+    rng = np.random.default_rng([R, new_hi])
+    c = case(rng, R, new_hi, 40, 4, False, ended=0.02)
+    hit = rng.choice(R, 12, replace=False)
+    c["added"][hit] = new_hi
+    c["capacity"] = max(1, int(c["added"].clip(0).sum()))
+    want = check(with_bad_pages(c, rng, hit, c["blocks"]), in_place)
+    assert (want["status"][hit] == O.E_BLOCK).all()
