@@ -513,14 +513,14 @@ class PreparedCommit(_Prepared):
             if a.row_bytes % 16 or not 16 <= a.row_bytes <= 65536 or any(s % 16 for s in strides):
                 raise ValueError("cache rows must be multiples of 16 bytes, 16-byte aligned")
             a.c_block, a.c_token, a.c_head = strides
-            addresses = [t.data_ptr() for t in caches]
+            addresses = list(dict.fromkeys(t.data_ptr() for t in caches))  # one listed twice is moved once
             if upload:
                 pointers = torch.tensor(addresses, dtype=torch.int64, device=dev)
                 a.caches = pointers.data_ptr()
             else:
-                pointers = (ctypes.c_void_p * len(caches))(*addresses)
+                pointers = (ctypes.c_void_p * len(addresses))(*addresses)
                 a.host_caches = ctypes.addressof(pointers)
-            a.cache_count = len(caches)
+            a.cache_count = len(addresses)
         elif page is None or blocks is None:
             raise ValueError("without caches, page and blocks are needed")
         else:
@@ -541,7 +541,8 @@ def commit_tree(parents, tokens, sampled, offsets, kv_lengths, table, caches, *,
                 eos_ids=None, page: int | None = None, blocks: int | None = None, lengths=None, pending=None,
                 plan_status=None) -> CommitResult:
     """The accepted path of each request's drafted tree, and its cache rows
-    moved together in every one of ``caches``.
+    moved together in every one of ``caches`` (once in one that is listed twice,
+    as keys that are also the values).
 
     ``tokens`` and ``sampled`` (int32) are each node's drafted token and the
     target's token drawn after it (``batch.sample_rows`` over the nodes' rows:

@@ -190,8 +190,8 @@ typedef struct dsr_tree_attention_args {
  * matches, is the new pending token.  Stops are those of verify_drafts: an
  * accepted draft whose token is an EOS id or reaches output_limit ends the
  * path there, with no pending token (-1); a pending token can stop likewise.
- * Then, in each of the `caches`, the path's rows are moved together: path node
- * j's row to place lengths + j.
+ * Then, in each of the `caches` (no two of which overlap), the path's rows are
+ * moved together: path node j's row to place lengths + j.
  * Status: DSR_E_TREE (parents, or more than 64 nodes), DSR_E_LENGTH
  * (kv_lengths below the new tokens or above width * page, output_limit < 1),
  * DSR_E_TOKEN (a negative sampled token on the path), DSR_E_BLOCK (a page id

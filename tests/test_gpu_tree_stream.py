@@ -87,3 +87,19 @@ def test_the_call_in_a_graph():
         eager = tree.commit_tree(*args, [t.clone() for t in start], output_limit=limit)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(vars(got).values(), vars(eager).values())), turn
+
+
+@pytest.mark.parametrize("upload", [False, True])
+def test_a_cache_listed_twice_is_moved_once(upload):
+    """Keys that are also the values: moved twice, a path's rows would move on."""
+    rng = np.random.default_rng(4)
+    c = case(rng, [40] * 5, 8)
+    for r in range(5):  # every second node of a chain's siblings is kept
+        c["parents"][40 * r:40 * r + 40] = [-1] + [2 * ((i - 1) // 2) for i in range(1, 40)]
+    c["tokens"][:], c["sampled"][:], c["limit"][:] = np.arange(200) % 2, 0, 64
+    caches, args = caches_of(rng, c, 3, 2, 64), arguments(c)
+    want = moved(c, caches)
+    assert not all(torch.equal(x, y) for x, y in zip(caches, want))
+    often = 50 * caches  # more than one launch's, where the addresses go with it
+    tree.PreparedCommit(*args, often, output_limit=i32(c["limit"]), upload=upload).launch()
+    assert all(torch.equal(x, y) for x, y in zip(caches, want))
