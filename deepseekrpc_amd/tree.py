@@ -72,6 +72,17 @@ def _rows(t, name, dtype, dev, shape):
     return (t.data_ptr(), *t.stride()[:-1])
 
 
+def _overlap(a, b):
+    def span(t):
+        first = t.data_ptr()
+        return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _table(t, rows, dev):
     if _device_of(t, "table") != dev:
         raise ValueError(f"table must be on {dev}")
@@ -187,6 +198,7 @@ class PreparedPlan(_Prepared):
         if parents is not None:
             a.parents = _array(parents, "parents", torch.int32, dev, capacity)
         out = dict(out or {})
+        given = [key for key, t in out.items() if t is not None]
         i32 = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
 
         def result(key, n, default):
@@ -204,6 +216,16 @@ class PreparedPlan(_Prepared):
                          result("status", R, lambda: i32(R)))
         if out:
             raise ValueError(f"unused out tensors: {sorted(out)}")
+        # Results are written while inputs and other results are still read.
+        memory = dict(lengths=lengths, added=added, table=table, held=held, pool=pool, state=state, parents=parents)
+        for key in given:
+            t = getattr(res, key)
+            if key in ("held", "state") and t.data_ptr() == memory[key].data_ptr():
+                continue  # in place
+            for name, other in memory.items():
+                if other is not None and _overlap(t, other):
+                    raise ValueError(f"out['{key}'] must not overlap {name}")
+            memory[f"out['{key}']"] = t
         a.requests, a.capacity, a.page, a.pool_size, a.blocks = R, capacity, page, pool.numel(), blocks
         for field, t in (("held_out", res.held), ("pool_state_out", res.state), ("offsets", res.offsets),
                          ("kv_lengths", res.kv_lengths), ("status", res.status), ("slots", res.slots),
@@ -227,7 +249,7 @@ def plan_blocks(lengths, added, table, held, pool, state, *, blocks: int, page: 
     ``parents`` (int32 ``[capacity]``, the index of each node's parent among
     its request's new tokens, -1 for none) makes them trees.  ``held`` and
     ``state`` are updated in place unless ``out`` has others; ``out`` may
-    supply any of the int32 results.  Requests that cannot be served are
+    supply any of the int32 results, in memory of their own.  Requests that cannot be served are
     refused with a status, and their tokens get slot -1."""
     return PreparedPlan(lengths, added, table, held, pool, state, blocks=blocks, page=page, capacity=capacity,
                         parents=parents, out=out).launch()

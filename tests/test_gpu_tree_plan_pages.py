@@ -2,9 +2,12 @@
 whatever page they would lie and in whatever part of the work they fall."""
 import numpy as np
 import pytest
+import torch
 
+from deepseekrpc_amd import tree
 from oracle import tree_oracle as O
 from tests.test_gpu_tree_plan import case, check
+from tests.tree_util import i32
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +77,20 @@ def test_pages_held_and_pool_replaced_in_place(R, new_hi, in_place):
     c["capacity"] = max(1, int(c["added"].clip(0).sum()))
     want = check(with_bad_pages(c, rng, hit, c["blocks"]), in_place)
     assert (want["status"][hit] == O.E_BLOCK).all()
+
+
+def test_results_in_memory_that_is_still_read():
+    """Lengths replaced by the plan's own lengths would move every later token."""
+    lengths, added, held, state = i32([9, 20]), i32([3, 2]), i32([2, 3]), i32([0, 4])
+    table, pool = i32([[0, 1, -1], [2, 3, 4]]), i32([5, 6, 7, 8])
+    args, kw = (lengths, added, table, held, pool, state), dict(blocks=9, page=8, capacity=5)
+    buffer = i32(np.zeros(40))
+    good = [dict(held=held, state=state), dict(held=torch.empty_like(held)), dict(slots=buffer[:5], owners=buffer[5:10]),
+            dict(slots=None, kv_lengths=buffer[:2])]
+    for out in good:
+        tree.PreparedPlan(*args, **kw, out=out)
+    for out in (dict(kv_lengths=lengths), dict(kv_lengths=added), dict(status=lengths), dict(status=held),
+                dict(held=lengths), dict(state=added), dict(offsets=pool[:3]), dict(kv_lengths=table[1, :2]),
+                dict(slots=buffer[:5], owners=buffer[4:9]), dict(slots=buffer[:5], positions=buffer[:5])):
+        with pytest.raises(ValueError, match="overlap"):
+            tree.PreparedPlan(*args, **kw, out=out)
