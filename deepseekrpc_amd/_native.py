@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 LIB_NAME = "libdsr_sampling.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 

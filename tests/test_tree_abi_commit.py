@@ -34,3 +34,9 @@ def test_the_state_before_the_step_is_no_output(field, output):
     a.caches, a.lengths_in, a.pending_in, a.plan_status = 4096, 4, 4, 4
     setattr(a, field, getattr(a, output))
     assert N.load().dsr_commit_tree(ctypes.byref(a), None) == -1
+
+
+def test_structs_and_the_version_that_gates_them():
+    """A library reads whole structs: whoever makes one longer raises the version."""
+    sizes = {s: ctypes.sizeof(getattr(N, s)) for s in ("PlanArgs", "RotaryArgs", "TreeAttentionArgs", "CommitArgs")}
+    assert (N.ABI_VERSION, sizes) == (7, dict(PlanArgs=184, RotaryArgs=280, TreeAttentionArgs=232, CommitArgs=248))
