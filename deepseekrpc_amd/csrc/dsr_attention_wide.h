@@ -38,8 +38,8 @@ constexpr int attn_round(int DP) { return kAttnThreads / (DP / 8); }
 // What bounds a step: the instructions a SIMD has to issue for its two waves
 // (a 32 x 32 x 16 product takes 16 of the issue cycles and 32 of the matrix
 // core's, an exponential 13, others 4), not the products themselves.  8 trees
-// of 64 nodes over 32,001 tokens, 64 and 8 heads of 128: 684 to 705 us, 760 to
-// 785 TFLOP/s; 32 ragged trees over up to 8,192 tokens 203 to 207.  64 rows
+// of 64 nodes over 32,001 tokens, 64 and 8 heads of 128: 681 to 705 us, 760 to
+// 787 TFLOP/s; 32 ragged trees over up to 8,192 tokens 196 to 200.  64 rows
 // a wave, with half the LDS reads a row, came out no faster (8 trees of 64
 // nodes over 32,065 tokens: 710 us against 706 then) and wasted more on ragged
 // rows.

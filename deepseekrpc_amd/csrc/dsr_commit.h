@@ -1,5 +1,5 @@
 // Acceptance of drafted trees and their cache rows moved together
-// (dsr_commit_tree).
+// (dsr_commit_tree).  What a step refused keeps its length and pending token.
 //
 // A workgroup takes one request and a few caches.  Its first wave walks the
 // tree with one node per lane: the children of the current node whose token
@@ -14,7 +14,8 @@
 // thread owns a 16-byte column of the rows and does just that.
 // What bounds it: a chain of a few dependent reads (tree, page ids, rows),
 // then 2 x row bytes per move and cache.  64 trees, 48 layers of keys and
-// values, about 35 MB moved: 9.6 us, 3.7 TB/s; 8 trees 3.6 to 4.0.
+// values, about 35 MB moved: 10.5 to 11.5 us, 3.1 to 3.4 TB/s, on caches that
+// change from call to call; 8 trees, 4 layers, 3.8 to 4.3.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -25,13 +26,14 @@
 namespace dsr {
 
 constexpr int kCommitThreads = 256;
-constexpr int kCommitBatch = 4;  // rows in flight per thread (64 trees: 10.1 us with two, 9.6 with four, 9.7 with eight)
+// Rows in flight per thread (64 trees, the same caches again and again: 10.1 us with two, 9.6 with four, 9.7 with eight).
+constexpr int kCommitBatch = 4;
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 // Caches per workgroup: as many as its threads cover with one 16-byte column
-// each, at most 8 (64 trees: 11.9 us with one, 9.6 with two to sixteen; the
-// fewer, the more often a request's tree is walked).
+// each, at most 8 (64 trees, as above: 11.9 us with one, 9.6 with two to
+// sixteen; the fewer, the more often a request's tree is walked).
 __host__ __device__ inline int commit_caches(const dsr_commit_args_t& a) {
   const int columns = a.heads * (a.row_bytes / 16);
   const int c = columns > 0 ? kCommitThreads / columns : 1;

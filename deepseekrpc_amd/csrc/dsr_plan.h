@@ -11,9 +11,9 @@
 //
 // What bounds it is latency: a call reads and writes a few KB to a few MB,
 // and its chain is load -> three scans -> offset search -> table entry ->
-// store.  64 requests of one token 5.3 us in one launch; 256 trees of 9 to 33
-// nodes 7.7 in two; 1,024 prompts with 523,000 tokens (6.3 MB written) 12.6:
-// 6.5 the one workgroup's scan, 6.2 the rest.
+// store.  64 requests of one token 6.0 us in one launch; 256 trees of 9 to 33
+// nodes 7.7 to 8.2 in two; 1,024 prompts with 523,000 tokens (6.3 MB written)
+// 12.6: 6.1 the one workgroup's scan, 6.0 the rest.
 #pragma once
 
 #include <hip/hip_runtime.h>

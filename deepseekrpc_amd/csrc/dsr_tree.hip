@@ -21,9 +21,9 @@ bool page_ok(int32_t page, int32_t blocks) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // Plans of at most this many tokens and requests (trees) run in one workgroup
-// and launch.  Us a call in one launch against two: 64 requests of 1 token 5.7
-// and 7.6, of 16 7.3 and 8.2, of 32 8.7 and 8.3; 128 of 8 7.0 and 7.4, 256 of
-// 2 7.6 and 7.0; 16 trees of 8 nodes 5.5 and 6.4, 32 7.5 and 6.9.
+// and launch.  Us a call in one launch against two: 64 requests of 1 token 6.6
+// and 7.1, of 16 8.3 and 8.8; 128 of 8 8.3 and 8.2, 256 of 2 8.9 and 7.9; 16
+// trees of 8 nodes 6.5 and 7.1, of 32 6.9 and 7.3, 24 of 8 7.5 and 7.3.
 constexpr int kPlanSmallTokens = 1024, kPlanSmallRequests = 128, kPlanSmallTrees = 16;
 static_assert(kPlanSmallTokens <= kPlanThreads, "a token a thread");
 
