@@ -1,5 +1,5 @@
-"""ctypes binding of ``libdsr_sampling.so`` (declared in include/dsr_sampling.h
-and include/dsr_tree.h).
+"""ctypes binding of ``libdsr_sampling.so`` (declared in include/dsr_sampling.h,
+include/dsr_tree.h and include/dsr_branch.h).
 
 The library is built in-tree by ``deepseekrpc_amd.build`` and is loaded from
 next to this file.  There is no fallback: if the library is missing, or its
@@ -58,17 +58,27 @@ EXPORTS = (
 TREE_EXPORTS = (
     "dsr_plan_workspace_bytes", "dsr_tree_attention_workspace_bytes", "dsr_plan_blocks", "dsr_rotary", "dsr_tree_attention", "dsr_commit_tree",
 )
+# include/dsr_branch.h
+BRANCH_EXPORTS = (
+    "dsr_select_beams_workspace_bytes", "dsr_fork_workspace_bytes", "dsr_compact_workspace_bytes",
+    "dsr_prefix_attention_workspace_bytes", "dsr_select_beams", "dsr_fork_pages", "dsr_compact_pages",
+    "dsr_prefix_attention",
+)
 F16 = 4
 E_LENGTH = 16
 E_BLOCKS = 17
 E_CAPACITY = 18
 E_TREE = 19
 E_BLOCK = 20
+E_PARENT = 21
 TREE_MAX_NODES = 64
 TREE_MAX_PAGE = 1024
 TREE_MAX_REQUESTS = 16384
 ROTARY_MAX_DIM = 512
 ATTENTION_MAX_DIM = 256
+BEAMS_MAX_KEEP = 64
+BEAMS_MAX_VOCAB = 1048576
+BEAMS_MAX_ROWS = 65536
 NOALLOC_SCRATCH_BYTES = 268435456
 HEAD_TILE = 128
 STATS_MAX_ROWS = 16
@@ -182,6 +192,42 @@ class CommitArgs(ctypes.Structure):
     ]
 
 
+class SelectBeamsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _p), ("scores", _p), ("finished", _p), ("offsets", _p), ("parents", _p), ("tokens", _p),
+        ("out_scores", _p), ("status", _p), ("dtype", _i32), ("keep", _i32), ("rows", _i64), ("groups", _i64),
+        ("vocab", _i64), ("ld", _i64), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class ForkArgs(ctypes.Structure):
+    _fields_ = [
+        ("lengths", _p), ("held", _p), ("table", _p), ("parents", _p), ("shared", _p), ("pool_state", _p),
+        ("pool", _p), ("table_out", _p), ("held_out", _p), ("lengths_out", _p), ("shared_out", _p),
+        ("pool_state_out", _p), ("status", _p), ("source_status", _p), ("caches", _p), ("host_caches", _p),
+        ("sources", _i64), ("rows", _i64), ("table_ld", _i64), ("table_out_ld", _i64), ("width", _i32),
+        ("page", _i32), ("blocks", _i32), ("pool_size", _i32), ("cache_count", _i32), ("heads", _i32),
+        ("row_bytes", _i32), ("reserved", _i32), ("c_block", _i64), ("c_token", _i64), ("c_head", _i64),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class CompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("held", _p), ("table", _p), ("shared", _p), ("pool", _p), ("pool_state", _p), ("table_out", _p),
+        ("shared_out", _p), ("pool_out", _p), ("pool_state_out", _p), ("remap", _p), ("status", _p), ("caches", _p),
+        ("host_caches", _p), ("rows", _i64), ("table_ld", _i64), ("table_out_ld", _i64), ("width", _i32),
+        ("page", _i32), ("blocks", _i32), ("first", _i32), ("pool_size", _i32), ("cache_count", _i32),
+        ("heads", _i32), ("row_bytes", _i32), ("c_block", _i64), ("c_token", _i64), ("c_head", _i64),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    _anonymous_ = ("a",)
+    _fields_ = [("a", TreeAttentionArgs), ("groups", _p), ("prefix_lengths", _p), ("group_count", _i64)]
+
+
 class NativeUnavailable(RuntimeError):
     """The HIP library is missing or incompatible; there is no CPU fallback."""
 
@@ -249,6 +295,13 @@ def load(path: str = LIB_PATH):
                        ("dsr_tree_attention", TreeAttentionArgs), ("dsr_commit_tree", CommitArgs)):
         getattr(lib, name).restype = _i32
         getattr(lib, name).argtypes = [ctypes.POINTER(args), _p]
+    for name, args in (("select_beams", SelectBeamsArgs), ("fork", ForkArgs), ("compact", CompactArgs),
+                       ("prefix_attention", PrefixAttentionArgs)):
+        getattr(lib, f"dsr_{name}_workspace_bytes").restype = ctypes.c_size_t
+        getattr(lib, f"dsr_{name}_workspace_bytes").argtypes = [ctypes.POINTER(args)]
+        call = getattr(lib, f"dsr_{name}" + ("_pages" if name in ("fork", "compact") else ""))
+        call.restype = _i32
+        call.argtypes = [ctypes.POINTER(args), _p]
     _lib = lib
     return lib
 

@@ -27,6 +27,8 @@ SOURCES = {
                          "dsr_wide.h", "dsr_wide_verify.h"],
     "dsr_tree.hip": ["dsr_plan.h", "dsr_rotary.h", "dsr_attention.h", "dsr_attention_wide.h",
                      "dsr_commit.h"],
+    "dsr_branch.hip": ["dsr_beams.h", "dsr_pages.h"],
+    "dsr_prefix.hip": ["dsr_prefix.h", "dsr_attention.h", "dsr_attention_wide.h"],
 }
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

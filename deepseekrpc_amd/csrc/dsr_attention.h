@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dsr_tree.h"
 
 namespace dsr {
@@ -41,6 +43,15 @@ struct AttnType<_Float16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
 };
+
+// Parts for a later join keep bf16 weights at most 1 (of a running maximum
+// that may be passed by 2^8): their sums of values near the type's largest
+// stay in float32's range as long as the values' weighted mean times the sum
+// of weights does.
+template <class T, bool BRANCH>
+constexpr float attn_lift() {
+  return AttnType<T>::kLift - (BRANCH && AttnType<T>::kLift == 0.f ? 8.f : 0.f);
+}
 
 // Transposing LDS read: of the 16 lanes of a group, lane i points at four
 // elements of row i / 4 (columns 4 (i % 4) ...) of a 4 x 16 block and gets the
@@ -79,18 +90,54 @@ struct AttnCall {
   dsr_tree_attention_args_t a;
   AttnPlan p;
 };
-__device__ __forceinline__ const AttnCall& attn_call() {
-  typedef const AttnCall __attribute__((address_space(4))) * Args;
+
+// dsr_prefix_attention goes over the rows twice, with these kernels: once over
+// the groups' prefixes (a "request" is a group then, with the tokens of all
+// its requests, and every row sees every token), once over each request's own
+// tokens behind its prefix.  Every result is a part, whose join is another
+// launch: whole tiles go to rows of float32.
+struct AttnBranch {
+  const int32_t* groups;  // the groups' pass: [count + 1], else null
+  const int32_t* prefix;  // the groups' pass: [count]
+  const int32_t* low;     // the requests' pass: first token of each one's own, -1: refused
+  int32_t* begin;         // [count + 1]: steps before each request
+  int32_t* bad;           // [count]: a page id outside the cache
+  float* row_o;           // [tokens, query heads, head dim of the kernel]
+  float2* row_ml;         // [tokens, query heads]: base (log2) and sum
+  int64_t count;          // groups or requests
+  int32_t* lows;          // the groups' pass writes these: `low`,
+  int32_t* group_of;      // and each request's group, -1: none
+  int64_t requests;
+};
+struct AttnBranchCall {
+  dsr_tree_attention_args_t a;
+  AttnPlan p;
+  AttnBranch b;
+};
+template <bool BRANCH>
+struct AttnArgs {
+  typedef AttnCall type;
+};
+template <>
+struct AttnArgs<true> {
+  typedef AttnBranchCall type;
+};
+template <bool BRANCH = false>
+__device__ __forceinline__ const typename AttnArgs<BRANCH>::type& attn_call() {
+  typedef typename AttnArgs<BRANCH>::type Call;
+  typedef const Call __attribute__((address_space(4))) * Args;
   Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(args));
-  return *(const AttnCall*)args;
+  return *(const Call*)args;
 }
 
 struct AttnRequest {
   int lo, n, kv;  // first new token, new tokens, cached tokens (0: nothing to read)
   int rows, tiles;
   bool fine;
+  int low;        // BRANCH: first token that is read
 };
+constexpr int kAttnAlign = 32;  // steps begin at multiples of it, so that a round of loads is on one page
 
 // A row's token among the request's new ones.
 __device__ __forceinline__ int attn_token(const AttnPlan& p, int row) {
@@ -110,7 +157,49 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   q.rows = q.n * p.group;
   q.kv = q.fine && q.n > 0 ? kv : 0;
   q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
+  q.low = 0;
   return q;
+}
+
+// The same of a group or, behind its prefix, of a request.
+__device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_args_t& a, const AttnPlan& p,
+                                                    const AttnBranch& b, int r) {
+  if (!b.groups) {
+    AttnRequest q = attn_request(a, p, r);
+    q.low = b.low[r];
+    if (q.low < 0 || a.kv_lengths[r] - q.n < q.low) q.fine = false;
+    if (!q.fine) q.kv = 0;
+    if (q.kv == 0) q.low = 0;
+    return q;
+  }
+  AttnRequest q;
+  const int N = (int)a.tokens, R = (int)b.requests, r0 = b.groups[r], r1 = b.groups[r + 1], kv = b.prefix[r];
+  q.fine = r0 >= 0 && r0 < r1 && r1 <= R && kv > 0 && kv <= (int64_t)a.width * a.page;
+  int lo = q.fine ? a.offsets[r0] : 0, hi = q.fine ? a.offsets[r1] : 0;
+  lo = lo < 0 ? 0 : lo > N ? N : lo;
+  hi = hi < lo ? lo : hi > N ? N : hi;
+  q.lo = lo;
+  q.n = hi - lo;
+  q.kv = q.n > 0 ? kv : 0;
+  q.rows = q.n * p.group;
+  q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
+  q.low = 0;
+  return q;
+}
+// A pass's requests, the context that every row sees, the table row, the mask words.
+__device__ __forceinline__ int64_t attn_count(const AttnCall& c) { return c.a.requests; }
+__device__ __forceinline__ int64_t attn_count(const AttnBranchCall& c) { return c.b.count; }
+__device__ __forceinline__ AttnRequest attn_request(const AttnCall& c, int r) { return attn_request(c.a, c.p, r); }
+__device__ __forceinline__ AttnRequest attn_request(const AttnBranchCall& c, int r) {
+  return attn_request(c.a, c.p, c.b, r);
+}
+__device__ __forceinline__ int attn_context(const AttnCall&, const AttnRequest& q) { return q.kv - q.n; }
+__device__ __forceinline__ int attn_context(const AttnBranchCall& c, const AttnRequest& q) {
+  return c.b.groups ? q.kv : q.kv - q.n;
+}
+__device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r) { return c.a.table + r * c.a.table_ld; }
+__device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int r) {
+  return c.a.table + (c.b.groups ? c.b.groups[r] : r) * c.a.table_ld;
 }
 
 // Inclusive sums over the lanes of a wave, without LDS (row shifts, then the
@@ -133,6 +222,13 @@ struct AttnSegment {
   uint32_t from, to;  // the tile's place in the order of all steps
 };
 
+// Steps of a share.
+__device__ __forceinline__ uint32_t attn_quota(const AttnPlan& p, uint32_t total) {
+  // Most calls of one step per tile have a workgroup for each: no division then.
+  const uint32_t quota = total <= (uint32_t)p.groups ? 1 : (total + p.groups - 1) / (uint32_t)p.groups;
+  return quota < (uint32_t)p.min_steps ? p.min_steps : quota;
+}
+
 // A workgroup's share of the work.
 //
 // All work is put in one order of steps (p.tokens tokens of a tile): request
@@ -148,43 +244,56 @@ struct AttnSegment {
 // The host chooses p.tokens so that the steps of a call number less than 2^31.
 // HOLD: each lane keeps its request of the 64 looked at last (for kernels with
 // registers to spare), else a segment's request is read again.
-template <bool HOLD>
+template <bool HOLD, class Call = AttnCall>
 struct AttnWork {
+  static constexpr bool BRANCH = !std::is_same<Call, AttnCall>::value;
   uint32_t at, stop, quota;  // steps
   uint32_t base;             // steps of the requests before r
   int r, me;
   int r0;                    // lane l holds request r0 + l:
   AttnRequest mine;
 
-  __device__ __forceinline__ int steps_of(const AttnPlan& p, const AttnRequest& q) {
-    return q.rows == 0 ? 0 : q.kv > p.tokens ? (q.kv + p.tokens - 1) >> p.token_shift : 1;
+  static __device__ __forceinline__ int steps_of(const AttnPlan& p, const AttnRequest& q) {
+    const int kv = BRANCH ? q.kv - (q.low & -kAttnAlign) : q.kv;
+    return q.rows == 0 ? 0 : kv > p.tokens ? (kv + p.tokens - 1) >> p.token_shift : 1;
   }
 
   // Steps of the lane's request of the 64 from `first` on.
-  __device__ __forceinline__ int hold(const dsr_tree_attention_args_t& a, const AttnPlan& p, int first) {
-    const int l = threadIdx.x & 63, R = (int)a.requests;
+  __device__ __forceinline__ int hold(const Call& c, int first) {
+    const int l = threadIdx.x & 63, R = (int)attn_count(c);
     r0 = first;
-    mine = attn_request(a, p, first + l < R ? first + l : R - 1);
-    return first + l < R ? mine.tiles * steps_of(p, mine) * a.kv_heads : 0;
+    mine = attn_request(c, first + l < R ? first + l : R - 1);
+    return first + l < R ? mine.tiles * steps_of(c.p, mine) * c.a.kv_heads : 0;
   }
 
   // `border` 0: this workgroup's share.  Else the work from where share `border` begins.
-  __device__ __forceinline__ AttnWork(const dsr_tree_attention_args_t& a, const AttnPlan& p, int border) {
-    const int R = (int)a.requests;
+  __device__ __forceinline__ AttnWork(const Call& c, int border) {
+    const dsr_tree_attention_args_t& a = c.a;
+    const AttnPlan& p = c.p;
+    const int R = (int)attn_count(c);
     int upto = 0, steps = 0;
     uint32_t total = 0;
     for (int first = 0; first < R; first += 64) {
-      steps = hold(a, p, first);
+      steps = hold(c, first);
       upto = attn_wave_scan(steps);
+      if constexpr (BRANCH) {  // for the join
+        const int r = first + (int)(threadIdx.x & 63);
+        if (blockIdx.x == 0 && threadIdx.x < 64 && r < R) c.b.begin[r] = (int)total + upto - steps;
+      }
       total += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
       // Requests without rows have no work: the first workgroup tells their status.
       const int l = threadIdx.x & 63;
-      if (blockIdx.x == 0 && border == 0 && threadIdx.x < 64 && first + l < R && mine.rows == 0)
-        a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
+      if (blockIdx.x == 0 && border == 0 && threadIdx.x < 64 && first + l < R && mine.rows == 0) {
+        if constexpr (BRANCH) {
+          if (!c.b.groups) a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
+        } else {
+          a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
+        }
+      }
     }
-    // Most calls of one step per tile have a workgroup for each: no division then.
-    quota = total <= (uint32_t)p.groups ? 1 : (total + p.groups - 1) / (uint32_t)p.groups;
-    if (quota < (uint32_t)p.min_steps) quota = p.min_steps;
+    if constexpr (BRANCH)
+      if (blockIdx.x == 0 && threadIdx.x == 0) c.b.begin[R] = (int)total;
+    quota = attn_quota(p, total);
     const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
       me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
@@ -199,7 +308,7 @@ struct AttnWork {
     if (at >= stop) return;
     for (int first = 0; first < R; first += 64) {
       if (R > 64) {
-        steps = hold(a, p, first);
+        steps = hold(c, first);
         upto = attn_wave_scan(steps);
       }
       const uint64_t past = __ballot(base + (uint32_t)upto > at);
@@ -214,15 +323,17 @@ struct AttnWork {
   }
 
   // The next segment and its request; false at the end.
-  __device__ __forceinline__ bool next(const dsr_tree_attention_args_t& a, const AttnPlan& p, AttnSegment& s,
-                                       AttnRequest& q) {
+  __device__ __forceinline__ bool next(const Call& c, AttnSegment& s, AttnRequest& q) {
+    const dsr_tree_attention_args_t& a = c.a;
+    const AttnPlan& p = c.p;
+    const int64_t R = attn_count(c);
     if (at >= stop) return false;
     uint32_t steps, length;
     for (;;) {  // past requests that end here or have no rows
-      if (r >= a.requests) return false;
+      if (r >= R) return false;
       if (!HOLD || r - r0 >= 64) {
         r0 = r;
-        mine = attn_request(a, p, HOLD && r + (int)(threadIdx.x & 63) < a.requests ? r + (threadIdx.x & 63) : r);
+        mine = attn_request(c, HOLD && r + (int)(threadIdx.x & 63) < R ? r + (threadIdx.x & 63) : r);
       }
       const int l = r - r0;
       q.lo = __builtin_amdgcn_readlane(mine.lo, l);
@@ -231,6 +342,7 @@ struct AttnWork {
       q.rows = __builtin_amdgcn_readlane(mine.rows, l);
       q.tiles = __builtin_amdgcn_readlane(mine.tiles, l);
       q.fine = __builtin_amdgcn_readlane((int)mine.fine, l);
+      q.low = BRANCH ? __builtin_amdgcn_readlane(mine.low, l) : 0;
       steps = steps_of(p, q);
       length = q.tiles * steps * a.kv_heads;
       if (at - base < length) break;
@@ -243,9 +355,12 @@ struct AttnWork {
     s.head = q.tiles == 1 ? unit : unit / (uint32_t)q.tiles;
     s.tile = unit - (uint32_t)s.head * q.tiles;
     if (!p.cut && !a.visible) s.tile = q.tiles - 1 - s.tile;  // a chunk's longest tiles first
-    s.begin = s0 * p.tokens;
-    s.end = s1 == steps ? q.kv : s1 * p.tokens;
-    if (!a.visible && q.kv > 0) {  // causal rows: nothing past the tile's last one
+    const int origin = BRANCH ? q.low & -kAttnAlign : 0;
+    s.begin = origin + s0 * p.tokens;
+    s.end = s1 == steps ? q.kv : origin + s1 * p.tokens;
+    bool causal = !a.visible;
+    if constexpr (BRANCH) causal &= !c.b.groups;
+    if (causal && q.kv > 0) {  // causal rows: nothing past the tile's last one
       const int last = attn_token(p, (s.tile + 1) * p.tile_rows - 1);
       if (s.end - (q.kv - q.n) > last + 1) s.end = q.kv - q.n + last + 1;
     }
@@ -261,10 +376,10 @@ struct AttnWork {
 // Rows of no request, before the first one's and past the last one's, give 0
 // and -inf.  The workgroups past p.groups take them in turn: looked for by the
 // workgroups that have shares, they cost every small call 0.2 us of 8.5.
-template <class T>
+template <class T, bool BRANCH = false>
 __device__ __forceinline__ void attn_clear(int groups, int threads) {
   typedef typename AttnType<T>::x8 x8;
-  const dsr_tree_attention_args_t& a = attn_call().a;
+  const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
   const int N = (int)a.tokens, lo = a.offsets[0], hi = a.offsets[a.requests];
   const int lead = lo < 0 ? 0 : lo > N ? N : lo, rest = hi < lead ? lead : hi > N ? N : hi;
   const int none = lead + N - rest, chunks = a.head_dim / 8;
@@ -275,6 +390,42 @@ __device__ __forceinline__ void attn_clear(int groups, int threads) {
       *(x8*)((T*)a.out + t * a.out_token + h * a.out_head + 8 * d) = x8{};
       if (a.lse && d == 0) a.lse[t * a.q_heads + h] = -INFINITY;
     }
+  }
+}
+
+// Each request's group and prefix, for the second pass; by the workgroups past
+// p.groups of the first, 64 threads or more.  Groups that do not ascend refuse
+// every request.
+__device__ __forceinline__ void attn_branch_lows(int threads) {
+  const AttnBranchCall& c = attn_call<true>();
+  if (!c.b.groups) return;
+  __shared__ int wrong;
+  const int G = (int)c.b.count, R = (int)c.b.requests;
+  if (threadIdx.x == 0) wrong = 0;
+  __syncthreads();
+  for (int g = threadIdx.x; g <= G; g += threads) {
+    const int r = c.b.groups[g];
+    if (r < 0 || r > R || (g > 0 && c.b.groups[g - 1] > r)) wrong = 1;
+  }
+  __syncthreads();
+  const int step = ((int)gridDim.x - c.p.groups) * threads;
+  for (int r = ((int)blockIdx.x - c.p.groups) * threads + threadIdx.x; r < R; r += step) {
+    int lo = 0, hi = G;  // the groups that begin at or before r
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (c.b.groups[mid] <= r)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    int low = wrong ? -1 : 0, mine = -1;
+    if (!wrong && lo > 0 && r < c.b.groups[lo]) {
+      const int prefix = c.b.prefix[lo - 1];
+      low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
+      mine = low > 0 ? lo - 1 : -1;
+    }
+    c.b.lows[r] = low;
+    c.b.group_of[r] = mine;
   }
 }
 
@@ -302,19 +453,28 @@ __device__ __forceinline__ bool attn_make_finite(typename AttnType<T>::x8& v) {
 // have.  Adding a term that was in the product already changes nothing, so the
 // tokens from `from` on are all looked at.  A thread takes a row; `base` is
 // its scores' base.  Nothing of this runs for ordinary values.
-template <class T, int DP>
-__device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, const AttnPlan& p, const AttnSegment& u,
-                                            const AttnRequest& q, int from, const float* base) {
+template <class T, int DP, class Call>
+__device__ __forceinline__ void attn_poison(const Call& c, const AttnSegment& u, const AttnRequest& q, int from,
+                                            const float* base) {
   typedef typename AttnType<T>::x8 x8;
-  const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = p.group, ctx = q.kv - q.n;
+  constexpr bool BRANCH = !std::is_same<Call, AttnCall>::value;
+  const dsr_tree_attention_args_t& a = c.a;
+  const AttnPlan& p = c.p;
+  const int r = threadIdx.x, row = u.tile * p.tile_rows + r, group = p.group, ctx = attn_context(c, q);
   if (r >= p.tile_rows || row >= q.rows) return;
   const int t = attn_token(p, row), h = u.head * group + row - t * group;
   const T* query = (const T*)a.q + (int64_t)(q.lo + t) * a.q_token + (int64_t)h * a.q_head;
   T* out = (T*)a.out + (int64_t)(q.lo + t) * a.out_token + (int64_t)h * a.out_head;
   float* o = &p.part_o[((int64_t)u.part * p.tile_rows + r) * DP];
+  bool part = !u.whole;
+  if constexpr (BRANCH) {
+    if (u.whole) o = &c.b.row_o[((int64_t)(q.lo + t) * a.q_heads + h) * DP];
+    part = true;
+    if (from < q.low) from = q.low;
+  }
 #pragma unroll 1
   for (int at = from; at < u.end; ++at) {
-    const int id = a.table[u.r * a.table_ld + (at >> p.page_shift)], place = at & (a.page - 1);
+    const int id = attn_pages(c, u.r)[at >> p.page_shift], place = at & (a.page - 1);
     if ((unsigned)id >= (unsigned)a.blocks) continue;
     const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
     const T* k = (const T*)a.k_cache + id * a.k_block + place * a.k_token + u.head * a.k_head;
@@ -335,7 +495,7 @@ __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if ((float)x[i] == (float)whole[i]) continue;
-        if (!u.whole)
+        if (part)
           o[d + i] += weight * (float)whole[i];
         else
           out[d + i] = (T)((float)out[d + i] + weight * (float)whole[i]);
@@ -347,13 +507,17 @@ __device__ __forceinline__ void attn_poison(const dsr_tree_attention_args_t& a, 
 // What a segment says of its page ids: the request's status, or its part's
 // (its last tile of its first head speaks for all: causal tiles see all of the
 // pages that the ones before them see).
-__device__ __forceinline__ void attn_report(const dsr_tree_attention_args_t& a, const AttnPlan& p,
-                                            const AttnSegment& u, const AttnRequest& q, int bad) {
+template <class Call>
+__device__ __forceinline__ void attn_report(const Call& c, const AttnSegment& u, const AttnRequest& q, int bad) {
   if (threadIdx.x != 0) return;
-  if (!u.whole)
-    p.part_bad[u.part] = bad;
-  else if (u.head == 0 && u.tile == q.tiles - 1)
-    a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
+  if (!u.whole) {
+    c.p.part_bad[u.part] = bad;
+  } else if (u.head == 0 && u.tile == q.tiles - 1) {
+    if constexpr (std::is_same<Call, AttnCall>::value)
+      c.a.status[u.r] = !q.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
+    else
+      c.b.bad[u.r] = bad;
+  }
 }
 
 __device__ __forceinline__ uint32_t attn_low_bits(int n) {
@@ -397,8 +561,10 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
 //
 // What bounds it: the cache's read.  64 requests of one token over 8,192
 // tokens, 8 heads of 128: 370 us, 5.8 TB/s.
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(AttnCall) {
+template <class T, int DP, int WAVES, bool BRANCH = false>
+__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
+    typename AttnArgs<BRANCH>::type) {
+  typedef typename AttnArgs<BRANCH>::type Call;
   constexpr int kThreads = 64 * WAVES;
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
@@ -412,28 +578,31 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  if ((int)blockIdx.x >= attn_call().p.groups) return attn_clear<T>(attn_call().p.groups, kThreads);
-  AttnWork<DP <= 128> work(attn_call().a, attn_call().p, 0);
+  if ((int)blockIdx.x >= attn_call<BRANCH>().p.groups) {
+    if constexpr (BRANCH) attn_branch_lows(kThreads);
+    return attn_clear<T, BRANCH>(attn_call<BRANCH>().p.groups, kThreads);
+  }
+  AttnWork<DP <= 128, Call> work(attn_call<BRANCH>(), 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(attn_call().a, attn_call().p, u, q)) {  // the same for the whole workgroup
-    const dsr_tree_attention_args_t& a = attn_call().a;
-    const AttnPlan& p = attn_call().p;
+  while (work.next(attn_call<BRANCH>(), u, q)) {  // the same for the whole workgroup
+    const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
+    const AttnPlan& p = attn_call<BRANCH>().p;
     const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
     __syncthreads();  // the last segment's LDS is read
     if (threadIdx.x == 0) sbad = spoison = 0;
-    const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
+    const int ctx = attn_context(attn_call<BRANCH>(), q), begin = u.begin, end = u.end;
     const int row0 = u.tile << row_shift;
 
     attn_f32x4 acc[DB];
     float m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x4{};
-    const dsr_tree_attention_args_t& c = attn_call().a;
-    const int32_t* pages = c.table + u.r * c.table_ld;
+    const dsr_tree_attention_args_t& c = attn_call<BRANCH>().a;
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
-    const int shift = attn_call().p.page_shift, page = c.page;
+    const int shift = attn_call<BRANCH>().p.page_shift, page = c.page;
     const unsigned blocks = c.blocks;
     const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
     const bool masks = c.visible != nullptr;
@@ -518,7 +687,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     __syncthreads();  // the flags
     for (int p0 = first; p0 < end; p0 += step) {
       const uint32_t bad = bad_next;
-      const bool masked = p0 + kAttnTile > ctx || bad;  // some row may not see some token
+      const bool masked = p0 + kAttnTile > ctx || bad || (BRANCH && p0 < q.low);  // some row may not see some token
       any_bad |= bad != 0;
       if (masked) {
         bool poison = false;
@@ -559,7 +728,9 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
       x8 pv;
       float top = -INFINITY;
       if (masked) {
-        const uint32_t see = attn_sees(masks, mask, tok, p0, ctx, end, bad) >> (4 * g);
+        uint32_t see = attn_sees(masks, mask, tok, p0, ctx, end, bad);
+        if constexpr (BRANCH) see &= ~attn_low_bits(q.low - p0);
+        see >>= 4 * g;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -570,7 +741,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[k][e]);
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32)) * scale - AttnType<T>::kLift;
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale - attn_lift<T, BRANCH>();
       if (__ballot(top > m + 8.f)) {
         const float next = fmaxf(m, top);
         const float f = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
@@ -603,7 +774,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     if (g == 0) sm[w][n] = m;
     if (any_bad && l == 0) sbad = 1;
     __syncthreads();
-    const AttnCall& e = attn_call();
+    const Call& e = attn_call<BRANCH>();
     const bool split = !u.whole;
     const int64_t part = u.part;
     constexpr int OS = DP + 4;  // LDS row of outputs
@@ -633,6 +804,12 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
         if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + row] = float2{M, L};
       } else if (row0 + row < q.rows && d < dim) {
         const int t = attn_token(e.p, row0 + row), head = u.head * group + row0 + row - t * group;
+        if constexpr (BRANCH) {
+          const int64_t at = (int64_t)(q.lo + t) * e.a.q_heads + head;
+          *(attn_f32x4*)&e.b.row_o[at * DP + d] = o;
+          if (d == 0) e.b.row_ml[at] = float2{M, L};
+          continue;
+        }
         const float inv = L == 0.f ? 0.f : 1.f / L;
         x4 y;
 #pragma unroll
@@ -644,8 +821,10 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     }
     __threadfence_block();
     __syncthreads();
-    if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, min(ctx, end) - kAttnTile), sbase);
-    attn_report(e.a, e.p, u, q, sbad);
+    if (spoison)
+      attn_poison<T, DP>(e, u, q, sbad || (BRANCH && begin < q.low) ? begin : max(begin, min(ctx, end) - kAttnTile),
+                         sbase);
+    attn_report(e, u, q, sbad);
   }
 }
 
@@ -666,11 +845,11 @@ __global__ __launch_bounds__(kAttnThreads) void k_tree_join(AttnCall) {
   __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const int border = blockIdx.x + 1;
-  AttnWork<true> work(attn_call().a, attn_call().p, border);
+  AttnWork<true> work(attn_call(), border);
   AttnSegment u;
   AttnRequest q;
   const uint32_t at = work.at;
-  if (!work.next(attn_call().a, attn_call().p, u, q) || u.from == at) return;  // no work there; a tile begins there
+  if (!work.next(attn_call(), u, q) || u.from == at) return;  // no work there; a tile begins there
   const int first = u.from / work.quota, last = (u.to - 1) / work.quota;
   if (first != border - 1) return;
   const dsr_tree_attention_args_t& a = attn_call().a;

@@ -46,8 +46,10 @@ constexpr int attn_round(int DP) { return kAttnThreads / (DP / 8); }
 //
 // FLAT: a page holds every token of a round of loads, so that a round's page
 // id and address are the same for the workgroup and a lane adds one offset.
-template <class T, int DP, int WR, bool FLAT>
-__global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_tree_attention_wide(AttnCall) {
+template <class T, int DP, int WR, bool FLAT, bool BRANCH = false>
+__global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_tree_attention_wide(
+    typename AttnArgs<BRANCH>::type) {
+  typedef typename AttnArgs<BRANCH>::type Call;
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
   typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -72,18 +74,21 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  if ((int)blockIdx.x >= attn_call().p.groups) return attn_clear<T>(attn_call().p.groups, kAttnThreads);
-  AttnWork<false> work(attn_call().a, attn_call().p, 0);
+  if ((int)blockIdx.x >= attn_call<BRANCH>().p.groups) {
+    if constexpr (BRANCH) attn_branch_lows(kAttnThreads);
+    return attn_clear<T, BRANCH>(attn_call<BRANCH>().p.groups, kAttnThreads);
+  }
+  AttnWork<false, Call> work(attn_call<BRANCH>(), 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(attn_call().a, attn_call().p, u, q)) {  // the same for the whole workgroup
-    const dsr_tree_attention_args_t& a = attn_call().a;
-    const AttnPlan& p = attn_call().p;
+  while (work.next(attn_call<BRANCH>(), u, q)) {  // the same for the whole workgroup
+    const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
+    const AttnPlan& p = attn_call<BRANCH>().p;
     const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
     __syncthreads();  // the last segment's LDS is read
     if (threadIdx.x < 4 * WK) sbits[threadIdx.x / WK][threadIdx.x % WK] = 0;
     if (threadIdx.x == 0) sbad = spoison = 0;
-    const int ctx = q.kv - q.n, begin = u.begin, end = u.end;
+    const int ctx = attn_context(attn_call<BRANCH>(), q), begin = u.begin, end = u.end;
     const int clear = min(ctx, end);  // every row sees the tokens before
     const int steps = end > begin ? (end - begin + NT - 1) / NT : 0;
 
@@ -110,11 +115,11 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
     float m = -INFINITY, sum = 0.f, top;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x16{};
-    const dsr_tree_attention_args_t& c = attn_call().a;
-    const int32_t* pages = c.table + u.r * c.table_ld;
+    const dsr_tree_attention_args_t& c = attn_call<BRANCH>().a;
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
-    const int shift = attn_call().p.page_shift, page = c.page;
+    const int shift = attn_call<BRANCH>().p.page_shift, page = c.page;
     const unsigned blocks = c.blocks;
     const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
     const bool masks = c.visible != nullptr;
@@ -203,13 +208,15 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
     // What rows may not see becomes -inf (rare); then the running maximum.
     auto settle = [&](attn_f32x16& s, int step, uint32_t bad) __attribute__((always_inline)) {
       const int p0 = begin + step * NT + 32 * wk;
-      if (p0 + kAttnTile > clear || bad) {
-        const uint32_t see = attn_sees(masks, mask, tok, p0, ctx, end, bad) >> (4 * h);
+      if (p0 + kAttnTile > clear || bad || (BRANCH && p0 < q.low)) {
+        uint32_t see = attn_sees(masks, mask, tok, p0, ctx, end, bad);
+        if constexpr (BRANCH) see &= ~attn_low_bits(q.low - p0);
+        see >>= 4 * h;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : -INFINITY;
         largest(s);
       }
-      top = __builtin_fmaf(top, scale, -AttnType<T>::kLift);
+      top = __builtin_fmaf(top, scale, -attn_lift<T, BRANCH>());
       if (__ballot(top > m + 8.f)) {
         const float next = fmaxf(m, top), f = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
         m = next;
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
       vals_of(0);
       __syncthreads();  // the flags
       if (outside(kid)) check_keys(kid, 0);
-      if (begin + NT > clear || outside(vid)) check_vals(vr, 0);
+      if (begin + NT > clear || outside(vid) || (BRANCH && begin < q.low)) check_vals(vr, 0);
       store(keys, KS, 0, kr, true);
       store(vals, VS, 0, vr, false);
       next_ids();
@@ -356,19 +363,26 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
         }
       }
     }
-    const AttnCall& e = attn_call();
+    const Call& e = attn_call<BRANCH>();
     if (wk == 0 && live) {
       if (h == 0) sbase[in_tile] = m;
-      if (!u.whole) {
-        const int64_t at = ((int64_t)u.part << row_shift) + in_tile;
+      if (BRANCH || !u.whole) {
+        int64_t at = ((int64_t)u.part << row_shift) + in_tile;
         float* o = &e.p.part_o[at * DP];
+        float2* ml = &e.p.part_ml[at];
+        if constexpr (BRANCH)
+          if (u.whole) {
+            at = (int64_t)(q.lo + tok) * e.a.q_heads + head;
+            o = &e.b.row_o[at * DP];
+            ml = &e.b.row_ml[at];
+          }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *(attn_f32x4*)&o[32 * d + 8 * i + 4 * h] =
                 attn_f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
-        if (h == 0) e.p.part_ml[at] = float2{m, sum};
+        if (h == 0) *ml = float2{m, sum};
       } else {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T* o = (T*)e.a.out + (int64_t)(q.lo + tok) * e.a.out_token + (int64_t)head * e.a.out_head;
@@ -388,8 +402,9 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
     }
     __threadfence_block();
     __syncthreads();
-    if (spoison) attn_poison<T, DP>(e.a, e.p, u, q, sbad ? begin : max(begin, clear - NT), sbase);
-    attn_report(e.a, e.p, u, q, sbad);
+    if (spoison)
+      attn_poison<T, DP>(e, u, q, sbad || (BRANCH && begin < q.low) ? begin : max(begin, clear - NT), sbase);
+    attn_report(e, u, q, sbad);
   }
 }
 

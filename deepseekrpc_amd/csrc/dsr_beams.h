@@ -1,0 +1,391 @@
+// The best continuations of groups of beams (dsr_select_beams).
+//
+// Two launches.  k_beam_slices: a workgroup takes a slice of one row, reads it
+// once into registers, and leaves its `keep` largest logits, in order, with
+// the slice's largest value and sum of exponentials.  k_beam_groups: a
+// workgroup takes a group, makes each row's log sum of its slices, and picks
+// the best of their candidates.
+//
+// Which of two rows' candidates is better hangs on the difference of two log
+// sums, so these, and the scores, are float64: an exponential costs about 13
+// float64 instructions (beam_exp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "dsr_branch.h"
+
+namespace dsr {
+
+constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
+constexpr int kBeamEach = 32;                            // logits of a thread
+constexpr int kBeamSlice = kBeamThreads * kBeamEach;     // and of a workgroup
+constexpr int kBeamGroupThreads = 512, kBeamGroupWaves = kBeamGroupThreads / 64;
+
+// One slice of a row.
+struct BeamPart {
+  double sum;  // of exp(logit - top)
+  float top;   // -inf: nothing but -inf
+  int32_t bad; // a NaN or +inf among the logits
+};
+
+// a.workspace: parts [rows, slices], terms [rows], candidates [rows, slices, keep].
+// A row's candidates are worth (logit - top) - rest + score each, in this
+// order: top + rest, their log sum, would lose `rest` where all of a row's
+// logits are the type's lowest value.
+struct BeamTerm {
+  double top, rest;  // largest logit, log sum exp(logit - top)
+  double score;      // NaN: the row offers nothing
+};
+struct BeamSpace {
+  BeamPart* parts;
+  BeamTerm* terms;
+  uint64_t* found; // order of the logit, ~token; 0: none
+};
+__host__ __device__ inline int beam_slices(int64_t vocab) { return (int)((vocab + kBeamSlice - 1) / kBeamSlice); }
+__host__ __device__ inline BeamSpace beam_space(const dsr_select_beams_args_t& a) {
+  BeamSpace s;
+  s.parts = (BeamPart*)a.workspace;
+  s.terms = (BeamTerm*)(s.parts + a.rows * beam_slices(a.vocab));
+  s.found = (uint64_t*)(s.terms + a.rows);
+  return s;
+}
+
+// The value of lane ^ J.
+template <int J>
+__device__ __forceinline__ uint32_t beam_xor(uint32_t x) {
+  if constexpr (J == 1) return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, false);   // quads 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, false);   // quads 2 3 0 1
+  if constexpr (J == 4) {                                                                  // 7 - i, then quads 3 2 1 0
+    const uint32_t y = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false);
+    return __builtin_amdgcn_update_dpp(0, y, 0x1B, 0xf, 0xf, false);
+  }
+  if constexpr (J == 8) return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // rows of 16 turned by 8
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (J == 16) {
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, x, false, false));
+    return threadIdx.x & 16 ? y[0] : y[1];
+  }
+  if constexpr (J == 32) {
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(x, x, false, false));
+    return threadIdx.x & 32 ? y[0] : y[1];
+  }
+}
+template <int J>
+__device__ __forceinline__ uint64_t beam_xor(uint64_t x) {
+  return (uint64_t)beam_xor<J>((uint32_t)(x >> 32)) << 32 | beam_xor<J>((uint32_t)x);
+}
+
+// A candidate among all of a group's: the greater is better.
+struct BeamOffer {
+  uint64_t key;   // order of its score; 0: none
+  uint32_t place; // ~place: of equal scores the earliest
+  __device__ __forceinline__ bool operator<(const BeamOffer& o) const {
+    return key < o.key || (key == o.key && place < o.place);
+  }
+};
+template <int J>
+__device__ __forceinline__ BeamOffer beam_xor(BeamOffer x) {
+  return BeamOffer{beam_xor<J>(x.key), beam_xor<J>(x.place)};
+}
+
+// One step of a bitonic network over a wave's lanes: the greater of a pair goes to the lane where `up`.
+template <int J, class K>
+__device__ __forceinline__ void beam_step(K& x, bool up) {
+  const K y = beam_xor<J>(x);
+  if ((x < y) == up) x = y;
+}
+// Lanes of a bitonic sequence, the greatest first.
+template <class K>
+__device__ __forceinline__ void beam_merge(K& x) {
+  const int l = threadIdx.x;
+  beam_step<32>(x, !(l & 32));
+  beam_step<16>(x, !(l & 16));
+  beam_step<8>(x, !(l & 8));
+  beam_step<4>(x, !(l & 4));
+  beam_step<2>(x, !(l & 2));
+  beam_step<1>(x, !(l & 1));
+}
+// Any lanes, the greatest first (Batcher's bitonic sort).
+template <class K>
+__device__ __forceinline__ void beam_sort(K& x) {
+  const int l = threadIdx.x;
+  beam_step<1>(x, !(l & 1) == !(l & 2));
+  beam_step<2>(x, !(l & 2) == !(l & 4));
+  beam_step<1>(x, !(l & 1) == !(l & 4));
+  beam_step<4>(x, !(l & 4) == !(l & 8));
+  beam_step<2>(x, !(l & 2) == !(l & 8));
+  beam_step<1>(x, !(l & 1) == !(l & 8));
+  beam_step<8>(x, !(l & 8) == !(l & 16));
+  beam_step<4>(x, !(l & 4) == !(l & 16));
+  beam_step<2>(x, !(l & 2) == !(l & 16));
+  beam_step<1>(x, !(l & 1) == !(l & 16));
+  beam_step<16>(x, !(l & 16) == !(l & 32));
+  beam_step<8>(x, !(l & 8) == !(l & 32));
+  beam_step<4>(x, !(l & 4) == !(l & 32));
+  beam_step<2>(x, !(l & 2) == !(l & 32));
+  beam_step<1>(x, !(l & 1) == !(l & 32));
+  beam_merge(x);
+}
+// The lanes in the opposite order.
+__device__ __forceinline__ uint64_t beam_turn(uint64_t x) { return __shfl(x, 63 - (int)(threadIdx.x & 63)); }
+__device__ __forceinline__ BeamOffer beam_turn(BeamOffer x) {
+  const int l = 63 - (int)(threadIdx.x & 63);
+  return BeamOffer{(uint64_t)__shfl(x.key, l), (uint32_t)__shfl((int)x.place, l)};
+}
+// The 64 greatest of two sorted 64, `y` in the opposite order.
+template <class K>
+__device__ __forceinline__ void beam_join(K& x, const K& y) {
+  if (x < y) x = y;
+  beam_merge(x);
+}
+
+// Order of float values as unsigned numbers (both zeros alike), and back.
+__device__ __forceinline__ uint32_t beam_order(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float beam_value(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ uint64_t beam_order(double x) {
+  const uint64_t u = __double_as_longlong(x + 0.0);
+  return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double beam_value(uint64_t u) {
+  return __longlong_as_double(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u);
+}
+
+// exp(d) for d <= 0, to about 2^-52: 2^(n / 64) from a table times a polynomial
+// of what is left, |r| <= ln 2 / 128, whose next term would be below 2^-60
+// (Tang, Table-driven implementation of the exponential function, 1989).
+// Values below e^-800 count as 0.
+__device__ __forceinline__ void beam_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
+}
+__device__ __forceinline__ double beam_exp(double d, const double* table) {
+  d = d > -800.0 ? d : -800.0;
+  const double n = __builtin_rint(d * 92.33248261893824);  // 64 / ln 2
+  const double r = __builtin_fma(n, -0.010830424696249145, d);
+  double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
+  p = __builtin_fma(p, r, 1.0 / 6);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  const int k = (int)n;
+  return __builtin_ldexp(p * table[k & 63], k >> 6);
+}
+
+__device__ __forceinline__ double beam_sum(double x) {  // over the wave's lanes
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s);
+  return x;
+}
+
+// VEC: rows are 16-byte aligned and read 16 bytes at a time.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_args_t a) {
+  typedef T xv __attribute__((ext_vector_type(16 / sizeof(T))));
+  constexpr int VE = VEC ? 16 / sizeof(T) : 1, C = kBeamEach / VE;
+  __shared__ double table[64];
+  __shared__ uint64_t list[kBeamWaves][128];
+  __shared__ BeamPart part[kBeamWaves];
+  const int slices = beam_slices(a.vocab), l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x / (unsigned)slices;
+  const int slice = blockIdx.x - (unsigned)row * slices;
+  if (slice == 0 && threadIdx.x == 0) a.status[row] = DSR_OK;
+  if (a.finished && a.finished[row]) return;
+  beam_table(table);
+  const T* logits = (const T*)a.logits + row * a.ld;
+  const int first = slice * kBeamSlice, V = (int)a.vocab;
+
+  // Element e of the thread is token first + (e / VE * threads + thread) VE + e % VE.
+  float x[kBeamEach];
+  auto token = [&](int e) { return first + (e / VE * kBeamThreads + (int)threadIdx.x) * VE + e % VE; };
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int at = token(c * VE);
+    if constexpr (VEC) {
+      xv v;
+      if (at + VE <= V) {
+        v = *(const xv*)(logits + at);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[c * VE + i] = (float)v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[c * VE + i] = at + i < V ? (float)logits[at + i] : -INFINITY;
+      }
+    } else {
+      x[c] = at < V ? (float)logits[at] : -INFINITY;
+    }
+  }
+  bool bad = false;
+  float most = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kBeamEach; ++e) {
+    bad |= !(x[e] < INFINITY);
+    most = fmaxf(most, x[e]);
+  }
+  // The keep-th largest of the lanes' largest: at least `keep` of the wave's
+  // logits are not below it, and few more.
+  uint64_t top = (uint64_t)beam_order(most) << 32;
+  beam_sort(top);
+  const float base = beam_value((uint32_t)(__shfl(top, 0) >> 32));
+  const uint64_t none = (uint64_t)beam_order(-INFINITY) << 32 | 0xFFFFFFFFull;
+  uint64_t floor = __shfl(top, a.keep - 1);  // candidates have to be above it
+  floor = floor ? floor - 1 : 0;
+  if (floor < none) floor = none;
+
+  // They go through the wave's list, 64 at a time, into the sorted `top`.
+  top = 0;
+  int n = 0;
+  auto take = [&](uint64_t key) __attribute__((always_inline)) {
+    beam_sort(key);
+    beam_join(top, beam_turn(key));
+    const uint64_t last = __shfl(top, a.keep - 1);
+    if (last > floor) floor = last;
+  };
+#pragma unroll
+  for (int e = 0; e < kBeamEach; ++e) {
+    const uint64_t key = (uint64_t)beam_order(x[e]) << 32 | (uint32_t)~token(e);
+    const bool in = key > floor;
+    const uint64_t which = __ballot(in);
+    if (which) {
+      if (in) list[w][n + __popcll(which & ((1ull << l) - 1))] = key;
+      n += __popcll(which);
+      if (n >= 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const uint64_t now = list[w][l], rest = list[w][64 + l];
+        __builtin_amdgcn_wave_barrier();
+        list[w][l] = rest;
+        n -= 64;
+        take(now);
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (n > 0) take(l < n ? list[w][l] : 0);
+  __syncthreads();  // the table
+  double sum = 0.0;
+  if (base > -INFINITY)
+#pragma unroll
+    for (int e = 0; e < kBeamEach; ++e) sum += beam_exp((double)x[e] - (double)base, table);
+  sum = beam_sum(sum);
+  const int wrong = __ballot(bad) != 0;
+  list[w][l] = top;
+  if (l == 0) part[w] = BeamPart{sum, base, wrong};
+  __syncthreads();
+  if (w > 0) return;
+  const BeamSpace space = beam_space(a);
+  const int64_t at = row * slices + slice;
+#pragma unroll
+  for (int i = 1; i < kBeamWaves; ++i) beam_join(top, list[i][63 - l]);
+  if (l < a.keep) space.found[at * a.keep + l] = top;
+  if (l == 0) {
+    BeamPart p = part[0];
+#pragma unroll
+    for (int i = 1; i < kBeamWaves; ++i) {
+      p.top = fmaxf(p.top, part[i].top);
+      p.bad |= part[i].bad;
+    }
+    p.sum = 0.0;
+    if (p.top > -INFINITY)
+#pragma unroll
+      for (int i = 0; i < kBeamWaves; ++i)
+        p.sum += part[i].sum * beam_exp((double)part[i].top - (double)p.top, table);
+    space.parts[at] = p;
+  }
+}
+
+__global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_beams_args_t a) {
+  __shared__ double table[64];
+  __shared__ uint64_t keys[kBeamGroupWaves][64];
+  __shared__ uint32_t places[kBeamGroupWaves][64];
+  const int g = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6, slices = beam_slices(a.vocab), keep = a.keep;
+  const int rows = (int)a.rows;
+  int lo = a.offsets[g], hi = a.offsets[g + 1];
+  lo = lo < 0 ? 0 : lo > rows ? rows : lo;
+  hi = hi < lo ? lo : hi > rows ? rows : hi;
+  const BeamSpace space = beam_space(a);
+  beam_table(table);
+  __syncthreads();
+  for (int r = lo + (int)threadIdx.x; r < hi; r += kBeamGroupThreads) {
+    const double score = a.scores[r];
+    int status = !(score < INFINITY) ? DSR_E_LOGITS : DSR_OK;
+    BeamTerm term{0.0, 0.0, score};
+    if (!(a.finished && a.finished[r])) {
+      const BeamPart* p = space.parts + (int64_t)r * slices;
+      float top = -INFINITY;
+      int bad = 0;
+      for (int s = 0; s < slices; ++s) {
+        top = fmaxf(top, p[s].top);
+        bad |= p[s].bad;
+      }
+      double sum = 0.0;
+      for (int s = 0; s < slices; ++s)
+        if (p[s].top > -INFINITY) sum += p[s].sum * beam_exp((double)p[s].top - (double)top, table);
+      if (bad)
+        status = DSR_E_LOGITS;
+      else if (top == -INFINITY && status == DSR_OK)
+        status = DSR_E_MASKED;
+      term.top = top;
+      term.rest = log(sum);
+    }
+    if (status != DSR_OK) a.status[r] = status;
+    if (status != DSR_OK) term.score = NAN;
+    space.terms[r] = term;
+  }
+  __threadfence_block();
+  __syncthreads();
+
+  // Candidates, 64 of a wave at a time, into its sorted `best`.
+  const int each = slices * keep, count = (hi - lo) * each;
+  BeamOffer best{0, 0}, last{0, 0};
+  for (int i0 = 64 * w; i0 < count; i0 += kBeamGroupThreads) {
+    const int i = i0 + l;
+    BeamOffer mine{0, 0};
+    if (i < count) {
+      const int r = i / each, in = i - r * each;
+      const BeamTerm term = space.terms[lo + r];
+      double score = NAN;
+      if (a.finished && a.finished[lo + r]) {
+        if (in == 0) score = term.score;
+      } else {
+        const uint64_t found = space.found[(int64_t)(lo + r) * each + in];
+        if (found) score = ((double)beam_value((uint32_t)(found >> 32)) - term.top) - term.rest + term.score;
+      }
+      if (score > -INFINITY) mine = BeamOffer{beam_order(score), ~(uint32_t)i};
+    }
+    if (!__ballot(last < mine)) continue;
+    beam_sort(mine);
+    beam_join(best, beam_turn(mine));
+    last = BeamOffer{(uint64_t)__shfl(best.key, keep - 1), (uint32_t)__shfl((int)best.place, keep - 1)};
+  }
+#pragma unroll
+  for (int half = kBeamGroupWaves / 2; half > 0; half /= 2) {
+    if (w >= half && w < 2 * half) {
+      keys[w][l] = best.key;
+      places[w][l] = best.place;
+    }
+    __syncthreads();
+    if (w < half) beam_join(best, BeamOffer{keys[w + half][63 - l], places[w + half][63 - l]});
+  }
+  if (w > 0 || l >= keep) return;
+  const int64_t at = (int64_t)g * keep + l;
+  int parent = -1, token = -1;
+  if (best.key) {
+    const uint32_t i = ~best.place, r = i / each;
+    parent = lo + (int)r;
+    if (!(a.finished && a.finished[parent]))
+      token = (int)~(uint32_t)space.found[(int64_t)parent * each + (i - r * each)];
+  }
+  a.parents[at] = parent;
+  a.tokens[at] = token;
+  a.out_scores[at] = best.key ? beam_value(best.key) : -INFINITY;
+}
+
+}  // namespace dsr

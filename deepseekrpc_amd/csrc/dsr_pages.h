@@ -1,0 +1,518 @@
+// Pages that several rows hold: rows that continue other rows
+// (dsr_fork_pages), and held pages moved to the front (dsr_compact_pages).
+//
+// Every decision is made from counts and prefix sums, so that no result
+// depends on timing: pages are taken from the pool in row order and given
+// back in ascending order, which a bit per page makes a matter of counting
+// the bits before it.
+//
+// What bounds both, beside a few launches that each wait for the one before,
+// is the moved rows of the caches, read and written once.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "dsr_branch.h"
+
+namespace dsr {
+
+constexpr int kPagesThreads = 256;
+constexpr int kForkThreads = 1024;
+constexpr int kBitsChunk = 4 * kPagesThreads;  // words of 32 pages that a workgroup counts
+constexpr int kPagesInline = 128;              // caches whose pointers are a launch's arguments
+
+typedef uint32_t pages_u32x4 __attribute__((ext_vector_type(4)));
+
+template <int COUNT>
+struct PagesCaches {
+  void* at[COUNT];
+};
+template <>
+struct PagesCaches<0> {};
+
+// Tokens [0, tokens) of page `from` go to page `to`, in every cache.
+struct PageCopy {
+  int32_t from, to, tokens;
+};
+
+__host__ __device__ inline int64_t pages_words(int32_t blocks) { return ((int64_t)blocks + 31) / 32; }
+__host__ __device__ inline int pages_chunks(int32_t blocks) {
+  return (int)((pages_words(blocks) + kBitsChunk - 1) / kBitsChunk);
+}
+
+// Sum over the workgroup (256 threads), for every thread; `part` is LDS of 4.
+__device__ __forceinline__ int pages_total(int x, int* part) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return part[0] + part[1] + part[2] + part[3];
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int pages_scan(int x) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int y = __shfl_up(x, s);
+    if ((int)(threadIdx.x & 63) >= s) x += y;
+  }
+  return x;
+}
+
+// Sum over the threads before this one (256 threads).
+__device__ __forceinline__ int pages_before(int x, int* part) {
+  const int upto = pages_scan(x), w = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) part[w] = upto;
+  __syncthreads();
+  int before = upto - x;
+  for (int i = 0; i < w; ++i) before += part[i];
+  return before;
+}
+
+// One page's tokens of one cache, by a workgroup.  Units of 16 bytes; the
+// rows of a page that lies in one piece are one run.
+struct PageShape {
+  int32_t heads, row_bytes;
+  int64_t c_block, c_token, c_head;
+};
+constexpr int kPagesFlight = 8;  // reads of a thread in flight
+__device__ __forceinline__ void pages_copy(const PageShape& s, char* cache, const PageCopy& c) {
+  const char* src = cache + c.from * s.c_block;
+  char* dst = cache + c.to * s.c_block;
+  // A page of a cache is less than 2^31 bytes.
+  const uint32_t cols = s.row_bytes / 16, per = cols * s.heads, units = c.tokens * per;
+  const bool flat = (s.heads == 1 || s.c_head == s.row_bytes) && (c.tokens == 1 || s.c_token == (int64_t)per * 16);
+  auto offset = [&](uint32_t u) __attribute__((always_inline)) -> int64_t {
+    if (flat) return (int64_t)u * 16;
+    const uint32_t t = u / per, in = u - t * per, h = in / cols;
+    return t * s.c_token + h * s.c_head + (in - h * cols) * 16;
+  };
+  for (uint32_t u = threadIdx.x; u < units; u += kPagesFlight * kPagesThreads) {
+    pages_u32x4 v[kPagesFlight];
+    int64_t at[kPagesFlight];
+#pragma unroll
+    for (int i = 0; i < kPagesFlight; ++i)
+      if (u + i * kPagesThreads < units) {
+        at[i] = offset(u + i * kPagesThreads);
+        v[i] = *(const pages_u32x4*)(src + at[i]);
+      }
+#pragma unroll
+    for (int i = 0; i < kPagesFlight; ++i)
+      if (u + i * kPagesThreads < units) *(pages_u32x4*)(dst + at[i]) = v[i];
+  }
+}
+
+// Items (copy, cache), a workgroup each in turn.
+template <int COUNT>
+__device__ __forceinline__ void pages_copies(const PageShape& s, const PageCopy* copies, int count,
+                                             void* const* device, const PagesCaches<COUNT>& caches, int cache_count,
+                                             int group, int groups) {
+  const int64_t items = (int64_t)count * cache_count;
+  for (int64_t i = group; i < items; i += groups) {
+    const int k = (int)(i / cache_count), c = (int)(i - (int64_t)k * cache_count);
+    char* cache;
+    if constexpr (COUNT > 0)
+      cache = (char*)caches.at[c];
+    else
+      cache = (char*)device[c];
+    pages_copy(s, cache, copies[k]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Fork.
+
+struct ForkRow {
+  int32_t source;  // -1: the row is empty
+  int32_t full;    // pages shared with its siblings
+  int32_t pages;   // pages in all
+  int32_t fresh;   // the page from the pool that comes behind the shared ones, with `copied`
+  int32_t copied;
+};
+struct ForkHead {
+  int32_t first, count, taken;  // the pool's first free entry, their number, pages taken
+};
+// a.workspace: head, rows, children of each source, copies, a bit per page that is freed.
+struct ForkSpace {
+  ForkHead* head;
+  ForkRow* rows;
+  int32_t* children;  // rows that continue a source; -1: its length or pages are out of bounds
+  PageCopy* copies;
+  uint32_t* freed;
+};
+__host__ __device__ inline int64_t fork_space(const dsr_fork_args_t& a, ForkSpace& s) {
+  char* p = (char*)a.workspace;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* q = p + at;
+    at += (bytes + 15) / 16 * 16;
+    return q;
+  };
+  s.head = (ForkHead*)take(sizeof(ForkHead));
+  s.rows = (ForkRow*)take(a.rows * sizeof(ForkRow));
+  s.children = (int32_t*)take(a.sources * 4);
+  s.copies = (PageCopy*)take(a.rows * sizeof(PageCopy));
+  s.freed = (uint32_t*)take(pages_words(a.blocks) * 4);
+  return at;
+}
+
+// The first workgroup decides what each row gets; the others clear the bits
+// and copy the counts.
+__global__ __launch_bounds__(kForkThreads) void k_fork_scan(dsr_fork_args_t a) {
+  __shared__ int32_t heir[DSR_TREE_MAX_REQUESTS];      // the first row that continues a source
+  __shared__ int32_t children[DSR_TREE_MAX_REQUESTS];
+  __shared__ int part[kForkThreads / 64];
+  __shared__ int taken;
+  ForkSpace space;
+  fork_space(a, space);
+  const int S = (int)a.sources, R = (int)a.rows, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (blockIdx.x > 0) {
+    const int64_t step = (int64_t)(gridDim.x - 1) * kForkThreads, words = pages_words(a.blocks);
+    const int64_t first = (int64_t)(blockIdx.x - 1) * kForkThreads + threadIdx.x;
+    for (int64_t i = first; i < words; i += step) space.freed[i] = 0;
+    if (a.shared_out != a.shared)
+      for (int64_t i = first; i < a.blocks; i += step) a.shared_out[i] = a.shared[i];
+    return;
+  }
+  for (int s = threadIdx.x; s < S; s += kForkThreads) {
+    heir[s] = INT_MAX;
+    children[s] = 0;
+  }
+  if (threadIdx.x == 0) taken = 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < R; r += kForkThreads) {
+    const int s = a.parents[r];
+    if ((unsigned)s < (unsigned)S) atomicMin(&heir[s], r);
+  }
+  __syncthreads();
+  const int shift = __ffs(a.page) - 1, size = a.pool_size;
+  int head = a.pool_state[0], count = a.pool_state[1];
+  if (head < 0 || head >= size || count < 0 || count > size) head = count = 0;  // not a pool: empty
+  auto fine = [&](int length, int held) {
+    return length >= 0 && (uint32_t)held <= (uint32_t)a.width && (uint32_t)length <= (uint32_t)held << shift;
+  };
+  int base = 0;  // pages wanted by the rows before these
+  for (int r0 = 0; r0 < R; r0 += kForkThreads) {
+    const int r = r0 + (int)threadIdx.x;
+    int status = DSR_OK, s = r < R ? a.parents[r] : -1, length = 0, held = 0;
+    if (s < -1 || s >= S) {
+      status = DSR_E_PARENT;
+      s = -1;
+    }
+    if (s >= 0) {
+      length = a.lengths[s];
+      held = a.held[s];
+      if (!fine(length, held)) {
+        status = DSR_E_LENGTH;
+        s = -1;
+      }
+    }
+    const bool first = s >= 0 && heir[s] == r;
+    const int want = s >= 0 && !first && (length & (a.page - 1)) != 0;
+    int upto = pages_scan(want);
+    __syncthreads();
+    if (l == 63) part[w] = upto;
+    __syncthreads();
+    for (int i = 0; i < kForkThreads / 64; ++i) {
+      if (i < w) upto += part[i];
+    }
+    upto += base;
+    for (int i = 0; i < kForkThreads / 64; ++i) base += part[i];
+    if (want && upto > count) {
+      status = DSR_E_BLOCKS;
+      s = -1;
+    }
+    if (r >= R) continue;  // no barrier is passed over: the others of the round have none left
+    ForkRow row{s, 0, 0, -1, 0};
+    if (s >= 0) {
+      row.full = length >> shift;
+      row.pages = first ? held : row.full + want;
+      atomicAdd(&children[s], 1);
+      if (want) {
+        const int at = head + upto - 1;
+        row.fresh = a.pool[at >= size ? at - size : at];
+        row.copied = 1;
+        const int from = a.table[s * a.table_ld + row.full];
+        const bool in = (unsigned)from < (unsigned)a.blocks && (unsigned)row.fresh < (unsigned)a.blocks;
+        space.copies[upto - 1] = PageCopy{in ? from : 0, in ? row.fresh : 0, in ? length & (a.page - 1) : 0};
+        atomicMax(&taken, upto);
+      }
+    }
+    space.rows[r] = row;
+    a.held_out[r] = row.pages;
+    a.lengths_out[r] = s >= 0 ? length : 0;
+    a.status[r] = status;
+  }
+  __syncthreads();
+  for (int s = threadIdx.x; s < S; s += kForkThreads)
+    space.children[s] = fine(a.lengths[s], a.held[s]) ? children[s] : -1;
+  if (threadIdx.x == 0) *space.head = ForkHead{head, count, taken};
+}
+
+// Table rows, a workgroup each; then the sources' pages gain and lose rows.
+__global__ __launch_bounds__(kPagesThreads) void k_fork_rows(dsr_fork_args_t a) {
+  __shared__ int outside;
+  ForkSpace space;
+  fork_space(a, space);
+  const unsigned blocks = a.blocks;
+  if (threadIdx.x == 0) outside = 0;
+  __syncthreads();
+  if ((int64_t)blockIdx.x < a.rows) {
+    const int64_t r = blockIdx.x;
+    const ForkRow row = space.rows[r];
+    const int32_t* from = a.table + row.source * a.table_ld;
+    int32_t* to = a.table_out + r * a.table_out_ld;
+    bool bad = false;
+    for (int64_t c = threadIdx.x; c < a.width; c += kPagesThreads) {
+      const int id = c >= row.pages ? -1 : row.copied && c == row.full ? row.fresh : from[c];
+      bad |= c < row.pages && (unsigned)id >= blocks;
+      to[c] = id;
+    }
+    if (bad) outside = 1;
+    __syncthreads();
+    if (threadIdx.x == 0 && outside) a.status[r] = DSR_E_BLOCK;
+    return;
+  }
+  const int64_t s = (int64_t)blockIdx.x - a.rows;
+  const int children = space.children[s];
+  if (children >= 0) {
+    const int full = a.lengths[s] / a.page, held = a.held[s];
+    const int32_t* pages = a.table + s * a.table_ld;
+    bool bad = false;
+    for (int c = threadIdx.x; c < held; c += kPagesThreads) {
+      const int id = pages[c], change = c < full ? children - 1 : children > 0 ? 0 : -1;
+      if ((unsigned)id >= blocks)
+        bad = true;
+      else if (change != 0 && atomicAdd(&a.shared_out[id], change) + change < 0)
+        atomicOr(&space.freed[id >> 5], 1u << (id & 31));
+    }
+    if (bad) outside = 1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) a.source_status[s] = children < 0 ? DSR_E_LENGTH : outside ? DSR_E_BLOCK : DSR_OK;
+}
+
+// Freed pages to the pool, a chunk of the bits a workgroup: each counts the
+// bits before its own.
+__device__ __forceinline__ void fork_free(const dsr_fork_args_t& a, const ForkSpace& space, int chunk) {
+  __shared__ int part[4];
+  const int64_t words = pages_words(a.blocks), begin = (int64_t)chunk * kBitsChunk;
+  int mine = 0;
+  for (int64_t i = threadIdx.x; i < begin; i += kPagesThreads) mine += __popc(space.freed[i]);
+  int before = pages_total(mine, part);
+  uint32_t bits[4];
+  mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = begin + 4 * (int)threadIdx.x + i;
+    bits[i] = at < words ? space.freed[at] : 0;
+    mine += __popc(bits[i]);
+  }
+  const ForkHead head = *space.head;
+  const int64_t size = a.pool_size, room = size - head.count + head.taken;
+  const int all = before + pages_total(mine, part);
+  before += pages_before(mine, part);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    for (uint32_t b = bits[i]; b; b &= b - 1, ++before) {
+      const int id = (int)((begin + 4 * (int)threadIdx.x + i) * 32) + __ffs(b) - 1;
+      a.shared_out[id] = 0;
+      if (before < room) a.pool[(head.first + (int64_t)head.count + before) % size] = id;
+    }
+  if (chunk == pages_chunks(a.blocks) - 1 && threadIdx.x == 0) {
+    a.pool_state_out[0] = (int32_t)((head.first + (int64_t)head.taken) % size);
+    a.pool_state_out[1] = head.count - head.taken + (int32_t)(all < room ? all : room);
+  }
+}
+
+// `chunks` workgroups free pages, the others copy.
+template <int COUNT>
+__global__ __launch_bounds__(kPagesThreads) void k_fork_finish(dsr_fork_args_t a, PagesCaches<COUNT> caches,
+                                                               int chunks) {
+  ForkSpace space;
+  fork_space(a, space);
+  if ((int)blockIdx.x < chunks) return fork_free(a, space, blockIdx.x);
+  pages_copies<COUNT>(PageShape{a.heads, a.row_bytes, a.c_block, a.c_token, a.c_head}, space.copies,
+                      space.head->taken, a.caches, caches, a.cache_count, blockIdx.x - chunks, gridDim.x - chunks);
+}
+
+// ---------------------------------------------------------------------------
+// Compact.
+
+struct CompactHead {
+  int32_t refused;  // some row has a status
+  int32_t limit;    // first page behind the held ones afterwards
+  int32_t moves;
+};
+// a.workspace: head, a bit per held page, rank of each page that moves or is moved to, copies.
+struct CompactSpace {
+  CompactHead* head;
+  uint32_t* held;
+  int32_t* rank;
+  PageCopy* copies;
+};
+__host__ __device__ inline int64_t compact_space(const dsr_compact_args_t& a, CompactSpace& s) {
+  char* p = (char*)a.workspace;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* q = p + at;
+    at += (bytes + 15) / 16 * 16;
+    return q;
+  };
+  s.head = (CompactHead*)take(sizeof(CompactHead));
+  s.held = (uint32_t*)take(pages_words(a.blocks) * 4);
+  s.rank = (int32_t*)take((int64_t)a.blocks * 4);
+  s.copies = (PageCopy*)take((int64_t)(a.blocks / 2 + 1) * sizeof(PageCopy));  // a move needs two pages
+  return at;
+}
+
+__global__ __launch_bounds__(kPagesThreads) void k_compact_clear(dsr_compact_args_t a) {
+  CompactSpace space;
+  compact_space(a, space);
+  const int64_t first = (int64_t)blockIdx.x * kPagesThreads + threadIdx.x;
+  if (first == 0) *space.head = CompactHead{0, 0, 0};
+  for (int64_t i = first; i < pages_words(a.blocks); i += (int64_t)gridDim.x * kPagesThreads) space.held[i] = 0;
+}
+
+// Rows, a workgroup each.
+__global__ __launch_bounds__(kPagesThreads) void k_compact_mark(dsr_compact_args_t a) {
+  __shared__ int outside;
+  CompactSpace space;
+  compact_space(a, space);
+  const int64_t r = blockIdx.x;
+  if (threadIdx.x == 0) outside = 0;
+  __syncthreads();
+  const int held = a.held[r];
+  const bool fine = (uint32_t)held <= (uint32_t)a.width;
+  const int32_t* pages = a.table + r * a.table_ld;
+  bool bad = false;
+  for (int c = threadIdx.x; fine && c < held; c += kPagesThreads) {
+    const int id = pages[c];
+    if ((unsigned)id >= (unsigned)a.blocks)
+      bad = true;
+    else
+      atomicOr(&space.held[id >> 5], 1u << (id & 31));
+  }
+  if (bad) outside = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.status[r] = !fine ? DSR_E_LENGTH : outside ? DSR_E_BLOCK : DSR_OK;
+    if (!fine || outside) space.head->refused = 1;
+  }
+}
+
+// The pages from `lo` on and before `hi` that are among word i's 32, a bit each.
+__device__ __forceinline__ uint32_t pages_range(int64_t i, int64_t lo, int64_t hi) {
+  const int64_t a = lo - 32 * i, b = hi - 32 * i;
+  const uint32_t from = a <= 0 ? ~0u : a >= 32 ? 0u : ~0u << a, to = b <= 0 ? 0u : b >= 32 ? ~0u : ~(~0u << b);
+  return from & to;
+}
+
+// Which page moves where: the k-th held page from the limit on, to the k-th
+// free one before it.
+__global__ __launch_bounds__(kPagesThreads) void k_compact_plan(dsr_compact_args_t a) {
+  __shared__ int part[4];
+  CompactSpace space;
+  compact_space(a, space);
+  const int64_t words = pages_words(a.blocks), begin = (int64_t)blockIdx.x * kBitsChunk;
+  const int64_t first = a.first, blocks = a.blocks;
+  int mine = 0;
+  for (int64_t i = threadIdx.x; i < words; i += kPagesThreads)
+    mine += __popc(space.held[i] & pages_range(i, first, blocks));
+  const int64_t limit = first + pages_total(mine, part);
+  int moved = 0, open = 0;  // held pages behind the limit, free ones before it
+  for (int64_t i = threadIdx.x; i < begin; i += kPagesThreads) {
+    const uint32_t held = space.held[i];
+    moved += __popc(held & pages_range(i, limit, blocks));
+    open += __popc(~held & pages_range(i, first, limit));
+  }
+  moved = pages_total(moved, part);
+  open = pages_total(open, part);
+  uint32_t from[4], to[4];
+  int m = 0, o = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = begin + 4 * (int)threadIdx.x + i;
+    const uint32_t held = at < words ? space.held[at] : 0;
+    from[i] = at < words ? held & pages_range(at, limit, blocks) : 0;
+    to[i] = at < words ? ~held & pages_range(at, first, limit) : 0;
+    m += __popc(from[i]);
+    o += __popc(to[i]);
+  }
+  const int all = moved + pages_total(m, part);
+  moved += pages_before(m, part);
+  open += pages_before(o, part);
+  const bool refused = space.head->refused;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = (int)((begin + 4 * (int)threadIdx.x + i) * 32) - 1;
+    for (uint32_t b = from[i]; b; b &= b - 1, ++moved) {
+      space.rank[id + __ffs(b)] = moved;
+      space.copies[moved].from = id + __ffs(b);
+    }
+    for (uint32_t b = to[i]; b; b &= b - 1, ++open) {
+      space.rank[id + __ffs(b)] = open;
+      space.copies[open].to = id + __ffs(b);
+      space.copies[open].tokens = a.page;
+    }
+  }
+  if (begin + kBitsChunk >= words && threadIdx.x == 0) {
+    space.head->limit = (int32_t)limit;
+    space.head->moves = refused ? 0 : all;
+  }
+}
+
+// `rows` workgroups write table rows, `others` what is kept per page and the
+// pool, the rest copy.
+template <int COUNT>
+__global__ __launch_bounds__(kPagesThreads) void k_compact_apply(dsr_compact_args_t a, PagesCaches<COUNT> caches,
+                                                                 int rows, int others) {
+  CompactSpace space;
+  compact_space(a, space);
+  const CompactHead head = *space.head;
+  if ((int)blockIdx.x < rows) {
+    const int64_t r = blockIdx.x;
+    const int held = head.refused ? 0 : a.held[r];
+    for (int64_t c = threadIdx.x; c < a.width; c += kPagesThreads) {
+      int id = a.table[r * a.table_ld + c];
+      if (c < held && id >= head.limit) id = space.copies[space.rank[id]].to;
+      a.table_out[r * a.table_out_ld + c] = id;
+    }
+    return;
+  }
+  if ((int)blockIdx.x < rows + others) {
+    const int64_t step = (int64_t)others * kPagesThreads;
+    const int64_t thread = (int64_t)((int)blockIdx.x - rows) * kPagesThreads + threadIdx.x;
+    for (int64_t p = thread; p < a.blocks; p += step) {
+      const bool held = space.held[p >> 5] >> (p & 31) & 1;
+      if (head.refused || p < a.first || (held && p < head.limit)) {
+        a.remap[p] = (int32_t)p;
+        if (a.shared) a.shared_out[p] = a.shared[p];
+      } else if (held) {  // moves: its place's thread writes its count
+        a.remap[p] = space.copies[space.rank[p]].to;
+      } else {
+        a.remap[p] = -1;
+        if (a.shared && p < head.limit) {
+          const int from = space.copies[space.rank[p]].from;
+          a.shared_out[p] = a.shared[from];
+          a.shared_out[from] = 0;
+        } else if (a.shared) {
+          a.shared_out[p] = 0;
+        }
+      }
+    }
+    for (int64_t i = thread; i < a.pool_size; i += step)
+      a.pool_out[i] = head.refused ? a.pool[i] : i < a.blocks - head.limit ? (int32_t)(head.limit + i) : -1;
+    if (thread < 2)
+      a.pool_state_out[thread] = head.refused ? a.pool_state[thread] : thread == 0 ? 0 : a.blocks - head.limit;
+    return;
+  }
+  pages_copies<COUNT>(PageShape{a.heads, a.row_bytes, a.c_block, a.c_token, a.c_head}, space.copies, head.moves,
+                      a.caches, caches, a.cache_count, blockIdx.x - rows - others, gridDim.x - rows - others);
+}
+
+}  // namespace dsr

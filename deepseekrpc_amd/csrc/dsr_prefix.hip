@@ -1,0 +1,173 @@
+// C ABI of dsr_prefix_attention: argument checks and launches.
+#include "dsr_prefix.h"
+
+using namespace dsr;
+
+namespace {
+
+int32_t launched() { return hipGetLastError() == hipSuccess ? 0 : DSR_ERR_LAUNCH; }
+
+// Dimensions of the kernel that takes a head dimension.
+int prefix_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+
+// The work split of one pass over `count` groups or requests, from sizes alone.
+AttnPlan prefix_plan(const dsr_tree_attention_args_t& a, int64_t count) {
+  AttnPlan p{};
+  const int64_t group = a.q_heads / a.kv_heads;
+  const int64_t rows = count > 0 ? (a.tokens * group + count - 1) / count : 0;  // of a usual one
+  const bool big = a.head_dim > 128;
+  p.tile_rows = rows <= 16 ? 16 : big ? (rows <= 64 ? 64 : 128) : rows <= 32 ? 32 : 128;
+  p.tokens = p.tile_rows <= 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
+  p.min_steps = 128 / p.tokens;
+  p.cut = true;
+  p.groups = p.tile_rows < 128 || big ? 256 : 512;
+  const int64_t tiles = (a.tokens * group / p.tile_rows + count) * a.kv_heads, span = (int64_t)a.width * a.page;
+  while ((span / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
+  auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
+  p.group = (int)group;
+  p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
+  p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
+  const int64_t shares = tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;
+  if (shares < p.groups) p.groups = (int)((shares + 7) / 8 * 8);
+  return p;
+}
+
+// Addresses in the workspace; their end.
+int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
+  const dsr_tree_attention_args_t& a = x.a;
+  const int64_t counts[2] = {x.group_count, a.requests}, dim = prefix_dim(a.head_dim);
+  char* base = (char*)a.workspace;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* p = base + at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  int32_t* lows = (int32_t*)take(a.requests * 4);
+  int32_t* group_of = (int32_t*)take(a.requests * 4);
+  for (int pass = 0; pass < 2; ++pass) {
+    AttnPlan& p = j.p[pass] = prefix_plan(a, counts[pass]);
+    AttnBranch& b = j.b[pass];
+    const int64_t parts = 2 * (int64_t)p.groups * p.tile_rows;
+    p.part_o = (float*)take(parts * dim * 4);
+    p.part_ml = (float2*)take(parts * 8);
+    p.part_bad = (int32_t*)take(2 * (int64_t)p.groups * 4);
+    b.groups = pass == 0 ? x.groups : nullptr;
+    b.prefix = pass == 0 ? x.prefix_lengths : nullptr;
+    b.low = b.lows = lows;
+    b.group_of = group_of;
+    b.begin = (int32_t*)take((counts[pass] + 1) * 4);
+    b.bad = (int32_t*)take(counts[pass] * 4);
+    b.row_o = (float*)take(a.tokens * a.q_heads * dim * 4);
+    b.row_ml = (float2*)take(a.tokens * a.q_heads * 8);
+    b.count = counts[pass];
+    b.requests = a.requests;
+  }
+  return at;
+}
+
+template <class T, int DP>
+int32_t prefix_pass(const AttnBranchCall& c, hipStream_t s) {
+  const dsr_tree_attention_args_t& a = c.a;
+  // Workgroups for rows of no request, and for the requests' groups.
+  int64_t others = 0;
+  if (c.b.groups) {
+    others = (a.tokens * a.q_heads * a.head_dim * 2 + (1 << 18) - 1) >> 18;
+    const int64_t lows = (a.requests + kAttnThreads - 1) / kAttnThreads;
+    others = others < lows ? lows : others;
+    others = others > 256 ? 256 : others < 8 ? 8 : others;
+  }
+  const dim3 grid((unsigned)(c.p.groups + others)), threads(kAttnThreads);
+  auto wide = [&](auto WR) {
+    constexpr int wr = decltype(WR)::value;
+    constexpr bool whole = kAttnThreads % (DP / 8) == 0;
+    if (whole && a.page >= attn_round(DP) && a.k_token <= 1 << 24 && a.v_token <= 1 << 24)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, wr, whole, true>), grid, threads, 0, s, c);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, wr, false, true>), grid, threads, 0, s, c);
+  };
+  switch (c.p.tile_rows) {
+    case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4, true>), grid, threads, 0, s, c); break;
+    case 128: wide(std::integral_constant<int, 4>{}); break;
+    default: wide(std::integral_constant<int, DP <= 128 ? 1 : 2>{});
+  }
+  return launched();
+}
+
+template <class T, int DP>
+int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j, hipStream_t s) {
+  for (int pass = 0; pass < 2; ++pass) {
+    AttnBranchCall c{x.a, j.p[pass], j.b[pass]};
+    if (pass == 0) c.a.visible = nullptr;  // every row sees the whole prefix
+    const int32_t rc = prefix_pass<T, DP>(c, s);
+    if (rc != 0) return rc;
+  }
+  const int64_t rows = x.a.tokens * x.a.q_heads;
+  const dim3 threads(kAttnThreads);
+  auto grid = [&](int64_t each) {
+    const int64_t items = x.a.tokens * ((x.a.q_heads + each - 1) / each);
+    return dim3((unsigned)(items < (1 << 20) ? items : 1 << 20));
+  };
+  if (rows == 0) return 0;
+  if (rows <= 16384)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), grid(2), threads, 0, s, j);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), grid(8), threads, 0, s, j);
+  return launched();
+}
+
+template <class T>
+int32_t prefix_typed(const dsr_prefix_attention_args_t& x, const PrefixJoin& j, hipStream_t s) {
+  switch (prefix_dim(x.a.head_dim)) {
+    case 64: return prefix_launch<T, 64>(x, j, s);
+    case 128: return prefix_launch<T, 128>(x, j, s);
+    case 192: return prefix_launch<T, 192>(x, j, s);
+    default: return prefix_launch<T, 256>(x, j, s);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dsr_prefix_attention_workspace_bytes(const dsr_prefix_attention_args_t* args) {
+  if (!args || args->group_count < 0 || args->group_count > args->a.requests) return 0;
+  const size_t tree = dsr_tree_attention_workspace_bytes(&args->a);
+  if (tree == 0) return 0;
+  PrefixJoin j;
+  const size_t own = (size_t)prefix_space(*args, j);
+  return own > tree ? own : tree;
+}
+
+int32_t dsr_prefix_attention(const dsr_prefix_attention_args_t* args, void* stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_prefix_attention_args_t& x = *args;
+  const dsr_tree_attention_args_t& a = x.a;
+  if (x.group_count < 0 || x.group_count > a.requests) return DSR_ERR_ARG;
+  if (x.group_count == 0) return dsr_tree_attention(&x.a, stream);
+  if (!x.groups || !x.prefix_lengths) return DSR_ERR_ARG;
+  // What dsr_tree_attention asks.
+  if (a.page < 1 || (a.page & (a.page - 1)) || a.blocks < 1 || (int64_t)a.blocks * a.page > INT_MAX ||
+      a.table_ld < a.width || !(a.scale == a.scale) || a.scale - a.scale != 0.f)
+    return DSR_ERR_ARG;
+  const size_t need = dsr_prefix_attention_workspace_bytes(args);
+  if (need == 0) return DSR_ERR_ARG;
+  if (!a.table || !a.offsets || !a.kv_lengths || !a.status || !a.k_cache || !a.v_cache ||
+      (a.tokens > 0 && (!a.q || !a.out)))
+    return DSR_ERR_ARG;
+  for (const void* p : {a.q, a.k_cache, a.v_cache, (const void*)a.out})
+    if ((uintptr_t)p & 15u) return DSR_ERR_ARG;
+  for (int64_t st : {a.q_token, a.q_head, a.out_token, a.out_head, a.k_block, a.k_token, a.k_head, a.v_block,
+                     a.v_token, a.v_head})
+    if (st % 8 != 0 || st < 0) return DSR_ERR_ARG;
+  for (int64_t st : {a.k_block, a.k_token, a.v_block, a.v_token})
+    if (st > INT_MAX) return DSR_ERR_ARG;  // multiplied in 32 x 32 bits
+  if (!a.workspace || ((uintptr_t)a.workspace & 255u) || a.workspace_bytes < need) return DSR_ERR_WORKSPACE;
+  PrefixJoin j;
+  j.a = a;
+  prefix_space(x, j);
+  hipStream_t s = (hipStream_t)stream;
+  return a.dtype == DSR_BF16 ? prefix_typed<__bf16>(x, j, s) : prefix_typed<_Float16>(x, j, s);
+}
+
+}  // extern "C"

@@ -32,7 +32,7 @@
 #include "dsr_split.h"
 #include "dsr_verify.h"
 #include "dsr_wide.h"
-#include "dsr_tree.h"
+#include "dsr_branch.h"
 #include "dsr_wide_verify.h"
 
 namespace dsr {
@@ -1185,6 +1185,7 @@ const char* dsr_status_message(int32_t code) {
     case DSR_E_CAPACITY: return "the new tokens do not fit the token arrays";
     case DSR_E_TREE: return "drafted nodes are not a tree of at most 64 nodes in parent-first order";
     case DSR_E_BLOCK: return "a page id or slot lies outside the cache";
+    case DSR_E_PARENT: return "a parent is no row of the step before";
     default: return "unknown sampling status";
   }
 }

@@ -87,7 +87,7 @@ def _table(t, rows, dev):
     if _device_of(t, "table") != dev:
         raise ValueError(f"table must be on {dev}")
     if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or \
-            (t.shape[1] > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < t.shape[1]):
+            (rows > 0 and t.shape[1] > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < t.shape[1]):
         raise ValueError("table must be int32 [requests, pages], contiguous within rows")
     return t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[1]
 
@@ -399,62 +399,69 @@ class AttentionResult:
     status: torch.Tensor      # int32 [requests]
 
 
+def _attention(a, name, q, k_cache, v_cache, table, offsets, kv_lengths, visible, scale, lse, out):
+    """Checks a call over a paged cache and fills ``a`` (TreeAttentionArgs) but
+    for the workspace: the result, its device and what has to be kept."""
+    dev = _device_of(q, "q")
+    _unrecorded(name, q, k_cache, v_cache, out)
+    if q.dim() != 3 or q.dtype not in _ATTENTION_TYPES:
+        raise ValueError("q must be bf16/f16 of shape [tokens, heads, dim]")
+    n, heads, dim = q.shape
+    if _device_of(k_cache, "k_cache") != dev or k_cache.dim() != 4:
+        raise ValueError(f"k_cache must be [blocks, page, heads, dim] on {dev}")
+    blocks, page, kv_heads = k_cache.shape[0], _page(k_cache.shape[1]), k_cache.shape[2]
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("query heads must be a multiple of key heads")
+    if not 8 <= dim <= N.ATTENTION_MAX_DIM or dim % 8:
+        raise ValueError(f"the head dimension must be a multiple of 8 up to {N.ATTENTION_MAX_DIM}")
+    R = _requests(kv_lengths.numel())
+    if blocks < 1 or blocks * page > 2**31 - 1 or (n + R) * heads >= 2**29:
+        raise ValueError("the cache must hold 1 to 2^31 - 1 tokens, and (tokens + requests) x heads be below 2^29")
+    shape = (blocks, page, kv_heads, dim)
+    a.q, a.q_token, a.q_head = _rows(q, "q", q.dtype, dev, q.shape)
+    a.k_cache, a.k_block, a.k_token, a.k_head = _rows(k_cache, "k_cache", q.dtype, dev, shape)
+    a.v_cache, a.v_block, a.v_token, a.v_head = _rows(v_cache, "v_cache", q.dtype, dev, shape)
+    if max(a.k_block, a.k_token, a.v_block, a.v_token) > 2**31 - 1:
+        raise ValueError("strides of the caches' pages and tokens must be below 2^31")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    a.out, a.out_token, a.out_head = _rows(out, "out", q.dtype, dev, q.shape)
+    for t, what in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")):
+        if t.data_ptr() % 16 or any(s % 8 for s, size in zip(t.stride()[:-1], t.shape[:-1]) if size > 1):
+            raise ValueError(f"rows of {what} must be 16-byte aligned")
+    for field in ("q_token", "q_head", "out_token", "out_head", "k_block", "k_token", "k_head", "v_block",
+                  "v_token", "v_head"):  # strides of dimensions of one element are free
+        setattr(a, field, getattr(a, field) // 8 * 8)
+    a.kv_lengths = _array(kv_lengths, "kv_lengths", torch.int32, dev)
+    a.offsets = _array(offsets, "offsets", torch.int32, dev, R + 1)
+    a.table, a.table_ld, a.width = _table(table, R, dev)
+    if a.width * page > 2**31 - 1:
+        raise ValueError("a table row must span less than 2^31 tokens")
+    if n > 0 and R == 0:
+        raise ValueError("tokens need requests")
+    if visible is not None:
+        a.visible = _array(visible, "visible", torch.int64, dev, n)
+    a.scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(a.scale):
+        raise ValueError("scale must be finite")
+    res = AttentionResult(out, torch.empty(n, heads, dtype=torch.float32, device=dev) if lse else None,
+                          torch.empty(R, dtype=torch.int32, device=dev))
+    a.lse = res.lse.data_ptr() if lse else None
+    a.status = res.status.data_ptr()
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim = _ATTENTION_TYPES[q.dtype], heads, kv_heads, dim
+    a.page, a.blocks, a.requests, a.tokens = page, blocks, R, n
+    return res, dev, (q, k_cache, v_cache, table, offsets, kv_lengths, visible, *vars(res).values())
+
+
 class PreparedTreeAttention(_Prepared):
     """See ``tree_attention``."""
 
     def __init__(self, q, k_cache, v_cache, table, offsets, kv_lengths, *, visible=None, scale: float | None = None,
                  lse: bool = False, out=None):
-        dev = _device_of(q, "q")
-        _unrecorded("tree_attention", q, k_cache, v_cache, out)
-        if q.dim() != 3 or q.dtype not in _ATTENTION_TYPES:
-            raise ValueError("q must be bf16/f16 of shape [tokens, heads, dim]")
-        n, heads, dim = q.shape
-        if _device_of(k_cache, "k_cache") != dev or k_cache.dim() != 4:
-            raise ValueError(f"k_cache must be [blocks, page, heads, dim] on {dev}")
-        blocks, page, kv_heads = k_cache.shape[0], _page(k_cache.shape[1]), k_cache.shape[2]
-        if heads < 1 or kv_heads < 1 or heads % kv_heads:
-            raise ValueError("query heads must be a multiple of key heads")
-        if not 8 <= dim <= N.ATTENTION_MAX_DIM or dim % 8:
-            raise ValueError(f"the head dimension must be a multiple of 8 up to {N.ATTENTION_MAX_DIM}")
-        R = _requests(kv_lengths.numel())
-        if blocks < 1 or blocks * page > 2**31 - 1 or (n + R) * heads >= 2**29:
-            raise ValueError("the cache must hold 1 to 2^31 - 1 tokens, and (tokens + requests) x heads be below 2^29")
         a = N.TreeAttentionArgs()
-        shape = (blocks, page, kv_heads, dim)
-        a.q, a.q_token, a.q_head = _rows(q, "q", q.dtype, dev, q.shape)
-        a.k_cache, a.k_block, a.k_token, a.k_head = _rows(k_cache, "k_cache", q.dtype, dev, shape)
-        a.v_cache, a.v_block, a.v_token, a.v_head = _rows(v_cache, "v_cache", q.dtype, dev, shape)
-        if max(a.k_block, a.k_token, a.v_block, a.v_token) > 2**31 - 1:
-            raise ValueError("strides of the caches' pages and tokens must be below 2^31")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        a.out, a.out_token, a.out_head = _rows(out, "out", q.dtype, dev, q.shape)
-        for t, name in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")):
-            if t.data_ptr() % 16 or any(s % 8 for s, size in zip(t.stride()[:-1], t.shape[:-1]) if size > 1):
-                raise ValueError(f"rows of {name} must be 16-byte aligned")
-        for field in ("q_token", "q_head", "out_token", "out_head", "k_block", "k_token", "k_head", "v_block",
-                      "v_token", "v_head"):  # strides of dimensions of one element are free
-            setattr(a, field, getattr(a, field) // 8 * 8)
-        a.kv_lengths = _array(kv_lengths, "kv_lengths", torch.int32, dev)
-        a.offsets = _array(offsets, "offsets", torch.int32, dev, R + 1)
-        a.table, a.table_ld, a.width = _table(table, R, dev)
-        if a.width * page > 2**31 - 1:
-            raise ValueError("a table row must span less than 2^31 tokens")
-        if n > 0 and R == 0:
-            raise ValueError("tokens need requests")
-        if visible is not None:
-            a.visible = _array(visible, "visible", torch.int64, dev, n)
-        a.scale = dim ** -0.5 if scale is None else float(scale)
-        if not math.isfinite(a.scale):
-            raise ValueError("scale must be finite")
-        res = AttentionResult(out, torch.empty(n, heads, dtype=torch.float32, device=dev) if lse else None,
-                              torch.empty(R, dtype=torch.int32, device=dev))
-        a.lse = res.lse.data_ptr() if lse else None
-        a.status = res.status.data_ptr()
-        a.dtype, a.q_heads, a.kv_heads, a.head_dim = _ATTENTION_TYPES[q.dtype], heads, kv_heads, dim
-        a.page, a.blocks, a.requests, a.tokens = page, blocks, R, n
-        self._setup("dsr_tree_attention", a, dev, res,
-                    (q, k_cache, v_cache, table, offsets, kv_lengths, visible, *vars(res).values()),
+        res, dev, keep = _attention(a, "tree_attention", q, k_cache, v_cache, table, offsets, kv_lengths, visible,
+                                    scale, lse, out)
+        self._setup("dsr_tree_attention", a, dev, res, keep,
                     N.load().dsr_tree_attention_workspace_bytes(ctypes.byref(a)))
 
 
