@@ -100,13 +100,14 @@ struct AttnBranch {
   const int32_t* groups;  // the groups' pass: [count + 1], else null
   const int32_t* prefix;  // the groups' pass: [count]
   const int32_t* low;     // the requests' pass: first token of each one's own, -1: refused
-  int32_t* begin;         // [count + 1]: steps before each request
+  int2* tiles;            // [key heads, rows of a head]: a tile's first share and their number, at its first row
   int32_t* bad;           // [count]: a page id outside the cache
   float* row_o;           // [tokens, query heads, head dim of the kernel]
   float2* row_ml;         // [tokens, query heads]: base (log2) and sum
   int64_t count;          // groups or requests
   int32_t* lows;          // the groups' pass writes these: `low`,
-  int32_t* group_of;      // and each request's group, -1: none
+  int32_t* group_of;      // each request's group, -1: none,
+  int32_t* group_lo;      // and its group's first new token
   int64_t requests;
 };
 struct AttnBranchCall {
@@ -276,10 +277,6 @@ struct AttnWork {
     for (int first = 0; first < R; first += 64) {
       steps = hold(c, first);
       upto = attn_wave_scan(steps);
-      if constexpr (BRANCH) {  // for the join
-        const int r = first + (int)(threadIdx.x & 63);
-        if (blockIdx.x == 0 && threadIdx.x < 64 && r < R) c.b.begin[r] = (int)total + upto - steps;
-      }
       total += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
       // Requests without rows have no work: the first workgroup tells their status.
       const int l = threadIdx.x & 63;
@@ -291,8 +288,6 @@ struct AttnWork {
         }
       }
     }
-    if constexpr (BRANCH)
-      if (blockIdx.x == 0 && threadIdx.x == 0) c.b.begin[R] = (int)total;
     quota = attn_quota(p, total);
     const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
@@ -368,6 +363,10 @@ struct AttnWork {
     s.part = 2 * me + (s0 > 0 ? 0 : 1);  // a tile begun elsewhere can only be a workgroup's first
     s.from = base + unit * steps;
     s.to = s.from + steps;
+    if constexpr (BRANCH)  // for the join
+      if (s0 == 0 && threadIdx.x == 0)
+        c.b.tiles[((int64_t)s.head * a.tokens + q.lo) * p.group + s.tile * p.tile_rows] =
+            int2{me, s.whole ? 1 : (int)((s.to - 1) / quota) - me + 1};
     at += s1 - s0;
     return true;
   }
@@ -419,13 +418,20 @@ __device__ __forceinline__ void attn_branch_lows(int threads) {
         hi = mid;
     }
     int low = wrong ? -1 : 0, mine = -1;
+    AttnRequest q{};
     if (!wrong && lo > 0 && r < c.b.groups[lo]) {
       const int prefix = c.b.prefix[lo - 1];
       low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
-      mine = low > 0 ? lo - 1 : -1;
+      if (low > 0) {
+        mine = lo - 1;
+        q = attn_request(c, mine);
+        const AttnRequest own = attn_request(c.a, c.p, r);
+        if (own.lo < q.lo || own.lo + own.n > q.lo + q.n) low = mine = -1;  // offsets that do not ascend
+      }
     }
     c.b.lows[r] = low;
     c.b.group_of[r] = mine;
+    c.b.group_lo[r] = q.lo;
   }
 }
 

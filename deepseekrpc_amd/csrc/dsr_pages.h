@@ -20,7 +20,7 @@ namespace dsr {
 
 constexpr int kPagesThreads = 256;
 constexpr int kForkThreads = 1024;
-constexpr int kBitsChunk = 4 * kPagesThreads;  // words of 32 pages that a workgroup counts
+constexpr int kBitsChunk = kPagesThreads;      // words of 32 pages that a workgroup counts
 constexpr int kPagesInline = 128;              // caches whose pointers are a launch's arguments
 
 typedef uint32_t pages_u32x4 __attribute__((ext_vector_type(4)));
@@ -51,6 +51,9 @@ __device__ __forceinline__ int pages_total(int x, int* part) {
   __syncthreads();
   return part[0] + part[1] + part[2] + part[3];
 }
+
+// A place in a ring: x < 2 size <= 2^31.
+__device__ __forceinline__ int pages_wrap(int x, int size) { return x >= size ? x - size : x; }
 
 // Inclusive sum over the lanes of a wave.
 __device__ __forceinline__ int pages_scan(int x) {
@@ -297,35 +300,33 @@ __global__ __launch_bounds__(kPagesThreads) void k_fork_rows(dsr_fork_args_t a) 
 }
 
 // Freed pages to the pool, a chunk of the bits a workgroup: each counts the
-// bits before its own.
+// bits before its own, then its threads take its pages, side by side.
 __device__ __forceinline__ void fork_free(const dsr_fork_args_t& a, const ForkSpace& space, int chunk) {
-  __shared__ int part[4];
+  __shared__ int part[4], base[kBitsChunk];
+  __shared__ uint32_t word[kBitsChunk];
   const int64_t words = pages_words(a.blocks), begin = (int64_t)chunk * kBitsChunk;
   int mine = 0;
   for (int64_t i = threadIdx.x; i < begin; i += kPagesThreads) mine += __popc(space.freed[i]);
-  int before = pages_total(mine, part);
-  uint32_t bits[4];
-  mine = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t at = begin + 4 * (int)threadIdx.x + i;
-    bits[i] = at < words ? space.freed[at] : 0;
-    mine += __popc(bits[i]);
-  }
+  const int before = chunk > 0 ? pages_total(mine, part) : 0;
+  const uint32_t bits = begin + threadIdx.x < words ? space.freed[begin + threadIdx.x] : 0;
   const ForkHead head = *space.head;
-  const int64_t size = a.pool_size, room = size - head.count + head.taken;
-  const int all = before + pages_total(mine, part);
-  before += pages_before(mine, part);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    for (uint32_t b = bits[i]; b; b &= b - 1, ++before) {
-      const int id = (int)((begin + 4 * (int)threadIdx.x + i) * 32) + __ffs(b) - 1;
-      a.shared_out[id] = 0;
-      if (before < room) a.pool[(head.first + (int64_t)head.count + before) % size] = id;
-    }
+  word[threadIdx.x] = bits;
+  const int upto = pages_before(__popc(bits), part);
+  base[threadIdx.x] = before + upto;
+  __syncthreads();
+  const int size = a.pool_size, room = size - head.count + head.taken;
+  const int all = base[kBitsChunk - 1] + __popc(word[kBitsChunk - 1]);
+  const int end = (int)(a.blocks - begin * 32 < kBitsChunk * 32 ? a.blocks - begin * 32 : kBitsChunk * 32);
+  for (int p = threadIdx.x; p < end; p += kPagesThreads) {
+    const uint32_t w = word[p >> 5], bit = 1u << (p & 31);
+    if (!(w & bit)) continue;
+    const int id = (int)(begin * 32) + p, at = base[p >> 5] + __popc(w & (bit - 1));
+    a.shared_out[id] = 0;
+    if (at < room) a.pool[pages_wrap(pages_wrap(head.first + head.count, size) + at, size)] = id;
+  }
   if (chunk == pages_chunks(a.blocks) - 1 && threadIdx.x == 0) {
-    a.pool_state_out[0] = (int32_t)((head.first + (int64_t)head.taken) % size);
-    a.pool_state_out[1] = head.count - head.taken + (int32_t)(all < room ? all : room);
+    a.pool_state_out[0] = pages_wrap(head.first + head.taken, size);
+    a.pool_state_out[1] = head.count - head.taken + (all < room ? all : room);
   }
 }
 
@@ -430,39 +431,38 @@ __global__ __launch_bounds__(kPagesThreads) void k_compact_plan(dsr_compact_args
     moved += __popc(held & pages_range(i, limit, blocks));
     open += __popc(~held & pages_range(i, first, limit));
   }
-  moved = pages_total(moved, part);
-  open = pages_total(open, part);
-  uint32_t from[4], to[4];
-  int m = 0, o = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t at = begin + 4 * (int)threadIdx.x + i;
-    const uint32_t held = at < words ? space.held[at] : 0;
-    from[i] = at < words ? held & pages_range(at, limit, blocks) : 0;
-    to[i] = at < words ? ~held & pages_range(at, first, limit) : 0;
-    m += __popc(from[i]);
-    o += __popc(to[i]);
+  if (begin > 0) {
+    moved = pages_total(moved, part);
+    open = pages_total(open, part);
   }
-  const int all = moved + pages_total(m, part);
-  moved += pages_before(m, part);
-  open += pages_before(o, part);
-  const bool refused = space.head->refused;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int id = (int)((begin + 4 * (int)threadIdx.x + i) * 32) - 1;
-    for (uint32_t b = from[i]; b; b &= b - 1, ++moved) {
-      space.rank[id + __ffs(b)] = moved;
-      space.copies[moved].from = id + __ffs(b);
-    }
-    for (uint32_t b = to[i]; b; b &= b - 1, ++open) {
-      space.rank[id + __ffs(b)] = open;
-      space.copies[open].to = id + __ffs(b);
-      space.copies[open].tokens = a.page;
+  __shared__ uint32_t from[kBitsChunk], to[kBitsChunk];
+  __shared__ int from_base[kBitsChunk], to_base[kBitsChunk];
+  const int x = threadIdx.x;
+  const uint32_t held = begin + x < words ? space.held[begin + x] : 0;
+  from[x] = begin + x < words ? held & pages_range(begin + x, limit, blocks) : 0;
+  to[x] = begin + x < words ? ~held & pages_range(begin + x, first, limit) : 0;
+  const int m = pages_before(__popc(from[x]), part), o = pages_before(__popc(to[x]), part);
+  from_base[x] = moved + m;
+  to_base[x] = open + o;
+  __syncthreads();
+  const int end = (int)(blocks - begin * 32 < kBitsChunk * 32 ? blocks - begin * 32 : kBitsChunk * 32);
+  for (int p = x; p < end; p += kPagesThreads) {
+    const int w = p >> 5, id = (int)(begin * 32) + p;
+    const uint32_t bit = 1u << (p & 31);
+    if (from[w] & bit) {
+      const int at = from_base[w] + __popc(from[w] & (bit - 1));
+      space.rank[id] = at;
+      space.copies[at].from = id;
+    } else if (to[w] & bit) {
+      const int at = to_base[w] + __popc(to[w] & (bit - 1));
+      space.rank[id] = at;
+      space.copies[at].to = id;
+      space.copies[at].tokens = a.page;
     }
   }
-  if (begin + kBitsChunk >= words && threadIdx.x == 0) {
+  if (begin + kBitsChunk >= words && x == 0) {
     space.head->limit = (int32_t)limit;
-    space.head->moves = refused ? 0 : all;
+    space.head->moves = space.head->refused ? 0 : from_base[kBitsChunk - 1] + __popc(from[kBitsChunk - 1]);
   }
 }
 

@@ -36,124 +36,118 @@ __device__ __forceinline__ int prefix_owner(const dsr_tree_attention_args_t& a, 
   return lo;
 }
 
-// The shares that hold a tile of head `head` of request (or group) r.
-__device__ __forceinline__ void prefix_shares(const AttnPlan& p, const AttnBranch& b, const AttnRequest& q, int r,
-                                              int head, int tile, int& first, int& last) {
-  const uint32_t quota = attn_quota(p, b.begin[b.count]);
-  const uint32_t steps = AttnWork<false, AttnBranchCall>::steps_of(p, q);
-  const uint32_t from = b.begin[r] + (head * (uint32_t)q.tiles + tile) * steps;
-  first = from / quota;
-  last = (from + steps - 1) / quota;
+// Where the shares of the tile of row `row` (of a request's, or group's, rows
+// of key head `head`; its first token is `lo`) are told.
+__device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int lo, int head, int row) {
+  return j.b[pass].tiles[((int64_t)head * j.a.tokens + lo) * j.p[0].group + (row & -j.p[pass].tile_rows)];
 }
 
-// JR rows (heads of a token) at a time; the threads left over take every
-// SLOTS-th part each, summed in a fixed order.
+// An item is a token and `each` blocks of JR of its rows (heads), a block at a
+// time.  The threads left over take every SLOTS-th part each, summed in a fixed
+// order; a thread has FLIGHT parts in flight.
 template <class T, int DP, int JR>
-__global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j) {
+__global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int each) {
   typedef typename AttnType<T>::x4 x4;
   constexpr int E = JR * DP / 4;  // four dimensions of a row each
   constexpr int SLOTS = E < kAttnThreads ? kAttnThreads / E : 1;
+  constexpr int FLIGHT = 4;
   __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const dsr_tree_attention_args_t& a = j.a;
-  const int heads = a.q_heads, group = j.p[0].group, blocks = (heads + JR - 1) / JR;
+  const int heads = a.q_heads, group = j.p[0].group, chunks = (heads + JR * each - 1) / (JR * each);
   const int slot = SLOTS > 1 ? threadIdx.x / E : 0;
   const bool spare = slot >= SLOTS;  // 192 dimensions
-  const int64_t items = a.tokens * blocks;
+  const int64_t items = a.tokens * chunks;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int t = (int)(item / blocks), h0 = (int)(item - (int64_t)t * blocks) * JR;
+    const int t = chunks == 1 ? (int)item : (int)(item / chunks), chunk = (int)(item - (int64_t)t * chunks);
     const int r = prefix_owner(a, t);
     if (r >= a.requests) continue;
+    const int g = j.b[1].group_of[r], g_lo = j.b[1].group_lo[r];
     const AttnRequest own = attn_request(a, j.p[1], j.b[1], r);
-    if (t < own.lo || t >= own.lo + own.n) continue;  // a row of no request
-    int g = own.fine ? j.b[1].group_of[r] : -1;
-    AttnRequest all{};
-    if (g >= 0) {
-      all = attn_request(a, j.p[0], j.b[0], g);
-      if (t < all.lo || t >= all.lo + all.n) g = -1;  // offsets that do not ascend
-    }
+    const int lo = own.lo;
+    if (t < lo || t >= lo + own.n) continue;  // a row of no request
+    const int h_end = min(heads, (chunk + 1) * JR * each);
+    for (int h0 = chunk * JR * each; h0 < h_end; h0 += JR) {
 #pragma unroll
-    for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
-      const int in = x / (DP / 4), h = h0 + in, d = x % (DP / 4) * 4;
-      const bool live = h < heads && !spare;
-      const int kv_head = h / group, of_group = h - kv_head * group;
-      const int64_t row = (int64_t)t * heads + h;
-      float M = -INFINITY, L = 0.f;
-      attn_f32x4 o = {};
-      auto add = [&](float m, float l, attn_f32x4 x) {
-        const float both = fmaxf(M, m), f = M == both ? 1.f : __builtin_amdgcn_exp2f(M - both);
-        const float g = m == both ? 1.f : __builtin_amdgcn_exp2f(m - both);
-        M = both;
-        L = L * f + l * g;
-        o = o * f + x * g;
-      };
-      if (live && own.fine) {
-        int at = slot;  // parts of both passes, counted on
+      for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
+        const int in = x / (DP / 4), h = h0 + in, d = x % (DP / 4) * 4;
+        const bool live = h < heads && !spare;
+        const int64_t row = (int64_t)t * heads + h;
+        float M = -INFINITY, L = 0.f;
+        attn_f32x4 o = {};
+        auto add = [&](float m, float l, attn_f32x4 x) {
+          const float both = fmaxf(M, m), f = M == both ? 1.f : __builtin_amdgcn_exp2f(M - both);
+          const float g = m == both ? 1.f : __builtin_amdgcn_exp2f(m - both);
+          M = both;
+          L = L * f + l * g;
+          o = o * f + x * g;
+        };
+        if (live && own.fine) {
+          const int kv_head = attn_token(j.p[0], h), of_group = h - kv_head * group;
+          const int row0 = (t - g_lo) * group + of_group, row1 = (t - lo) * group + of_group;
+          const int2 s0 = g >= 0 ? prefix_tile(j, 0, g_lo, kv_head, row0) : int2{0, 0};
+          const int2 s1 = prefix_tile(j, 1, lo, kv_head, row1);
+          const int in0 = row0 & (j.p[0].tile_rows - 1), in1 = row1 & (j.p[1].tile_rows - 1);
+          const int count = s0.y + s1.y;
+          for (int i0 = slot; i0 < count; i0 += FLIGHT * SLOTS) {
+            float2 ml[FLIGHT];
+            attn_f32x4 v[FLIGHT];
 #pragma unroll
-        for (int pass = 0; pass < 2; ++pass) {
-          if (pass == 0 && g < 0) continue;
-          const AttnPlan& p = j.p[pass];
-          const AttnBranch& b = j.b[pass];
-          const AttnRequest& q = pass == 0 ? all : own;
-          const int in_tiles = (t - q.lo) * group + of_group, tile = in_tiles >> p.tile_shift;
-          const int in_tile = in_tiles - (tile << p.tile_shift);
-          int first, last;
-          prefix_shares(p, b, q, pass == 0 ? g : r, kv_head, tile, first, last);
-          if (first == last) {
-            if (at == 0) {
-              const float2 ml = b.row_ml[row];
-              add(ml.x, ml.y, *(const attn_f32x4*)&b.row_o[row * DP + d]);
-              at += SLOTS;
-            }
-            at -= 1;
-          } else {
-            const int n = last - first + 1;
-#pragma unroll 4
-            for (; at < n; at += SLOTS) {
+            for (int k = 0; k < FLIGHT; ++k) {
+              const int i = min(i0 + k * SLOTS, count - 1);
+              const bool second = i >= s0.y;
+              const int c = second ? i - s0.y : i, first = second ? s1.x : s0.x;
+              const bool whole = (second ? s1.y : s0.y) == 1;
               // The first part is its workgroup's last (an odd place), the others their workgroups' first.
-              const int64_t place = ((int64_t)(2 * (first + at) + (at == 0)) << p.tile_shift) + in_tile;
-              const float2 ml = p.part_ml[place];
-              add(ml.x, ml.y, *(const attn_f32x4*)&p.part_o[place * DP + d]);
+              const int place = 2 * (first + c) + (c == 0);
+              const int64_t part = second ? ((int64_t)place << j.p[1].tile_shift) + in1
+                                          : ((int64_t)place << j.p[0].tile_shift) + in0;
+              const int64_t at = whole ? row : part;
+              const float2* m_at = second ? (whole ? j.b[1].row_ml : j.p[1].part_ml)
+                                          : (whole ? j.b[0].row_ml : j.p[0].part_ml);
+              const float* o_at = second ? (whole ? j.b[1].row_o : j.p[1].part_o)
+                                         : (whole ? j.b[0].row_o : j.p[0].part_o);
+              ml[k] = m_at[at];
+              v[k] = *(const attn_f32x4*)&o_at[at * DP + d];
             }
-            at -= n;
+#pragma unroll
+            for (int k = 0; k < FLIGHT; ++k)
+              if (i0 + k * SLOTS < count) add(ml[k].x, ml[k].y, v[k]);
           }
         }
-      }
-      if constexpr (SLOTS > 1) {
-        if (!spare) so[slot][x] = o;
-        if (d == 0 && !spare) {
-          sm[slot][in] = M;
-          sl[slot][in] = L;
-        }
-        __syncthreads();
-        if (slot == 0) {
+        if constexpr (SLOTS > 1) {
+          if (!spare) so[slot][x] = o;
+          if (d == 0 && !spare) {
+            sm[slot][in] = M;
+            sl[slot][in] = L;
+          }
+          __syncthreads();
+          if (slot == 0) {
 #pragma unroll
-          for (int i = 1; i < SLOTS; ++i) add(sm[i][in], sl[i][in], so[i][x]);
+            for (int i = 1; i < SLOTS; ++i) add(sm[i][in], sl[i][in], so[i][x]);
+          }
+          __syncthreads();  // the next block's
         }
-        __syncthreads();  // the next item's
-      }
-      if (slot > 0 || !live || d >= a.head_dim) continue;
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      x4 y;
+        if (slot > 0 || !live || d >= a.head_dim) continue;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        x4 y;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
-      *(x4*)((T*)a.out + (int64_t)t * a.out_token + (int64_t)h * a.out_head + d) = y;
-      if (a.lse && d == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+        *(x4*)((T*)a.out + (int64_t)t * a.out_token + (int64_t)h * a.out_head + d) = y;
+        if (a.lse && d == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+      }
     }
-    if (t == own.lo && h0 == 0 && threadIdx.x == 0) {
+    if (t == lo && chunk == 0 && threadIdx.x == 0) {
       // A request's (a group's) last tile of its first head speaks for its page ids.
       int bad = 0;
       if (own.fine)
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
           if (pass == 0 && g < 0) continue;
-          const AttnRequest& q = pass == 0 ? all : own;
-          int first, last;
-          prefix_shares(j.p[pass], j.b[pass], q, pass == 0 ? g : r, 0, q.tiles - 1, first, last);
-          if (first == last)
-            bad |= j.b[pass].bad[pass == 0 ? g : r];
-          else
-            for (int c = first; c <= last; ++c) bad |= j.p[pass].part_bad[2 * c + (c == first)];
+          const AttnRequest q = pass == 0 ? attn_request(a, j.p[0], j.b[0], g) : own;
+          const int2 s = prefix_tile(j, pass, q.lo, 0, (q.tiles - 1) * j.p[pass].tile_rows);
+          if (s.y == 1) bad |= j.b[pass].bad[pass == 0 ? g : r];
+          for (int c = 0; s.y > 1 && c < s.y; ++c) bad |= j.p[pass].part_bad[2 * (s.x + c) + (c == 0)];
         }
       a.status[r] = !own.fine ? DSR_E_LENGTH : bad ? DSR_E_BLOCK : DSR_OK;
     }

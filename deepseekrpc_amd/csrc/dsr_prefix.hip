@@ -20,7 +20,7 @@ AttnPlan prefix_plan(const dsr_tree_attention_args_t& a, int64_t count) {
   p.tokens = p.tile_rows <= 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
   p.min_steps = 128 / p.tokens;
   p.cut = true;
-  p.groups = p.tile_rows < 128 || big ? 256 : 512;
+  p.groups = big || (p.tile_rows < 128 && p.tile_rows > 16) ? 256 : 512;
   const int64_t tiles = (a.tokens * group / p.tile_rows + count) * a.kv_heads, span = (int64_t)a.width * a.page;
   while ((span / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
   auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
@@ -45,6 +45,7 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
   };
   int32_t* lows = (int32_t*)take(a.requests * 4);
   int32_t* group_of = (int32_t*)take(a.requests * 4);
+  int32_t* group_lo = (int32_t*)take(a.requests * 4);
   for (int pass = 0; pass < 2; ++pass) {
     AttnPlan& p = j.p[pass] = prefix_plan(a, counts[pass]);
     AttnBranch& b = j.b[pass];
@@ -56,7 +57,8 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
     b.prefix = pass == 0 ? x.prefix_lengths : nullptr;
     b.low = b.lows = lows;
     b.group_of = group_of;
-    b.begin = (int32_t*)take((counts[pass] + 1) * 4);
+    b.group_lo = group_lo;
+    b.tiles = (int2*)take(a.tokens * a.q_heads * 8);
     b.bad = (int32_t*)take(counts[pass] * 4);
     b.row_o = (float*)take(a.tokens * a.q_heads * dim * 4);
     b.row_ml = (float2*)take(a.tokens * a.q_heads * 8);
@@ -94,6 +96,8 @@ int32_t prefix_pass(const AttnBranchCall& c, hipStream_t s) {
   return launched();
 }
 
+constexpr int64_t kPrefixFewRows = 16384, kPrefixItems = 4096;
+
 template <class T, int DP>
 int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j, hipStream_t s) {
   for (int pass = 0; pass < 2; ++pass) {
@@ -103,16 +107,17 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
     if (rc != 0) return rc;
   }
   const int64_t rows = x.a.tokens * x.a.q_heads;
-  const dim3 threads(kAttnThreads);
-  auto grid = [&](int64_t each) {
-    const int64_t items = x.a.tokens * ((x.a.q_heads + each - 1) / each);
-    return dim3((unsigned)(items < (1 << 20) ? items : 1 << 20));
-  };
   if (rows == 0) return 0;
-  if (rows <= 16384)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), grid(2), threads, 0, s, j);
+  const int jr = rows <= kPrefixFewRows ? 2 : 8;
+  // Blocks of rows of an item: one where there are few, else so many that the chip still has items enough.
+  const int64_t blocks = (x.a.q_heads + jr - 1) / jr, most = x.a.tokens * blocks / kPrefixItems;
+  const int each = (int)(most < 1 ? 1 : most < blocks ? most : blocks);
+  const int64_t items = x.a.tokens * ((blocks + each - 1) / each);
+  const dim3 grid((unsigned)(items < (1 << 20) ? items : 1 << 20)), threads(kAttnThreads);
+  if (jr == 2)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), grid, threads, 0, s, j, each);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), grid(8), threads, 0, s, j);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), grid, threads, 0, s, j, each);
   return launched();
 }
 
