@@ -91,30 +91,31 @@ struct AttnCall {
   AttnPlan p;
 };
 
-// dsr_prefix_attention goes over the rows twice, with these kernels: once over
-// the groups' prefixes (a "request" is a group then, with the tokens of all
-// its requests, and every row sees every token), once over each request's own
-// tokens behind its prefix.  Every result is a part, whose join is another
-// launch: whole tiles go to rows of float32.
+// dsr_prefix_attention goes over the rows twice, with these kernels' bodies:
+// once over the groups' prefixes (a "request" is a group then, with the tokens
+// of all its requests, and every row sees every token), once over each
+// request's own tokens behind its prefix.  Every result is a part, whose join is
+// another launch: whole tiles go to rows of float32.
 struct AttnBranch {
-  const int32_t* groups;  // the groups' pass: [count + 1], else null
-  const int32_t* prefix;  // the groups' pass: [count]
-  const int32_t* low;     // the requests' pass: first token of each one's own, -1: refused
+  const int32_t* groups;  // [group_count + 1]
+  const int32_t* prefix;  // [group_count]
+  int32_t group_count;
+  int32_t own;            // the requests' pass, else the groups'
+  int64_t count;          // requests or groups
   int2* tiles;            // [key heads, rows of a head]: a tile's first share and their number, at its first row
   int32_t* bad;           // [count]: a page id outside the cache
   float* row_o;           // [tokens, query heads, head dim of the kernel]
   float2* row_ml;         // [tokens, query heads]: base (log2) and sum
-  int64_t count;          // groups or requests
-  int32_t* lows;          // the groups' pass writes these: `low`,
-  int32_t* group_of;      // each request's group, -1: none,
+  int32_t* low;           // each request's first own token, -1: refused,
+  int32_t* group_of;      // its group, -1: none,
   int32_t* group_lo;      // and its group's first new token
-  int64_t requests;
 };
 struct AttnBranchCall {
   dsr_tree_attention_args_t a;
   AttnPlan p;
   AttnBranch b;
 };
+constexpr int kAttnLows = 1024;  // requests whose `low` every workgroup finds for itself (attn_branch_lows)
 template <bool BRANCH>
 struct AttnArgs {
   typedef AttnCall type;
@@ -124,12 +125,12 @@ struct AttnArgs<true> {
   typedef AttnBranchCall type;
 };
 template <bool BRANCH = false>
-__device__ __forceinline__ const typename AttnArgs<BRANCH>::type& attn_call() {
+__device__ __forceinline__ const typename AttnArgs<BRANCH>::type& attn_call(int pass = 0) {
   typedef typename AttnArgs<BRANCH>::type Call;
   typedef const Call __attribute__((address_space(4))) * Args;
   Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(args));
-  return *(const Call*)args;
+  return ((const Call*)args)[pass];
 }
 
 struct AttnRequest {
@@ -162,19 +163,20 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   return q;
 }
 
-// The same of a group or, behind its prefix, of a request.
-__device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_args_t& a, const AttnPlan& p,
-                                                    const AttnBranch& b, int r) {
-  if (!b.groups) {
-    AttnRequest q = attn_request(a, p, r);
-    q.low = b.low[r];
-    if (q.low < 0 || a.kv_lengths[r] - q.n < q.low) q.fine = false;
-    if (!q.fine) q.kv = 0;
-    if (q.kv == 0) q.low = 0;
-    return q;
-  }
+// The same of a request behind its prefix,
+__device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t& a, const AttnPlan& p, int r, int low) {
+  AttnRequest q = attn_request(a, p, r);
+  q.low = low;
+  if (low < 0 || a.kv_lengths[r] - q.n < low) q.fine = false;
+  if (!q.fine) q.kv = 0;
+  if (q.kv == 0) q.low = 0;
+  return q;
+}
+// and of a group.
+__device__ __forceinline__ AttnRequest attn_group(const dsr_tree_attention_args_t& a, const AttnPlan& p,
+                                                  const AttnBranch& b, int g) {
   AttnRequest q;
-  const int N = (int)a.tokens, R = (int)b.requests, r0 = b.groups[r], r1 = b.groups[r + 1], kv = b.prefix[r];
+  const int N = (int)a.tokens, R = (int)a.requests, r0 = b.groups[g], r1 = b.groups[g + 1], kv = b.prefix[g];
   q.fine = r0 >= 0 && r0 < r1 && r1 <= R && kv > 0 && kv <= (int64_t)a.width * a.page;
   int lo = q.fine ? a.offsets[r0] : 0, hi = q.fine ? a.offsets[r1] : 0;
   lo = lo < 0 ? 0 : lo > N ? N : lo;
@@ -187,20 +189,26 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   q.low = 0;
   return q;
 }
+// What attn_branch_lows left for the workgroup.
+__device__ __forceinline__ int* attn_lows() {
+  __shared__ int lows[kAttnLows];
+  return lows;
+}
 // A pass's requests, the context that every row sees, the table row, the mask words.
 __device__ __forceinline__ int64_t attn_count(const AttnCall& c) { return c.a.requests; }
 __device__ __forceinline__ int64_t attn_count(const AttnBranchCall& c) { return c.b.count; }
 __device__ __forceinline__ AttnRequest attn_request(const AttnCall& c, int r) { return attn_request(c.a, c.p, r); }
 __device__ __forceinline__ AttnRequest attn_request(const AttnBranchCall& c, int r) {
-  return attn_request(c.a, c.p, c.b, r);
+  if (!c.b.own) return attn_group(c.a, c.p, c.b, r);
+  return attn_own(c.a, c.p, r, c.a.requests <= kAttnLows ? attn_lows()[r] : c.b.low[r]);
 }
 __device__ __forceinline__ int attn_context(const AttnCall&, const AttnRequest& q) { return q.kv - q.n; }
 __device__ __forceinline__ int attn_context(const AttnBranchCall& c, const AttnRequest& q) {
-  return c.b.groups ? q.kv : q.kv - q.n;
+  return c.b.own ? q.kv - q.n : q.kv;
 }
 __device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r) { return c.a.table + r * c.a.table_ld; }
 __device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int r) {
-  return c.a.table + (c.b.groups ? c.b.groups[r] : r) * c.a.table_ld;
+  return c.a.table + (c.b.own ? r : c.b.groups[r]) * c.a.table_ld;
 }
 
 // Inclusive sums over the lanes of a wave, without LDS (row shifts, then the
@@ -282,7 +290,7 @@ struct AttnWork {
       const int l = threadIdx.x & 63;
       if (blockIdx.x == 0 && border == 0 && threadIdx.x < 64 && first + l < R && mine.rows == 0) {
         if constexpr (BRANCH) {
-          if (!c.b.groups) a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
+          if (c.b.own) a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
         } else {
           a.status[first + l] = mine.fine ? DSR_OK : DSR_E_LENGTH;
         }
@@ -291,8 +299,11 @@ struct AttnWork {
     quota = attn_quota(p, total);
     const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
-      me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-      at = (blockIdx.x >> 3) < each ? me * quota : total;
+      // The groups' pass has its shares from the other end, so that where both have few they are not the same workgroups'.
+      uint32_t group = blockIdx.x;
+      if constexpr (BRANCH) group = c.b.own ? group : p.groups - 1 - group;
+      me = (group & 7) * each + (group >> 3);
+      at = (group >> 3) < each ? me * quota : total;
     } else {
       me = border;
       at = (uint32_t)border < 8 * each ? border * quota : total;
@@ -354,7 +365,7 @@ struct AttnWork {
     s.begin = origin + s0 * p.tokens;
     s.end = s1 == steps ? q.kv : origin + s1 * p.tokens;
     bool causal = !a.visible;
-    if constexpr (BRANCH) causal &= !c.b.groups;
+    if constexpr (BRANCH) causal &= c.b.own != 0;
     if (causal && q.kv > 0) {  // causal rows: nothing past the tile's last one
       const int last = attn_token(p, (s.tile + 1) * p.tile_rows - 1);
       if (s.end - (q.kv - q.n) > last + 1) s.end = q.kv - q.n + last + 1;
@@ -392,47 +403,51 @@ __device__ __forceinline__ void attn_clear(int groups, int threads) {
   }
 }
 
-// Each request's group and prefix, for the second pass; by the workgroups past
-// p.groups of the first, 64 threads or more.  Groups that do not ascend refuse
-// every request.
-__device__ __forceinline__ void attn_branch_lows(int threads) {
-  const AttnBranchCall& c = attn_call<true>();
-  if (!c.b.groups) return;
+// Each request's group and prefix.  Up to kAttnLows requests every workgroup
+// finds them for itself, in LDS (a launch for it would cost 2 us or more), the
+// first one also for the join; `groups` is LDS for kAttnLows + 1 numbers.  More
+// requests have a launch of their own, and `groups` null.  Groups that do not
+// ascend refuse every request.
+__device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, int threads, int* groups) {
   __shared__ int wrong;
-  const int G = (int)c.b.count, R = (int)c.b.requests;
+  const int G = c.b.group_count, R = (int)c.a.requests;
   if (threadIdx.x == 0) wrong = 0;
   __syncthreads();
   for (int g = threadIdx.x; g <= G; g += threads) {
     const int r = c.b.groups[g];
     if (r < 0 || r > R || (g > 0 && c.b.groups[g - 1] > r)) wrong = 1;
+    if (groups) groups[g] = r;
   }
   __syncthreads();
-  const int step = ((int)gridDim.x - c.p.groups) * threads;
-  for (int r = ((int)blockIdx.x - c.p.groups) * threads + threadIdx.x; r < R; r += step) {
+  const int first = groups ? 0 : (int)blockIdx.x * threads, step = groups ? threads : (int)gridDim.x * threads;
+  for (int r = first + (int)threadIdx.x; r < R; r += step) {
     int lo = 0, hi = G;  // the groups that begin at or before r
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      if (c.b.groups[mid] <= r)
+      if ((groups ? groups[mid] : c.b.groups[mid]) <= r)
         lo = mid + 1;
       else
         hi = mid;
     }
-    int low = wrong ? -1 : 0, mine = -1;
-    AttnRequest q{};
-    if (!wrong && lo > 0 && r < c.b.groups[lo]) {
+    int low = wrong ? -1 : 0, mine = -1, group_lo = 0;
+    if (!wrong && lo > 0 && r < (groups ? groups[lo] : c.b.groups[lo])) {
       const int prefix = c.b.prefix[lo - 1];
       low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
       if (low > 0) {
         mine = lo - 1;
-        q = attn_request(c, mine);
-        const AttnRequest own = attn_request(c.a, c.p, r);
+        const AttnRequest q = attn_group(c.a, c.p, c.b, mine), own = attn_request(c.a, c.p, r);
+        group_lo = q.lo;
         if (own.lo < q.lo || own.lo + own.n > q.lo + q.n) low = mine = -1;  // offsets that do not ascend
       }
     }
-    c.b.lows[r] = low;
-    c.b.group_of[r] = mine;
-    c.b.group_lo[r] = q.lo;
+    if (groups) attn_lows()[r] = low;
+    if (!groups || blockIdx.x == 0) {
+      c.b.low[r] = low;
+      c.b.group_of[r] = mine;
+      c.b.group_lo[r] = group_lo;
+    }
   }
+  __syncthreads();
 }
 
 // v with 0 in the place of infinities and NaN; whether there were any.
@@ -567,9 +582,12 @@ __device__ __forceinline__ uint32_t attn_sees(bool masks, uint64_t mask, int tok
 //
 // What bounds it: the cache's read.  64 requests of one token over 8,192
 // tokens, 8 heads of 128: 370 us, 5.8 TB/s.
-template <class T, int DP, int WAVES, bool BRANCH = false>
-__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(
-    typename AttnArgs<BRANCH>::type) {
+template <class T, int DP, int WAVES>
+constexpr int attn_few_lds() {
+  return WAVES * kAttnTile * (DP + 8 + DP + 16) * (int)sizeof(T);
+}
+template <class T, int DP, int WAVES, bool BRANCH>
+__device__ __forceinline__ void attn_few(char* lds, int pass) {
   typedef typename AttnArgs<BRANCH>::type Call;
   constexpr int kThreads = 64 * WAVES;
   typedef typename AttnType<T>::x4 x4;
@@ -577,38 +595,36 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
   constexpr int KS = DP / 32;   // k steps of the score product
   constexpr int DB = DP / 16;   // 16-wide output blocks
   constexpr int VS = DP + 16;   // LDS row of values: 32 bytes of padding spread the transposing reads over the banks
-  __shared__ __align__(16) T keys[WAVES][kAttnTile][DP + 8];  // 16 bytes of padding for the 16-byte reads of 16 keys
-  __shared__ __align__(16) T vals[WAVES][kAttnTile][VS];
+  typedef T KeyRows[kAttnTile][DP + 8];  // 16 bytes of padding for the 16-byte reads of 16 keys
+  typedef T ValRows[kAttnTile][VS];
+  KeyRows* keys = (KeyRows*)lds;
+  ValRows* vals = (ValRows*)(lds + WAVES * sizeof(KeyRows));
   __shared__ float sm[WAVES][16], sl[WAVES][16];
   __shared__ float sbase[16];
   __shared__ int sbad, spoison;  // a page id outside the cache; a value left out (attn_poison)
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-  if ((int)blockIdx.x >= attn_call<BRANCH>().p.groups) {
-    if constexpr (BRANCH) attn_branch_lows(kThreads);
-    return attn_clear<T, BRANCH>(attn_call<BRANCH>().p.groups, kThreads);
-  }
-  AttnWork<DP <= 128, Call> work(attn_call<BRANCH>(), 0);
+  AttnWork<DP <= 128, Call> work(attn_call<BRANCH>(pass), 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(attn_call<BRANCH>(), u, q)) {  // the same for the whole workgroup
-    const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
-    const AttnPlan& p = attn_call<BRANCH>().p;
+  while (work.next(attn_call<BRANCH>(pass), u, q)) {  // the same for the whole workgroup
+    const dsr_tree_attention_args_t& a = attn_call<BRANCH>(pass).a;
+    const AttnPlan& p = attn_call<BRANCH>(pass).p;
     const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
     __syncthreads();  // the last segment's LDS is read
     if (threadIdx.x == 0) sbad = spoison = 0;
-    const int ctx = attn_context(attn_call<BRANCH>(), q), begin = u.begin, end = u.end;
+    const int ctx = attn_context(attn_call<BRANCH>(pass), q), begin = u.begin, end = u.end;
     const int row0 = u.tile << row_shift;
 
     attn_f32x4 acc[DB];
     float m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x4{};
-    const dsr_tree_attention_args_t& c = attn_call<BRANCH>().a;
-    const int32_t* pages = attn_pages(attn_call<BRANCH>(), u.r);
+    const dsr_tree_attention_args_t& c = attn_call<BRANCH>(pass).a;
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
-    const int shift = attn_call<BRANCH>().p.page_shift, page = c.page;
+    const int shift = attn_call<BRANCH>(pass).p.page_shift, page = c.page;
     const unsigned blocks = c.blocks;
     const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
     const bool masks = c.visible != nullptr;
@@ -780,7 +796,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
     if (g == 0) sm[w][n] = m;
     if (any_bad && l == 0) sbad = 1;
     __syncthreads();
-    const Call& e = attn_call<BRANCH>();
+    const Call& e = attn_call<BRANCH>(pass);
     const bool split = !u.whole;
     const int64_t part = u.part;
     constexpr int OS = DP + 4;  // LDS row of outputs
@@ -832,6 +848,13 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_
                          sbase);
     attn_report(e, u, q, sbad);
   }
+}
+
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP <= 128 || WAVES > 4 ? 2 : 1) void k_tree_attention(AttnCall) {
+  __shared__ __align__(16) char lds[attn_few_lds<T, DP, WAVES>()];
+  if ((int)blockIdx.x >= attn_call().p.groups) return attn_clear<T>(attn_call().p.groups, 64 * WAVES);
+  attn_few<T, DP, WAVES, false>(lds, 0);
 }
 
 // Joins the parts of the tiles that borders between shares cut:

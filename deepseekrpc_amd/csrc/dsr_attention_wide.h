@@ -46,9 +46,12 @@ constexpr int attn_round(int DP) { return kAttnThreads / (DP / 8); }
 //
 // FLAT: a page holds every token of a round of loads, so that a round's page
 // id and address are the same for the workgroup and a lane adds one offset.
-template <class T, int DP, int WR, bool FLAT, bool BRANCH = false>
-__global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_tree_attention_wide(
-    typename AttnArgs<BRANCH>::type) {
+template <class T, int DP, int WR>
+constexpr int attn_wide_lds() {
+  return 2 * kAttnTile * (kAttnWaves / WR) * (DP + 8 + DP + 16) * (int)sizeof(T);
+}
+template <class T, int DP, int WR, bool FLAT, bool BRANCH>
+__device__ __forceinline__ void attn_wide_rows(char* attn_lds, int pass) {
   typedef typename AttnArgs<BRANCH>::type Call;
   typedef typename AttnType<T>::x4 x4;
   typedef typename AttnType<T>::x8 x8;
@@ -64,7 +67,6 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
   static_assert(NT * CH % kAttnThreads == 0, "every thread stages as much");
   static_assert(!FLAT || kAttnThreads % CH == 0, "a round is a whole number of tokens");
   constexpr int kKeys = 2 * NT * KS, kVals = 2 * NT * VS;  // elements, double-buffered
-  __shared__ __align__(16) char attn_lds[(kKeys + kVals) * sizeof(T)];
   T* keys = (T*)attn_lds;        // [2][NT][KS]
   T* vals = keys + kKeys;        // [2][NT][VS]
   __shared__ float sm[kAttnWaves][32], sl[kAttnWaves][32];
@@ -74,21 +76,17 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 31, h = l >> 5;
   const int wr = w / WK, wk = w % WK;
-  if ((int)blockIdx.x >= attn_call<BRANCH>().p.groups) {
-    if constexpr (BRANCH) attn_branch_lows(kAttnThreads);
-    return attn_clear<T, BRANCH>(attn_call<BRANCH>().p.groups, kAttnThreads);
-  }
-  AttnWork<false, Call> work(attn_call<BRANCH>(), 0);
+  AttnWork<false, Call> work(attn_call<BRANCH>(pass), 0);
   AttnSegment u;
   AttnRequest q;
-  while (work.next(attn_call<BRANCH>(), u, q)) {  // the same for the whole workgroup
-    const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
-    const AttnPlan& p = attn_call<BRANCH>().p;
+  while (work.next(attn_call<BRANCH>(pass), u, q)) {  // the same for the whole workgroup
+    const dsr_tree_attention_args_t& a = attn_call<BRANCH>(pass).a;
+    const AttnPlan& p = attn_call<BRANCH>(pass).p;
     const int group = p.group, dim = a.head_dim, row_shift = p.tile_shift;
     __syncthreads();  // the last segment's LDS is read
     if (threadIdx.x < 4 * WK) sbits[threadIdx.x / WK][threadIdx.x % WK] = 0;
     if (threadIdx.x == 0) sbad = spoison = 0;
-    const int ctx = attn_context(attn_call<BRANCH>(), q), begin = u.begin, end = u.end;
+    const int ctx = attn_context(attn_call<BRANCH>(pass), q), begin = u.begin, end = u.end;
     const int clear = min(ctx, end);  // every row sees the tokens before
     const int steps = end > begin ? (end - begin + NT - 1) / NT : 0;
 
@@ -115,11 +113,11 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
     float m = -INFINITY, sum = 0.f, top;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x16{};
-    const dsr_tree_attention_args_t& c = attn_call<BRANCH>().a;
-    const int32_t* pages = attn_pages(attn_call<BRANCH>(), u.r);
+    const dsr_tree_attention_args_t& c = attn_call<BRANCH>(pass).a;
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
-    const int shift = attn_call<BRANCH>().p.page_shift, page = c.page;
+    const int shift = attn_call<BRANCH>(pass).p.page_shift, page = c.page;
     const unsigned blocks = c.blocks;
     const uint32_t k_block = c.k_block, k_token = c.k_token, v_block = c.v_block, v_token = c.v_token;
     const bool masks = c.visible != nullptr;
@@ -363,7 +361,7 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
         }
       }
     }
-    const Call& e = attn_call<BRANCH>();
+    const Call& e = attn_call<BRANCH>(pass);
     if (wk == 0 && live) {
       if (h == 0) sbase[in_tile] = m;
       if (BRANCH || !u.whole) {
@@ -406,6 +404,13 @@ __global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_t
       attn_poison<T, DP>(e, u, q, sbad || (BRANCH && begin < q.low) ? begin : max(begin, clear - NT), sbase);
     attn_report(e, u, q, sbad);
   }
+}
+
+template <class T, int DP, int WR, bool FLAT>
+__global__ __launch_bounds__(kAttnThreads, DP * (4 / WR) < 512 ? 2 : 1) void k_tree_attention_wide(AttnCall) {
+  __shared__ __align__(16) char lds[attn_wide_lds<T, DP, WR>()];
+  if ((int)blockIdx.x >= attn_call().p.groups) return attn_clear<T>(attn_call().p.groups, kAttnThreads);
+  attn_wide_rows<T, DP, WR, FLAT, false>(lds, 0);
 }
 
 }  // namespace dsr

@@ -7,10 +7,11 @@
 // the best of their candidates.
 //
 // Which of two rows' candidates is better hangs on the difference of two log
-// sums, so these, and the scores, are float64: an exponential costs about 13
+// sums, so these, and the scores, are float64: an exponential costs a dozen
 // float64 instructions (beam_exp).
 #pragma once
 
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -20,8 +21,7 @@
 namespace dsr {
 
 constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
-constexpr int kBeamEach = 32;                            // logits of a thread
-constexpr int kBeamSlice = kBeamThreads * kBeamEach;     // and of a workgroup
+constexpr int kBeamList = 256;                            // candidates a wave sorts from LDS
 constexpr int kBeamGroupThreads = 512, kBeamGroupWaves = kBeamGroupThreads / 64;
 
 // One slice of a row.
@@ -44,11 +44,20 @@ struct BeamSpace {
   BeamTerm* terms;
   uint64_t* found; // order of the logit, ~token; 0: none
 };
-__host__ __device__ inline int beam_slices(int64_t vocab) { return (int)((vocab + kBeamSlice - 1) / kBeamSlice); }
+// Logits of a thread: many where that leaves workgroups enough for the chip,
+// because a wave's sorts cost as much as 30 logits of each thread.
+__host__ __device__ inline int beam_each(int64_t rows, int64_t vocab) {
+  auto groups = [&](int each) { return rows * ((vocab + kBeamThreads * each - 1) / (kBeamThreads * each)); };
+  return groups(64) >= 512 ? 64 : groups(32) >= 512 ? 32 : 8;
+}
+__host__ __device__ inline int beam_slices(const dsr_select_beams_args_t& a) {
+  const int slice = kBeamThreads * beam_each(a.rows, a.vocab);
+  return (int)((a.vocab + slice - 1) / slice);
+}
 __host__ __device__ inline BeamSpace beam_space(const dsr_select_beams_args_t& a) {
   BeamSpace s;
   s.parts = (BeamPart*)a.workspace;
-  s.terms = (BeamTerm*)(s.parts + a.rows * beam_slices(a.vocab));
+  s.terms = (BeamTerm*)(s.parts + a.rows * beam_slices(a));
   s.found = (uint64_t*)(s.terms + a.rows);
   return s;
 }
@@ -56,13 +65,13 @@ __host__ __device__ inline BeamSpace beam_space(const dsr_select_beams_args_t& a
 // The value of lane ^ J.
 template <int J>
 __device__ __forceinline__ uint32_t beam_xor(uint32_t x) {
-  if constexpr (J == 1) return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, false);   // quads 1 0 3 2
-  if constexpr (J == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, false);   // quads 2 3 0 1
+  if constexpr (J == 1) return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, true);   // quads 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, true);   // quads 2 3 0 1
   if constexpr (J == 4) {                                                                  // 7 - i, then quads 3 2 1 0
-    const uint32_t y = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false);
-    return __builtin_amdgcn_update_dpp(0, y, 0x1B, 0xf, 0xf, false);
+    const uint32_t y = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true);
+    return __builtin_amdgcn_update_dpp(0, y, 0x1B, 0xf, 0xf, true);
   }
-  if constexpr (J == 8) return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // rows of 16 turned by 8
+  if constexpr (J == 8) return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);  // rows of 16 turned by 8
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   if constexpr (J == 16) {
     const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, x, false, false));
@@ -130,6 +139,7 @@ __device__ __forceinline__ void beam_sort(K& x) {
   beam_merge(x);
 }
 // The lanes in the opposite order.
+__device__ __forceinline__ uint32_t beam_turn(uint32_t x) { return __shfl(x, 63 - (int)(threadIdx.x & 63)); }
 __device__ __forceinline__ uint64_t beam_turn(uint64_t x) { return __shfl(x, 63 - (int)(threadIdx.x & 63)); }
 __device__ __forceinline__ BeamOffer beam_turn(BeamOffer x) {
   const int l = 63 - (int)(threadIdx.x & 63);
@@ -158,24 +168,31 @@ __device__ __forceinline__ double beam_value(uint64_t u) {
   return __longlong_as_double(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u);
 }
 
-// exp(d) for d <= 0, to about 2^-52: 2^(n / 64) from a table times a polynomial
-// of what is left, |r| <= ln 2 / 128, whose next term would be below 2^-60
-// (Tang, Table-driven implementation of the exponential function, 1989).
-// Values below e^-800 count as 0.
+// exp(d) for -700 <= d <= 0, to about 2^-52: 2^(n / 256) from a table times a
+// polynomial of what is left, |r| <= ln 2 / 512, whose next term would be below
+// 2^-54 (Tang, Table-driven implementation of the exponential function, 1989).
+// n is rounded by adding 1.5 x 2^52, which leaves it in the low bits; the power
+// of two goes to the table value's exponent, which d >= -700 keeps in range.
+constexpr double kBeamFar = 700.0;  // what is farther below the largest counts as that far: e^-700
+constexpr int kBeamTable = 256;
 __device__ __forceinline__ void beam_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
+  for (int i = threadIdx.x; i < kBeamTable; i += blockDim.x) table[i] = exp2(i / (double)kBeamTable);
 }
 __device__ __forceinline__ double beam_exp(double d, const double* table) {
-  d = d > -800.0 ? d : -800.0;
-  const double n = __builtin_rint(d * 92.33248261893824);  // 64 / ln 2
-  const double r = __builtin_fma(n, -0.010830424696249145, d);
-  double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
-  p = __builtin_fma(p, r, 1.0 / 6);
+  constexpr double kRound = 6755399441055744.0;
+  const double t = __builtin_fma(d, 369.3299304675746, kRound);  // 256 / ln 2
+  const double r = __builtin_fma(t - kRound, -0.0027076061740622863, d);
+  double p = __builtin_fma(r, 1.0 / 24, 1.0 / 6);
   p = __builtin_fma(p, r, 0.5);
   p = __builtin_fma(p, r, 1.0);
   p = __builtin_fma(p, r, 1.0);
-  const int k = (int)n;
-  return __builtin_ldexp(p * table[k & 63], k >> 6);
+  const int k = (int)__double_as_longlong(t);
+  const int64_t scale = (int64_t)((uint64_t)(uint32_t)(k >> 8) << 52);
+  return p * __longlong_as_double(__double_as_longlong(table[k & (kBeamTable - 1)]) + scale);
+}
+// exp(x - top); x may be -inf or NaN, top not.
+__device__ __forceinline__ double beam_exp(float x, float top, const double* table) {
+  return beam_exp(__builtin_fmax((double)x - (double)top, -kBeamFar), table);
 }
 
 __device__ __forceinline__ double beam_sum(double x) {  // over the wave's lanes
@@ -184,33 +201,31 @@ __device__ __forceinline__ double beam_sum(double x) {  // over the wave's lanes
   return x;
 }
 
-// VEC: rows are 16-byte aligned and read 16 bytes at a time.
-template <class T, bool VEC>
+// EACH: logits of a thread.  VEC: rows are 16-byte aligned and read 16 bytes at a time.
+template <class T, int EACH, bool VEC>
 __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_args_t a) {
   typedef T xv __attribute__((ext_vector_type(16 / sizeof(T))));
-  constexpr int VE = VEC ? 16 / sizeof(T) : 1, C = kBeamEach / VE;
-  __shared__ double table[64];
-  __shared__ uint64_t list[kBeamWaves][128];
+  constexpr int VE = VEC ? 16 / sizeof(T) : 1, C = EACH / VE;
+  __shared__ double table[kBeamTable];
+  __shared__ uint64_t list[kBeamWaves][kBeamList];
   __shared__ BeamPart part[kBeamWaves];
-  const int slices = beam_slices(a.vocab), l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int V = (int)a.vocab, slices = (V + kBeamThreads * EACH - 1) / (kBeamThreads * EACH);
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t row = blockIdx.x / (unsigned)slices;
-  const int slice = blockIdx.x - (unsigned)row * slices;
+  const int slice = blockIdx.x - (unsigned)row * slices, first = slice * kBeamThreads * EACH;
   if (slice == 0 && threadIdx.x == 0) a.status[row] = DSR_OK;
   if (a.finished && a.finished[row]) return;
-  beam_table(table);
   const T* logits = (const T*)a.logits + row * a.ld;
-  const int first = slice * kBeamSlice, V = (int)a.vocab;
 
   // Element e of the thread is token first + (e / VE * threads + thread) VE + e % VE.
-  float x[kBeamEach];
+  float x[EACH];
   auto token = [&](int e) { return first + (e / VE * kBeamThreads + (int)threadIdx.x) * VE + e % VE; };
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int at = token(c * VE);
     if constexpr (VEC) {
-      xv v;
       if (at + VE <= V) {
-        v = *(const xv*)(logits + at);
+        const xv v = *(const xv*)(logits + at);
 #pragma unroll
         for (int i = 0; i < VE; ++i) x[c * VE + i] = (float)v[i];
       } else {
@@ -221,59 +236,59 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
       x[c] = at < V ? (float)logits[at] : -INFINITY;
     }
   }
+  beam_table(table);
   bool bad = false;
   float most = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < kBeamEach; ++e) {
-    bad |= !(x[e] < INFINITY);
-    most = fmaxf(most, x[e]);
+  for (int e = 0; e < EACH; e += 2) {
+    bad |= __builtin_isunordered(x[e], x[e + 1]);
+    most = fmaxf(most, fmaxf(x[e], x[e + 1]));
   }
+  bad |= most == INFINITY;
   // The keep-th largest of the lanes' largest: at least `keep` of the wave's
   // logits are not below it, and few more.
-  uint64_t top = (uint64_t)beam_order(most) << 32;
-  beam_sort(top);
-  const float base = beam_value((uint32_t)(__shfl(top, 0) >> 32));
-  const uint64_t none = (uint64_t)beam_order(-INFINITY) << 32 | 0xFFFFFFFFull;
-  uint64_t floor = __shfl(top, a.keep - 1);  // candidates have to be above it
-  floor = floor ? floor - 1 : 0;
-  if (floor < none) floor = none;
-
-  // They go through the wave's list, 64 at a time, into the sorted `top`.
-  top = 0;
+  uint32_t tops = beam_order(most);
+  beam_sort(tops);
+  const float base = beam_value(__shfl(tops, 0)), least = fmaxf(beam_value(__shfl(tops, a.keep - 1)), -FLT_MAX);
+  auto key_of = [&](float v, int e) { return (uint64_t)beam_order(v) << 32 | (uint32_t)~token(e); };
   int n = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const bool in = x[e] >= least;
+    const uint64_t which = __ballot(in);
+    if (which) {
+      const int at = n + __popcll(which & ((1ull << l) - 1));
+      if (in && at < kBeamList) list[w][at] = key_of(x[e], e);
+      n += __popcll(which);
+    }
+  }
+  uint64_t top = 0, floor = 0;
   auto take = [&](uint64_t key) __attribute__((always_inline)) {
     beam_sort(key);
     beam_join(top, beam_turn(key));
-    const uint64_t last = __shfl(top, a.keep - 1);
-    if (last > floor) floor = last;
+    floor = __shfl(top, a.keep - 1);
   };
-#pragma unroll
-  for (int e = 0; e < kBeamEach; ++e) {
-    const uint64_t key = (uint64_t)beam_order(x[e]) << 32 | (uint32_t)~token(e);
-    const bool in = key > floor;
-    const uint64_t which = __ballot(in);
-    if (which) {
-      if (in) list[w][n + __popcll(which & ((1ull << l) - 1))] = key;
-      n += __popcll(which);
-      if (n >= 64) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const uint64_t now = list[w][l], rest = list[w][64 + l];
-        __builtin_amdgcn_wave_barrier();
-        list[w][l] = rest;
-        n -= 64;
-        take(now);
-      }
-    }
-  }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  if (n > 0) take(l < n ? list[w][l] : 0);
+  if (n <= kBeamList) {
+#pragma unroll 1
+    for (int i = 0; i < n; i += 64) take(i + l < n ? list[w][i + l] : 0);
+  } else {
+    // Hundreds of equal logits, or a few lanes with all the large ones: the
+    // wave's logits once more, 64 at a time.
+#pragma unroll 1
+    for (int e = 0; e < EACH; ++e) {
+      const int at = token(e);
+      const float v = at < V ? (float)logits[at] : -INFINITY;
+      const uint64_t key = v >= least ? key_of(v, e) : 0;
+      if (__ballot(key > floor)) take(key);
+    }
+  }
   __syncthreads();  // the table
   double sum = 0.0;
   if (base > -INFINITY)
 #pragma unroll
-    for (int e = 0; e < kBeamEach; ++e) sum += beam_exp((double)x[e] - (double)base, table);
+    for (int e = 0; e < EACH; ++e) sum += beam_exp(x[e], base, table);
   sum = beam_sum(sum);
   const int wrong = __ballot(bad) != 0;
   list[w][l] = top;
@@ -296,16 +311,16 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
     if (p.top > -INFINITY)
 #pragma unroll
       for (int i = 0; i < kBeamWaves; ++i)
-        p.sum += part[i].sum * beam_exp((double)part[i].top - (double)p.top, table);
+        p.sum += part[i].sum * beam_exp(part[i].top, p.top, table);
     space.parts[at] = p;
   }
 }
 
 __global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_beams_args_t a) {
-  __shared__ double table[64];
+  __shared__ double table[kBeamTable];
   __shared__ uint64_t keys[kBeamGroupWaves][64];
   __shared__ uint32_t places[kBeamGroupWaves][64];
-  const int g = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6, slices = beam_slices(a.vocab), keep = a.keep;
+  const int g = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6, slices = beam_slices(a), keep = a.keep;
   const int rows = (int)a.rows;
   int lo = a.offsets[g], hi = a.offsets[g + 1];
   lo = lo < 0 ? 0 : lo > rows ? rows : lo;
@@ -313,50 +328,65 @@ __global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_be
   const BeamSpace space = beam_space(a);
   beam_table(table);
   __syncthreads();
-  for (int r = lo + (int)threadIdx.x; r < hi; r += kBeamGroupThreads) {
+  // Candidates do not wait for the rows' sums: the first ones are on their way.
+  const int each = slices * keep, count = (hi - lo) * each;
+  const uint64_t* found = space.found + (int64_t)lo * each;
+  uint64_t next = (int)threadIdx.x < count ? found[threadIdx.x] : 0;
+  // A row's sum, a wave each, a slice a lane.
+  for (int r = lo + w; r < hi; r += kBeamGroupWaves) {
     const double score = a.scores[r];
+    const bool ended = a.finished && a.finished[r];
     int status = !(score < INFINITY) ? DSR_E_LOGITS : DSR_OK;
     BeamTerm term{0.0, 0.0, score};
-    if (!(a.finished && a.finished[r])) {
+    if (!ended) {
       const BeamPart* p = space.parts + (int64_t)r * slices;
-      float top = -INFINITY;
-      int bad = 0;
-      for (int s = 0; s < slices; ++s) {
-        top = fmaxf(top, p[s].top);
-        bad |= p[s].bad;
+      BeamPart mine{0.0, -INFINITY, 0};
+      for (int s = l; s < slices; s += 64) {
+        const BeamPart x = p[s];
+        const float top = fmaxf(mine.top, x.top);
+        if (top > -INFINITY && !(x.bad | mine.bad))
+          mine.sum = mine.sum * beam_exp(mine.top, top, table) + x.sum * beam_exp(x.top, top, table);
+        mine.top = top;
+        mine.bad |= x.bad;
       }
-      double sum = 0.0;
-      for (int s = 0; s < slices; ++s)
-        if (p[s].top > -INFINITY) sum += p[s].sum * beam_exp((double)p[s].top - (double)top, table);
+      float top = mine.top;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+      const bool bad = __ballot(mine.bad) != 0;
       if (bad)
         status = DSR_E_LOGITS;
       else if (top == -INFINITY && status == DSR_OK)
         status = DSR_E_MASKED;
-      term.top = top;
-      term.rest = log(sum);
+      if (status == DSR_OK) {
+        term.top = top;
+        term.rest = log(beam_sum(mine.sum * beam_exp(mine.top, top, table)));
+      }
     }
-    if (status != DSR_OK) a.status[r] = status;
     if (status != DSR_OK) term.score = NAN;
-    space.terms[r] = term;
+    if (l == 0) {
+      if (status != DSR_OK) a.status[r] = status;
+      space.terms[r] = term;
+    }
   }
   __threadfence_block();
   __syncthreads();
 
   // Candidates, 64 of a wave at a time, into its sorted `best`.
-  const int each = slices * keep, count = (hi - lo) * each;
   BeamOffer best{0, 0}, last{0, 0};
+#pragma unroll 1
   for (int i0 = 64 * w; i0 < count; i0 += kBeamGroupThreads) {
     const int i = i0 + l;
+    const uint64_t now = next;
+    next = i + kBeamGroupThreads < count ? found[i + kBeamGroupThreads] : 0;
     BeamOffer mine{0, 0};
     if (i < count) {
-      const int r = i / each, in = i - r * each;
+      const int r = (unsigned)i / (unsigned)each, in = i - r * each;
       const BeamTerm term = space.terms[lo + r];
       double score = NAN;
       if (a.finished && a.finished[lo + r]) {
         if (in == 0) score = term.score;
-      } else {
-        const uint64_t found = space.found[(int64_t)(lo + r) * each + in];
-        if (found) score = ((double)beam_value((uint32_t)(found >> 32)) - term.top) - term.rest + term.score;
+      } else if (now) {
+        score = ((double)beam_value((uint32_t)(now >> 32)) - term.top) - term.rest + term.score;
       }
       if (score > -INFINITY) mine = BeamOffer{beam_order(score), ~(uint32_t)i};
     }
@@ -381,7 +411,7 @@ __global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_be
     const uint32_t i = ~best.place, r = i / each;
     parent = lo + (int)r;
     if (!(a.finished && a.finished[parent]))
-      token = (int)~(uint32_t)space.found[(int64_t)parent * each + (i - r * each)];
+      token = (int)~(uint32_t)found[i];
   }
   a.parents[at] = parent;
   a.tokens[at] = token;

@@ -22,13 +22,22 @@ bool beams_shape_ok(const dsr_select_beams_args_t& a) {
          a.groups <= DSR_BEAMS_MAX_ROWS && a.vocab >= 1 && a.vocab <= DSR_BEAMS_MAX_VOCAB;
 }
 
-template <class T>
+template <class T, int EACH>
 void beams_launch(const dsr_select_beams_args_t& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * beam_slices(a.vocab))), threads(kBeamThreads);
+  const dim3 grid((unsigned)(a.rows * beam_slices(a))), threads(kBeamThreads);
   if ((uintptr_t)a.logits % 16 == 0 && (a.rows == 1 || a.ld * sizeof(T) % 16 == 0))
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_beam_slices<T, true>), grid, threads, 0, s, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_beam_slices<T, EACH, true>), grid, threads, 0, s, a);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_beam_slices<T, false>), grid, threads, 0, s, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_beam_slices<T, EACH, false>), grid, threads, 0, s, a);
+}
+
+template <class T>
+void beams_typed(const dsr_select_beams_args_t& a, hipStream_t s) {
+  switch (beam_each(a.rows, a.vocab)) {
+    case 8: return beams_launch<T, 8>(a, s);
+    case 32: return beams_launch<T, 32>(a, s);
+    default: return beams_launch<T, 64>(a, s);
+  }
 }
 
 // What fork and compact ask of caches; without caches the rest is free.
@@ -88,7 +97,7 @@ extern "C" {
 
 size_t dsr_select_beams_workspace_bytes(const dsr_select_beams_args_t* args) {
   if (!args || !beams_shape_ok(*args)) return 0;
-  const int64_t slices = beam_slices(args->vocab);
+  const int64_t slices = beam_slices(*args);
   return (size_t)(args->rows * (slices * (int64_t)sizeof(BeamPart) + (int64_t)sizeof(BeamTerm) + slices * args->keep * 8));
 }
 
@@ -104,9 +113,9 @@ int32_t dsr_select_beams(const dsr_select_beams_args_t* args, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   if (a.rows > 0) {
     switch (a.dtype) {
-      case DSR_BF16: beams_launch<__bf16>(a, s); break;
-      case DSR_F16: beams_launch<_Float16>(a, s); break;
-      default: beams_launch<float>(a, s);
+      case DSR_BF16: beams_typed<__bf16>(a, s); break;
+      case DSR_F16: beams_typed<_Float16>(a, s); break;
+      default: beams_typed<float>(a, s);
     }
     if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   }

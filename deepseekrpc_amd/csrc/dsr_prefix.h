@@ -18,6 +18,68 @@
 
 namespace dsr {
 
+// The kernels' argument: the groups' pass and the requests'.
+struct PrefixCall {
+  AttnBranchCall c[2];
+};
+
+// Both passes in one launch.  Tiles of the groups' pass have A rows, of the
+// requests' B.  Prefixes are bound by the matrix cores, the tokens of single
+// requests by memory, so one half of the workgroups (64 in turn) begins with the
+// prefixes and the other with the requests.  64 requests over one prefix of
+// 32,768 tokens, up to 1,024 of their own: 163 us so, 169 with the prefixes first
+// everywhere, 171 with the requests, 171 where 256 in turn do, 190 in two
+// launches; 8 prefixes of 8 requests 95, 119 in two launches.
+template <int ROWS, class T, int DP, bool FLAT>
+__device__ __forceinline__ void prefix_pass(char* lds, int pass) {
+  if constexpr (ROWS == 16)
+    attn_few<T, DP, kAttnWaves, true>(lds, pass);
+  else
+    attn_wide_rows<T, DP, ROWS / 32, FLAT, true>(lds, pass);
+}
+template <int ROWS, class T, int DP>
+constexpr int prefix_lds() {
+  if constexpr (ROWS == 16)
+    return attn_few_lds<T, DP, kAttnWaves>();
+  else
+    return attn_wide_lds<T, DP, ROWS / 32>();
+}
+template <int ROWS, int DP>
+constexpr bool prefix_two() {  // a CU has room for two workgroups
+  return ROWS == 16 ? DP <= 128 : DP * (128 / ROWS) < 512;
+}
+template <class T, int DP, int A, int B, bool FLAT>
+__global__ __launch_bounds__(kAttnThreads, (prefix_two<A, DP>() && prefix_two<B, DP>() ? 2 : 1)) void
+k_prefix_attention(PrefixCall) {
+  constexpr int kLds = prefix_lds<A, T, DP>() > prefix_lds<B, T, DP>() ? prefix_lds<A, T, DP>() : prefix_lds<B, T, DP>();
+  static_assert(kLds >= (kAttnLows + 1) * 4, "the groups fit");
+  __shared__ __align__(16) char lds[kLds];
+  const int shares = attn_call<true>(0).p.groups;
+  if ((int)blockIdx.x >= shares) return attn_clear<T, true>(shares, kAttnThreads);
+  if (attn_call<true>(0).a.requests <= kAttnLows) attn_branch_lows(attn_call<true>(0), kAttnThreads, (int*)lds);
+  const int first = blockIdx.x >> 6 & 1;
+  if constexpr (A == B) {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      __syncthreads();
+      prefix_pass<A, T, DP, FLAT>(lds, first ^ i);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      __syncthreads();
+      if ((first ^ i) == 0)
+        prefix_pass<A, T, DP, FLAT>(lds, 0);
+      else
+        prefix_pass<B, T, DP, FLAT>(lds, 1);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kAttnThreads) void k_prefix_lows(PrefixCall) {
+  attn_branch_lows(attn_call<true>(0), kAttnThreads, nullptr);
+}
+
 struct PrefixJoin {
   dsr_tree_attention_args_t a;
   AttnPlan p[2];    // of the groups' pass and of the requests'
@@ -63,7 +125,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
     const int r = prefix_owner(a, t);
     if (r >= a.requests) continue;
     const int g = j.b[1].group_of[r], g_lo = j.b[1].group_lo[r];
-    const AttnRequest own = attn_request(a, j.p[1], j.b[1], r);
+    const AttnRequest own = attn_own(a, j.p[1], r, j.b[1].low[r]);
     const int lo = own.lo;
     if (t < lo || t >= lo + own.n) continue;  // a row of no request
     const int h_end = min(heads, (chunk + 1) * JR * each);
@@ -144,7 +206,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
           if (pass == 0 && g < 0) continue;
-          const AttnRequest q = pass == 0 ? attn_request(a, j.p[0], j.b[0], g) : own;
+          const AttnRequest q = pass == 0 ? attn_group(a, j.p[0], j.b[0], g) : own;
           const int2 s = prefix_tile(j, pass, q.lo, 0, (q.tiles - 1) * j.p[pass].tile_rows);
           if (s.y == 1) bad |= j.b[pass].bad[pass == 0 ? g : r];
           for (int c = 0; s.y > 1 && c < s.y; ++c) bad |= j.p[pass].part_bad[2 * (s.x + c) + (c == 0)];

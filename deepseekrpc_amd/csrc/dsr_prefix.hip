@@ -10,26 +10,38 @@ int32_t launched() { return hipGetLastError() == hipSuccess ? 0 : DSR_ERR_LAUNCH
 // Dimensions of the kernel that takes a head dimension.
 int prefix_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
-// The work split of one pass over `count` groups or requests, from sizes alone.
-AttnPlan prefix_plan(const dsr_tree_attention_args_t& a, int64_t count) {
-  AttnPlan p{};
-  const int64_t group = a.q_heads / a.kv_heads;
-  const int64_t rows = count > 0 ? (a.tokens * group + count - 1) / count : 0;  // of a usual one
+// Rows of a tile for a usual group's, or request's, rows.
+int prefix_rows(const dsr_tree_attention_args_t& a, int64_t count) {
+  const int64_t rows = count > 0 ? (a.tokens * (a.q_heads / a.kv_heads) + count - 1) / count : 0;
+  return rows <= 16 ? 16 : a.head_dim > 128 ? (rows <= 64 ? 64 : 128) : rows <= 32 ? 32 : 128;
+}
+
+// The work splits of both passes, from sizes alone.
+void prefix_plan(const dsr_tree_attention_args_t& a, const int64_t* counts, AttnPlan* plans) {
+  const int64_t group = a.q_heads / a.kv_heads, span = (int64_t)a.width * a.page;
   const bool big = a.head_dim > 128;
-  p.tile_rows = rows <= 16 ? 16 : big ? (rows <= 64 ? 64 : 128) : rows <= 32 ? 32 : 128;
-  p.tokens = p.tile_rows <= 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
-  p.min_steps = 128 / p.tokens;
-  p.cut = true;
-  p.groups = big || (p.tile_rows < 128 && p.tile_rows > 16) ? 256 : 512;
-  const int64_t tiles = (a.tokens * group / p.tile_rows + count) * a.kv_heads, span = (int64_t)a.width * a.page;
-  while ((span / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
-  auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
-  p.group = (int)group;
-  p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
-  p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
-  const int64_t shares = tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;
-  if (shares < p.groups) p.groups = (int)((shares + 7) / 8 * 8);
-  return p;
+  int rows[2] = {prefix_rows(a, counts[0]), prefix_rows(a, counts[1])};
+  if (rows[1] > 16) rows[1] = rows[0];  // the kernels that there are
+  int64_t most = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    AttnPlan& p = plans[pass] = AttnPlan{};
+    p.tile_rows = rows[pass];
+    p.tokens = p.tile_rows <= 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
+    p.min_steps = 128 / p.tokens;
+    p.cut = true;
+    const int64_t tiles = (a.tokens * group / p.tile_rows + counts[pass]) * a.kv_heads;
+    while ((span / p.tokens + 1) * tiles >= INT_MAX) p.tokens *= 2;  // steps are counted in 32 bits
+    auto log2_of = [](int64_t x) { return x & (x - 1) ? -1 : __builtin_ctzll(x); };
+    p.group = (int)group;
+    p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
+    p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
+    most += tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;  // shares of the fewest steps
+  }
+  // Workgroups that the chip holds at once: 256 CUs, two each where there is room.
+  const bool mid = rows[0] > 16 && rows[0] < 128;
+  int groups = big || mid ? 256 : 512;
+  if (most < groups) groups = (int)((most + 7) / 8 * 8);
+  plans[0].groups = plans[1].groups = groups;
 }
 
 // Addresses in the workspace; their end.
@@ -43,69 +55,70 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
     at += (bytes + 255) / 256 * 256;
     return p;
   };
-  int32_t* lows = (int32_t*)take(a.requests * 4);
+  int32_t* low = (int32_t*)take(a.requests * 4);
   int32_t* group_of = (int32_t*)take(a.requests * 4);
   int32_t* group_lo = (int32_t*)take(a.requests * 4);
+  prefix_plan(a, counts, j.p);
   for (int pass = 0; pass < 2; ++pass) {
-    AttnPlan& p = j.p[pass] = prefix_plan(a, counts[pass]);
+    AttnPlan& p = j.p[pass];
     AttnBranch& b = j.b[pass];
     const int64_t parts = 2 * (int64_t)p.groups * p.tile_rows;
     p.part_o = (float*)take(parts * dim * 4);
     p.part_ml = (float2*)take(parts * 8);
     p.part_bad = (int32_t*)take(2 * (int64_t)p.groups * 4);
-    b.groups = pass == 0 ? x.groups : nullptr;
-    b.prefix = pass == 0 ? x.prefix_lengths : nullptr;
-    b.low = b.lows = lows;
-    b.group_of = group_of;
-    b.group_lo = group_lo;
+    b.groups = x.groups;
+    b.prefix = x.prefix_lengths;
+    b.group_count = (int32_t)x.group_count;
+    b.own = pass;
+    b.count = counts[pass];
     b.tiles = (int2*)take(a.tokens * a.q_heads * 8);
     b.bad = (int32_t*)take(counts[pass] * 4);
     b.row_o = (float*)take(a.tokens * a.q_heads * dim * 4);
     b.row_ml = (float2*)take(a.tokens * a.q_heads * 8);
-    b.count = counts[pass];
-    b.requests = a.requests;
+    b.low = low;
+    b.group_of = group_of;
+    b.group_lo = group_lo;
   }
   return at;
-}
-
-template <class T, int DP>
-int32_t prefix_pass(const AttnBranchCall& c, hipStream_t s) {
-  const dsr_tree_attention_args_t& a = c.a;
-  // Workgroups for rows of no request, and for the requests' groups.
-  int64_t others = 0;
-  if (c.b.groups) {
-    others = (a.tokens * a.q_heads * a.head_dim * 2 + (1 << 18) - 1) >> 18;
-    const int64_t lows = (a.requests + kAttnThreads - 1) / kAttnThreads;
-    others = others < lows ? lows : others;
-    others = others > 256 ? 256 : others < 8 ? 8 : others;
-  }
-  const dim3 grid((unsigned)(c.p.groups + others)), threads(kAttnThreads);
-  auto wide = [&](auto WR) {
-    constexpr int wr = decltype(WR)::value;
-    constexpr bool whole = kAttnThreads % (DP / 8) == 0;
-    if (whole && a.page >= attn_round(DP) && a.k_token <= 1 << 24 && a.v_token <= 1 << 24)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, wr, whole, true>), grid, threads, 0, s, c);
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention_wide<T, DP, wr, false, true>), grid, threads, 0, s, c);
-  };
-  switch (c.p.tile_rows) {
-    case 16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_tree_attention<T, DP, 4, true>), grid, threads, 0, s, c); break;
-    case 128: wide(std::integral_constant<int, 4>{}); break;
-    default: wide(std::integral_constant<int, DP <= 128 ? 1 : 2>{});
-  }
-  return launched();
 }
 
 constexpr int64_t kPrefixFewRows = 16384, kPrefixItems = 4096;
 
 template <class T, int DP>
 int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j, hipStream_t s) {
-  for (int pass = 0; pass < 2; ++pass) {
-    AttnBranchCall c{x.a, j.p[pass], j.b[pass]};
-    if (pass == 0) c.a.visible = nullptr;  // every row sees the whole prefix
-    const int32_t rc = prefix_pass<T, DP>(c, s);
-    if (rc != 0) return rc;
+  const dsr_tree_attention_args_t& a = x.a;
+  PrefixCall c{{{a, j.p[0], j.b[0]}, {a, j.p[1], j.b[1]}}};
+  c.c[0].a.visible = nullptr;  // every row sees the whole prefix
+  const dim3 threads(kAttnThreads);
+  if (a.requests > kAttnLows) {
+    const int64_t lows = (a.requests + kAttnThreads - 1) / kAttnThreads;
+    hipLaunchKernelGGL(k_prefix_lows, dim3((unsigned)lows), threads, 0, s, c);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   }
+  // Workgroups for rows of no request: one for each 256 KB that all rows have.
+  const int64_t clear = (a.tokens * a.q_heads * a.head_dim * 2 + (1 << 18) - 1) >> 18;
+  const dim3 grid((unsigned)(j.p[0].groups + (clear > 256 ? 256 : clear < 8 ? 8 : clear)));
+  constexpr int kMid = DP <= 128 ? 32 : 64;
+  constexpr bool whole = kAttnThreads % (DP / 8) == 0;
+  const bool flat = whole && a.page >= attn_round(DP) && a.k_token <= 1 << 24 && a.v_token <= 1 << 24;
+  auto launch = [&](auto A, auto B) {
+    constexpr int rows = decltype(A)::value, own = decltype(B)::value;
+    if (flat && rows > 16)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, whole && (rows > 16)>), grid, threads, 0, s,
+                         c);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, false>), grid, threads, 0, s, c);
+  };
+  constexpr std::integral_constant<int, 16> few{};
+  constexpr std::integral_constant<int, kMid> mid{};
+  constexpr std::integral_constant<int, 128> many{};
+  // A group's rows are no fewer than a request's.
+  switch (j.p[0].tile_rows) {
+    case 16: launch(few, few); break;
+    case 128: j.p[1].tile_rows == 16 ? launch(many, few) : launch(many, many); break;
+    default: j.p[1].tile_rows == 16 ? launch(mid, few) : launch(mid, mid);
+  }
+  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   const int64_t rows = x.a.tokens * x.a.q_heads;
   if (rows == 0) return 0;
   const int jr = rows <= kPrefixFewRows ? 2 : 8;
@@ -113,11 +126,11 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   const int64_t blocks = (x.a.q_heads + jr - 1) / jr, most = x.a.tokens * blocks / kPrefixItems;
   const int each = (int)(most < 1 ? 1 : most < blocks ? most : blocks);
   const int64_t items = x.a.tokens * ((blocks + each - 1) / each);
-  const dim3 grid((unsigned)(items < (1 << 20) ? items : 1 << 20)), threads(kAttnThreads);
+  const dim3 join((unsigned)(items < (1 << 20) ? items : 1 << 20));
   if (jr == 2)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), grid, threads, 0, s, j, each);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), join, threads, 0, s, j, each);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), grid, threads, 0, s, j, each);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), join, threads, 0, s, j, each);
   return launched();
 }
 

@@ -126,6 +126,9 @@ def test_far_scores_and_logits():
     x[1] = 3e38
     x[2] = -3e38
     check(x, [-10.0] * 4, [0, 4], 16)
+    x[1, 5:] = 1e38  # a step of float32 here is far more than the exponential's range
+    x[3] += 1e12
+    check(x, [-10.0, -1e38, -10, -10], [0, 1, 2, 3, 4], 16)
 
 
 def test_a_prepared_call_in_a_graph_and_on_another_stream():
