@@ -167,7 +167,7 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
 __device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t& a, const AttnPlan& p, int r, int low) {
   AttnRequest q = attn_request(a, p, r);
   q.low = low;
-  if (low < 0 || a.kv_lengths[r] - q.n < low) q.fine = false;
+  if (low < 0) q.fine = false;
   if (!q.fine) q.kv = 0;
   if (q.kv == 0) q.low = 0;
   return q;
@@ -408,7 +408,8 @@ __device__ __forceinline__ void attn_clear(int groups, int threads) {
 // first one also for the join; `groups` is LDS for kAttnLows + 1 numbers.  More
 // requests have a launch of their own, and `groups` null.  Groups that do not
 // ascend refuse every request.
-__device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, int threads, int* groups) {
+__device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const AttnBranchCall& requests, int threads,
+                                                 int* groups) {
   __shared__ int wrong;
   const int G = c.b.group_count, R = (int)c.a.requests;
   if (threadIdx.x == 0) wrong = 0;
@@ -435,9 +436,10 @@ __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, int th
       low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
       if (low > 0) {
         mine = lo - 1;
-        const AttnRequest q = attn_group(c.a, c.p, c.b, mine), own = attn_request(c.a, c.p, r);
+        const AttnRequest q = attn_group(c.a, c.p, c.b, mine), own = attn_request(requests.a, requests.p, r);
         group_lo = q.lo;
-        if (own.lo < q.lo || own.lo + own.n > q.lo + q.n) low = mine = -1;  // offsets that do not ascend
+        // A context shorter than the prefix, a length out of bounds, offsets that do not ascend.
+        if (!own.fine || c.a.kv_lengths[r] - own.n < low || own.lo < q.lo || own.lo + own.n > q.lo + q.n) low = mine = -1;
       }
     }
     if (groups) attn_lows()[r] = low;

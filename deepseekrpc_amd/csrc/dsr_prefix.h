@@ -56,7 +56,8 @@ k_prefix_attention(PrefixCall) {
   __shared__ __align__(16) char lds[kLds];
   const int shares = attn_call<true>(0).p.groups;
   if ((int)blockIdx.x >= shares) return attn_clear<T, true>(shares, kAttnThreads);
-  if (attn_call<true>(0).a.requests <= kAttnLows) attn_branch_lows(attn_call<true>(0), kAttnThreads, (int*)lds);
+  if (attn_call<true>(0).a.requests <= kAttnLows)
+    attn_branch_lows(attn_call<true>(0), attn_call<true>(1), kAttnThreads, (int*)lds);
   const int first = blockIdx.x >> 6 & 1;
   if constexpr (A == B) {
 #pragma unroll 1
@@ -77,7 +78,7 @@ k_prefix_attention(PrefixCall) {
 }
 
 __global__ __launch_bounds__(kAttnThreads) void k_prefix_lows(PrefixCall) {
-  attn_branch_lows(attn_call<true>(0), kAttnThreads, nullptr);
+  attn_branch_lows(attn_call<true>(0), attn_call<true>(1), kAttnThreads, nullptr);
 }
 
 struct PrefixJoin {
@@ -106,28 +107,30 @@ __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int l
 
 // An item is a token and `each` blocks of JR of its rows (heads), a block at a
 // time.  The threads left over take every SLOTS-th part each, summed in a fixed
-// order; a thread has FLIGHT parts in flight.
+// order; a thread has FLIGHT parts in flight.  A refused request's rows are one
+// part without weight.
+// What bounds it: a chain of reads (the token's request, its tiles' shares, the
+// parts), then the parts' way through the caches.
 template <class T, int DP, int JR>
-__global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int each) {
+__global__ __launch_bounds__(kAttnThreads, 7) void k_prefix_join(PrefixJoin j, int each) {
   typedef typename AttnType<T>::x4 x4;
   constexpr int E = JR * DP / 4;  // four dimensions of a row each
   constexpr int SLOTS = E < kAttnThreads ? kAttnThreads / E : 1;
-  constexpr int FLIGHT = 4;
+  constexpr int FLIGHT = 3;
   __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const dsr_tree_attention_args_t& a = j.a;
-  const int heads = a.q_heads, group = j.p[0].group, chunks = (heads + JR * each - 1) / (JR * each);
+  const int heads = a.q_heads, group = j.p[0].group;
   const int slot = SLOTS > 1 ? threadIdx.x / E : 0;
   const bool spare = slot >= SLOTS;  // 192 dimensions
-  const int64_t items = a.tokens * chunks;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int t = chunks == 1 ? (int)item : (int)(item / chunks), chunk = (int)(item - (int64_t)t * chunks);
+  const int chunk = blockIdx.y;
+  for (int64_t item = blockIdx.x; item < a.tokens; item += gridDim.x) {
+    const int t = (int)item;
     const int r = prefix_owner(a, t);
     if (r >= a.requests) continue;
     const int g = j.b[1].group_of[r], g_lo = j.b[1].group_lo[r];
-    const AttnRequest own = attn_own(a, j.p[1], r, j.b[1].low[r]);
-    const int lo = own.lo;
-    if (t < lo || t >= lo + own.n) continue;  // a row of no request
+    const int lo = max(a.offsets[r], 0);
+    if (t < lo) continue;  // a row of no request
     const int h_end = min(heads, (chunk + 1) * JR * each);
     for (int h0 = chunk * JR * each; h0 < h_end; h0 += JR) {
 #pragma unroll
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
           L = L * f + l * g;
           o = o * f + x * g;
         };
-        if (live && own.fine) {
+        if (live) {
           const int kv_head = attn_token(j.p[0], h), of_group = h - kv_head * group;
           const int row0 = (t - g_lo) * group + of_group, row1 = (t - lo) * group + of_group;
           const int2 s0 = g >= 0 ? prefix_tile(j, 0, g_lo, kv_head, row0) : int2{0, 0};
@@ -201,6 +204,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
     }
     if (t == lo && chunk == 0 && threadIdx.x == 0) {
       // A request's (a group's) last tile of its first head speaks for its page ids.
+      const AttnRequest own = attn_own(a, j.p[1], r, j.b[1].low[r]);
       int bad = 0;
       if (own.fine)
 #pragma unroll

@@ -13,7 +13,7 @@ int prefix_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 
 // Rows of a tile for a usual group's, or request's, rows.
 int prefix_rows(const dsr_tree_attention_args_t& a, int64_t count) {
   const int64_t rows = count > 0 ? (a.tokens * (a.q_heads / a.kv_heads) + count - 1) / count : 0;
-  return rows <= 16 ? 16 : a.head_dim > 128 ? (rows <= 64 ? 64 : 128) : rows <= 32 ? 32 : 128;
+  return rows <= 16 ? 16 : a.head_dim > 128 && rows <= 64 ? 64 : 128;
 }
 
 // The work splits of both passes, from sizes alone.
@@ -26,7 +26,7 @@ void prefix_plan(const dsr_tree_attention_args_t& a, const int64_t* counts, Attn
   for (int pass = 0; pass < 2; ++pass) {
     AttnPlan& p = plans[pass] = AttnPlan{};
     p.tile_rows = rows[pass];
-    p.tokens = p.tile_rows <= 32 ? 128 : p.tile_rows == 64 ? 64 : 32;
+    p.tokens = p.tile_rows == 16 ? 128 : p.tile_rows == 64 ? 64 : 32;
     p.min_steps = 128 / p.tokens;
     p.cut = true;
     const int64_t tiles = (a.tokens * group / p.tile_rows + counts[pass]) * a.kv_heads;
@@ -38,8 +38,7 @@ void prefix_plan(const dsr_tree_attention_args_t& a, const int64_t* counts, Attn
     most += tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;  // shares of the fewest steps
   }
   // Workgroups that the chip holds at once: 256 CUs, two each where there is room.
-  const bool mid = rows[0] > 16 && rows[0] < 128;
-  int groups = big || mid ? 256 : 512;
+  int groups = big ? 256 : 512;
   if (most < groups) groups = (int)((most + 7) / 8 * 8);
   plans[0].groups = plans[1].groups = groups;
 }
@@ -82,7 +81,7 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
   return at;
 }
 
-constexpr int64_t kPrefixFewRows = 16384, kPrefixItems = 4096;
+constexpr int64_t kPrefixItems = 1024;
 
 template <class T, int DP>
 int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j, hipStream_t s) {
@@ -98,7 +97,6 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   // Workgroups for rows of no request: one for each 256 KB that all rows have.
   const int64_t clear = (a.tokens * a.q_heads * a.head_dim * 2 + (1 << 18) - 1) >> 18;
   const dim3 grid((unsigned)(j.p[0].groups + (clear > 256 ? 256 : clear < 8 ? 8 : clear)));
-  constexpr int kMid = DP <= 128 ? 32 : 64;
   constexpr bool whole = kAttnThreads % (DP / 8) == 0;
   const bool flat = whole && a.page >= attn_round(DP) && a.k_token <= 1 << 24 && a.v_token <= 1 << 24;
   auto launch = [&](auto A, auto B) {
@@ -110,27 +108,33 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, false>), grid, threads, 0, s, c);
   };
   constexpr std::integral_constant<int, 16> few{};
-  constexpr std::integral_constant<int, kMid> mid{};
   constexpr std::integral_constant<int, 128> many{};
   // A group's rows are no fewer than a request's.
   switch (j.p[0].tile_rows) {
     case 16: launch(few, few); break;
     case 128: j.p[1].tile_rows == 16 ? launch(many, few) : launch(many, many); break;
-    default: j.p[1].tile_rows == 16 ? launch(mid, few) : launch(mid, mid);
+    default:
+      if constexpr (DP > 128) {
+        constexpr std::integral_constant<int, 64> mid{};
+        j.p[1].tile_rows == 16 ? launch(mid, few) : launch(mid, mid);
+      }
   }
   if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   const int64_t rows = x.a.tokens * x.a.q_heads;
   if (rows == 0) return 0;
-  const int jr = rows <= kPrefixFewRows ? 2 : 8;
-  // Blocks of rows of an item: one where there are few, else so many that the chip still has items enough.
+  // Parts of a row, about: the chip's workgroups over all tiles, or as many as the longest row has steps.
+  const int64_t tiles = (rows + j.p[0].tile_rows - 1) / j.p[0].tile_rows, span = (int64_t)a.width * a.page;
+  const int64_t cuts = j.p[0].groups / tiles, steps = span / 128, parts = 2 + (cuts < steps ? cuts : steps);
+  const int jr = parts > 6 ? 2 : 8;
+  // Blocks of rows of an item: one where there are few, else so many that the chip holds about all items at once.
   const int64_t blocks = (x.a.q_heads + jr - 1) / jr, most = x.a.tokens * blocks / kPrefixItems;
-  const int each = (int)(most < 1 ? 1 : most < blocks ? most : blocks);
-  const int64_t items = x.a.tokens * ((blocks + each - 1) / each);
-  const dim3 join((unsigned)(items < (1 << 20) ? items : 1 << 20));
+  const int64_t each = most < 1 ? 1 : most < blocks ? most : blocks, chunks = (blocks + each - 1) / each;
+  const int64_t tokens = x.a.tokens < (1 << 20) / chunks ? x.a.tokens : (1 << 20) / chunks;
+  const dim3 join((unsigned)tokens, (unsigned)chunks);
   if (jr == 2)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), join, threads, 0, s, j, each);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), join, threads, 0, s, j, (int)each);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), join, threads, 0, s, j, each);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), join, threads, 0, s, j, (int)each);
   return launched();
 }
 

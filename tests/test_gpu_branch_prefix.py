@@ -111,6 +111,11 @@ def test_requests_that_are_refused():
     assert res.status.tolist() == [0, 16, 0, 0, 16, 0, 0]
     for r in (1, 4):
         assert not res.out[2 * r:2 * r + 2].any() and torch.isneginf(res.lse[2 * r:2 * r + 2]).all()
+    many = PrefixStep(rng, 2, [32], [70, 3], [9, 9], 4, 2, 64, 16, "bf16")
+    many.visible = np.full(73, 7, np.int64)  # more new tokens than a mask has bits
+    more = branches.prefix_attention(*many.prefix_args()[0], visible=many.args()[1], lse=True)
+    assert more.status.tolist() == [16, 0] and not more.out[:70].any() and torch.isneginf(more.lse[:70]).all()
+    assert more.out[70:].any(-1).all()
     step.kv_lengths[[1, 4]] = step.kv_lengths[[0, 3]]
     fine = branches.prefix_attention(*step.prefix_args()[0], lse=True)
     keep = torch.tensor([0, 2, 3, 5, 6], device="cuda")
