@@ -146,15 +146,23 @@ int32_t dsr_fork_pages(const dsr_fork_args_t* args, void* stream) {
   if (!a.workspace || ((uintptr_t)a.workspace & 15u) || a.workspace_bytes < dsr_fork_workspace_bytes(args))
     return DSR_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t words = a.shared_out != a.shared ? a.blocks : pages_words(a.blocks);
-  const int64_t helpers = (words + 8 * kForkThreads - 1) / (8 * kForkThreads);
-  hipLaunchKernelGGL(k_fork_scan, dim3(1 + (unsigned)(helpers < 256 ? helpers : 256)), dim3(kForkThreads), 0, s, a);
-  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
-  if (a.rows + a.sources > 0) {
-    hipLaunchKernelGGL(k_fork_rows, dim3((unsigned)(a.rows + a.sources)), dim3(kPagesThreads), 0, s, a);
+  int chunks = 0;  // of pages that the last launch frees
+  if (a.rows <= kForkSmallRows && a.sources <= kForkSmallRows && a.blocks <= kForkSmallBlocks &&
+      (a.rows + a.sources) * a.width <= kForkSmallEntries) {
+    hipLaunchKernelGGL(k_fork_small, dim3(1), dim3(kForkThreads), 0, s, a);
     if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    if (a.cache_count == 0) return 0;
+  } else {
+    const int64_t words = a.shared_out != a.shared ? a.blocks : pages_words(a.blocks);
+    const int64_t helpers = (words + 8 * kForkThreads - 1) / (8 * kForkThreads);
+    hipLaunchKernelGGL(k_fork_scan, dim3(1 + (unsigned)(helpers < 256 ? helpers : 256)), dim3(kForkThreads), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    if (a.rows + a.sources > 0) {
+      hipLaunchKernelGGL(k_fork_rows, dim3((unsigned)(a.rows + a.sources)), dim3(kPagesThreads), 0, s, a);
+      if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    }
+    chunks = pages_chunks(a.blocks);
   }
-  const int chunks = pages_chunks(a.blocks);
   return pages_launch(
       a, a.rows,
       [&](const dsr_fork_args_t& part, const PagesCaches<kPagesInline>& caches, unsigned copiers, bool first) {
@@ -164,7 +172,8 @@ int32_t dsr_fork_pages(const dsr_fork_args_t* args, void* stream) {
                              s, part, caches, free);
       },
       [&](const dsr_fork_args_t& all, unsigned copiers) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_fork_finish<0>), dim3(chunks + copiers), dim3(kPagesThreads), 0, s, all,
+        if (chunks + copiers > 0)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(k_fork_finish<0>), dim3(chunks + copiers), dim3(kPagesThreads), 0, s, all,
                            PagesCaches<0>{}, chunks);
       });
 }
@@ -187,15 +196,20 @@ int32_t dsr_compact_pages(const dsr_compact_args_t* args, void* stream) {
     return DSR_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   const dim3 threads(kPagesThreads);
-  const int64_t clear = (pages_words(a.blocks) + 8 * kPagesThreads - 1) / (8 * kPagesThreads);
-  hipLaunchKernelGGL(k_compact_clear, dim3((unsigned)(clear < 256 ? clear : 256)), threads, 0, s, a);
-  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
-  if (a.rows > 0) {
-    hipLaunchKernelGGL(k_compact_mark, dim3((unsigned)a.rows), threads, 0, s, a);
+  if (a.blocks <= kCompactSmallBlocks && a.rows * a.width <= kCompactSmallEntries) {
+    hipLaunchKernelGGL(k_compact_small, dim3(1), dim3(kForkThreads), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+  } else {
+    const int64_t clear = (pages_words(a.blocks) + 8 * kPagesThreads - 1) / (8 * kPagesThreads);
+    hipLaunchKernelGGL(k_compact_clear, dim3((unsigned)(clear < 256 ? clear : 256)), threads, 0, s, a);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    if (a.rows > 0) {
+      hipLaunchKernelGGL(k_compact_mark, dim3((unsigned)a.rows), threads, 0, s, a);
+      if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL(k_compact_plan, dim3((unsigned)pages_chunks(a.blocks)), threads, 0, s, a);
     if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   }
-  hipLaunchKernelGGL(k_compact_plan, dim3((unsigned)pages_chunks(a.blocks)), threads, 0, s, a);
-  if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   const int64_t entries = a.blocks > a.pool_size ? a.blocks : a.pool_size;
   const int64_t each = (entries + kPagesThreads - 1) / kPagesThreads;
   const int rows = (int)a.rows, others = (int)(each < 512 ? each : 512);
