@@ -231,11 +231,11 @@ struct AttnSegment {
   uint32_t from, to;  // the tile's place in the order of all steps
 };
 
-// Steps of a share.
-__device__ __forceinline__ uint32_t attn_quota(const AttnPlan& p, uint32_t total) {
+// Steps of a share, `least` at least.
+__device__ __forceinline__ uint32_t attn_quota(const AttnPlan& p, uint32_t total, uint32_t least) {
   // Most calls of one step per tile have a workgroup for each: no division then.
   const uint32_t quota = total <= (uint32_t)p.groups ? 1 : (total + p.groups - 1) / (uint32_t)p.groups;
-  return quota < (uint32_t)p.min_steps ? p.min_steps : quota;
+  return quota < least ? least : quota;
 }
 
 // A workgroup's share of the work.
@@ -281,11 +281,15 @@ struct AttnWork {
     const AttnPlan& p = c.p;
     const int R = (int)attn_count(c);
     int upto = 0, steps = 0;
-    uint32_t total = 0;
+    uint32_t total = 0, tiles = 0;
     for (int first = 0; first < R; first += 64) {
       steps = hold(c, first);
       upto = attn_wave_scan(steps);
       total += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+      if constexpr (BRANCH) {
+        const int mine_tiles = first + (int)(threadIdx.x & 63) < R && mine.rows > 0 ? mine.tiles * a.kv_heads : 0;
+        tiles += (uint32_t)__builtin_amdgcn_readlane(attn_wave_scan(mine_tiles), 63);
+      }
       // Requests without rows have no work: the first workgroup tells their status.
       const int l = threadIdx.x & 63;
       if (blockIdx.x == 0 && border == 0 && threadIdx.x < 64 && first + l < R && mine.rows == 0) {
@@ -296,7 +300,12 @@ struct AttnWork {
         }
       }
     }
-    quota = attn_quota(p, total);
+    uint32_t least = p.min_steps;
+    if constexpr (BRANCH) {
+      // Tiles of fewer steps are shares of their own (drafted trees of 16 rows behind 32 tokens: 46 us of 4 steps a share, 23 so).
+      if (total < least * tiles) least = total / tiles > 1 ? total / tiles : 1;
+    }
+    quota = attn_quota(p, total, least);
     const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
       // The groups' pass has its shares from the other end, so that where both have few they are not the same workgroups'.

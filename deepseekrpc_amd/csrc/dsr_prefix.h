@@ -111,12 +111,11 @@ __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int l
 // part without weight.
 // What bounds it: a chain of reads (the token's request, its tiles' shares, the
 // parts), then the parts' way through the caches.
-template <class T, int DP, int JR>
-__global__ __launch_bounds__(kAttnThreads, 7) void k_prefix_join(PrefixJoin j, int each) {
+template <class T, int DP, int JR, int FLIGHT>
+__global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int each) {
   typedef typename AttnType<T>::x4 x4;
   constexpr int E = JR * DP / 4;  // four dimensions of a row each
   constexpr int SLOTS = E < kAttnThreads ? kAttnThreads / E : 1;
-  constexpr int FLIGHT = 3;
   __shared__ float sm[SLOTS][JR], sl[SLOTS][JR];
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const dsr_tree_attention_args_t& a = j.a;

@@ -35,7 +35,8 @@ void prefix_plan(const dsr_tree_attention_args_t& a, const int64_t* counts, Attn
     p.group = (int)group;
     p.tile_shift = log2_of(p.tile_rows), p.token_shift = log2_of(p.tokens), p.group_shift = log2_of(group);
     p.page_shift = a.page > 0 ? log2_of(a.page) : 0;
-    most += tiles * ((span + p.tokens - 1) / p.tokens) / p.min_steps + 1;  // shares of the fewest steps
+    const int64_t cuts = (span + p.tokens - 1) / p.tokens / p.min_steps;  // shares of the fewest steps
+    most += tiles * (cuts > 1 ? cuts : 1) + 1;
   }
   // Workgroups that the chip holds at once: 256 CUs, two each where there is room.
   int groups = big ? 256 : 512;
@@ -125,16 +126,16 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   // Parts of a row, about: the chip's workgroups over all tiles, or as many as the longest row has steps.
   const int64_t tiles = (rows + j.p[0].tile_rows - 1) / j.p[0].tile_rows, span = (int64_t)a.width * a.page;
   const int64_t cuts = j.p[0].groups / tiles, steps = span / 128, parts = 2 + (cuts < steps ? cuts : steps);
-  const int jr = parts > 6 ? 2 : 8;
+  const int jr = parts > 6 ? 4 : 8;
   // Blocks of rows of an item: one where there are few, else so many that the chip holds about all items at once.
   const int64_t blocks = (x.a.q_heads + jr - 1) / jr, most = x.a.tokens * blocks / kPrefixItems;
   const int64_t each = most < 1 ? 1 : most < blocks ? most : blocks, chunks = (blocks + each - 1) / each;
   const int64_t tokens = x.a.tokens < (1 << 20) / chunks ? x.a.tokens : (1 << 20) / chunks;
   const dim3 join((unsigned)tokens, (unsigned)chunks);
-  if (jr == 2)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 2>), join, threads, 0, s, j, (int)each);
+  if (jr == 4)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 4, 5>), join, threads, 0, s, j, (int)each);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8>), join, threads, 0, s, j, (int)each);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_join<T, DP, 8, 4>), join, threads, 0, s, j, (int)each);
   return launched();
 }
 
