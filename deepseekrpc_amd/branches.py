@@ -25,8 +25,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as N
-from .tree import (AttentionResult, _array, _attention, _device_of, _overlap, _page, _Prepared, _requests, _rows, _table,
-                   _unrecorded)
+from .tree import (AttentionResult, _array, _attention, _device_of, _overlap, _page, _Prepared, _requests, _rows,
+                   _table, _unrecorded)
 
 E_PARENT = N.E_PARENT
 _LOGITS_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16, torch.float32: N.F32}

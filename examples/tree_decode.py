@@ -54,7 +54,7 @@ class Model:
         x = x.float()
         return (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)).to(torch.bfloat16)
 
-    def forward(self, tokens, plan, k_caches, v_caches):
+    def forward(self, tokens, plan, k_caches, v_caches, attend=tree.tree_attention):
         """Hidden states of the step's tokens; their keys and values go to the caches."""
         x = self.embed[tokens]
         n, split = tokens.numel(), [self.dim, self.kv * self.head, self.kv * self.head]
@@ -63,8 +63,8 @@ class Model:
             q, k, v = (t.view(n, -1, self.head) for t in (q, k, v))
             q = tree.rotary(q, k, plan.positions, self.freqs, v=v, magnitude=self.magnitude, slots=plan.slots,
                             k_cache=k_caches[i], v_cache=v_caches[i]).q
-            out = tree.tree_attention(q, k_caches[i], v_caches[i], plan.table, plan.offsets, plan.kv_lengths,
-                                      visible=plan.visible).out
+            out = attend(q, k_caches[i], v_caches[i], plan.table, plan.offsets, plan.kv_lengths,
+                         visible=plan.visible).out
             x = x + out.view(n, -1) @ self.out[i].t()
             a, b = (self.norm(x) @ self.up[i].t()).chunk(2, -1)
             x = x + (torch.nn.functional.silu(a) * b) @ self.down[i].t()

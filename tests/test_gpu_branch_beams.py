@@ -105,7 +105,8 @@ def test_equal_offers_go_to_the_lowest_row_and_token(dtype):
     x[:] = torch.from_numpy(rng.integers(-3, 4, (4, 20000)).astype(np.float32))  # thousands of equals
     x[2] = x[0]
     check(x, [-1.0, -1.5, -1.0, -2.0], [0, 4], 64)
-    y = torch.arange(20000, device="cuda").float().expand(4, -1).div(64).to(DTYPES[dtype])  # ascending: the last are best
+    # Ascending: the last are best.
+    y = torch.arange(20000, device="cuda").float().expand(4, -1).div(64).to(DTYPES[dtype])
     check(y, [-1.0, -1.5, -1.25, -2.0], [0, 4], 64)
     z = y.flip(1).contiguous()
     check(z, [-1.0, -1.5, -1.25, -2.0], [0, 4], 64)

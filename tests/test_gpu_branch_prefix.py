@@ -84,7 +84,8 @@ def test_values_that_are_not_numbers(where, value):
         ctx = int(step.kv_lengths[1]) - new
         at = dict(prefix=60, own=ctx - 5, tree=ctx + 1, behind=None)[where]
         if at is None:  # a page that no row holds, and what lies behind a request's last token
-            step.v[int(step.table[1, (ctx + new - 1) // 8]), (ctx + new) % 8 or 7:, :, 3] = value if (ctx + new) % 8 else 0
+            rest = (ctx + new) % 8
+            step.v[int(step.table[1, (ctx + new - 1) // 8]), rest or 7:, :, 3] = value if rest else 0
         else:
             step.v[int(step.table[1, at // 8]), at % 8, 0, 5] = value
         run(step, "bf16")
