@@ -138,6 +138,7 @@ struct AttnRequest {
   int rows, tiles;
   bool fine;
   int low;        // BRANCH: first token that is read
+  int pages;      // BRANCH: the table row with its page ids
 };
 constexpr int kAttnAlign = 32;  // steps begin at multiples of it, so that a round of loads is on one page
 
@@ -160,6 +161,7 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   q.kv = q.fine && q.n > 0 ? kv : 0;
   q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
   q.low = 0;
+  q.pages = r;
   return q;
 }
 
@@ -172,17 +174,26 @@ __device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t&
   if (q.kv == 0) q.low = 0;
   return q;
 }
-// and of a group.
+// and of a group.  Its page ids are those of its first request that has tokens
+// behind the prefix: others may be empty rows.
 __device__ __forceinline__ AttnRequest attn_group(const dsr_tree_attention_args_t& a, const AttnPlan& p,
                                                   const AttnBranch& b, int g) {
   AttnRequest q;
   const int N = (int)a.tokens, R = (int)a.requests, r0 = b.groups[g], r1 = b.groups[g + 1], kv = b.prefix[g];
   q.fine = r0 >= 0 && r0 < r1 && r1 <= R && kv > 0 && kv <= (int64_t)a.width * a.page;
-  int lo = q.fine ? a.offsets[r0] : 0, hi = q.fine ? a.offsets[r1] : 0;
-  lo = lo < 0 ? 0 : lo > N ? N : lo;
-  hi = hi < lo ? lo : hi > N ? N : hi;
-  q.lo = lo;
-  q.n = hi - lo;
+  const int r = q.fine ? r0 : 0, s = q.fine ? r1 : 0;
+  auto token = [&](int x) { return x < 0 ? 0 : x > N ? N : x; };
+  int first = token(a.offsets[r]), next = token(a.offsets[r + 1]), length = a.kv_lengths[r];
+  const int hi = token(a.offsets[s]);
+  q.lo = q.fine ? first : 0;
+  q.n = q.fine && hi > first ? hi - first : 0;
+  q.pages = r0;
+  while (q.n > 0 && !(next > first && length - (next - first) >= kv) && ++q.pages < r1) {
+    first = next;
+    next = token(a.offsets[q.pages + 1]);
+    length = a.kv_lengths[q.pages];
+  }
+  if (q.pages == r1) q.n = 0;  // no row sees the prefix
   q.kv = q.n > 0 ? kv : 0;
   q.rows = q.n * p.group;
   q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
@@ -206,9 +217,11 @@ __device__ __forceinline__ int attn_context(const AttnCall&, const AttnRequest& 
 __device__ __forceinline__ int attn_context(const AttnBranchCall& c, const AttnRequest& q) {
   return c.b.own ? q.kv - q.n : q.kv;
 }
-__device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r) { return c.a.table + r * c.a.table_ld; }
-__device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int r) {
-  return c.a.table + (c.b.own ? r : c.b.groups[r]) * c.a.table_ld;
+__device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r, const AttnRequest&) {
+  return c.a.table + r * c.a.table_ld;
+}
+__device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int, const AttnRequest& q) {
+  return c.a.table + q.pages * c.a.table_ld;
 }
 
 // Inclusive sums over the lanes of a wave, without LDS (row shifts, then the
@@ -358,6 +371,7 @@ struct AttnWork {
       q.tiles = __builtin_amdgcn_readlane(mine.tiles, l);
       q.fine = __builtin_amdgcn_readlane((int)mine.fine, l);
       q.low = BRANCH ? __builtin_amdgcn_readlane(mine.low, l) : 0;
+      q.pages = BRANCH ? __builtin_amdgcn_readlane(mine.pages, l) : 0;
       steps = steps_of(p, q);
       length = q.tiles * steps * a.kv_heads;
       if (at - base < length) break;
@@ -430,25 +444,33 @@ __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const 
   }
   __syncthreads();
   const int first = groups ? 0 : (int)blockIdx.x * threads, step = groups ? threads : (int)gridDim.x * threads;
+  auto at = [&](int g) { return groups ? groups[g] : c.b.groups[g]; };
   for (int r = first + (int)threadIdx.x; r < R; r += step) {
     int lo = 0, hi = G;  // the groups that begin at or before r
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      if ((groups ? groups[mid] : c.b.groups[mid]) <= r)
+      if (at(mid) <= r)
         lo = mid + 1;
       else
         hi = mid;
     }
     int low = wrong ? -1 : 0, mine = -1, group_lo = 0;
-    if (!wrong && lo > 0 && r < (groups ? groups[lo] : c.b.groups[lo])) {
-      const int prefix = c.b.prefix[lo - 1];
+    const int begin = lo > 0 ? at(lo - 1) : 0, end = lo > 0 ? at(lo) : 0;
+    if (!wrong && r < end) {
+      const int N = (int)c.a.tokens, prefix = c.b.prefix[lo - 1], last = c.a.offsets[end];
+      const AttnRequest own = attn_request(requests.a, requests.p, r);
+      group_lo = c.a.offsets[begin];
+      group_lo = group_lo < 0 ? 0 : group_lo > N ? N : group_lo;
       low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
       if (low > 0) {
         mine = lo - 1;
-        const AttnRequest q = attn_group(c.a, c.p, c.b, mine), own = attn_request(requests.a, requests.p, r);
-        group_lo = q.lo;
-        // A context shorter than the prefix, a length out of bounds, offsets that do not ascend.
-        if (!own.fine || c.a.kv_lengths[r] - own.n < low || own.lo < q.lo || own.lo + own.n > q.lo + q.n) low = mine = -1;
+        // A context shorter than the prefix, a length out of bounds, offsets that do not ascend.  Without new tokens
+        // nothing is read.
+        if (own.n == 0)
+          low = own.fine ? 0 : -1, mine = -1;
+        else if (!own.fine || c.a.kv_lengths[r] - own.n < low || own.lo < group_lo ||
+                 own.lo + own.n > (last < N ? last : N))
+          low = mine = -1;
       }
     }
     if (groups) attn_lows()[r] = low;
@@ -506,7 +528,7 @@ __device__ __forceinline__ void attn_poison(const Call& c, const AttnSegment& u,
   }
 #pragma unroll 1
   for (int at = from; at < u.end; ++at) {
-    const int id = attn_pages(c, u.r)[at >> p.page_shift], place = at & (a.page - 1);
+    const int id = attn_pages(c, u.r, q)[at >> p.page_shift], place = at & (a.page - 1);
     if ((unsigned)id >= (unsigned)a.blocks) continue;
     const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
     const T* k = (const T*)a.k_cache + id * a.k_block + place * a.k_token + u.head * a.k_head;
@@ -632,7 +654,7 @@ __device__ __forceinline__ void attn_few(char* lds, int pass) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x4{};
     const dsr_tree_attention_args_t& c = attn_call<BRANCH>(pass).a;
-    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r);
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r, q);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
     const int shift = attn_call<BRANCH>(pass).p.page_shift, page = c.page;

@@ -173,13 +173,16 @@ typedef struct dsr_compact_args {
  * a prefix.  Group g is requests [groups[g], groups[g + 1]); the first
  * prefix_lengths[g] tokens of their contexts are the same, on the same pages:
  * their keys and values are read once for all of the group's rows, from the
- * table row of its first request, and may be from that of each.  Requests of
- * no group have no shared prefix.  out, lse and `visible` are as there, and so
+ * table row of its first request with new tokens, and may be from that of each.
+ * Requests without new tokens may be anything, empty rows too.  Requests of no
+ * group have no shared prefix.  out, lse and `visible` are as there, and so
  * is the rounding.
  * Status per request: as there, and DSR_E_LENGTH too where groups do not
  * ascend within 0 .. requests (every request), prefix_lengths[g] is negative or
- * more than width * page, or a request's context (kv_lengths less its new
- * tokens) is shorter than its group's prefix.
+ * more than width * page (requests of that group), or the context of a request
+ * with new tokens (kv_lengths less these) is shorter than its group's prefix.
+ * Values are summed with weights of at most 1 before the sum is divided by that
+ * of the weights: values near the type's largest in many places overflow.
  * `a.workspace` holds dsr_prefix_attention_workspace_bytes(args). */
 typedef struct dsr_prefix_attention_args {
   dsr_tree_attention_args_t a;

@@ -169,8 +169,48 @@ def test_padding_rows_and_empty_requests():
     # Tiles are chosen by the length of the arrays, so not bit by bit what a call without padding gives.
     check(step, tree.AttentionResult(out[5:10], res.lse[5:10], res.status), "f16")
     assert not res.status.any()
+    # Fewer tokens than the offsets say: the last request has what there is of its own.
+    for have in (1, 3, 4):
+        cut = branches.prefix_attention(args[0][:have].contiguous(), *args[1:], lse=True)
+        assert not cut.status.any() and torch.isfinite(cut.lse).all()
     none = branches.prefix_attention(q[:0], *args[1:4], torch.zeros_like(args[4]), *args[5:], lse=True)
     assert none.out.numel() == 0 and not none.status.any()
+
+
+@pytest.mark.parametrize("n,dim", [(1, 64), (12, 128), (2, 256)])
+def test_groups_with_empty_rows(n, dim):
+    """Ended branches: rows without pages, tokens or a context, first ones of their group among them."""
+    rng = np.random.default_rng([n, dim])
+    new = [0, n, 0, n, 0, 0, 0, n, n]
+    step = PrefixStep(rng, 4, [160, 96], new, [30] * 9, 4, 2, dim, 16, "bf16", 1)
+    for r in (0, 4, 5, 6):
+        step.table[r] = -1
+        step.kv_lengths[r] = 0
+    assert not run(step, "bf16").status.any()
+    step.kv_lengths[[1, 7]] = 20 + n  # shorter than their prefixes: the next ones lead, or none
+    args, _ = step.prefix_args()
+    res = branches.prefix_attention(*args, lse=True)
+    assert res.status.tolist() == [0, 16, 0, 0, 0, 0, 0, 16, 0]
+    lo = step.offsets
+    for r in (1, 7):
+        assert not res.out[lo[r]:lo[r + 1]].any() and torch.isneginf(res.lse[lo[r]:lo[r + 1]]).all()
+    want = tree.tree_attention(*args[:6], lse=True)
+    for r in (3, 8):  # two results, each off by 2^-8 of itself and of the values' mean size (below 4 together)
+        rows = slice(lo[r], lo[r + 1])
+        assert (res.out[rows].float() - want.out[rows].float()).abs().max() <= 2.0**-5
+        assert (res.lse[rows] - want.lse[rows]).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("family", [1, 7])
+def test_many_requests(family):
+    """More than every workgroup finds the groups of for itself."""
+    rng = np.random.default_rng(family)
+    R, alone = 1099, 1099 % family + 6 * family
+    groups = (R - alone) // family
+    prefix = [int(x) * 8 for x in rng.integers(0, 8, groups)]
+    step = PrefixStep(rng, family, prefix, list(rng.integers(0, 3, R)), list(rng.integers(0, 20, R)), 2, 1, 64, 8,
+                      "bf16", alone)
+    assert not run(step, "bf16").status.any()
 
 
 def test_strided_rows_and_another_stream():
