@@ -168,7 +168,7 @@ __device__ __forceinline__ double beam_value(uint64_t u) {
   return __longlong_as_double(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u);
 }
 
-// exp(d) for -700 <= d <= 0, to about 2^-52: 2^(n / 256) from a table times a
+// A sum and exp(d), -700 <= d <= 0, to about 2^-52: 2^(n / 256) from a table times a
 // polynomial of what is left, |r| <= ln 2 / 512, whose next term would be below
 // 2^-54 (Tang, Table-driven implementation of the exponential function, 1989).
 // n is rounded by adding 1.5 x 2^52, which leaves it in the low bits; the power
@@ -178,7 +178,7 @@ constexpr int kBeamTable = 256;
 __device__ __forceinline__ void beam_table(double* table) {
   for (int i = threadIdx.x; i < kBeamTable; i += blockDim.x) table[i] = exp2(i / (double)kBeamTable);
 }
-__device__ __forceinline__ double beam_exp(double d, const double* table) {
+__device__ __forceinline__ double beam_add(double sum, double d, const double* table) {  // sum + exp(d)
   constexpr double kRound = 6755399441055744.0;
   const double t = __builtin_fma(d, 369.3299304675746, kRound);  // 256 / ln 2
   const double r = __builtin_fma(t - kRound, -0.0027076061740622863, d);
@@ -188,11 +188,11 @@ __device__ __forceinline__ double beam_exp(double d, const double* table) {
   p = __builtin_fma(p, r, 1.0);
   const int k = (int)__double_as_longlong(t);
   const int64_t scale = (int64_t)((uint64_t)(uint32_t)(k >> 8) << 52);
-  return p * __longlong_as_double(__double_as_longlong(table[k & (kBeamTable - 1)]) + scale);
+  return __builtin_fma(p, __longlong_as_double(__double_as_longlong(table[k & (kBeamTable - 1)]) + scale), sum);
 }
 // exp(x - top); x may be -inf or NaN, top not.
 __device__ __forceinline__ double beam_exp(float x, float top, const double* table) {
-  return beam_exp(__builtin_fmax((double)x - (double)top, -kBeamFar), table);
+  return beam_add(0.0, __builtin_fmax((double)x - (double)top, -kBeamFar), table);
 }
 
 __device__ __forceinline__ double beam_sum(double x) {  // over the wave's lanes
@@ -265,7 +265,10 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
   uint64_t top = 0, floor = 0;
   auto take = [&](uint64_t key) __attribute__((always_inline)) {
     beam_sort(key);
-    beam_join(top, beam_turn(key));
+    if (__ballot(top != 0))
+      beam_join(top, beam_turn(key));
+    else
+      top = key;
     floor = __shfl(top, a.keep - 1);
   };
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -288,7 +291,8 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
   double sum = 0.0;
   if (base > -INFINITY)
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) sum += beam_exp(x[e], base, table);
+    for (int e = 0; e < EACH; ++e)
+      sum = beam_add(sum, __builtin_fmax((double)x[e] - (double)base, -kBeamFar), table);
   sum = beam_sum(sum);
   const int wrong = __ballot(bad) != 0;
   list[w][l] = top;
@@ -392,7 +396,10 @@ __global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_be
     }
     if (!__ballot(last < mine)) continue;
     beam_sort(mine);
-    beam_join(best, beam_turn(mine));
+    if (__ballot(best.key != 0))
+      beam_join(best, beam_turn(mine));
+    else
+      best = mine;
     last = BeamOffer{(uint64_t)__shfl(best.key, keep - 1), (uint32_t)__shfl((int)best.place, keep - 1)};
   }
 #pragma unroll
