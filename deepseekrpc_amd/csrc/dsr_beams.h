@@ -202,10 +202,15 @@ __device__ __forceinline__ double beam_sum(double x) {  // over the wave's lanes
 }
 
 // EACH: logits of a thread.  VEC: rows are 16-byte aligned and read 16 bytes at a time.
+//
+// What bounds it: the issue of vector instructions, 26 a logit, of which the
+// exponential takes 17, most of them float64.  128 rows of 129,280 bf16 (33 MB)
+// 18.2 us, 512 of float32 (265 MB) 68 us, 3.9 TB/s; 4 rows of 32,000 6.5 us, one
+// wave's chain of a read and sorts.
 template <class T, int EACH, bool VEC>
 __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_args_t a) {
-  typedef T xv __attribute__((ext_vector_type(16 / sizeof(T))));
   constexpr int VE = VEC ? 16 / sizeof(T) : 1, C = EACH / VE;
+  typedef T xv __attribute__((ext_vector_type(VE)));
   __shared__ double table[kBeamTable];
   __shared__ uint64_t list[kBeamWaves][kBeamList];
   __shared__ BeamPart part[kBeamWaves];
@@ -220,10 +225,18 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
   // Element e of the thread is token first + (e / VE * threads + thread) VE + e % VE.
   float x[EACH];
   auto token = [&](int e) { return first + (e / VE * kBeamThreads + (int)threadIdx.x) * VE + e % VE; };
+  // No read stands behind a branch of its own (129,281 bf16 logits, which are read
+  // one by one, 42 us where each did, 28 so), but in rows that end inside 16 bytes.
+  if (V % VE == 0) {
+    xv v[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = token(c * VE);
-    if constexpr (VEC) {
+    for (int c = 0; c < C; ++c) v[c] = *(const xv*)(logits + (token(c * VE) < V ? token(c * VE) : 0));
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) x[e] = token(e / VE * VE) < V ? (float)v[e / VE][e % VE] : -INFINITY;
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int at = token(c * VE);
       if (at + VE <= V) {
         const xv v = *(const xv*)(logits + at);
 #pragma unroll
@@ -232,8 +245,6 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
 #pragma unroll
         for (int i = 0; i < VE; ++i) x[c * VE + i] = at + i < V ? (float)logits[at + i] : -INFINITY;
       }
-    } else {
-      x[c] = at < V ? (float)logits[at] : -INFINITY;
     }
   }
   beam_table(table);
@@ -320,6 +331,9 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_slices(dsr_select_beams_a
   }
 }
 
+// What bounds it: a chain of reads, a logarithm and sorts, with nothing to fill the
+// chip beside (1 group of 4 rows 6.6 us, 64 of 8 9.8).  Eight waves share a group so
+// that the chain is short: its rows' sums and the candidates go to all of them.
 __global__ __launch_bounds__(kBeamGroupThreads) void k_beam_groups(dsr_select_beams_args_t a) {
   __shared__ double table[kBeamTable];
   __shared__ uint64_t keys[kBeamGroupWaves][64];

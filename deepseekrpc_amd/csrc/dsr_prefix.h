@@ -27,9 +27,14 @@ struct PrefixCall {
 // requests' B.  Prefixes are bound by the matrix cores, the tokens of single
 // requests by memory, so one half of the workgroups (64 in turn) begins with the
 // prefixes and the other with the requests.  64 requests over one prefix of
-// 32,768 tokens, up to 1,024 of their own: 163 us so, 169 with the prefixes first
-// everywhere, 171 with the requests, 171 where 256 in turn do, 190 in two
-// launches; 8 prefixes of 8 requests 95, 119 in two launches.
+// 32,768 tokens, up to 1,024 of their own: 158 us so, 164 with the prefixes first
+// everywhere, 168 with the requests, 160 where every other one does, 169 where 256
+// in turn do (in two launches 190, 163 then in one); 8 prefixes of 8 requests 92,
+// and 94 in each of the other orders.
+//
+// What bounds it: long prefixes by the issue of the products' instructions (650 to
+// 700 TFLOP/s of 128-row tiles), few and short tokens by a share's beginning and
+// end, which are each a chain of reads.
 template <int ROWS, class T, int DP, bool FLAT>
 __device__ __forceinline__ void prefix_pass(char* lds, int pass) {
   if constexpr (ROWS == 16)
@@ -110,7 +115,9 @@ __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int l
 // order; a thread has FLIGHT parts in flight.  A refused request's rows are one
 // part without weight.
 // What bounds it: a chain of reads (the token's request, its tiles' shares, the
-// parts), then the parts' way through the caches.
+// parts; 4 tokens of 32 heads 6.6 us), then the parts' way through the caches of
+// other XCDs (64 tokens of 64 heads and 17 parts a row 13 us, 2,900 of 32 and few
+// parts 40).
 template <class T, int DP, int JR, int FLIGHT>
 __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int each) {
   typedef typename AttnType<T>::x4 x4;
