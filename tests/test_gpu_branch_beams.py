@@ -118,6 +118,24 @@ def test_many_rows_of_one_group():
     check(rows_of(rng, 700, 30, "bf16"), -20 * rng.random(700), np.arange(701), 3)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,V,ld,offset", [
+    (512, 16384, 16384, 0), (512, 16389, 16392, 0), (512, 4099, 4099, 0), (515, 2048, 2056, 8),
+    (256, 9001, 9001, 0), (256, 8200, 8200, 0), (256, 12289, 12296, 0), (300, 8193, 8200, 1)])
+def test_many_logits_a_thread(rows, V, ld, offset, dtype):
+    """Rows enough for 64 or 32 logits a thread.  64 additions in a row in place of
+    32 are 32 roundings more, of which check()'s bound has 5 x 40 to spare."""
+    rng = np.random.default_rng([rows, V, ld, offset])
+    offsets = [rows - 20, rows - 17, rows - 8, rows - 8, rows]
+    x = rows_of(rng, rows, V, dtype, ld, offset)
+    x[-18, V // 2:] = -math.inf
+    x[-16, : V - 1] = -math.inf
+    x[-15, V - 1] = math.nan
+    finished = np.arange(rows) % 24 != rows % 24  # the others are there for their number
+    finished[-20:] = rng.random(20) < 0.1
+    check(x, -20 * rng.random(rows), offsets, 9, finished.astype(np.int32).tolist())
+
+
 def test_far_scores_and_logits():
     """Scores a long output's, logits far apart: nothing is lost in between."""
     rng = np.random.default_rng(6)
