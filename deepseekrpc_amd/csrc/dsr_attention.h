@@ -175,24 +175,21 @@ __device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t&
   return q;
 }
 // and of a group.  Its page ids are those of its first request that has tokens
-// behind the prefix: others may be empty rows.
+// behind the prefix: others may be empty rows.  `low` is as in AttnBranch: above 0
+// for no other request, and for none where the groups do not ascend.
+template <class Low>
 __device__ __forceinline__ AttnRequest attn_group(const dsr_tree_attention_args_t& a, const AttnPlan& p,
-                                                  const AttnBranch& b, int g) {
+                                                  const AttnBranch& b, int g, Low low) {
   AttnRequest q;
   const int N = (int)a.tokens, R = (int)a.requests, r0 = b.groups[g], r1 = b.groups[g + 1], kv = b.prefix[g];
   q.fine = r0 >= 0 && r0 < r1 && r1 <= R && kv > 0 && kv <= (int64_t)a.width * a.page;
-  const int r = q.fine ? r0 : 0, s = q.fine ? r1 : 0;
   auto token = [&](int x) { return x < 0 ? 0 : x > N ? N : x; };
-  int first = token(a.offsets[r]), next = token(a.offsets[r + 1]), length = a.kv_lengths[r];
-  const int hi = token(a.offsets[s]);
+  int leads = low(q.fine ? r0 : 0);
+  const int first = token(a.offsets[q.fine ? r0 : 0]), hi = token(a.offsets[q.fine ? r1 : 0]);
   q.lo = q.fine ? first : 0;
   q.n = q.fine && hi > first ? hi - first : 0;
   q.pages = r0;
-  while (q.n > 0 && !(next > first && length - (next - first) >= kv) && ++q.pages < r1) {
-    first = next;
-    next = token(a.offsets[q.pages + 1]);
-    length = a.kv_lengths[q.pages];
-  }
+  while (q.n > 0 && leads <= 0 && ++q.pages < r1) leads = low(q.pages);
   if (q.pages == r1) q.n = 0;  // no row sees the prefix
   q.kv = q.n > 0 ? kv : 0;
   q.rows = q.n * p.group;
@@ -210,8 +207,8 @@ __device__ __forceinline__ int64_t attn_count(const AttnCall& c) { return c.a.re
 __device__ __forceinline__ int64_t attn_count(const AttnBranchCall& c) { return c.b.count; }
 __device__ __forceinline__ AttnRequest attn_request(const AttnCall& c, int r) { return attn_request(c.a, c.p, r); }
 __device__ __forceinline__ AttnRequest attn_request(const AttnBranchCall& c, int r) {
-  if (!c.b.own) return attn_group(c.a, c.p, c.b, r);
-  return attn_own(c.a, c.p, r, c.a.requests <= kAttnLows ? attn_lows()[r] : c.b.low[r]);
+  const auto low = [&](int i) { return c.a.requests <= kAttnLows ? attn_lows()[i] : c.b.low[i]; };
+  return c.b.own ? attn_own(c.a, c.p, r, low(r)) : attn_group(c.a, c.p, c.b, r, low);
 }
 __device__ __forceinline__ int attn_context(const AttnCall&, const AttnRequest& q) { return q.kv - q.n; }
 __device__ __forceinline__ int attn_context(const AttnBranchCall& c, const AttnRequest& q) {

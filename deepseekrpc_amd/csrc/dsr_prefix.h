@@ -105,9 +105,13 @@ __device__ __forceinline__ int prefix_owner(const dsr_tree_attention_args_t& a, 
 }
 
 // Where the shares of the tile of row `row` (of a request's, or group's, rows
-// of key head `head`; its first token is `lo`) are told.
+// of key head `head`; its first token is `lo`) are told.  Where offsets out of
+// order make more steps than are counted, a tile may have been told none: nothing
+// is read for it then.
 __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int lo, int head, int row) {
-  return j.b[pass].tiles[((int64_t)head * j.a.tokens + lo) * j.p[0].group + (row & -j.p[pass].tile_rows)];
+  const int2 s = j.b[pass].tiles[((int64_t)head * j.a.tokens + lo) * j.p[0].group + (row & -j.p[pass].tile_rows)];
+  const uint32_t shares = j.p[0].groups, first = s.x, count = s.y;
+  return first < shares && count <= shares - first ? s : int2{0, 0};
 }
 
 // An item is a token and `each` blocks of JR of its rows (heads), a block at a
@@ -212,11 +216,12 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
       // A request's (a group's) last tile of its first head speaks for its page ids.
       const AttnRequest own = attn_own(a, j.p[1], r, j.b[1].low[r]);
       int bad = 0;
+      const auto low = [&](int i) { return j.b[0].low[i]; };
       if (own.fine)
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
           if (pass == 0 && g < 0) continue;
-          const AttnRequest q = pass == 0 ? attn_group(a, j.p[0], j.b[0], g) : own;
+          const AttnRequest q = pass == 0 ? attn_group(a, j.p[0], j.b[0], g, low) : own;
           const int2 s = prefix_tile(j, pass, q.lo, 0, (q.tiles - 1) * j.p[pass].tile_rows);
           if (s.y == 1) bad |= j.b[pass].bad[pass == 0 ? g : r];
           for (int c = 0; s.y > 1 && c < s.y; ++c) bad |= j.p[pass].part_bad[2 * (s.x + c) + (c == 0)];

@@ -127,7 +127,8 @@ def test_requests_that_are_refused():
 @pytest.mark.parametrize("groups,prefix,status", [
     ([0, 3, 6], [64, -1], [0, 0, 0, 16, 16, 16, 0]), ([0, 3, 6], [1 << 30, 96], [16, 16, 16, 0, 0, 0, 0]),
     ([0, 5, 3], [64, 64], [16] * 7), ([-1, 3, 6], [64, 64], [16] * 7), ([0, 3, 8], [64, 64], [16] * 7),
-    ([1, 3, 3], [64, 64], [0] * 7), ([0, 0, 0], [64, 9], [0] * 7), ([7, 7, 7], [64, 9], [0] * 7)])
+    ([1, 3, 3], [64, 64], [0] * 7), ([0, 0, 0], [64, 9], [0] * 7), ([7, 7, 7], [64, 9], [0] * 7),
+    ([0, 7, 0, 7, 0, 7], [64] * 5, [16] * 7)])
 def test_groups_out_of_bounds(groups, prefix, status):
     rng = np.random.default_rng(5)
     step = PrefixStep(rng, 3, [64, 96], [2] * 7, [30] * 7, 4, 2, 64, 16, "bf16", 1)
@@ -211,6 +212,10 @@ def test_many_requests(family):
     step = PrefixStep(rng, family, prefix, list(rng.integers(0, 3, R)), list(rng.integers(0, 20, R)), 2, 1, 64, 8,
                       "bf16", alone)
     assert not run(step, "bf16").status.any()
+    step.groups[1::2], step.groups[::2] = R, 0  # all requests in every second group: nothing is read
+    step.prefix[:] = 8
+    res = branches.prefix_attention(*step.prefix_args()[0], lse=True)
+    assert (res.status == 16).all() and not res.out.any() and torch.isneginf(res.lse).all()
 
 
 def test_strided_rows_and_another_stream():
