@@ -43,6 +43,16 @@ def caches_of(rng, p, count, kv, dim, dtype="bf16", by_head=False):
     return [t.transpose(1, 2) for t in made] if by_head else made
 
 
+def far_apart(cache):
+    """The cache with its pages spread over more than 2^32 bytes."""
+    blocks, *page = cache.shape
+    elements = cache[0].numel()
+    step = max(elements, ((5 << 30) // cache.element_size() // blocks + 127) // 128 * 128)
+    strides = [elements // page[0], page[2], 1]
+    far = torch.empty((blocks - 1) * step + elements, dtype=cache.dtype, device=cache.device)
+    return far.as_strided(cache.shape, (step, *strides)).copy_(cache)
+
+
 def copied(caches, copies):
     """The caches after the copies (from, to, tokens)."""
     out = []

@@ -5,7 +5,7 @@ import torch
 
 from deepseekrpc_amd import branches
 from oracle import branch_oracle as O
-from tests.branch_util import Pages, caches_of, copied
+from tests.branch_util import Pages, caches_of, copied, far_apart
 from tests.tree_util import i32
 
 pytestmark = pytest.mark.gpu
@@ -61,6 +61,13 @@ def test_pages_before_the_first_stay():
     p = Pages(rng, [64, 40, 20], 1, 16, spare=30, first=6)
     p.table[0, 0], p.table[2, 1] = 2, 5
     check(p, caches_of(rng, p, 2, 1, 8))
+
+
+def test_caches_past_32_bits():
+    rng = np.random.default_rng(13)
+    p = Pages(rng, [64, 40, 20, 90], 2, 8, spare=30, first=2)
+    _, want = check(p, [far_apart(caches_of(rng, p, 1, 2, 16)[0])])
+    assert want["copies"]
 
 
 @pytest.mark.parametrize("count", [1, 128, 129, 300])

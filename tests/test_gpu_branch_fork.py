@@ -6,7 +6,7 @@ import torch
 
 from deepseekrpc_amd import branches
 from oracle import branch_oracle as O
-from tests.branch_util import Pages, caches_of, copied
+from tests.branch_util import Pages, caches_of, copied, far_apart
 from tests.tree_util import i32
 
 pytestmark = pytest.mark.gpu
@@ -146,6 +146,13 @@ def test_many_pages():
     assert p.blocks > 2 * 32768
     _, want, _ = check(p, rng.integers(-1, 64, 64), caches_of(rng, p, 1, 1, 8))
     consistent(p, want)
+
+
+def test_caches_past_32_bits():
+    rng = np.random.default_rng(12)
+    p = Pages(rng, [37, 50, 5, 63, 64, 30], 3, 8, spare=20)
+    cache = far_apart(caches_of(rng, p, 1, 2, 16)[0])
+    check(p, [0, 0, 1, 3, 3, 3, 5, 5, 2, 2], [cache])
 
 
 def test_given_results_leave_the_inputs():

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from deepseekrpc_amd import branches, tree
-from tests.branch_util import PrefixStep
+from tests.branch_util import PrefixStep, far_apart
 from tests.tree_exact import check
 from tests.tree_util import i32
 
@@ -216,6 +216,17 @@ def test_many_requests(family):
     step.prefix[:] = 8
     res = branches.prefix_attention(*step.prefix_args()[0], lse=True)
     assert (res.status == 16).all() and not res.out.any() and torch.isneginf(res.lse).all()
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_caches_past_32_bits(new):
+    rng = np.random.default_rng(new)
+    step = PrefixStep(rng, 4, [160, 96], [new] * 8, [30] * 8, 4, 2, 128, 16, "bf16")
+    args, _ = step.prefix_args()
+    near = branches.prefix_attention(*args, lse=True)
+    far = branches.prefix_attention(args[0], far_apart(args[1]), far_apart(args[2]), *args[3:], lse=True)
+    check(step, far, "bf16")
+    assert torch.equal(far.out, near.out) and torch.equal(far.lse, near.lse) and not far.status.any()
 
 
 def test_strided_rows_and_another_stream():
