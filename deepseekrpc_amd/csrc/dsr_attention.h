@@ -852,6 +852,7 @@ __device__ __forceinline__ void attn_few(char* lds, int pass) {
         o += *(const attn_f32x4*)((const float*)&vals[i][0][0] + row * OS + d);
       }
       if (split) {
+        if (BRANCH && d >= dim) continue;  // the join reads no more
         *(attn_f32x4*)&e.p.part_o[(((int64_t)part << row_shift) + row) * DP + d] = o;
         if (d == 0) e.p.part_ml[((int64_t)part << row_shift) + row] = float2{M, L};
       } else if (row0 + row < q.rows && d < dim) {

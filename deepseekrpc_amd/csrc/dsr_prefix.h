@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
 #pragma unroll
       for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
         const int in = x / (DP / 4), h = h0 + in, d = x % (DP / 4) * 4;
-        const bool live = h < heads && !spare;
+        const bool live = h < heads && !spare && d < a.head_dim;
         const int64_t row = (int64_t)t * heads + h;
         float M = -INFINITY, L = 0.f;
         attn_f32x4 o = {};
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
           }
           __syncthreads();  // the next block's
         }
-        if (slot > 0 || !live || d >= a.head_dim) continue;
+        if (slot > 0 || !live) continue;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         x4 y;
 #pragma unroll
