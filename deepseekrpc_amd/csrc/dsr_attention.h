@@ -312,13 +312,15 @@ struct AttnWork {
     }
     uint32_t least = p.min_steps;
     if constexpr (BRANCH) {
-      // Tiles of fewer steps are shares of their own (drafted trees of 16 rows behind 32 tokens: 46 us of 4 steps a share, 23 so).
+      // Tiles of fewer steps are shares of their own (drafted trees of 16 rows behind 32 tokens: 46 us of 4 steps a
+      // share, 23 so).
       if (total < least * tiles) least = total / tiles > 1 ? total / tiles : 1;
     }
     quota = attn_quota(p, total, least);
     const uint32_t each = quota == 1 ? (total + 7) / 8 : (total + 8 * quota - 1) / (8 * quota);  // workgroups, per XCD
     if (border == 0) {
-      // The groups' pass has its shares from the other end, so that where both have few they are not the same workgroups'.
+      // The groups' pass has its shares from the other end, so that where both have few they are not the same
+      // workgroups'.
       uint32_t group = blockIdx.x;
       if constexpr (BRANCH) group = c.b.own ? group : p.groups - 1 - group;
       me = (group & 7) * each + (group >> 3);

@@ -98,7 +98,8 @@ extern "C" {
 size_t dsr_select_beams_workspace_bytes(const dsr_select_beams_args_t* args) {
   if (!args || !beams_shape_ok(*args)) return 0;
   const int64_t slices = beam_slices(*args);
-  return (size_t)(args->rows * (slices * (int64_t)sizeof(BeamPart) + (int64_t)sizeof(BeamTerm) + slices * args->keep * 8));
+  const int64_t row = slices * (int64_t)sizeof(BeamPart) + (int64_t)sizeof(BeamTerm) + slices * args->keep * 8;
+  return (size_t)(args->rows * row);
 }
 
 int32_t dsr_select_beams(const dsr_select_beams_args_t* args, void* stream) {

@@ -56,7 +56,7 @@ constexpr bool prefix_two() {  // a CU has room for two workgroups
 template <class T, int DP, int A, int B, bool FLAT>
 __global__ __launch_bounds__(kAttnThreads, (prefix_two<A, DP>() && prefix_two<B, DP>() ? 2 : 1)) void
 k_prefix_attention(PrefixCall) {
-  constexpr int kLds = prefix_lds<A, T, DP>() > prefix_lds<B, T, DP>() ? prefix_lds<A, T, DP>() : prefix_lds<B, T, DP>();
+  constexpr int kA = prefix_lds<A, T, DP>(), kB = prefix_lds<B, T, DP>(), kLds = kA > kB ? kA : kB;
   static_assert(kLds >= (kAttnLows + 1) * 4, "the groups fit");
   __shared__ __align__(16) char lds[kLds];
   const int shares = attn_call<true>(0).p.groups;

@@ -103,8 +103,8 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   auto launch = [&](auto A, auto B) {
     constexpr int rows = decltype(A)::value, own = decltype(B)::value;
     if (flat && rows > 16)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, whole && (rows > 16)>), grid, threads, 0, s,
-                         c);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, whole && (rows > 16)>), grid, threads, 0,
+                         s, c);
     else
       hipLaunchKernelGGL(HIP_KERNEL_NAME(k_prefix_attention<T, DP, rows, own, false>), grid, threads, 0, s, c);
   };
