@@ -106,7 +106,7 @@ struct AttnBranch {
   int32_t* bad;           // [count]: a page id outside the cache
   float* row_o;           // [tokens, query heads, head dim of the kernel]
   float2* row_ml;         // [tokens, query heads]: base (log2) and sum
-  int32_t* low;           // each request's first own token, -1: refused,
+  int32_t* low;           // each request's first own token, -1: refused, kAttnNone (every one): nothing is read,
   int32_t* group_of;      // its group, -1: none,
   int32_t* group_lo;      // and its group's first new token
 };
@@ -115,6 +115,7 @@ struct AttnBranchCall {
   AttnPlan p;
   AttnBranch b;
 };
+constexpr int kAttnNone = -2;
 constexpr int kAttnLows = 1024;  // requests whose `low` every workgroup finds for itself (attn_branch_lows)
 template <bool BRANCH>
 struct AttnArgs {
@@ -169,6 +170,7 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
 __device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t& a, const AttnPlan& p, int r, int low) {
   AttnRequest q = attn_request(a, p, r);
   q.low = low;
+  if (low == kAttnNone) q.n = q.rows = 0, q.tiles = 1;
   if (low < 0) q.fine = false;
   if (!q.fine) q.kv = 0;
   if (q.kv == 0) q.low = 0;
@@ -406,13 +408,14 @@ struct AttnWork {
 };
 
 // Rows of no request, before the first one's and past the last one's, give 0
-// and -inf.  The workgroups past p.groups take them in turn: looked for by the
-// workgroups that have shares, they cost every small call 0.2 us of 8.5.
+// and -inf; with `all`, every row does.  The workgroups past p.groups take them
+// in turn: looked for by the workgroups that have shares, they cost every small
+// call 0.2 us of 8.5.
 template <class T, bool BRANCH = false>
-__device__ __forceinline__ void attn_clear(int groups, int threads) {
+__device__ __forceinline__ void attn_clear(int groups, int threads, bool all = false) {
   typedef typename AttnType<T>::x8 x8;
   const dsr_tree_attention_args_t& a = attn_call<BRANCH>().a;
-  const int N = (int)a.tokens, lo = a.offsets[0], hi = a.offsets[a.requests];
+  const int N = (int)a.tokens, lo = all ? N : a.offsets[0], hi = a.offsets[a.requests];
   const int lead = lo < 0 ? 0 : lo > N ? N : lo, rest = hi < lead ? lead : hi > N ? N : hi;
   const int none = lead + N - rest, chunks = a.head_dim / 8;
   for (int i = blockIdx.x - groups; i < none; i += gridDim.x - groups) {
@@ -425,23 +428,30 @@ __device__ __forceinline__ void attn_clear(int groups, int threads) {
   }
 }
 
+// Whether the groups do not ascend within the requests, or the offsets, held
+// to the tokens, descend: whose rows are whose cannot be told then, every
+// request is refused and every row is 0.  `groups`, if not null, is LDS that
+// gets a copy of them.  (Reads one after the other cost a call 0.3 us of 20.)
+__device__ __forceinline__ bool attn_branch_wrong(const AttnBranchCall& c, int threads, int* groups) {
+  const int G = c.b.group_count, R = (int)c.a.requests, N = (int)c.a.tokens;
+  bool wrong = false;
+  for (int i = threadIdx.x; i <= R; i += threads) {  // all reads of a round side by side
+    const int g = min(i, G), begin = c.b.groups[max(g - 1, 0)], r = c.b.groups[g];
+    const int lo = c.a.offsets[max(i - 1, 0)], hi = c.a.offsets[i];
+    wrong |= r < 0 || r > R || begin > r || min(max(lo, 0), N) > min(max(hi, 0), N);
+    if (groups && i <= G) groups[i] = r;
+  }
+  return __syncthreads_or(wrong);
+}
+
 // Each request's group and prefix.  Up to kAttnLows requests every workgroup
 // finds them for itself, in LDS (a launch for it would cost 2 us or more), the
 // first one also for the join; `groups` is LDS for kAttnLows + 1 numbers.  More
-// requests have a launch of their own, and `groups` null.  Groups that do not
-// ascend refuse every request.
+// requests have a launch of their own, and `groups` null.
 __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const AttnBranchCall& requests, int threads,
                                                  int* groups) {
-  __shared__ int wrong;
   const int G = c.b.group_count, R = (int)c.a.requests;
-  if (threadIdx.x == 0) wrong = 0;
-  __syncthreads();
-  for (int g = threadIdx.x; g <= G; g += threads) {
-    const int r = c.b.groups[g];
-    if (r < 0 || r > R || (g > 0 && c.b.groups[g - 1] > r)) wrong = 1;
-    if (groups) groups[g] = r;
-  }
-  __syncthreads();
+  const bool wrong = attn_branch_wrong(c, threads, groups);
   const int first = groups ? 0 : (int)blockIdx.x * threads, step = groups ? threads : (int)gridDim.x * threads;
   auto at = [&](int g) { return groups ? groups[g] : c.b.groups[g]; };
   for (int r = first + (int)threadIdx.x; r < R; r += step) {
@@ -453,22 +463,20 @@ __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const 
       else
         hi = mid;
     }
-    int low = wrong ? -1 : 0, mine = -1, group_lo = 0;
+    int low = wrong ? kAttnNone : 0, mine = -1, group_lo = 0;
     const int begin = lo > 0 ? at(lo - 1) : 0, end = lo > 0 ? at(lo) : 0;
     if (!wrong && r < end) {
-      const int N = (int)c.a.tokens, prefix = c.b.prefix[lo - 1], last = c.a.offsets[end];
+      const int N = (int)c.a.tokens, prefix = c.b.prefix[lo - 1];
       const AttnRequest own = attn_request(requests.a, requests.p, r);
       group_lo = c.a.offsets[begin];
       group_lo = group_lo < 0 ? 0 : group_lo > N ? N : group_lo;
       low = prefix >= 0 && prefix <= (int64_t)c.a.width * c.a.page ? prefix : -1;
       if (low > 0) {
         mine = lo - 1;
-        // A context shorter than the prefix, a length out of bounds, offsets that do not ascend.  Without new tokens
-        // nothing is read.
+        // A context shorter than the prefix, or a length out of bounds.  Without new tokens nothing is read.
         if (own.n == 0)
           low = own.fine ? 0 : -1, mine = -1;
-        else if (!own.fine || c.a.kv_lengths[r] - own.n < low || own.lo < group_lo ||
-                 own.lo + own.n > (last < N ? last : N))
+        else if (!own.fine || c.a.kv_lengths[r] - own.n < low)
           low = mine = -1;
       }
     }

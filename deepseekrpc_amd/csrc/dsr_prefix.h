@@ -60,8 +60,13 @@ k_prefix_attention(PrefixCall) {
   static_assert(kLds >= (kAttnLows + 1) * 4, "the groups fit");
   __shared__ __align__(16) char lds[kLds];
   const int shares = attn_call<true>(0).p.groups;
-  if ((int)blockIdx.x >= shares) return attn_clear<T, true>(shares, kAttnThreads);
-  if (attn_call<true>(0).a.requests <= kAttnLows)
+  const bool few = attn_call<true>(0).a.requests <= kAttnLows;
+  if ((int)blockIdx.x >= shares) {
+    const AttnBranchCall& c = attn_call<true>(0);
+    const bool none = few ? attn_branch_wrong(c, kAttnThreads, nullptr) : c.b.low[0] == kAttnNone;
+    return attn_clear<T, true>(shares, kAttnThreads, none);
+  }
+  if (few)
     attn_branch_lows(attn_call<true>(0), attn_call<true>(1), kAttnThreads, (int*)lds);
   const int first = blockIdx.x >> 6 & 1;
   if constexpr (A == B) {
@@ -105,13 +110,9 @@ __device__ __forceinline__ int prefix_owner(const dsr_tree_attention_args_t& a, 
 }
 
 // Where the shares of the tile of row `row` (of a request's, or group's, rows
-// of key head `head`; its first token is `lo`) are told.  Where offsets out of
-// order make more steps than are counted, a tile may have been told none: nothing
-// is read for it then.
+// of key head `head`; its first token is `lo`) are told: the first and their number.
 __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int lo, int head, int row) {
-  const int2 s = j.b[pass].tiles[((int64_t)head * j.a.tokens + lo) * j.p[0].group + (row & -j.p[pass].tile_rows)];
-  const uint32_t shares = j.p[0].groups, first = s.x, count = s.y;
-  return first < shares && count <= shares - first ? s : int2{0, 0};
+  return j.b[pass].tiles[((int64_t)head * j.a.tokens + lo) * j.p[0].group + (row & -j.p[pass].tile_rows)];
 }
 
 // An item is a token and `each` blocks of JR of its rows (heads), a block at a
@@ -134,10 +135,11 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
   const int slot = SLOTS > 1 ? threadIdx.x / E : 0;
   const bool spare = slot >= SLOTS;  // 192 dimensions
   const int chunk = blockIdx.y;
+  const bool none = j.b[1].low[0] == kAttnNone;  // rows and statuses are written
   for (int64_t item = blockIdx.x; item < a.tokens; item += gridDim.x) {
     const int t = (int)item;
     const int r = prefix_owner(a, t);
-    if (r >= a.requests) continue;
+    if (r >= a.requests || none) continue;
     const int g = j.b[1].group_of[r], g_lo = j.b[1].group_lo[r];
     const int lo = max(a.offsets[r], 0);
     if (t < lo) continue;  // a row of no request

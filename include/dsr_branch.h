@@ -178,7 +178,8 @@ typedef struct dsr_compact_args {
  * group have no shared prefix.  out, lse and `visible` are as there, and so
  * is the rounding.
  * Status per request: as there, and DSR_E_LENGTH too where groups do not
- * ascend within 0 .. requests (every request), prefix_lengths[g] is negative or
+ * ascend within 0 .. requests or offsets, held to 0 .. tokens, descend (every
+ * request, and every row gives 0 and -inf), prefix_lengths[g] is negative or
  * more than width * page (requests of that group), or the context of a request
  * with new tokens (kv_lengths less these) is shorter than its group's prefix.
  * Values are summed with weights of at most 1 before the sum is divided by that
