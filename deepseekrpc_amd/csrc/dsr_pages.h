@@ -227,6 +227,7 @@ __device__ __forceinline__ void fork_decide(const dsr_fork_args_t& a, const Fork
         row.copied = 1;
         const int from = a.table[s * a.table_ld + row.full];
         const bool in = (unsigned)from < (unsigned)a.blocks && (unsigned)row.fresh < (unsigned)a.blocks;
+        if (!in) status = DSR_E_BLOCK;  // a page of its own, but not its tokens
         space.copies[upto - 1] = PageCopy{in ? from : 0, in ? row.fresh : 0, in ? length & (a.page - 1) : 0};
         atomicMax(&taken, upto);
       }

@@ -91,8 +91,10 @@ typedef struct dsr_select_beams_args {
  * pool_state_out may be shared and pool_state; no other arrays may overlap.
  * Status per row: DSR_E_PARENT (parents[r] is neither -1 nor a source),
  * DSR_E_LENGTH (its source's length or pages are out of bounds), DSR_E_BLOCKS:
- * the row is empty; DSR_E_BLOCK (a page id outside the cache): the row is
- * made, but such a page is not copied and not counted.
+ * the row is empty; DSR_E_BLOCK (a page id outside the cache, among the row's
+ * or the one that it should have a copy of): the row is made, but such a page is
+ * not copied and not counted, and the page that was to have its tokens holds
+ * what it held.
  * Status per source: DSR_E_LENGTH (its pages stay as they are, in no row and
  * not in the pool), DSR_E_BLOCK. */
 typedef struct dsr_fork_args {

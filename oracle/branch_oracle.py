@@ -51,7 +51,7 @@ def fork(lengths, parents, table, held, shared, pool, state, blocks, page):
     fine = [L >= 0 and 0 <= h <= width and L <= h * page for L, h in zip(lengths, held)]
     rows, status, copies, children, wanted, taken = [], [], [], [0] * S, 0, 0
     for p in parents:
-        p, row, st, length = int(p), [], OK, 0
+        p, row, st, length, lost = int(p), [], OK, 0, False
         if p < -1 or p >= S:
             st = E_PARENT
         elif p >= 0 and not fine[p]:
@@ -72,12 +72,13 @@ def fork(lengths, parents, table, held, shared, pool, state, blocks, page):
                         fresh = int(pool[(head + taken) % size])
                         taken += 1
                         row = row + [fresh]
-                        if 0 <= source[full] < blocks and 0 <= fresh < blocks:
+                        lost = not 0 <= source[full] < blocks  # the tokens that it should have had
+                        if not lost and 0 <= fresh < blocks:
                             copies.append((source[full], fresh, part))
             if st == OK:
                 children[p] += 1
                 length = int(lengths[p])
-                if any(not 0 <= x < blocks for x in row):
+                if lost or any(not 0 <= x < blocks for x in row):
                     st = E_BLOCK
             else:
                 row = []
