@@ -252,12 +252,18 @@ __device__ __forceinline__ bool fork_entry(const dsr_fork_args_t& a, const ForkR
 }
 
 // A source's page gains the rows that share it besides one, or loses its row.
-// `freed` has a bit per page; whether the page id is outside the cache.
+// `freed` has a bit per page, which changes as often as the count passes 0: in
+// the end it says whether the count is below, whatever the order of the sources
+// (it matters where `shared` knows less holders than there are).
+// Returns whether the page id is outside the cache.
 __device__ __forceinline__ bool fork_count(const dsr_fork_args_t& a, int64_t s, int c, int children, int full,
                                            uint32_t* freed) {
   const int id = a.table[s * a.table_ld + c], change = c < full ? children - 1 : children > 0 ? 0 : -1;
   if ((unsigned)id >= (unsigned)a.blocks) return true;
-  if (change != 0 && atomicAdd(&a.shared_out[id], change) + change < 0) atomicOr(&freed[id >> 5], 1u << (id & 31));
+  if (change != 0) {
+    const int before = atomicAdd(&a.shared_out[id], change);
+    if ((before < 0) != (before + change < 0)) atomicXor(&freed[id >> 5], 1u << (id & 31));
+  }
   return false;
 }
 

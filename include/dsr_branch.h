@@ -18,11 +18,11 @@
  *
  * A page may be held by several rows.  shared[p] counts the rows that hold
  * page p besides one: 0 for a page that is free or held once, which is what
- * dsr_plan_blocks's pages are.  Only pages that are full are shared, so the
- * new tokens of a step, and dsr_commit_tree's moves, are always in pages of
- * their row's own.  A row with shared pages ends in dsr_fork_pages (no row
- * continues it), not in dsr_plan_blocks (added == -1), which would give the
- * shared pages back to the pool.
+ * dsr_plan_blocks's pages are, and never less.  Only pages that are full are
+ * shared, so the new tokens of a step, and dsr_commit_tree's moves, are always
+ * in pages of their row's own.  A row with shared pages ends in dsr_fork_pages
+ * (no row continues it), not in dsr_plan_blocks (added == -1), which would give
+ * the shared pages back to the pool.
  */
 #ifndef DSR_BRANCH_H
 #define DSR_BRANCH_H
@@ -81,10 +81,11 @@ typedef struct dsr_select_beams_args {
  * tokens in it are copied there in every cache.  Rows that the pool cannot
  * serve are refused (DSR_E_BLOCKS), once one is also all later ones that want
  * a page; refused rows are empty.  A page that no row holds any more (its
- * sources ended, or spare pages of a source without a row) goes back to the
- * pool, whose entries are as in dsr_plan_blocks: in ascending order behind the
- * last one, to be taken by the next call.  (Pages that a ring shorter than its
- * pages has no room for are lost.)
+ * sources ended, or spare pages of a source without a row: its count, less one
+ * for each that is gone and more for each row that joins, is below 0) goes back
+ * to the pool, whose entries are as in dsr_plan_blocks: in ascending order
+ * behind the last one, to be taken by the next call.  (Pages that a ring shorter
+ * than its pages has no room for are lost.)
  *
  * Table entries past a row's pages are -1.  table, held and lengths are new
  * arrays: rows may be more or fewer than sources.  shared_out and

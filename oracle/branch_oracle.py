@@ -84,7 +84,7 @@ def fork(lengths, parents, table, held, shared, pool, state, blocks, page):
                 row = []
         rows.append((row, length))
         status.append(st)
-    gone, source_status = set(), []
+    before, source_status = shared.copy(), []
     for s in range(S):
         if not fine[s]:
             source_status.append(E_LENGTH)
@@ -96,10 +96,8 @@ def fork(lengths, parents, table, held, shared, pool, state, blocks, page):
                 bad = True
                 continue
             shared[p] += children[s] - 1 if c < full else 0 if children[s] else -1
-            if shared[p] < 0:
-                gone.add(p)
         source_status.append(E_BLOCK if bad else OK)
-    room, freed = size - count + taken, sorted(gone)
+    room, freed = size - count + taken, [int(p) for p in np.flatnonzero((before < 0) != (shared < 0))]
     for p in freed:
         shared[p] = 0
     for i, p in enumerate(freed[:room]):
