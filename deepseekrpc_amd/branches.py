@@ -32,10 +32,11 @@ E_PARENT = N.E_PARENT
 _LOGITS_TYPES = {torch.bfloat16: N.BF16, torch.float16: N.F16, torch.float32: N.F32}
 
 
-def _caches(a, caches, dev, page, blocks, upload):
-    """Caches that share their strides: fills ``a``; the tensors to keep and
-    what holds their addresses."""
+def _caches(a, name, caches, dev, page, blocks, upload):
+    """Caches that share their strides and are written in place: fills ``a``; the
+    tensors to keep and what holds their addresses."""
     caches = list(caches)
+    _unrecorded(name, *caches)
     if not caches:
         if page is None or blocks is None:
             raise ValueError("without caches, page and blocks are needed")
@@ -190,7 +191,7 @@ class PreparedFork(_Prepared):
         dev = _device_of(lengths, "lengths")
         S, R = _requests(lengths.numel()), _requests(parents.numel())
         a = N.ForkArgs()
-        caches, pointers = _caches(a, caches, dev, page, blocks, upload)
+        caches, pointers = _caches(a, "fork_pages", caches, dev, page, blocks, upload)
         a.lengths = _array(lengths, "lengths", torch.int32, dev)
         a.parents = _array(parents, "parents", torch.int32, dev)
         a.held = _array(held, "held", torch.int32, dev, S)
@@ -236,7 +237,8 @@ def fork_pages(lengths, parents, table, held, shared, pool, state, caches, *, pa
 
     ``shared`` (int32 ``[blocks]``) and ``state`` are updated in place unless
     ``out`` has others; ``out`` may supply any of the results but the pool, in
-    memory of their own.  Without caches, ``page`` and ``blocks`` are given."""
+    memory of their own.  Without caches, ``page`` and ``blocks`` are given.
+    Caches that require a gradient are refused, but under ``torch.no_grad()``."""
     return PreparedFork(lengths, parents, table, held, shared, pool, state, caches, page=page, blocks=blocks, out=out,
                         upload=False).launch()
 
@@ -259,7 +261,7 @@ class PreparedCompact(_Prepared):
         dev = _device_of(held, "held")
         R = _requests(held.numel())
         a = N.CompactArgs()
-        caches, pointers = _caches(a, caches, dev, page, blocks, upload)
+        caches, pointers = _caches(a, "compact_pages", caches, dev, page, blocks, upload)
         a.held = _array(held, "held", torch.int32, dev)
         a.table, a.table_ld, a.width = _table(table, R, dev)
         a.pool = _array(pool, "pool", torch.int32, dev)
@@ -302,7 +304,8 @@ def compact_pages(table, held, pool, state, caches, *, shared=None, first: int =
     afterwards.  ``table``, ``pool``, ``state`` and ``shared`` are rewritten in
     place unless ``out`` has others.  ``remap`` of the result tells page ids that
     are kept elsewhere their new ones.  If any row has a status nothing moves.
-    Without caches, ``page`` and ``blocks`` are given."""
+    Without caches, ``page`` and ``blocks`` are given.  Caches that require a
+    gradient are refused, but under ``torch.no_grad()``."""
     return PreparedCompact(table, held, pool, state, caches, shared=shared, first=first, page=page, blocks=blocks,
                            out=out, upload=False).launch()
 
