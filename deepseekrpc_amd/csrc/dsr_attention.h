@@ -7,6 +7,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -109,6 +110,7 @@ struct AttnBranch {
   int32_t* low;           // each request's first own token, -1: refused, kAttnNone (every one): nothing is read,
   int32_t* group_of;      // its group, -1: none,
   int32_t* group_lo;      // and its group's first new token
+  int32_t* lead;          // each group's first request with tokens behind its prefix, INT_MAX: none
 };
 struct AttnBranchCall {
   dsr_tree_attention_args_t a;
@@ -139,7 +141,6 @@ struct AttnRequest {
   int rows, tiles;
   bool fine;
   int low;        // BRANCH: first token that is read
-  int pages;      // BRANCH: the table row with its page ids
 };
 constexpr int kAttnAlign = 32;  // steps begin at multiples of it, so that a round of loads is on one page
 
@@ -162,7 +163,6 @@ __device__ __forceinline__ AttnRequest attn_request(const dsr_tree_attention_arg
   q.kv = q.fine && q.n > 0 ? kv : 0;
   q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
   q.low = 0;
-  q.pages = r;
   return q;
 }
 
@@ -176,51 +176,52 @@ __device__ __forceinline__ AttnRequest attn_own(const dsr_tree_attention_args_t&
   if (q.kv == 0) q.low = 0;
   return q;
 }
-// and of a group.  Its page ids are those of its first request that has tokens
-// behind the prefix: others may be empty rows.  `low` is as in AttnBranch: above 0
-// for no other request, and for none where the groups do not ascend.
-template <class Low>
+// and of a group, given whether any of its requests has tokens behind the
+// prefix (else no row sees it).  Groups with such a request are within bounds.
 __device__ __forceinline__ AttnRequest attn_group(const dsr_tree_attention_args_t& a, const AttnPlan& p,
-                                                  const AttnBranch& b, int g, Low low) {
+                                                  const AttnBranch& b, int g, bool seen) {
   AttnRequest q;
-  const int N = (int)a.tokens, R = (int)a.requests, r0 = b.groups[g], r1 = b.groups[g + 1], kv = b.prefix[g];
-  q.fine = r0 >= 0 && r0 < r1 && r1 <= R && kv > 0 && kv <= (int64_t)a.width * a.page;
+  const int N = (int)a.tokens, r0 = b.groups[g], r1 = b.groups[g + 1], kv = b.prefix[g];
+  q.fine = seen;
   auto token = [&](int x) { return x < 0 ? 0 : x > N ? N : x; };
-  int leads = low(q.fine ? r0 : 0);
-  const int first = token(a.offsets[q.fine ? r0 : 0]), hi = token(a.offsets[q.fine ? r1 : 0]);
-  q.lo = q.fine ? first : 0;
-  q.n = q.fine && hi > first ? hi - first : 0;
-  q.pages = r0;
-  while (q.n > 0 && leads <= 0 && ++q.pages < r1) leads = low(q.pages);
-  if (q.pages == r1) q.n = 0;  // no row sees the prefix
+  q.lo = q.fine ? token(a.offsets[r0]) : 0;
+  q.n = q.fine ? token(a.offsets[r1]) - q.lo : 0;
   q.kv = q.n > 0 ? kv : 0;
   q.rows = q.n * p.group;
   q.tiles = q.rows > p.tile_rows ? (q.rows + p.tile_rows - 1) >> p.tile_shift : 1;
   q.low = 0;
   return q;
 }
-// What attn_branch_lows left for the workgroup.
+// What attn_branch_lows left for the workgroup: `low` and `lead` as in AttnBranch.
 __device__ __forceinline__ int* attn_lows() {
   __shared__ int lows[kAttnLows];
   return lows;
 }
-// A pass's requests, the context that every row sees, the table row, the mask words.
+__device__ __forceinline__ int* attn_leads() {
+  __shared__ int leads[kAttnLows];
+  return leads;
+}
+// The request whose table row has a group's page ids: others may be empty rows.
+__device__ __forceinline__ int attn_lead(const AttnBranchCall& c, int g) {
+  return c.a.requests <= kAttnLows ? attn_leads()[g] : c.b.lead[g];
+}
+// A pass's requests, the context that every row sees, the table row.
 __device__ __forceinline__ int64_t attn_count(const AttnCall& c) { return c.a.requests; }
 __device__ __forceinline__ int64_t attn_count(const AttnBranchCall& c) { return c.b.count; }
 __device__ __forceinline__ AttnRequest attn_request(const AttnCall& c, int r) { return attn_request(c.a, c.p, r); }
 __device__ __forceinline__ AttnRequest attn_request(const AttnBranchCall& c, int r) {
-  const auto low = [&](int i) { return c.a.requests <= kAttnLows ? attn_lows()[i] : c.b.low[i]; };
-  return c.b.own ? attn_own(c.a, c.p, r, low(r)) : attn_group(c.a, c.p, c.b, r, low);
+  if (c.b.own) return attn_own(c.a, c.p, r, c.a.requests <= kAttnLows ? attn_lows()[r] : c.b.low[r]);
+  return attn_group(c.a, c.p, c.b, r, attn_lead(c, r) < INT_MAX);
 }
 __device__ __forceinline__ int attn_context(const AttnCall&, const AttnRequest& q) { return q.kv - q.n; }
 __device__ __forceinline__ int attn_context(const AttnBranchCall& c, const AttnRequest& q) {
   return c.b.own ? q.kv - q.n : q.kv;
 }
-__device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r, const AttnRequest&) {
+__device__ __forceinline__ const int32_t* attn_pages(const AttnCall& c, int r) {
   return c.a.table + r * c.a.table_ld;
 }
-__device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int, const AttnRequest& q) {
-  return c.a.table + q.pages * c.a.table_ld;
+__device__ __forceinline__ const int32_t* attn_pages(const AttnBranchCall& c, int r) {
+  return c.a.table + (c.b.own ? r : __builtin_amdgcn_readfirstlane(attn_lead(c, r))) * c.a.table_ld;
 }
 
 // Inclusive sums over the lanes of a wave, without LDS (row shifts, then the
@@ -372,7 +373,6 @@ struct AttnWork {
       q.tiles = __builtin_amdgcn_readlane(mine.tiles, l);
       q.fine = __builtin_amdgcn_readlane((int)mine.fine, l);
       q.low = BRANCH ? __builtin_amdgcn_readlane(mine.low, l) : 0;
-      q.pages = BRANCH ? __builtin_amdgcn_readlane(mine.pages, l) : 0;
       steps = steps_of(p, q);
       length = q.tiles * steps * a.kv_heads;
       if (at - base < length) break;
@@ -435,6 +435,7 @@ __device__ __forceinline__ void attn_clear(int groups, int threads, bool all = f
 __device__ __forceinline__ bool attn_branch_wrong(const AttnBranchCall& c, int threads, int* groups) {
   const int G = c.b.group_count, R = (int)c.a.requests, N = (int)c.a.tokens;
   bool wrong = false;
+#pragma unroll 4
   for (int i = threadIdx.x; i <= R; i += threads) {  // all reads of a round side by side
     const int g = min(i, G), begin = c.b.groups[max(g - 1, 0)], r = c.b.groups[g];
     const int lo = c.a.offsets[max(i - 1, 0)], hi = c.a.offsets[i];
@@ -444,13 +445,23 @@ __device__ __forceinline__ bool attn_branch_wrong(const AttnBranchCall& c, int t
   return __syncthreads_or(wrong);
 }
 
+// A request of group `mine` (-1: none, or it does not lead) may be the group's
+// first.  Of a wave's requests in a row only the first one looks (r ascends
+// with the lane).
+__device__ __forceinline__ void attn_lead_of(int32_t* lead, int mine, int r) {
+  const int before = __shfl_up(mine, 1);
+  if (mine >= 0 && ((threadIdx.x & 63) == 0 || before != mine)) atomicMin(&lead[mine], r);
+}
+
 // Each request's group and prefix.  Up to kAttnLows requests every workgroup
 // finds them for itself, in LDS (a launch for it would cost 2 us or more), the
 // first one also for the join; `groups` is LDS for kAttnLows + 1 numbers.  More
-// requests have a launch of their own, and `groups` null.
+// requests have launches of their own, and `groups` null.
 __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const AttnBranchCall& requests, int threads,
                                                  int* groups) {
   const int G = c.b.group_count, R = (int)c.a.requests;
+  if (groups)
+    for (int g = threadIdx.x; g < G; g += threads) attn_leads()[g] = INT_MAX;
   const bool wrong = attn_branch_wrong(c, threads, groups);
   const int first = groups ? 0 : (int)blockIdx.x * threads, step = groups ? threads : (int)gridDim.x * threads;
   auto at = [&](int g) { return groups ? groups[g] : c.b.groups[g]; };
@@ -480,7 +491,12 @@ __device__ __forceinline__ void attn_branch_lows(const AttnBranchCall& c, const 
           low = mine = -1;
       }
     }
-    if (groups) attn_lows()[r] = low;
+    if (groups) {
+      attn_lows()[r] = low;
+      attn_lead_of(attn_leads(), mine, r);
+    } else if (r < G) {
+      c.b.lead[r] = INT_MAX;
+    }
     if (!groups || blockIdx.x == 0) {
       c.b.low[r] = low;
       c.b.group_of[r] = mine;
@@ -535,7 +551,7 @@ __device__ __forceinline__ void attn_poison(const Call& c, const AttnSegment& u,
   }
 #pragma unroll 1
   for (int at = from; at < u.end; ++at) {
-    const int id = attn_pages(c, u.r, q)[at >> p.page_shift], place = at & (a.page - 1);
+    const int id = attn_pages(c, u.r)[at >> p.page_shift], place = at & (a.page - 1);
     if ((unsigned)id >= (unsigned)a.blocks) continue;
     const T* v = (const T*)a.v_cache + id * a.v_block + place * a.v_token + u.head * a.v_head;
     const T* k = (const T*)a.k_cache + id * a.k_block + place * a.k_token + u.head * a.k_head;
@@ -661,7 +677,7 @@ __device__ __forceinline__ void attn_few(char* lds, int pass) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x4{};
     const dsr_tree_attention_args_t& c = attn_call<BRANCH>(pass).a;
-    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r, q);
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
     const int shift = attn_call<BRANCH>(pass).p.page_shift, page = c.page;

@@ -114,7 +114,7 @@ __device__ __forceinline__ void attn_wide_rows(char* attn_lds, int pass) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = attn_f32x16{};
     const dsr_tree_attention_args_t& c = attn_call<BRANCH>(pass).a;
-    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r, q);
+    const int32_t* pages = attn_pages(attn_call<BRANCH>(pass), u.r);
     const T* kb = (const T*)c.k_cache + u.head * c.k_head;
     const T* vb = (const T*)c.v_cache + u.head * c.v_head;
     const int shift = attn_call<BRANCH>(pass).p.page_shift, page = c.page;

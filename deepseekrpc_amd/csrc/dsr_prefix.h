@@ -87,8 +87,15 @@ k_prefix_attention(PrefixCall) {
   }
 }
 
+// More requests than every workgroup looks over for itself, a thread each: their
+// groups, then who leads these.
 __global__ __launch_bounds__(kAttnThreads) void k_prefix_lows(PrefixCall) {
   attn_branch_lows(attn_call<true>(0), attn_call<true>(1), kAttnThreads, nullptr);
+}
+__global__ __launch_bounds__(kAttnThreads) void k_prefix_leads(PrefixCall) {
+  const AttnBranchCall& c = attn_call<true>(0);
+  const int r = (int)blockIdx.x * kAttnThreads + (int)threadIdx.x;
+  attn_lead_of(c.b.lead, r < c.a.requests ? c.b.group_of[r] : -1, r);
 }
 
 struct PrefixJoin {
@@ -218,13 +225,13 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
       // A request's (a group's) last tile of its first head speaks for its page ids.
       const AttnRequest own = attn_own(a, j.p[1], r, j.b[1].low[r]);
       int bad = 0;
-      const auto low = [&](int i) { return j.b[0].low[i]; };
       if (own.fine)
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
           if (pass == 0 && g < 0) continue;
-          const AttnRequest q = pass == 0 ? attn_group(a, j.p[0], j.b[0], g, low) : own;
-          const int2 s = prefix_tile(j, pass, q.lo, 0, (q.tiles - 1) * j.p[pass].tile_rows);
+          const int q_lo = pass == 0 ? g_lo : own.lo;
+          const int end = pass == 0 ? min(a.offsets[j.b[0].groups[g + 1]], (int)a.tokens) : own.lo + own.n;
+          const int2 s = prefix_tile(j, pass, q_lo, 0, (end - q_lo) * group - 1);
           if (s.y == 1) bad |= j.b[pass].bad[pass == 0 ? g : r];
           for (int c = 0; s.y > 1 && c < s.y; ++c) bad |= j.p[pass].part_bad[2 * (s.x + c) + (c == 0)];
         }

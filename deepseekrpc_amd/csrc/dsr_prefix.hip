@@ -58,6 +58,7 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
   int32_t* low = (int32_t*)take(a.requests * 4);
   int32_t* group_of = (int32_t*)take(a.requests * 4);
   int32_t* group_lo = (int32_t*)take(a.requests * 4);
+  int32_t* lead = (int32_t*)take(x.group_count * 4);
   prefix_plan(a, counts, j.p);
   for (int pass = 0; pass < 2; ++pass) {
     AttnPlan& p = j.p[pass];
@@ -78,6 +79,7 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
     b.low = low;
     b.group_of = group_of;
     b.group_lo = group_lo;
+    b.lead = lead;
   }
   return at;
 }
@@ -93,6 +95,8 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   if (a.requests > kAttnLows) {
     const int64_t lows = (a.requests + kAttnThreads - 1) / kAttnThreads;
     hipLaunchKernelGGL(k_prefix_lows, dim3((unsigned)lows), threads, 0, s, c);
+    if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
+    hipLaunchKernelGGL(k_prefix_leads, dim3((unsigned)lows), threads, 0, s, c);
     if (hipGetLastError() != hipSuccess) return DSR_ERR_LAUNCH;
   }
   // Workgroups for rows of no request: one for each 256 KB that all rows have.
