@@ -66,8 +66,9 @@ bool compact_shape_ok(const dsr_compact_args_t& a) {
          a.first < a.blocks && a.pool_size >= a.blocks - a.first;
 }
 
-// The last launch of a call, once for every kPagesInline caches whose
-// addresses go with it; `plain` workgroups of the first one do other work.
+// The last launch of a call: once with the caches' addresses on the device, or
+// once for every kPagesInline caches whose addresses go with it (the first of
+// these has also the work that is not copying).
 // Workgroups that copy: as many as the chip holds a few times over.
 constexpr int64_t kPagesCopiers = 2048;
 template <class A, class Inline, class Device>

@@ -124,7 +124,8 @@ __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int l
 
 // An item is a token and `each` blocks of JR of its rows (heads), a block at a
 // time.  The threads left over take every SLOTS-th part each, summed in a fixed
-// order; a thread has FLIGHT parts in flight.  A refused request's rows are one
+// order (none are where a block has 192 or more dimensions, whose threads are no
+// power of two); a thread has FLIGHT parts in flight.  A refused request's rows are one
 // part without weight.
 // What bounds it: a chain of reads (the token's request, its tiles' shares, the
 // parts; 4 tokens of 32 heads 6.6 us), then the parts' way through the caches of
@@ -139,8 +140,8 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
   __shared__ attn_f32x4 so[SLOTS][SLOTS > 1 ? E : 1];
   const dsr_tree_attention_args_t& a = j.a;
   const int heads = a.q_heads, group = j.p[0].group;
+  static_assert(SLOTS == 1 || SLOTS * E == kAttnThreads, "every thread has a slot");
   const int slot = SLOTS > 1 ? threadIdx.x / E : 0;
-  const bool spare = slot >= SLOTS;  // 192 dimensions
   const int chunk = blockIdx.y;
   const bool none = j.b[1].low[0] == kAttnNone;  // rows and statuses are written
   for (int64_t item = blockIdx.x; item < a.tokens; item += gridDim.x) {
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
 #pragma unroll
       for (int x = SLOTS > 1 ? threadIdx.x % E : threadIdx.x; x < E; x += kAttnThreads) {
         const int in = x / (DP / 4), h = h0 + in, d = x % (DP / 4) * 4;
-        const bool live = h < heads && !spare && d < a.head_dim;
+        const bool live = h < heads && d < a.head_dim;
         const int64_t row = (int64_t)t * heads + h;
         float M = -INFINITY, L = 0.f;
         attn_f32x4 o = {};
@@ -200,8 +201,8 @@ __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int 
           }
         }
         if constexpr (SLOTS > 1) {
-          if (!spare) so[slot][x] = o;
-          if (d == 0 && !spare) {
+          so[slot][x] = o;
+          if (d == 0) {
             sm[slot][in] = M;
             sl[slot][in] = L;
           }

@@ -185,8 +185,10 @@ typedef struct dsr_compact_args {
  * request, and every row gives 0 and -inf), prefix_lengths[g] is negative or
  * more than width * page (requests of that group), or the context of a request
  * with new tokens (kv_lengths less these) is shorter than its group's prefix.
- * Values are summed with weights of at most 1 before the sum is divided by that
- * of the weights: values near the type's largest in many places overflow.
+ * Values are summed in float32 before the sum is divided by that of the weights.
+ * bf16 weights are at most 1: values near that type's largest in many places
+ * overflow.  f16 ones are at most 2^15, and no sum of f16 values does: 2^15 x
+ * 65504 x 2^31 tokens is below 2^62.
  * `a.workspace` holds dsr_prefix_attention_workspace_bytes(args). */
 typedef struct dsr_prefix_attention_args {
   dsr_tree_attention_args_t a;
