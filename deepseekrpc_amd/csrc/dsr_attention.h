@@ -529,7 +529,9 @@ __device__ __forceinline__ bool attn_make_finite(typename AttnType<T>::x8& v) {
 // added in memory: what they hold becomes infinite or NaN as the sum would
 // have.  Adding a term that was in the product already changes nothing, so the
 // tokens from `from` on are all looked at.  A thread takes a row; `base` is
-// its scores' base.  Nothing of this runs for ordinary values.
+// its scores' base.  Nothing of this runs for ordinary values, and the compiler is
+// told so: it spilled what it keeps for it otherwise (16 requests of 64 rows of
+// 256 dimensions over up to 8,000 tokens 107.5 us, 103.3 so).
 template <class T, int DP, class Call>
 __device__ __forceinline__ void attn_poison(const Call& c, const AttnSegment& u, const AttnRequest& q, int from,
                                             const float* base) {
@@ -900,7 +902,7 @@ __device__ __forceinline__ void attn_few(char* lds, int pass) {
     }
     __threadfence_block();
     __syncthreads();
-    if (spoison)
+    if (__builtin_expect(spoison, 0))
       attn_poison<T, DP>(e, u, q, sbad || (BRANCH && begin < q.low) ? begin : max(begin, min(ctx, end) - kAttnTile),
                          sbase);
     attn_report(e, u, q, sbad);

@@ -403,7 +403,7 @@ __device__ __forceinline__ void attn_wide_rows(char* attn_lds, int pass) {
     }
     __threadfence_block();
     __syncthreads();
-    if (spoison)
+    if (__builtin_expect(spoison, 0))
       attn_poison<T, DP>(e, u, q, sbad || (BRANCH && begin < q.low) ? begin : max(begin, clear - NT), sbase);
     attn_report(e, u, q, sbad);
   }
