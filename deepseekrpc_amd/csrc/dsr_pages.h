@@ -538,10 +538,10 @@ __global__ __launch_bounds__(kPagesThreads) void k_compact_plan(dsr_compact_args
   }
 }
 
-// Bits, statuses and moves of a small cache in one workgroup (512 entries and
-// 1,000 pages 4.3 us, 14.2 us a call in four launches and 10.5 so; 2,304 and 2,200
-// 7.6, three launches 14.7).
-constexpr int kCompactSmallEntries = 8192, kCompactSmallBlocks = 32 * kForkThreads;
+// Bits, statuses and moves of a small cache in one workgroup (table entries: 544
+// 7.5 us a call, 10.9 in four launches; 8,032 13.7 and 19.3; 13,400 17.7 and 21.6;
+// 26,800 the same).
+constexpr int kCompactSmallEntries = 16384, kCompactSmallBlocks = 32 * kForkThreads;
 __global__ __launch_bounds__(kForkThreads) void k_compact_small(dsr_compact_args_t a) {
   __shared__ uint32_t bits[kForkThreads];
   __shared__ int part[kForkThreads / 64];
