@@ -10,7 +10,12 @@ int32_t launched() { return hipGetLastError() == hipSuccess ? 0 : DSR_ERR_LAUNCH
 // Dimensions of the kernel that takes a head dimension.
 int prefix_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
-// Rows of a tile for a usual group's, or request's, rows.
+// Rows of a tile for a usual group's, or request's, rows.  64 only above 128
+// dimensions: 8 prefixes of 8 requests, 64 rows a head, 84 us in tiles of 128 rows
+// and 112 in ones of 64, whose steps are of twice the tokens and leave room for one
+// workgroup a CU.  Groups of 32 to 64 rows over 8,192 tokens and more, in tiles of 64
+// and of 128: 192 dimensions 133 to 223 us and 156 to 278; 256 dimensions 308 and 550
+// where requests have 32 rows, but 185 to 283 and 175 to 244 where they have 4 to 16.
 int prefix_rows(const dsr_tree_attention_args_t& a, int64_t count) {
   const int64_t rows = count > 0 ? (a.tokens * (a.q_heads / a.kv_heads) + count - 1) / count : 0;
   return rows <= 16 ? 16 : a.head_dim > 128 && rows <= 64 ? 64 : 128;
@@ -84,6 +89,8 @@ int64_t prefix_space(const dsr_prefix_attention_args_t& x, PrefixJoin& j) {
   return at;
 }
 
+// Items of the join that the chip holds about at once (8 prefixes of 8 requests 84 us, 91 with 256; trees of 96
+// dimensions 71.5 and 79.7; 4,096 as 1,024).
 constexpr int64_t kPrefixItems = 1024;
 
 template <class T, int DP>
@@ -130,6 +137,8 @@ int32_t prefix_launch(const dsr_prefix_attention_args_t& x, const PrefixJoin& j,
   // Parts of a row, about: the chip's workgroups over all tiles, or as many as the longest row has steps.
   const int64_t tiles = (rows + j.p[0].tile_rows - 1) / j.p[0].tile_rows, span = (int64_t)a.width * a.page;
   const int64_t cuts = j.p[0].groups / tiles, steps = span / 128, parts = 2 + (cuts < steps ? cuts : steps);
+  // Many parts: four rows a block, so that more threads share a row's (a single call over 1,000 tokens 19.7 us, 21.0
+  // with eight); few: eight (chunks of up to 400 tokens 591 us, 616 with four).
   const int jr = parts > 6 ? 4 : 8;
   // Blocks of rows of an item: one where there are few, else so many that the chip holds about all items at once.
   const int64_t blocks = (x.a.q_heads + jr - 1) / jr, most = x.a.tokens * blocks / kPrefixItems;
