@@ -279,11 +279,11 @@ __device__ __forceinline__ void fork_state(const dsr_fork_args_t& a, const ForkH
   a.pool_state_out[1] = head.count - head.taken + (freed < room ? freed : room);
 }
 
-// Everything but the copies in one workgroup, for batches that have an entry of
-// rows and sources for each of its threads (1,024 entries 7.9 us a call, 8.9 in
-// three launches).  A second round costs as much as the launches that it spares
-// (1,232 entries 10.3 and 9.3 us, the 1,728 of 32 beams 10.8 and 10.1).
-constexpr int kForkSmallRows = 1024, kForkSmallEntries = kForkThreads, kForkSmallBlocks = 32 * kForkThreads;
+// Everything but the copies in one workgroup, for batches whose tables it goes
+// over about as fast as another launch begins (entries of rows and sources: 1,728
+// 7.5 us, 12.0 in three launches' time in all and 11.2 so; 5,184 15.3, 158.7 and
+// 159.5).
+constexpr int kForkSmallRows = 1024, kForkSmallEntries = 2048, kForkSmallBlocks = 32 * kForkThreads;
 __global__ __launch_bounds__(kForkThreads) void k_fork_small(dsr_fork_args_t a) {
   __shared__ int32_t heir[kForkSmallRows], children[kForkSmallRows];
   __shared__ uint32_t freed[kForkThreads];
