@@ -112,8 +112,9 @@ __device__ __forceinline__ void pages_copy(const PageShape& s, char* cache, cons
 }
 
 // Items (copy, cache), a workgroup each in turn.  What bounds it: memory (224 copies
-// of 63 tokens at most, 16 caches of 8 heads of 256 bytes: 0.9 GB moved in 140 us;
-// whole pages of 64 tokens, 2.3 GB in 447 us, 5.1 TB/s).
+// of 63 tokens at most, 32 caches of 8 heads of 256 bytes: 516 MB written in 140 us,
+// and the 74 MB of the sources' tails, which each of seven copies reads anew from the
+// caches; whole pages of 64 tokens, 2.3 GB in 447 us, 5.1 TB/s).
 template <int COUNT>
 __device__ __forceinline__ void pages_copies(const PageShape& s, const PageCopy* copies, int count,
                                              void* const* device, const PagesCaches<COUNT>& caches, int cache_count,
@@ -280,9 +281,10 @@ __device__ __forceinline__ void fork_state(const dsr_fork_args_t& a, const ForkH
 }
 
 // Everything but the copies in one workgroup, for batches whose tables it goes
-// over about as fast as another launch begins (entries of rows and sources: 1,728
-// 7.5 us, 12.0 in three launches' time in all and 11.2 so; 5,184 15.3, 158.7 and
-// 159.5).
+// over about as fast as the launches begin that it spares (entries of rows and
+// sources, in one workgroup and in three launches: 1,024 7.9 and 8.9 us a call;
+// 1,728 10.8 to 11.0, and 10.1 to 12.2 with how fast the host launches; 2,688 11.6
+// and 9.7).
 constexpr int kForkSmallRows = 1024, kForkSmallEntries = 2048, kForkSmallBlocks = 32 * kForkThreads;
 __global__ __launch_bounds__(kForkThreads) void k_fork_small(dsr_fork_args_t a) {
   __shared__ int32_t heir[kForkSmallRows], children[kForkSmallRows];

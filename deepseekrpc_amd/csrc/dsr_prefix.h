@@ -128,9 +128,9 @@ __device__ __forceinline__ int2 prefix_tile(const PrefixJoin& j, int pass, int l
 // power of two); a thread has FLIGHT parts in flight.  A refused request's rows are one
 // part without weight.
 // What bounds it: a chain of reads (the token's request, its tiles' shares, the
-// parts; 4 tokens of 32 heads 6.6 us), then the parts' way through the caches of
-// other XCDs (64 tokens of 64 heads and 17 parts a row 13 us, 2,900 of 32 and few
-// parts 40).
+// parts; 4 tokens of 32 heads 6.2 us), then the parts' way through the caches of
+// other XCDs (64 tokens of 64 heads and 17 parts a row 12 us, 2,900 of 32 and few
+// parts 38).
 template <class T, int DP, int JR, int FLIGHT>
 __global__ __launch_bounds__(kAttnThreads) void k_prefix_join(PrefixJoin j, int each) {
   typedef typename AttnType<T>::x4 x4;
