@@ -50,7 +50,7 @@ constexpr int prefix_lds() {
     return attn_wide_lds<T, DP, ROWS / 32>();
 }
 template <int ROWS, int DP>
-constexpr bool prefix_two() {  // a CU has room for two workgroups
+constexpr bool prefix_two() {  // registers for two workgroups a CU (above 128 dimensions one is launched)
   return ROWS == 16 ? DP <= 128 : DP * (128 / ROWS) < 512;
 }
 template <class T, int DP, int A, int B, bool FLAT>
